@@ -533,4 +533,7 @@ int fx_hybrid_restore(const uint8_t *codes, const float *rows, const float *colu
 }
 #endif
 
+/* Cached attention with a sliding window and sinks, and the 4-bit key/value cache. */
+#include "fluxbin_attention.h"
+
 #endif /* FLUXBIN_AMD_H */

@@ -5,7 +5,8 @@ Drop-in for the deployment API of maxiu188-afk/Marlin_Style_Fluxbin's
 LUT Linear (``w3_lut_deployment``), fused RMSNorm / RoPE (``fused_modules``) and
 the static-KV decode session (``static_decode``), and the two-base binary-basis
 formats (``packing``, ``evaluation``, ``deployment``, ``engine_interface``; the
-benchmark's rank-one variant in ``two_base``).  GPU work runs in hand-written
+benchmark's rank-one variant in ``two_base``), and attention over long caches
+(``cached_attention``: sliding window with sinks, 4-bit key/value cache).  GPU work runs in hand-written
 HIP kernels behind the C ABI of ``libfluxbin_amd.so`` (``include/fluxbin_amd.h``).
 """
 from .gptq_deployment import (  # noqa: F401
@@ -50,6 +51,7 @@ from .fused_modules import (  # noqa: F401
     rms_norm_reference,
 )
 
+from .cached_attention import Int4KVCache, kv4_attention, window_attention  # noqa: F401
 from .packing import pack_two_bases, unpack_two_bases  # noqa: F401
 from .evaluation import materialize_global_two_base_weight, materialize_hybrid_s8_weight  # noqa: F401
 from .deployment import PackedHybridLinear  # noqa: F401

@@ -15,7 +15,7 @@ from pathlib import Path
 import torch
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libfluxbin_amd.so"
-ABI_VERSION = 20
+ABI_VERSION = 21
 PAYLOAD_PLANAR, PAYLOAD_FIELDS, PAYLOAD_FP6 = 0, 1, 2  # FX_W3_PLANAR / FX_W3_FIELDS / FX_W3_FP6
 
 FX_F32, FX_F16, FX_BF16 = 0, 1, 2
@@ -81,6 +81,16 @@ SIGNATURES: dict[str, tuple] = {
     "fx_hybrid_restore": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _p, _i, _i, _p]),
 }
 
+# mirrors include/fluxbin_attention.h
+ATTENTION_SIGNATURES: dict[str, tuple] = {
+    "fx_cached_attention_workspace_bytes": (_sz, [_i] * 9),
+    "fx_window_attention": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _sz, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _p]),
+    "fx_kv4_attention": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i,
+                              _p]),
+    "fx_kv4_append": (_i, [_p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p]),
+    "fx_kv4_restore": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p]),
+}
+
 _lock = threading.Lock()
 _library = None
 
@@ -99,7 +109,7 @@ def library():
                 "(or __graft_entry__.build()). There is no CPU substitute for the HIP kernels."
             )
         lib = ctypes.CDLL(str(LIBRARY_PATH))
-        for name, (restype, argtypes) in SIGNATURES.items():
+        for name, (restype, argtypes) in (SIGNATURES | ATTENTION_SIGNATURES).items():
             fn = getattr(lib, name)
             fn.restype = restype
             fn.argtypes = argtypes

@@ -1,0 +1,117 @@
+// Shared device code of the cached-attention kernels: matrix instructions, the keys
+// that a workgroup's queries see, and where they sit in the cache.
+#pragma once
+#include "attention_launch.h"
+
+namespace fx {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+
+// D = A B + C.  Lane l holds row (A) or column (B) l % 32 (l % 16), depth elements
+// 8 (l / 32).. (8 (l / 16)..); of C column l % 32 and rows (r & 3) + 8 (r >> 2) + 4 (l / 32)
+// (column l % 16, rows 4 (l / 16) + r).
+template <int DT>
+__device__ __forceinline__ f32x16_t mfma32(const u32x4_t& a, const u32x4_t& b, const f32x16_t& c) {
+  if constexpr (DT == kBF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                   c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                  0, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ f32x4_t mfma16(const u32x4_t& a, const u32x4_t& b, const f32x4_t& c) {
+  if constexpr (DT == kBF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                   c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                  0, 0, 0);
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// The sum / maximum over the two lanes l and l ^ 32 (every lane gets it).
+__device__ __forceinline__ float half_pair_max(float v) {
+  const unsigned u = __float_as_uint(v);
+  const u32x2_t r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_pair_sum(float v) {
+  const unsigned u = __float_as_uint(v);
+  const u32x2_t r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Two 16-bit values of one word: nonzero iff either is an infinity or a NaN (the exponent
+// field, all ones, carries into its sign bit).
+template <int DT>
+__device__ __forceinline__ unsigned nonfinite_pair(unsigned w) {
+  constexpr unsigned e = DT == kBF16 ? 0x7f807f80u : 0x7c007c00u;
+  constexpr unsigned one = DT == kBF16 ? 0x00800080u : 0x04000400u;
+  return ((w & e) + one) & 0x80008000u;
+}
+// The word with its infinities and NaNs replaced by zero.
+template <int DT>
+__device__ __forceinline__ unsigned finite_pair(unsigned w) {
+  const unsigned bad = nonfinite_pair<DT>(w);  // bit 15, bit 31
+  return w & ~((bad >> 15) * 0xffffu);
+}
+
+// A sequence's share of the call, and the keys that its query rows see.
+struct SequenceSpan {
+  int n, m;  // keys, queries
+};
+__device__ __forceinline__ SequenceSpan sequence_span(const CachedAttentionArgs& a, int b) {
+  SequenceSpan s{a.L, a.T};
+  if (a.lengths) s.n = min(max(a.lengths[b], 0), a.L);
+  if (a.query_lengths) s.m = min(max(a.query_lengths[b], 0), a.T);
+  return s;
+}
+
+// Key tiles (of KT keys) that queries at positions lo_pos .. hi_pos see: the sinks' first
+// tiles, then the window's.  Tile i of the list is tile_index(i); a tile inside both is
+// listed once.
+struct KeyTiles {
+  int sink_tiles, first, count;
+  __device__ __forceinline__ int tile_index(int i) const { return i < sink_tiles ? i : first + (i - sink_tiles); }
+};
+template <int KT>
+__device__ __forceinline__ KeyTiles key_tiles(int lo_pos, int hi_pos, int window, int sinks) {
+  KeyTiles k{0, 0, 0};
+  if (hi_pos < 0) return k;
+  const int lo = window > 0 ? max(0, lo_pos - window + 1) : 0;
+  const int last = hi_pos / KT + 1;
+  k.sink_tiles = min((min(sinks, lo) + KT - 1) / KT, last);
+  k.first = max(lo / KT, k.sink_tiles);
+  k.count = k.sink_tiles + last - k.first;
+  return k;
+}
+
+// Query at position p sees key j: j <= p, and inside the window or among the sinks.
+__device__ __forceinline__ bool sees(int p, int j, int window, int sinks) {
+  return j <= p && (window <= 0 || j > p - window || j < sinks);
+}
+// Every query at lo_pos .. hi_pos sees all keys j0 .. j1 - 1.
+__device__ __forceinline__ bool all_see(int lo_pos, int hi_pos, int j0, int j1, int window, int sinks) {
+  return j1 - 1 <= lo_pos && (window <= 0 || j0 > hi_pos - window || j1 <= sinks);
+}
+
+// Buffer resource over `rows` rows of D 16-bit values, `stride` elements apart.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_resource(const uint16_t* base, long long stride, int rows,
+                                                               int D) {
+  return buffer_resource_2g(base, rows > 0 ? unsigned(rows - 1) * unsigned(stride) * 2u + unsigned(D) * 2u : 0u);
+}
+
+// 1 / l of a finished row.  A row that sees no key is zero; one that sees only keys of
+// score -inf has no softmax (NaN).
+__device__ __forceinline__ float softmax_inverse(float l, int p) {
+  if (l > 0.f) return 1.f / l;
+  return p < 0 ? 0.f : __builtin_nanf("");
+}
+
+}  // namespace fx

@@ -1,0 +1,8 @@
+// attention_few.h for bf16 queries over the 4-bit cache.
+#include "attention_few.h"
+
+namespace fx {
+template void launch_attention_few<kBF16, 64, true>(const CachedAttentionArgs&, hipStream_t);
+template void launch_attention_few<kBF16, 128, true>(const CachedAttentionArgs&, hipStream_t);
+template void launch_attention_few<kBF16, 256, true>(const CachedAttentionArgs&, hipStream_t);
+}  // namespace fx

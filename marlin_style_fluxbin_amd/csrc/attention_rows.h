@@ -1,0 +1,463 @@
+// Cached attention of many query rows (a prompt, a chunk, several drafted tokens): one
+// pass over the keys with a running maximum and sum, both products on the matrix cores.
+//
+// A workgroup of four waves takes 128 query rows of one KV head, row = token * G + head
+// of the group, so every head grouping fills the tile and the four waves share each key
+// and value tile in LDS.  Per tile of KT keys a wave forms
+//   S^T = K Q^T   (32 x 32 x 16 products: column = query, so a query's scores sit in two
+//                  lanes: its maximum and sum are register work and one lane swap)
+//   P^T = 2^(S^T f - m), f = scale log2(e), rounded to the cache's 16-bit type
+//   O^T += V^T P^T (P^T is already in the operand layout: the key order of a product is
+//                  free as long as both operands use the same, and V^T is read from LDS
+//                  by the transposing read in the order that S^T has left P^T in)
+// with S, m, the sum and O in fp32.  O is rescaled only when some query's maximum grew by
+// more than 2^8 (p then stays below 2^8, which fp16 holds too).
+//
+// LDS: rows of D 16-bit values in 16-byte chunks, chunk c of key j at c ^ swizzle(j), so
+// that both the 16-byte reads of 8 consecutive keys (K) and the transposing reads of 4
+// keys x 32 bytes (V) touch every bank once.  16-bit caches load straight into LDS (the
+// swizzle is applied to the global address of each lane), the next tile while this one is
+// multiplied; the 4-bit cache is widened in registers and stored.
+#pragma once
+#include "attention_core.h"
+
+namespace fx {
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+template <int D>
+struct RowsShape {
+  static constexpr int KT = rows_key_tile(D);
+  static constexpr int kChunks = D / 8;         // 16-byte chunks of a row
+  static constexpr int kRowBytes = D * 2;
+  static constexpr int kTileBytes = KT * kRowBytes;
+  static constexpr int kSteps = D / 16;         // depth steps of S^T
+  static constexpr int kDims = D / 32;          // 32-row blocks of O^T
+  static constexpr int kSub = KT / 32;          // 32-key blocks of a tile
+};
+
+// A row of 128 bytes covers half the banks, so two keys share a swizzle there.
+template <int D>
+__device__ __forceinline__ int lds_swizzle(int key) {
+  return D == 64 ? ((key >> 1) & 3) << 1 : (key & 7) << 1;
+}
+
+__device__ __forceinline__ u32x4_t lds_b128(const lds_char* p) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(p);
+}
+// Four 16-bit values of one column from four rows: lane i of 16 gives the address of row
+// i / 4, columns 4 (i % 4).., and receives column i of the four rows.
+__device__ __forceinline__ u32x2_t lds_transposed(const lds_char* p) {
+  return __builtin_bit_cast(
+      u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p)));
+}
+
+// 16 bytes per lane from `resource` at the lane's offset to lds + 16 * lane, asynchronously
+// (vmcnt).  The instruction has no result register; written as the builtin, every later LDS
+// read of the kernel waits for it, whichever buffer it fills.
+__device__ __forceinline__ void load_to_lds(const u32x4_t& resource, int offset, lds_char* lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(unsigned(size_t(lds))),
+               "v"(offset), "s"(resource)
+               : "memory", "m0");
+}
+
+// One tile (rows left of it may be fewer than KT: the others become zero) into LDS.
+template <int D>
+__device__ __forceinline__ void load_rows_to_lds(const uint16_t* base, long long stride, int rows, lds_char* dst,
+                                                 int wave, int lane) {
+  using S = RowsShape<D>;
+  constexpr int kRowsPerLoad = 1024 / S::kRowBytes;  // one wave load: 64 lanes x 16 bytes
+  constexpr int kLoads = S::KT / kRowsPerLoad / 4;   // per wave
+  const int live = min(rows, S::KT);
+  const size_t address = reinterpret_cast<size_t>(base);
+  const u32x4_t r = {unsigned(address), unsigned(address >> 32) & 0xffffu,
+                     live > 0 ? unsigned(live - 1) * unsigned(stride) * 2u + unsigned(D) * 2u : 0u, 0x00020000u};
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int first = (wave * kLoads + i) * kRowsPerLoad, row = first + lane / S::kChunks;
+    const int chunk = (lane % S::kChunks) ^ lds_swizzle<D>(row);
+    load_to_lds(r, row * int(stride) * 2 + chunk * 16, dst + first * S::kRowBytes);
+  }
+}
+
+// The 4-bit cache's tile: each thread holds 16 bytes of codes (32 columns of one key) and
+// the key's (scale, minimum) pairs, widens them to fp16 (code * scale + minimum in one
+// rounding, 2^-11 of the value, as a 16-bit cache's own rounding) and stores the columns of
+// a chunk in the order a0 b0 a1 b1 a2 b2 a3 b3 of its two 4-column units: q and the output
+// are permuted alike (kv4_column), so no lane has to sort them.
+template <int D>
+struct Kv4Stage {
+  using S = RowsShape<D>;
+  static constexpr int kGroups = D / 64;
+  static constexpr int kPieces = D / 32;                    // 16-byte pieces of a key's codes
+  static constexpr int kKeysPerPass = 256 / kPieces;        // keys that the 256 threads take at once
+  static constexpr int kPasses = (S::KT + kKeysPerPass - 1) / kKeysPerPass;
+  u32x4_t codes[kPasses];
+  unsigned scales[kPasses][kGroups];
+
+  __device__ __forceinline__ void load(const uint8_t* c, const uint32_t* sc, int rows, int t) {
+    const int live = min(rows, S::KT);
+    const auto rc = buffer_resource_2g(c, unsigned(live) * (D / 2));
+    const auto rs = buffer_resource_2g(sc, unsigned(live) * (kGroups * 4));
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int key = i * kKeysPerPass + t / kPieces, piece = t % kPieces;
+      codes[i] = load_b128(rc, key * (D / 2) + piece * 16, 0);
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+        scales[i][g] = __builtin_amdgcn_raw_buffer_load_b32(rs, key * (kGroups * 4) + g * 4, 0, 0);
+    }
+  }
+
+  __device__ __forceinline__ void store(lds_char* dst, int t) const {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 bias = {_Float16(1024.f), _Float16(1024.f)};
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int key = i * kKeysPerPass + t / kPieces, piece = t % kPieces;
+      if (kKeysPerPass * kPasses > S::KT && key >= S::KT) continue;
+      // words (unit, group): unit u of the piece holds kGroups 16-bit words
+      constexpr int kUnits = 8 / kGroups;  // units of a piece
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const h2 pair = __builtin_bit_cast(h2, scales[i][g]);
+        const h2 sc = {pair.x, pair.x}, mn = {pair.y, pair.y};
+#pragma unroll
+        for (int u = 0; u < kUnits; u += 2) {
+          const int wa = u * kGroups + g, wb = wa + kGroups;  // 16-bit words of the piece
+          // both words in one register: lanes (a, b)
+          const unsigned xa = codes[i][wa >> 1], xb = codes[i][wb >> 1];
+          const unsigned ab = __builtin_amdgcn_perm(xb, xa, ((wb & 1) ? 0x07060000u : 0x05040000u) |
+                                                               ((wa & 1) ? 0x0302u : 0x0100u));
+          u32x4_t w;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const h2 code = __builtin_bit_cast(h2, ((ab >> (4 * r)) & 0x000f000fu) | 0x64006400u) - bias;
+            w[r] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(code, sc, mn));
+          }
+          // columns 64 g + 4 (units of the pieces before + u) .. + 7: chunk 8 g + that / 8
+          const int chunk = 8 * g + (piece * kUnits + u) / 2;
+          *reinterpret_cast<__attribute__((address_space(3))) u32x4_t*>(
+              dst + key * S::kRowBytes + ((chunk ^ lds_swizzle<D>(key)) * 16)) = w;
+        }
+      }
+    }
+  }
+};
+
+// Column of position x of a widened 4-bit row.
+__device__ __forceinline__ int kv4_column(int x) { return (x & ~7) | ((x & 1) << 2) | ((x >> 1) & 3); }
+
+template <int QDT, int D, bool KV4>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(const CachedAttentionArgs a) {
+  using S = RowsShape<D>;
+  constexpr int CDT = KV4 ? kF16 : QDT;  // the products' type
+  constexpr int KT = S::KT;
+  __shared__ __attribute__((aligned(1024))) char lds_memory[4 * S::kTileBytes];
+  lds_char* const lds = (lds_char*)lds_memory;
+  const int t = threadIdx.x, lane = t & 63, wave = wave_index();
+  const int half = lane >> 5, l31 = lane & 31;
+
+  // ---- which rows of which KV head, which part of its keys.  Workgroup ids go round the
+  // XCDs, so eight heads at a time each keep to one XCD and its L2; within a head the last
+  // (longest) row tiles come first.
+  const int heads = a.B * a.Hk, items = a.row_tiles * a.splits;
+  int id = blockIdx.x, head, item;
+  const int full = heads / kXcdCount * kXcdCount;
+  if (id < full * items) {
+    const int slot = id / kXcdCount;
+    head = id % kXcdCount + kXcdCount * (slot / items);
+    item = slot % items;
+  } else {
+    id -= full * items;
+    head = full + id % (heads - full);
+    item = id / (heads - full);
+  }
+  const int tile = a.row_tiles - 1 - item / a.splits, split = item % a.splits;
+  const int b = head / a.Hk, g = head - b * a.Hk;
+  const SequenceSpan span = sequence_span(a, b);
+  const int rows = span.m * a.G, r0 = tile * kRowsTile;
+  if (r0 >= rows) return;
+  const int base_pos = span.n - span.m;
+  const int lo_pos = base_pos + r0 / a.G, hi_pos = base_pos + (min(r0 + kRowsTile, rows) - 1) / a.G;
+  const KeyTiles tiles = key_tiles<KT>(lo_pos, hi_pos, a.window, a.sinks);
+  const int per = (tiles.count + a.splits - 1) / a.splits;
+  const int it0 = split * per, it1 = min(tiles.count, it0 + per);
+
+  // ---- this lane's query
+  const int wave_row = r0 + wave * 32;
+  const bool active = wave_row < rows;  // wave-uniform: the others only help loading
+  const int row = min(wave_row + l31, rows - 1);
+  const int tok = row / a.G, hq = g * a.G + row - tok * a.G;
+  const int p = base_pos + tok;
+  u32x4_t qf[S::kSteps];
+  float f = a.scale * kLog2e;
+  {
+    const uint16_t* q = a.q + b * a.q_stride[0] + hq * a.q_stride[1] + tok * a.q_stride[2];
+    if constexpr (!KV4) {
+#pragma unroll
+      for (int s = 0; s < S::kSteps; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(q + 16 * s + 8 * half);
+    } else {
+      // in fp16, scaled by a power of two so that the row's largest magnitude lies in
+      // [2^9, 2^10): exact for every element within 2^-23 of it
+      float mag = 0.f;
+#pragma unroll
+      for (int s = 0; s < S::kSteps; ++s) {
+        qf[s] = *reinterpret_cast<const u32x4_t*>(q + 16 * s + 8 * half);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mag = fmaxf(mag, fabsf(to_f32<QDT>(uint16_t(qf[s][e >> 1] >> (16 * (e & 1))))));
+      }
+      mag = half_pair_max(mag);
+      const int shift = mag > 0.f && mag < INFINITY ? 10 - __builtin_amdgcn_frexp_expf(mag) : 0;
+#pragma unroll
+      for (int s = 0; s < S::kSteps; ++s) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = ldexpf(to_f32<QDT>(uint16_t(qf[s][e >> 1] >> (16 * (e & 1)))), shift);
+        // a widened row's order
+        qf[s] = u32x4_t{f32x2_to_f16x2_bits(v[0], v[4]), f32x2_to_f16x2_bits(v[1], v[5]),
+                        f32x2_to_f16x2_bits(v[2], v[6]), f32x2_to_f16x2_bits(v[3], v[7])};
+      }
+      f = ldexpf(f, -shift);
+    }
+    // the loads end here: a first use inside the loop would wait, every time round, for
+    // the tiles in flight too
+#pragma unroll
+    for (int s = 0; s < S::kSteps; ++s) asm volatile("" : "+v"(qf[s]));
+  }
+
+  // ---- LDS read addresses: K chunk 2 s + half of key l31 (+ 32 u); V^T: keys 4 half +
+  // (i >> 2) (+ 16 kk + 8), columns 32 dt + 16 dg + 4 (i & 3)
+  const int xk = lds_swizzle<D>(l31) * 16;
+  const int kaddr = l31 * S::kRowBytes + half * 16;
+  const int i16 = lane & 15, dg = (lane >> 4) & 1, vkey = 4 * half + (i16 >> 2);
+  const int xv = lds_swizzle<D>(vkey) * 16;
+  const int vaddr = vkey * S::kRowBytes + (i16 & 1) * 8;
+  const int vcol = (2 * dg + ((i16 & 3) >> 1)) * 16;
+
+  f32x16_t o[S::kDims];
+#pragma unroll
+  for (int d = 0; d < S::kDims; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float m = -INFINITY, m_use = 0.f, l = 0.f;
+
+  const uint16_t* kb = nullptr;
+  const uint16_t* vb = nullptr;
+  size_t row_at = 0;  // 4-bit cache: first row of the head
+  if constexpr (!KV4) {
+    kb = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + g * a.k_stride[1];
+    vb = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + g * a.v_stride[1];
+  } else {
+    row_at = size_t(head) * a.L;
+  }
+  Kv4Stage<D> ks, vs;
+
+  // loads of tile `it` of the list: a 16-bit tile on its way into LDS, a 4-bit one into registers
+  auto fetch = [&](int it, lds_char* dst) __attribute__((always_inline)) {
+    const int j0 = tiles.tile_index(it) * KT;
+    if constexpr (!KV4) {
+      load_rows_to_lds<D>(kb + j0 * a.k_stride[2], a.k_stride[2], span.n - j0, dst, wave, lane);
+      load_rows_to_lds<D>(vb + j0 * a.v_stride[2], a.v_stride[2], span.n - j0, dst + S::kTileBytes, wave, lane);
+    } else {
+      const size_t at = row_at + j0;
+      ks.load(static_cast<const uint8_t*>(a.k) + at * (D / 2), a.k_scales + at * (D / 64), span.n - j0, t);
+      vs.load(static_cast<const uint8_t*>(a.v) + at * (D / 2), a.v_scales + at * (D / 64), span.n - j0, t);
+    }
+  };
+
+  auto scores = [&](const lds_char* kt, f32x16_t(&s)[S::kSub]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < S::kSub; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+#pragma unroll
+    for (int st = 0; st < S::kSteps; ++st)
+#pragma unroll
+      for (int u = 0; u < S::kSub; ++u)
+        s[u] = mfma32<CDT>(lds_b128(kt + kaddr + u * 32 * S::kRowBytes + ((st * 32) ^ xk)), qf[st], s[u]);
+  };
+
+  // running maximum and sum; s becomes p in the operand layout of P^T
+  auto softmax = [&](f32x16_t(&s)[S::kSub], u32x4_t(&pf)[2 * S::kSub]) __attribute__((always_inline)) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < S::kSub; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+    top = half_pair_max(top) * f;
+    if (__builtin_amdgcn_ballot_w64(top > m + 8.f)) {
+      const float mn = fmaxf(m, top);
+      m_use = mn == -INFINITY ? 0.f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(m - m_use);  // 0 before the first visible key
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < S::kDims; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+    }
+#pragma unroll
+    for (int u = 0; u < S::kSub; ++u) {
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], f, -m_use));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r + 1], f, -m_use));
+        l += p0 + p1;
+        float c0 = p0, c1 = p1;
+        pf[2 * u + r / 8][(r & 7) / 2] = round_pair_bits<CDT>(c0, c1);
+      }
+    }
+  };
+
+  auto values = [&](const lds_char* vt, const u32x4_t(&pf)[2 * S::kSub]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int kk = 0; kk < 2 * S::kSub; ++kk)
+#pragma unroll
+      for (int d = 0; d < S::kDims; ++d) {
+        const lds_char* at = vt + vaddr + kk * 16 * S::kRowBytes + ((vcol + d * 64) ^ xv);
+        const u32x2_t x = lds_transposed(at), y = lds_transposed(at + 8 * S::kRowBytes);
+        o[d] = mfma32<CDT>(u32x4_t{x[0], x[1], y[0], y[1]}, pf[kk], o[d]);
+      }
+  };
+
+  // A tile that some query sees only in part: hidden scores become -inf.  A product with a
+  // zero p would still carry a hidden value's infinity or NaN into the row, so a tile that
+  // holds any adds them by hand to the rows that see them and zeroes them in LDS.
+  auto masked_tile = [&](lds_char* cur, int j0) __attribute__((always_inline)) {
+    f32x16_t s[S::kSub];
+    u32x4_t pf[2 * S::kSub];
+    if (active) {
+      scores(cur, s);
+#pragma unroll
+      for (int u = 0; u < S::kSub; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!sees(p, j0 + 32 * u + (r & 3) + 8 * (r >> 2) + 4 * half, a.window, a.sinks)) s[u][r] = -INFINITY;
+      softmax(s, pf);
+    }
+    lds_char* vt = cur + S::kTileBytes;
+    unsigned bad = 0;
+    for (int i = t * 16; i < S::kTileBytes; i += 256 * 16) {
+      const u32x4_t w = lds_b128(vt + i);
+      bad |= nonfinite_pair<CDT>(w[0]) | nonfinite_pair<CDT>(w[1]) | nonfinite_pair<CDT>(w[2]) |
+             nonfinite_pair<CDT>(w[3]);
+    }
+    if (__syncthreads_or(bad != 0)) {
+      for (int j = 0; j < KT; ++j) {
+        if (!active || !sees(p, j0 + j, a.window, a.sinks)) continue;
+#pragma unroll
+        for (int d = 0; d < S::kDims; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int x = 32 * d + (r & 3) + 8 * (r >> 2) + 4 * half;
+            const uint16_t bits = *reinterpret_cast<const __attribute__((address_space(3))) uint16_t*>(
+                vt + j * S::kRowBytes + (((x >> 3) ^ lds_swizzle<D>(j)) * 16) + (x & 7) * 2);
+            o[d][r] += nonfinite_pair<CDT>(bits) ? to_f32<CDT>(bits) : 0.f;
+          }
+      }
+      __syncthreads();
+      for (int i = t * 16; i < S::kTileBytes; i += 256 * 16) {
+        u32x4_t w = lds_b128(vt + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = finite_pair<CDT>(w[e]);
+        *reinterpret_cast<__attribute__((address_space(3))) u32x4_t*>(vt + i) = w;
+      }
+      __syncthreads();
+    }
+    if (active) values(vt, pf);
+  };
+
+  if (it0 < it1) {
+    fetch(it0, lds);
+    if constexpr (KV4) {
+      ks.store(lds, t);
+      vs.store(lds + S::kTileBytes, t);
+    }
+  }
+  auto step = [&](lds_char* cur, lds_char* nxt, int it, bool more) __attribute__((always_inline)) {
+    if (more) fetch(it + 1, nxt);
+    const int j0 = tiles.tile_index(it) * KT;
+    if (all_see(lo_pos, hi_pos, j0, j0 + KT, a.window, a.sinks)) {
+      if (active) {
+        f32x16_t s[S::kSub];
+        u32x4_t pf[2 * S::kSub];
+        scores(cur, s);
+        softmax(s, pf);
+        values(cur + S::kTileBytes, pf);
+      }
+    } else {
+      masked_tile(cur, j0);
+    }
+  };
+  int parity = 0;
+  for (int it = it0; it < it1; ++it) {
+    lds_char* cur = lds + parity * 2 * S::kTileBytes;
+    lds_char* nxt = lds + (parity ^ 1) * 2 * S::kTileBytes;
+    // this tile has arrived (every wave waits for its own loads), and the other buffer's
+    // readers are done
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const bool more = it + 1 < it1;
+    step(cur, nxt, it, more);
+    if constexpr (KV4) {
+      if (more) {
+        ks.store(nxt, t);
+        vs.store(nxt + S::kTileBytes, t);
+      }
+    }
+    parity ^= 1;
+  }
+
+  if (!active || wave_row + l31 >= rows) return;
+  l = half_pair_sum(l);
+  if (a.splits > 1) {
+    const size_t slot = (size_t(head) * a.T * a.G + row) * a.splits + split;
+    float* po = a.partial + slot * D;
+#pragma unroll
+    for (int d = 0; d < S::kDims; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int x = 32 * d + 2 * r + 4 * half;
+        if constexpr (!KV4) {
+          *reinterpret_cast<float4*>(po + x) = make_float4(o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) po[kv4_column(x + e)] = o[d][r + e];
+        }
+      }
+    if (half == 0) {
+      float* ml = a.partial + size_t(heads) * a.T * a.G * a.splits * D + slot * 2;
+      ml[0] = m;
+      ml[1] = l;
+    }
+    return;
+  }
+  const float inv = softmax_inverse(l, p);
+  uint16_t* out = a.out + b * a.out_stride[0] + hq * a.out_stride[1] + tok * a.out_stride[2];
+#pragma unroll
+  for (int d = 0; d < S::kDims; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int x = 32 * d + 2 * r + 4 * half;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = o[d][r + e] * inv;
+      if constexpr (!KV4) {
+        const unsigned lo = round_pair_bits<QDT>(v[0], v[1]), hi = round_pair_bits<QDT>(v[2], v[3]);
+        *reinterpret_cast<u32x2_t*>(out + x) = u32x2_t{lo, hi};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[kv4_column(x + e)] = from_f32<QDT>(v[e]);
+      }
+    }
+}
+
+template <int DT, int D, bool KV4>
+void launch_attention_rows(const CachedAttentionArgs& a, hipStream_t s) {
+  const unsigned blocks = unsigned(a.B) * a.Hk * a.row_tiles * a.splits;
+  hipLaunchKernelGGL((attention_rows_kernel<DT, D, KV4>), dim3(blocks), dim3(256), 0, s, a);
+}
+
+}  // namespace fx

@@ -1,0 +1,8 @@
+// attention_rows.h for bf16 queries over a 16-bit cache.
+#include "attention_rows.h"
+
+namespace fx {
+template void launch_attention_rows<kBF16, 64, false>(const CachedAttentionArgs&, hipStream_t);
+template void launch_attention_rows<kBF16, 128, false>(const CachedAttentionArgs&, hipStream_t);
+template void launch_attention_rows<kBF16, 256, false>(const CachedAttentionArgs&, hipStream_t);
+}  // namespace fx

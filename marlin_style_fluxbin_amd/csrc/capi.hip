@@ -13,6 +13,7 @@
 #include "w3_lut.hip"
 #include "w3_mfma_launch.h"
 #include "norms_launch.h"
+#include "attention_launch.h"
 #include "decode_launch.h"
 #include "lm_head_launch.h"
 #include "two_base_launch.h"
@@ -597,7 +598,7 @@ bool two_base_config(int O, int G, int waves, int prefetch, int groups_per_split
 
 extern "C" {
 
-int fx_abi_version(void) { return 20; }
+int fx_abi_version(void) { return 21; }
 
 const char* fx_last_error(void) { return g_error; }
 
@@ -1739,6 +1740,229 @@ int fx_hybrid_restore(const uint8_t* codes, const float* rows, const float* colu
                                 sparse_columns, weight, bad,     O,       K / 128,      interleaved != 0};
   fx::launch_hybrid_restore(weight_dtype, a, static_cast<hipStream_t>(stream));
   return check_launch("hybrid_restore_kernel");
+}
+
+}  // extern "C"
+
+namespace {
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Sizes that every cached-attention and 4-bit cache call shares.
+int validate_cache_sizes(int batch, int n_kv_heads, int tokens, int max_len, int head_dim) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(FX_EINVAL, "head_dim must be 64, 128 or 256, got %d", head_dim);
+  if (batch < 0 || batch > (1 << 16)) return fail(FX_EINVAL, "batch must be in [0, 65536], got %d", batch);
+  if (n_kv_heads < 1 || n_kv_heads > 4096)
+    return fail(FX_EINVAL, "n_kv_heads must be in [1, 4096], got %d", n_kv_heads);
+  if (tokens < 0 || tokens > (1 << 24)) return fail(FX_EINVAL, "tokens must be in [0, 2^24], got %d", tokens);
+  if (max_len < 0 || max_len > (1 << 28)) return fail(FX_EINVAL, "max_len must be in [0, 2^28], got %d", max_len);
+  return FX_OK;
+}
+
+int validate_attention_sizes(int batch, int n_q_heads, int n_kv_heads, int tokens, int max_len, int head_dim,
+                             int window, int sinks) {
+  if (int rc = validate_cache_sizes(batch, n_kv_heads, tokens, max_len, head_dim)) return rc;
+  if (n_q_heads < 1 || n_q_heads % n_kv_heads != 0)
+    return fail(FX_EINVAL, "n_q_heads %d must be a positive multiple of n_kv_heads %d", n_q_heads, n_kv_heads);
+  if (window < 0 || sinks < 0) return fail(FX_EINVAL, "window and sinks must be non-negative");
+  // 31 bits hold every row index and the number of workgroups
+  if ((long long)(tokens) * n_q_heads > (1LL << 30) || (long long)(batch) * n_q_heads * (tokens / 8 + 1) > (1LL << 30))
+    return fail(FX_EINVAL, "batch %d x %d heads x %d tokens is too large for one call", batch, n_q_heads, tokens);
+  return FX_OK;
+}
+
+fx::CachedAttentionPlan attention_plan(int batch, int n_q_heads, int n_kv_heads, int tokens, int max_len,
+                                       int head_dim, int window, int sinks, bool kv4) {
+  return fx::plan_cached_attention(batch, n_kv_heads, n_q_heads / n_kv_heads, tokens, max_len, head_dim, window,
+                                   sinks, kv4);
+}
+
+size_t attention_workspace(const fx::CachedAttentionPlan& plan, int batch, int n_q_heads, int tokens, int head_dim) {
+  if (plan.splits <= 1) return 0;
+  return size_t(batch) * n_q_heads * tokens * plan.splits * (size_t(head_dim) + 2) * sizeof(float);
+}
+
+// (batch, head, row) strides of one tensor.
+int validate_strides(const char* name, const long long* s, long long row_limit) {
+  for (int i = 0; i < 3; ++i)
+    if (s[i] < 0 || s[i] % 8 != 0)
+      return fail(FX_EINVAL, "%s strides must be non-negative multiples of 8 elements, got %lld", name, s[i]);
+  if (s[2] > row_limit)
+    return fail(FX_EINVAL, "%s position stride must be at most %lld elements, got %lld", name, row_limit, s[2]);
+  return FX_OK;
+}
+
+constexpr long long kCacheRowLimit = 1LL << 22;    // 64 rows of a tile stay within 31 bits of bytes
+constexpr long long kTokenRowLimit = 1LL << 40;
+
+int run_cached_attention(bool kv4, fx::CachedAttentionArgs& a, const long long* q_strides,
+                         const long long* out_strides, void* workspace, size_t workspace_bytes, int n_q_heads,
+                         int head_dim, int dtype, void* stream) {
+  if (!is_half_dtype(dtype)) return fail(FX_EINVAL, "dtype must be fp16 or bf16");
+  if (!(a.scale > 0.f) || a.scale > 3.4e38f) return fail(FX_EINVAL, "scale must be positive and finite");
+  if (a.B == 0 || a.T == 0) return FX_OK;
+  if (!a.q || !a.out) return fail(FX_EINVAL, "q and out must be non-null");
+  if (!aligned16(a.q) || !aligned16(a.out)) return fail(FX_EINVAL, "q and out must be 16-byte aligned");
+  if (int rc = validate_strides("q", q_strides, kTokenRowLimit)) return rc;
+  if (int rc = validate_strides("out", out_strides, kTokenRowLimit)) return rc;
+  std::copy(q_strides, q_strides + 3, a.q_stride);
+  std::copy(out_strides, out_strides + 3, a.out_stride);
+  a.G = n_q_heads / a.Hk;
+  const fx::CachedAttentionPlan plan =
+      attention_plan(a.B, n_q_heads, a.Hk, a.T, a.L, head_dim, a.window, a.sinks, kv4);
+  const size_t need = attention_workspace(plan, a.B, n_q_heads, a.T, head_dim);
+  if (need) {
+    if (!workspace || workspace_bytes < need)
+      return fail(FX_EINVAL, "attention workspace needs %zu bytes, got %zu", need, workspace_bytes);
+    if (!aligned16(workspace)) return fail(FX_EINVAL, "workspace must be 16-byte aligned");
+  }
+  a.partial = static_cast<float*>(workspace);
+  a.splits = plan.splits;
+  a.row_tiles = plan.row_tiles;
+  fx::launch_cached_attention(dtype, head_dim, kv4, plan.few, a, static_cast<hipStream_t>(stream));
+  return check_launch(kv4 ? "fx_kv4_attention" : "fx_window_attention");
+}
+
+int validate_kv4_cache(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales) {
+  if (!k_codes || !k_scales || !v_codes || !v_scales) return fail(FX_EINVAL, "cache arrays must be non-null");
+  if (!aligned16(k_codes) || !aligned16(k_scales) || !aligned16(v_codes) || !aligned16(v_scales))
+    return fail(FX_EINVAL, "cache arrays must be 16-byte aligned");
+  return FX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fx_cached_attention_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int tokens, int max_len,
+                                           int head_dim, int window, int sinks, int kv4) {
+  if (validate_attention_sizes(batch, n_q_heads, n_kv_heads, tokens, max_len, head_dim, window, sinks)) return 0;
+  if (batch == 0 || tokens == 0) return 0;
+  return attention_workspace(attention_plan(batch, n_q_heads, n_kv_heads, tokens, max_len, head_dim, window, sinks,
+                                            kv4 != 0),
+                             batch, n_q_heads, tokens, head_dim);
+}
+
+int fx_window_attention(const void* q, const void* k, const void* v, void* out, const long long* strides,
+                        const int* lengths, const int* query_lengths, void* workspace, size_t workspace_bytes,
+                        int batch, int n_q_heads, int n_kv_heads, int tokens, int max_len, int head_dim, int window,
+                        int sinks, float scale, int dtype, void* stream) {
+  if (int rc = validate_attention_sizes(batch, n_q_heads, n_kv_heads, tokens, max_len, head_dim, window, sinks))
+    return rc;
+  if (!strides) return fail(FX_EINVAL, "strides must be non-null");
+  if (max_len > 0 && (!k || !v)) return fail(FX_EINVAL, "k and v must be non-null");
+  if (!aligned16(k) || !aligned16(v)) return fail(FX_EINVAL, "k and v must be 16-byte aligned");
+  if (int rc = validate_strides("k", strides + 3, kCacheRowLimit)) return rc;
+  if (int rc = validate_strides("v", strides + 6, kCacheRowLimit)) return rc;
+  fx::CachedAttentionArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.out = static_cast<uint16_t*>(out);
+  a.k = k;
+  a.v = v;
+  std::copy(strides + 3, strides + 6, a.k_stride);
+  std::copy(strides + 6, strides + 9, a.v_stride);
+  a.lengths = lengths;
+  a.query_lengths = query_lengths;
+  a.B = batch;
+  a.Hk = n_kv_heads;
+  a.T = tokens;
+  a.L = max_len;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale = scale;
+  return run_cached_attention(false, a, strides, strides + 9, workspace, workspace_bytes, n_q_heads, head_dim, dtype,
+                              stream);
+}
+
+int fx_kv4_attention(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                     const void* v_scales, void* out, const long long* strides, const int* lengths,
+                     const int* query_lengths, void* workspace, size_t workspace_bytes, int batch, int n_q_heads,
+                     int n_kv_heads, int tokens, int max_len, int head_dim, int window, int sinks, float scale,
+                     int dtype, void* stream) {
+  if (int rc = validate_attention_sizes(batch, n_q_heads, n_kv_heads, tokens, max_len, head_dim, window, sinks))
+    return rc;
+  if (!strides) return fail(FX_EINVAL, "strides must be non-null");
+  if (max_len > 0)
+    if (int rc = validate_kv4_cache(k_codes, k_scales, v_codes, v_scales)) return rc;
+  fx::CachedAttentionArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.out = static_cast<uint16_t*>(out);
+  a.k = k_codes;
+  a.v = v_codes;
+  a.k_scales = static_cast<const uint32_t*>(k_scales);
+  a.v_scales = static_cast<const uint32_t*>(v_scales);
+  a.lengths = lengths;
+  a.query_lengths = query_lengths;
+  a.B = batch;
+  a.Hk = n_kv_heads;
+  a.T = tokens;
+  a.L = max_len;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale = scale;
+  return run_cached_attention(true, a, strides, strides + 3, workspace, workspace_bytes, n_q_heads, head_dim, dtype,
+                              stream);
+}
+
+int fx_kv4_append(const void* k, const void* v, const long long* strides, const int* start, int start_all,
+                  const int* counts, void* k_codes, void* k_scales, void* v_codes, void* v_scales, int batch,
+                  int n_kv_heads, int tokens, int max_len, int head_dim, int dtype, void* stream) {
+  if (int rc = validate_cache_sizes(batch, n_kv_heads, tokens, max_len, head_dim)) return rc;
+  if (!is_half_dtype(dtype)) return fail(FX_EINVAL, "dtype must be fp16 or bf16");
+  if ((long long)(batch) * n_kv_heads * (tokens / 8 + 1) > (1LL << 30))
+    return fail(FX_EINVAL, "batch %d x %d heads x %d tokens is too large for one call", batch, n_kv_heads, tokens);
+  if (!strides) return fail(FX_EINVAL, "strides must be non-null");
+  if (int rc = validate_strides("k", strides, kTokenRowLimit)) return rc;
+  if (int rc = validate_strides("v", strides + 3, kTokenRowLimit)) return rc;
+  if (batch == 0 || tokens == 0 || max_len == 0) return FX_OK;
+  if (!k || !v) return fail(FX_EINVAL, "k and v must be non-null");
+  if (!aligned16(k) || !aligned16(v)) return fail(FX_EINVAL, "k and v must be 16-byte aligned");
+  if (int rc = validate_kv4_cache(k_codes, k_scales, v_codes, v_scales)) return rc;
+  fx::Kv4AppendArgs a{};
+  a.x[0] = static_cast<const uint16_t*>(k);
+  a.x[1] = static_cast<const uint16_t*>(v);
+  for (int i = 0; i < 2; ++i) std::copy(strides + 3 * i, strides + 3 * i + 3, a.stride[i]);
+  a.codes[0] = static_cast<uint32_t*>(k_codes);
+  a.codes[1] = static_cast<uint32_t*>(v_codes);
+  a.scales[0] = static_cast<uint32_t*>(k_scales);
+  a.scales[1] = static_cast<uint32_t*>(v_scales);
+  a.start = start;
+  a.counts = counts;
+  a.start0 = start_all;
+  a.B = batch;
+  a.Hk = n_kv_heads;
+  a.T = tokens;
+  a.L = max_len;
+  fx::launch_kv4_append(dtype, head_dim, a, static_cast<hipStream_t>(stream));
+  return check_launch("fx_kv4_append");
+}
+
+int fx_kv4_restore(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, void* k_out,
+                   void* v_out, int batch, int n_kv_heads, int max_len, int rows, int head_dim, int dtype,
+                   void* stream) {
+  if (int rc = validate_cache_sizes(batch, n_kv_heads, rows, max_len, head_dim)) return rc;
+  if (!is_half_dtype(dtype)) return fail(FX_EINVAL, "dtype must be fp16 or bf16");
+  if (rows > max_len) return fail(FX_EINVAL, "rows must be in [0, max_len], got %d of %d", rows, max_len);
+  if ((long long)(batch) * n_kv_heads * (rows / 8 + 1) > (1LL << 30))
+    return fail(FX_EINVAL, "batch %d x %d heads x %d rows is too large for one call", batch, n_kv_heads, rows);
+  if (batch == 0 || rows == 0) return FX_OK;
+  if (int rc = validate_kv4_cache(k_codes, k_scales, v_codes, v_scales)) return rc;
+  if (!k_out || !v_out) return fail(FX_EINVAL, "k_out and v_out must be non-null");
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail(FX_EINVAL, "k_out and v_out must be 16-byte aligned");
+  fx::Kv4RestoreArgs a{};
+  a.codes[0] = static_cast<const uint32_t*>(k_codes);
+  a.codes[1] = static_cast<const uint32_t*>(v_codes);
+  a.scales[0] = static_cast<const uint32_t*>(k_scales);
+  a.scales[1] = static_cast<const uint32_t*>(v_scales);
+  a.out[0] = static_cast<uint16_t*>(k_out);
+  a.out[1] = static_cast<uint16_t*>(v_out);
+  a.B = batch;
+  a.Hk = n_kv_heads;
+  a.L = max_len;
+  a.rows = rows;
+  fx::launch_kv4_restore(dtype, head_dim, a, static_cast<hipStream_t>(stream));
+  return check_launch("fx_kv4_restore");
 }
 
 }  // extern "C"
