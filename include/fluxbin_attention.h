@@ -32,7 +32,7 @@ extern "C" {
 
 /* kv4 0: for fx_window_attention, else for fx_kv4_attention. */
 size_t fx_cached_attention_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int tokens, int max_len,
-                                           int head_dim, int window, int sinks, int kv4);
+                                           int head_dim, int window, int sinks, int dtype, int kv4);
 /*
  * q [batch, n_q_heads, tokens, head_dim], k and v [batch, n_kv_heads, max_len, head_dim],
  * out as q, all of `dtype` (fp16 or bf16), the last axis contiguous; strides[12]: the

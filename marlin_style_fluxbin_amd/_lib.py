@@ -83,7 +83,7 @@ SIGNATURES: dict[str, tuple] = {
 
 # mirrors include/fluxbin_attention.h
 ATTENTION_SIGNATURES: dict[str, tuple] = {
-    "fx_cached_attention_workspace_bytes": (_sz, [_i] * 9),
+    "fx_cached_attention_workspace_bytes": (_sz, [_i] * 10),
     "fx_window_attention": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _sz, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _p]),
     "fx_kv4_attention": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i,
                               _p]),

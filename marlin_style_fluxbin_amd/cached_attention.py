@@ -31,93 +31,107 @@ def _workspace_bytes(*sizes) -> int:
     return _lib.library().fx_cached_attention_workspace_bytes(*sizes)
 
 
-def _strides(t: torch.Tensor) -> list[int]:
+def _strides(t: torch.Tensor) -> tuple[int, ...]:
     """(batch, head, row) strides; an axis of one element never moves."""
-    return [0 if n == 1 else s for n, s in zip(t.shape, t.stride()[:3])]
+    return tuple(0 if n == 1 else s for n, s in zip(t.shape, t.stride()[:3]))
 
 
-def _rows_ok(t: torch.Tensor) -> bool:
-    """16-byte aligned rows of contiguous columns."""
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in _strides(t))
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t``, or a copy of it whose rows the kernels can read."""
-    if _rows_ok(t):
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _rows(t: torch.Tensor, copy: bool = True):
+    """``t`` (or a copy of it, or None without ``copy``) as the kernels read it, rows of
+    contiguous columns at 16-byte boundaries: the tensor, its address and its strides."""
+    s, p = t.stride(), t.data_ptr()
+    if s[3] == 1 and not (s[0] | s[1] | s[2]) & 7 and not p & 15:
+        return t, p, s[:3]
+    s = _strides(t)
+    if t.stride(3) != 1 or (s[0] | s[1] | s[2]) & 7 or p & 15:
+        if not copy:
+            return None
+        t = t.contiguous()
+        t = t.clone() if t.data_ptr() & 15 else t
+        s = _strides(t)
+    return t, t.data_ptr(), s
 
 
 def _check_heads(name: str, t: torch.Tensor) -> None:
     if t.ndim != 4:
         raise ValueError(f"{name} must have shape [batch, heads, tokens, head_dim]")
-    _lib.require_gpu_tensor(t, name)
+    if not t.is_cuda:
+        _lib.require_gpu_tensor(t, name)
     if t.dtype not in _HALF:
         raise ValueError(f"{name} must be fp16 or bf16")
-    if t.shape[3] not in HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {t.shape[3]}")
 
 
-def _check_counts(name: str, t: torch.Tensor | None, batch: int, device: torch.device) -> int | None:
+def _check_head_dim(dim: int) -> None:
+    if dim not in HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {dim}")
+
+
+def _counts(name: str, t: torch.Tensor | None, batch: int, index: int) -> int | None:
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.shape != (batch,) or t.device != device or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != (batch,) or t.get_device() != index or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 [batch] tensor on the device of the cache")
     return t.data_ptr()
 
 
-def _check_inference(*tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError("cached attention has no backward pass; call it under torch.no_grad()")
+def _no_gradient() -> None:
+    raise ValueError("cached attention has no backward pass; call it under torch.no_grad()")
 
 
-def _on_device(device: torch.device, call, *args) -> int:
-    """Launch with ``device`` current (kernels launch on the current device)."""
+def _launch(name: str, device: torch.device, *args) -> None:
+    """The library call with ``device`` current (kernels launch on the current device)."""
+    call = getattr(_lib.library(), name)
     if torch.cuda.current_device() == device.index:
-        return call(*args, _lib.stream_handle(device))
-    with torch.cuda.device(device):
-        return call(*args, _lib.stream_handle(device))
+        rc = call(*args, _lib.stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            rc = call(*args, _lib.stream_handle(device))
+    if rc:
+        _lib.check(rc, name)
+
+
+_Strides6, _Strides12 = ctypes.c_longlong * 6, ctypes.c_longlong * 12
 
 
 def _attention(name, q, cache, cache_args, cache_strides, lengths, query_lengths, window, sinks, scale, out, kv4):
     """Checks and call shared by the two caches; ``cache`` is (batch, kv heads, max_len)."""
-    batch, heads, tokens, dim = q.shape
-    kv_heads, max_len = cache[1], cache[2]
-    device = q.device
-    if cache[0] != batch:
-        raise ValueError(f"q and the cache disagree on the batch: {batch} and {cache[0]}")
+    shape, dtype, device = q.shape, q.dtype, q.device
+    batch, heads, tokens, dim = shape
+    cache_batch, kv_heads, max_len = cache
+    if cache_batch != batch:
+        raise ValueError(f"q and the cache disagree on the batch: {batch} and {cache_batch}")
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError(f"query heads ({heads}) must be a positive multiple of KV heads ({kv_heads})")
     if window is None:
         window = 0
-    elif not isinstance(window, int) or isinstance(window, bool) or not 1 <= window <= _LIMIT:
+    elif not isinstance(window, int) or isinstance(window, bool) or window < 1:
         raise ValueError("window must be None or a positive integer")
-    if not isinstance(sinks, int) or isinstance(sinks, bool) or not 0 <= sinks <= _LIMIT:
+    if not isinstance(sinks, int) or isinstance(sinks, bool) or sinks < 0:
         raise ValueError("sinks must be a non-negative integer")
-    if scale is None:
-        scale = 1.0 / math.sqrt(dim)
     # no key lies beyond max_len, so neither a window nor sinks need to
     window, sinks = min(window, max_len + 1), min(sinks, max_len)
-    lengths_ptr = _check_counts("lengths", lengths, batch, device)
-    counts_ptr = _check_counts("query_lengths", query_lengths, batch, device)
+    index = device.index
+    lengths_ptr = _counts("lengths", lengths, batch, index)
+    counts_ptr = _counts("query_lengths", query_lengths, batch, index)
     if out is None:
         make = torch.empty if query_lengths is None else torch.zeros
-        out = make((batch, tokens, heads, dim), dtype=q.dtype, device=device).transpose(1, 2)
-    else:
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != device:
-            raise ValueError("out must have q's shape, dtype and device")
-        if not _rows_ok(out) or any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride())):
-            raise ValueError("out must have contiguous 16-byte aligned rows, each its own memory")
-    q = _rows(q)
-    nbytes = _workspace_bytes(batch, heads, kv_heads, tokens, max_len, dim, window, sinks, kv4)
+        out = make((batch, tokens, heads, dim), dtype=dtype, device=device).transpose(1, 2)
+    elif out.shape != shape or out.dtype is not dtype or out.device != device:
+        raise ValueError("out must have q's shape, dtype and device")
+    elif out.requires_grad and torch.is_grad_enabled():
+        _no_gradient()
+    rows = _rows(out, copy=False)
+    if rows is None or (0 in rows[2] and any(s == 0 and n > 1 for n, s in zip(shape, rows[2]))):
+        raise ValueError("out must have contiguous 16-byte aligned rows, each its own memory")
+    _, out_ptr, out_strides = rows
+    q, q_ptr, q_strides = _rows(q)
+    code = _lib.dtype_code(dtype)
+    nbytes = _workspace_bytes(batch, heads, kv_heads, tokens, max_len, dim, window, sinks, code, kv4)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    strides = (ctypes.c_longlong * (6 + len(cache_strides)))(*_strides(q), *cache_strides, *_strides(out))
-    rc = _on_device(device, getattr(_lib.library(), name), q.data_ptr(), *cache_args, out.data_ptr(), strides,
-                    lengths_ptr, counts_ptr, _lib.ptr(workspace), nbytes, batch, heads, kv_heads, tokens, max_len, dim,
-                    window, sinks, scale, _lib.dtype_code(q.dtype))
-    if rc:
-        _lib.check(rc, name)
+    strides = (_Strides6 if kv4 else _Strides12)(*q_strides, *cache_strides, *out_strides)
+    _launch(name, device, q_ptr, *cache_args, out_ptr, strides, lengths_ptr, counts_ptr, _lib.ptr(workspace), nbytes,
+            batch, heads, kv_heads, tokens, max_len, dim, window, sinks,
+            1.0 / math.sqrt(dim) if scale is None else scale, code)
     return out
 
 
@@ -135,16 +149,21 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengt
     ``query_lengths[b]`` stay as they are in ``out`` and are zeros in a new output.  ``scale``
     defaults to ``1 / sqrt(head_dim)``.  fp16 or bf16, head_dim 64, 128 or 256, any strides
     (rows that are not 16-byte aligned are copied first, ``out`` is refused)."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _check_heads(name, t)
-    if k.shape != v.shape or q.shape[3] != k.shape[3]:
+    _check_heads("q", q)
+    _check_heads("k", k)
+    _check_heads("v", v)
+    shape, dtype, device = k.shape, q.dtype, q.device
+    if v.shape != shape or q.shape[3] != shape[3]:
         raise ValueError("k and v must have one shape, with q's head_dim")
-    if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device:
+    _check_head_dim(shape[3])
+    if not dtype == k.dtype == v.dtype or not device == k.device == v.device:
         raise ValueError("q, k and v must share dtype and device")
-    _check_inference(q, k, v)
-    k, v = _rows(k), _rows(v)
-    return _attention("fx_window_attention", q, k.shape, (k.data_ptr(), v.data_ptr()), _strides(k) + _strides(v),
-                      lengths, query_lengths, window, sinks, scale, out, 0)
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        _no_gradient()
+    k, k_ptr, k_strides = _rows(k)
+    v, v_ptr, v_strides = _rows(v)
+    return _attention("fx_window_attention", q, shape[:3], (k_ptr, v_ptr), (*k_strides, *v_strides), lengths,
+                      query_lengths, window, sinks, scale, out, 0)
 
 
 class Int4KVCache:
@@ -154,8 +173,7 @@ class Int4KVCache:
     zeros.  The caller keeps the lengths, as it does for a 16-bit cache."""
 
     def __init__(self, batch: int, kv_heads: int, max_len: int, head_dim: int, *, device="cuda"):
-        if head_dim not in HEAD_DIMS:
-            raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
+        _check_head_dim(head_dim)
         if batch < 1 or kv_heads < 1 or max_len < 1:
             raise ValueError("batch, kv_heads and max_len must be positive")
         device = torch.device(device)
@@ -190,29 +208,28 @@ class Int4KVCache:
         [batch, kv_heads, tokens, head_dim]`` into positions ``start[b] + t`` (``start`` int32
         ``[batch]`` on the device, or one integer for all).  Positions outside the cache are
         dropped; nothing else of it changes."""
-        for name, t in (("k", k), ("v", v)):
-            _check_heads(name, t)
-        if k.shape != v.shape or k.dtype != v.dtype or not k.device == v.device == self.device:
+        _check_heads("k", k)
+        _check_heads("v", v)
+        device = self.device
+        if k.shape != v.shape or k.dtype != v.dtype or not k.device == v.device == device:
             raise ValueError("k and v must share shape and dtype, on the cache's device")
         batch, heads, tokens, dim = k.shape
         if (batch, heads, dim) != (self.batch, self.kv_heads, self.head_dim):
             raise ValueError("k and v must be [batch, kv_heads, tokens, head_dim] of the cache")
-        _check_inference(k, v)
+        if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+            _no_gradient()
         start_ptr, start_all = None, 0
         if isinstance(start, torch.Tensor):
-            start_ptr = _check_counts("start", start, batch, self.device)
+            start_ptr = _counts("start", start, batch, device.index)
         elif isinstance(start, int) and not isinstance(start, bool) and 0 <= start <= _LIMIT:
             start_all = start
         else:
             raise ValueError("start must be a non-negative integer or an int32 [batch] tensor")
-        counts_ptr = _check_counts("counts", counts, batch, self.device)
-        k, v = _rows(k), _rows(v)
-        strides = (ctypes.c_longlong * 6)(*_strides(k), *_strides(v))
-        rc = _on_device(self.device, _lib.library().fx_kv4_append, k.data_ptr(), v.data_ptr(), strides, start_ptr,
-                        start_all, counts_ptr, *self._pointers(), batch, heads, tokens, self.max_len, dim,
-                        _lib.dtype_code(k.dtype))
-        if rc:
-            _lib.check(rc, "fx_kv4_append")
+        counts_ptr = _counts("counts", counts, batch, device.index)
+        k, k_ptr, k_strides = _rows(k)
+        v, v_ptr, v_strides = _rows(v)
+        _launch("fx_kv4_append", device, k_ptr, v_ptr, _Strides6(*k_strides, *v_strides), start_ptr, start_all,
+                counts_ptr, *self._pointers(), batch, heads, tokens, self.max_len, dim, _lib.dtype_code(k.dtype))
 
     def restore(self, *, length: int | None = None, dtype: torch.dtype = torch.bfloat16):
         """The values that the first ``length`` positions (default all) stand for, as new
@@ -224,10 +241,8 @@ class Int4KVCache:
             raise ValueError("dtype must be fp16 or bf16")
         shape = (self.batch, self.kv_heads, length, self.head_dim)
         k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
-        rc = _on_device(self.device, _lib.library().fx_kv4_restore, *self._pointers(), k.data_ptr(), v.data_ptr(),
-                        self.batch, self.kv_heads, self.max_len, length, self.head_dim, _lib.dtype_code(dtype))
-        if rc:
-            _lib.check(rc, "fx_kv4_restore")
+        _launch("fx_kv4_restore", self.device, *self._pointers(), k.data_ptr(), v.data_ptr(), self.batch, self.kv_heads,
+                self.max_len, length, self.head_dim, _lib.dtype_code(dtype))
         return k, v
 
 
@@ -238,6 +253,7 @@ def kv4_attention(q: torch.Tensor, cache: Int4KVCache, *, lengths: torch.Tensor 
     _check_heads("q", q)
     if q.shape[3] != cache.head_dim or q.device != cache.device:
         raise ValueError("q must have the cache's head_dim and device")
-    _check_inference(q)
-    return _attention("fx_kv4_attention", q, (cache.batch, cache.kv_heads, cache.max_len), cache._pointers(), [],
+    if q.requires_grad and torch.is_grad_enabled():
+        _no_gradient()
+    return _attention("fx_kv4_attention", q, (cache.batch, cache.kv_heads, cache.max_len), cache._pointers(), (),
                       lengths, query_lengths, window, sinks, scale, out, 1)

@@ -5,96 +5,143 @@
 
 namespace fx {
 
-// grid: one wave per query row (row of all heads, four a workgroup).  o = sum_s w_s o_s /
-// sum_s w_s l_s with w_s = 2^(m_s - max m) over the row's splits (<= 64: lane s forms w_s).
-template <int DT, int D>
+// The join of a row's key splits: o = sum_s w_s o_s / sum_s w_s l_s, w_s = 2^(m_s - max m).
+// W waves a row (every wave forms the weights: lane s holds split s, splits <= 64), each
+// with its share of at most N splits loaded at once; four rows (W = 1) or one a workgroup.
+// Bound by one round trip: 64 splits of 32 rows took 17.7 us with one wave looping over them.
+template <int DT, int D, int N, int W>
 __global__ __launch_bounds__(256) void attention_combine_kernel(const CachedAttentionArgs a) {
+  constexpr int kRows = 4 / W, kCols = D / 64;
+  typedef float cols_t __attribute__((ext_vector_type(kCols)));
+  __shared__ float red[W > 1 ? W : 1][W > 1 ? D : 1];
   const int per_head = a.T * a.G, heads = a.B * a.Hk;
-  const int tiles = (per_head + 3) / 4;
-  const int head = blockIdx.x / tiles, lane = threadIdx.x & 63;
-  const int row = (blockIdx.x - head * tiles) * 4 + wave_index();
+  const int tiles = (per_head + kRows - 1) / kRows;
+  const int wave = wave_index(), lane = threadIdx.x & 63;
+  const int head = blockIdx.x / tiles, part = wave % W;
+  const int row = (blockIdx.x - head * tiles) * kRows + wave / W;
   const int b = head / a.Hk, g = head - b * a.Hk;
   const SequenceSpan span = sequence_span(a, b);
-  if (row >= span.m * a.G) return;
+  if (row >= span.m * a.G) return;  // W > 1: the whole workgroup
   const size_t first = (size_t(head) * per_head + row) * a.splits;
   const float* ml = a.partial + size_t(heads) * per_head * a.splits * D + first * 2;
+  const float* po = a.partial + first * D + lane * kCols;
+  cols_t v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i)  // splits past the last: the last again, with weight 0
+    v[i] = *reinterpret_cast<const cols_t*>(po + size_t(min(part + W * i, a.splits - 1)) * D);
   const bool live = lane < a.splits;
   const float m = live ? ml[lane * 2] : -INFINITY, ls = live ? ml[lane * 2 + 1] : 0.f;
   const float top = wave_max(m);
-  const float w = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
-  const float l = wave_total(live ? w * ls : 0.f);
-  const float* po = a.partial + first * D + lane;
-  constexpr int N = D / 64;
-  float o[N];
+  const float w = !live ? 0.f : m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+  const float l = wave_total(w * ls);
+  float o[kCols];
 #pragma unroll
-  for (int i = 0; i < N; ++i) o[i] = 0.f;
-#pragma unroll 8
-  for (int s = 0; s < a.splits; ++s) {
-    const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s));
+  for (int c = 0; c < kCols; ++c) o[c] = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] += ws * po[size_t(s) * D + 64 * i];
+  for (int i = 0; i < N; ++i) {
+    const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), min(part + W * i, 63)));
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) o[c] += ws * v[i][c];
   }
   const int tok = row / a.G;
   const float inv = softmax_inverse(l, span.n - span.m + tok);
   uint16_t* out = a.out + b * a.out_stride[0] + (g * a.G + row - tok * a.G) * a.out_stride[1] +
-                  tok * a.out_stride[2] + lane;
+                  tok * a.out_stride[2];
+  if constexpr (W == 1) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) out[64 * i] = from_f32<DT>(o[i] * inv);
+    for (int c = 0; c < kCols; ++c) out[lane * kCols + c] = from_f32<DT>(o[c] * inv);
+  } else {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) red[part][lane * kCols + c] = o[c];
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d < D) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) sum += red[i][d];
+      out[d] = from_f32<DT>(sum * inv);
+    }
+  }
 }
 
-CachedAttentionPlan plan_cached_attention(int B, int Hk, int G, int T, int L, int D, int window, int sinks,
+// Which kernel: up to 16 query rows of a KV head fit one operand of the few-rows kernel.  A
+// 4-bit cache keeps it for up to 64 rows (5 tokens of 7 heads over 4101 keys of 8 sequences
+// of 4 KV heads: 23 us, the rows kernel 25 us on half as exact fp16 results), and always for
+// fp16 queries: the rows kernel widens the cache to fp16, which a bf16 output does not show
+// and an fp16 output does (error of the output 1.5 to 2 times its own rounding's).
+CachedAttentionPlan plan_cached_attention(int dt, int B, int Hk, int G, int T, int L, int D, int window, int sinks,
                                           bool kv4) {
-  CachedAttentionPlan plan;
+  CachedAttentionPlan plan{};
   const long rows = long(T) * G, heads = long(B) * Hk;
-  plan.few = rows <= kFewRows;
-  plan.row_tiles = plan.few ? 1 : int((rows + kRowsTile - 1) / kRowsTile);
-  // the most key tiles that a row tile can see
-  const long tokens = plan.few ? T : (kRowsTile + G - 1) / G + 1;
-  long keys = L;
+  plan.few = rows <= 16 || (kv4 && (dt == kF16 || rows <= 64));
   const int kt = plan.few ? kFewKeys : rows_key_tile(D);
-  if (window > 0) keys = std::min<long>(L, long(sinks) + window + std::min<long>(tokens, T) - 1 + 2 * kt);
+  plan.waves = 4;
+  plan.row_blocks = plan.row_groups = 1;
+  if (plan.few && rows > 16) {
+    plan.waves = 8;
+    plan.row_blocks = D <= 128 ? 2 : 1;
+    while (plan.row_groups < plan.waves && plan.row_groups * plan.row_blocks * 16 < rows) plan.row_groups *= 2;
+  }
+  const long tile_rows = plan.few ? 16 * plan.row_blocks * plan.row_groups : kRowsTile;
+  plan.row_tiles = int((rows + tile_rows - 1) / tile_rows);
+  // the most key tiles that a row tile can see
+  const long tokens = std::min<long>(T, (tile_rows + G - 1) / G + 1);
+  long keys = L;
+  if (window > 0) keys = std::min<long>(L, long(sinks) + window + tokens - 1 + 2 * kt);
   const long tiles = (keys + kt - 1) / kt;
-  // enough workgroups for two (few rows: four) on each of the 256 CUs, each with at least a
-  // tile for every wave (few rows) or four tiles (the first one's latency is not hidden)
-  const long target = plan.few ? 1024 : 512;
-  const long smallest = 4;
+  // Key splits until the chip is full, each with a tile for every wave (four tiles in the
+  // rows kernel, whose first one's latency is not hidden).  Full is, measured over 256 to
+  // 2048 workgroups: 512 of the rows kernel (two a CU, LDS and registers); 1024 of the
+  // few-rows kernel (24 sequences, 4096 keys of 16 bits: 83 us, 512 or 2048 87 us), 2048 over
+  // a 4-bit cache (32 sequences of 32768 keys: 198 us, 1024 226, 512 219: ragged lengths even
+  // out); 256 with several row groups (35 rows: 31 us, 128 39, 512 39 us).
+  const long target = !plan.few ? 512 : rows > 16 ? 256 : kv4 ? 2048 : 1024;
+  const long smallest = plan.few ? plan.waves / plan.row_groups : 4;
   const long groups = heads * plan.row_tiles;
-  long splits = std::min((target + groups - 1) / groups, (tiles + smallest - 1) / smallest);
+  const long splits = std::min((target + groups - 1) / groups, (tiles + smallest - 1) / smallest);
   plan.splits = int(std::max<long>(1, std::min<long>(splits, kMaxAttentionSplits)));
   return plan;
 }
 
 template <int DT, int D>
 void launch_combine(const CachedAttentionArgs& a, hipStream_t s) {
-  const unsigned tiles = (unsigned(a.T) * a.G + 3) / 4;
-  hipLaunchKernelGGL((attention_combine_kernel<DT, D>), dim3(tiles * a.B * a.Hk), dim3(256), 0, s, a);
+  const unsigned rows = unsigned(a.T) * a.G, heads = unsigned(a.B) * a.Hk;
+  if (a.splits <= 4)
+    hipLaunchKernelGGL((attention_combine_kernel<DT, D, 4, 1>), dim3((rows + 3) / 4 * heads), dim3(256), 0, s, a);
+  else if (a.splits <= 16)
+    hipLaunchKernelGGL((attention_combine_kernel<DT, D, 16, 1>), dim3((rows + 3) / 4 * heads), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((attention_combine_kernel<DT, D, kMaxAttentionSplits / 4, 4>), dim3(rows * heads), dim3(256), 0,
+                       s, a);
 }
 
 template <int DT, int D>
-void launch_for_dim(bool kv4, bool few, const CachedAttentionArgs& a, hipStream_t s) {
-  if (few) {
-    if (kv4) launch_attention_few<DT, D, true>(a, s);
-    else launch_attention_few<DT, D, false>(a, s);
-  } else {
-    if (kv4) launch_attention_rows<DT, D, true>(a, s);
-    else launch_attention_rows<DT, D, false>(a, s);
+void launch_for_dim(bool kv4, const CachedAttentionPlan& plan, const CachedAttentionArgs& a, hipStream_t s) {
+  if (plan.few) {
+    if (kv4) launch_attention_few<DT, D, true>(plan, a, s);
+    else launch_attention_few<DT, D, false>(plan, a, s);
+  } else if (!kv4) {
+    launch_attention_rows<DT, D, false>(a, s);
+  } else if constexpr (DT == kBF16) {  // fp16 queries of a 4-bit cache always take the few-rows kernel
+    launch_attention_rows<DT, D, true>(a, s);
   }
   if (a.splits > 1) launch_combine<DT, D>(a, s);
 }
 
 template <int DT>
-bool launch_for_type(int D, bool kv4, bool few, const CachedAttentionArgs& a, hipStream_t s) {
+bool launch_for_type(int D, bool kv4, const CachedAttentionPlan& plan, const CachedAttentionArgs& a, hipStream_t s) {
   switch (D) {
-    case 64: launch_for_dim<DT, 64>(kv4, few, a, s); return true;
-    case 128: launch_for_dim<DT, 128>(kv4, few, a, s); return true;
-    case 256: launch_for_dim<DT, 256>(kv4, few, a, s); return true;
+    case 64: launch_for_dim<DT, 64>(kv4, plan, a, s); return true;
+    case 128: launch_for_dim<DT, 128>(kv4, plan, a, s); return true;
+    case 256: launch_for_dim<DT, 256>(kv4, plan, a, s); return true;
   }
   return false;
 }
 
-bool launch_cached_attention(int dt, int D, bool kv4, bool few, const CachedAttentionArgs& a, hipStream_t s) {
-  if (dt == kBF16) return launch_for_type<kBF16>(D, kv4, few, a, s);
-  if (dt == kF16) return launch_for_type<kF16>(D, kv4, few, a, s);
+bool launch_cached_attention(int dt, int D, bool kv4, const CachedAttentionPlan& plan, const CachedAttentionArgs& a,
+                             hipStream_t s) {
+  if (dt == kBF16) return launch_for_type<kBF16>(D, kv4, plan, a, s);
+  if (dt == kF16) return launch_for_type<kF16>(D, kv4, plan, a, s);
   return false;
 }
 

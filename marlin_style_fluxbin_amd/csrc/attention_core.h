@@ -73,32 +73,57 @@ __device__ __forceinline__ SequenceSpan sequence_span(const CachedAttentionArgs&
   return s;
 }
 
-// Key tiles (of KT keys) that queries at positions lo_pos .. hi_pos see: the sinks' first
-// tiles, then the window's.  Tile i of the list is tile_index(i); a tile inside both is
-// listed once.
+// Key tiles (of KT keys) that queries at positions lo_pos .. hi_pos see: those of the sinks,
+// from key 0, then the window's, from its first key on (no tile is cut at its front).  Tile i
+// of the list starts at tile_start(i).
 struct KeyTiles {
   int sink_tiles, first, count;
-  __device__ __forceinline__ int tile_index(int i) const { return i < sink_tiles ? i : first + (i - sink_tiles); }
+  bool joined;  // the sinks lie in the window's tiles
+  template <int KT>
+  __device__ __forceinline__ int tile_start(int i) const {
+    return i < sink_tiles ? i * KT : first + (i - sink_tiles) * KT;
+  }
+  // the first key behind those that some query sees (a tile of the list may reach past it)
+  __device__ __forceinline__ int tile_end(int i, int hi_pos, int sinks) const {
+    return i < sink_tiles ? sinks : hi_pos + 1;
+  }
 };
 template <int KT>
 __device__ __forceinline__ KeyTiles key_tiles(int lo_pos, int hi_pos, int window, int sinks) {
-  KeyTiles k{0, 0, 0};
+  KeyTiles k{0, 0, 0, false};
   if (hi_pos < 0) return k;
   const int lo = window > 0 ? max(0, lo_pos - window + 1) : 0;
-  const int last = hi_pos / KT + 1;
-  k.sink_tiles = min((min(sinks, lo) + KT - 1) / KT, last);
-  k.first = max(lo / KT, k.sink_tiles);
-  k.count = k.sink_tiles + last - k.first;
+  // sinks that reach the window, or leave a gap that costs no tile, join it (sinks at or
+  // behind lo always do: so the sinks of sink tiles all lie in front of the window's tiles)
+  const int s = min(sinks, lo);
+  k.sink_tiles = (s + KT - 1) / KT;
+  k.first = lo;
+  if (s > 0 && (hi_pos + KT) / KT <= k.sink_tiles + (hi_pos - lo + KT) / KT) k.sink_tiles = k.first = 0;
+  k.joined = window > 0 && sinks > k.first;
+  k.count = k.sink_tiles + (hi_pos - k.first + KT) / KT;
   return k;
 }
 
-// Query at position p sees key j: j <= p, and inside the window or among the sinks.
-__device__ __forceinline__ bool sees(int p, int j, int window, int sinks) {
-  return j <= p && (window <= 0 || j > p - window || j < sinks);
-}
-// Every query at lo_pos .. hi_pos sees all keys j0 .. j1 - 1.
-__device__ __forceinline__ bool all_see(int lo_pos, int hi_pos, int j0, int j1, int window, int sinks) {
-  return j1 - 1 <= lo_pos && (window <= 0 || j0 > hi_pos - window || j1 <= sinks);
+// The keys of one tile that the query at position p sees.  A tile of the sinks counts those
+// alone (its other keys come again in the window's tiles, or no query sees them); elsewhere
+// j <= p, and inside the window or among the sinks.
+struct TileMask {
+  int lo, width;  // window: keys lo .. lo + width - 1
+  int sinks, last;
+  __device__ __forceinline__ TileMask(int p, int window, int sinks_, bool sink_tile, bool joined) {
+    lo = window > 0 ? p - window + 1 : 0;
+    width = sink_tile ? 0 : window > 0 ? window : p + 1 > 0 ? p + 1 : 0;
+    sinks = sink_tile || joined ? sinks_ : 0;
+    last = p;
+  }
+  __device__ __forceinline__ bool sees_window(int j) const { return unsigned(j - lo) < unsigned(width); }
+  __device__ __forceinline__ bool sees(int j) const { return sees_window(j) | ((j < sinks) & (j <= last)); }
+};
+// Every query at lo_pos .. hi_pos sees all keys j0 .. j1 - 1 of a tile.
+__device__ __forceinline__ bool all_see(int lo_pos, int hi_pos, int j0, int j1, int window, int sinks,
+                                        bool sink_tile) {
+  if (j1 <= sinks && j1 - 1 <= lo_pos) return true;
+  return !sink_tile && j1 - 1 <= lo_pos && (window <= 0 || j0 > hi_pos - window);
 }
 
 // Buffer resource over `rows` rows of D 16-bit values, `stride` elements apart.

@@ -24,32 +24,35 @@ struct CachedAttentionArgs {
   float* partial;            // splits > 1: [rows, splits, D] outputs, then [rows, splits, 2] (max, sum)
   int B, Hk, G, T, L;        // G = Hq / Hk
   int window, sinks;         // window 0: none
-  int splits, row_tiles;
+  int splits, row_tiles, row_groups;  // row_groups: attention_few.h
   float scale;
 };
 
 // The kernel and split that a call takes, from its sizes alone.
 struct CachedAttentionPlan {
-  bool few;       // at most 16 query rows for a KV head: attention_few.h, else attention_rows.h
-  int row_tiles;  // workgroups along the T * G query rows of a KV head
-  int splits;     // workgroups along the keys
+  bool few;        // attention_few.h, else attention_rows.h
+  int waves;       // few: waves of a workgroup (4, 8),
+  int row_blocks;  //      16-row blocks of a wave (1, 2),
+  int row_groups;  //      waves of a workgroup along the rows; the others take other keys
+  int row_tiles;   // workgroups along the T * G query rows of a KV head
+  int splits;      // workgroups along the keys
 };
 
-constexpr int kFewRows = 16;    // query rows (token x head of the group) of the few-rows kernel
-constexpr int kFewKeys = 32;    // its keys per wave step
+constexpr int kFewKeys = 32;    // keys of a wave step of the few-rows kernel
 constexpr int kRowsTile = 128;  // query rows of a rows-kernel workgroup
 constexpr int kMaxAttentionSplits = 64;
 constexpr int rows_key_tile(int D) { return D == 256 ? 32 : 64; }
 
-CachedAttentionPlan plan_cached_attention(int B, int Hk, int G, int T, int L, int D, int window, int sinks,
+CachedAttentionPlan plan_cached_attention(int dt, int B, int Hk, int G, int T, int L, int D, int window, int sinks,
                                           bool kv4);
 // dt: the type of q and out (and of a 16-bit cache)
-bool launch_cached_attention(int dt, int D, bool kv4, bool few, const CachedAttentionArgs& a, hipStream_t s);
+bool launch_cached_attention(int dt, int D, bool kv4, const CachedAttentionPlan& plan, const CachedAttentionArgs& a,
+                             hipStream_t s);
 
 template <int DT, int D, bool KV4>
 void launch_attention_rows(const CachedAttentionArgs& a, hipStream_t s);
 template <int DT, int D, bool KV4>
-void launch_attention_few(const CachedAttentionArgs& a, hipStream_t s);
+void launch_attention_few(const CachedAttentionPlan& plan, const CachedAttentionArgs& a, hipStream_t s);
 
 // The 4-bit cache (format: kv4.hip).
 struct Kv4AppendArgs {

@@ -70,13 +70,15 @@ __device__ __forceinline__ void load_rows_to_lds(const uint16_t* base, long long
   constexpr int kRowsPerLoad = 1024 / S::kRowBytes;  // one wave load: 64 lanes x 16 bytes
   constexpr int kLoads = S::KT / kRowsPerLoad / 4;   // per wave
   const int live = min(rows, S::KT);
-  const size_t address = reinterpret_cast<size_t>(base);
-  const u32x4_t r = {unsigned(address), unsigned(address >> 32) & 0xffffu,
-                     live > 0 ? unsigned(live - 1) * unsigned(stride) * 2u + unsigned(D) * 2u : 0u, 0x00020000u};
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
-    const int first = (wave * kLoads + i) * kRowsPerLoad, row = first + lane / S::kChunks;
-    const int chunk = (lane % S::kChunks) ^ lds_swizzle<D>(row);
+    // the scalar part of the address in the resource, two or four lane offsets for all loads
+    const int first = (wave * kLoads + i) * kRowsPerLoad, left = live - first;
+    const size_t address = reinterpret_cast<size_t>(base + first * stride);
+    const u32x4_t r = {unsigned(address), unsigned(address >> 32) & 0xffffu,
+                       left > 0 ? unsigned(left - 1) * unsigned(stride) * 2u + unsigned(D) * 2u : 0u, 0x00020000u};
+    const int row = lane / S::kChunks;
+    const int chunk = (lane % S::kChunks) ^ lds_swizzle<D>(i * kRowsPerLoad + row);  // a wave's rows start at 8 w
     load_to_lds(r, row * int(stride) * 2 + chunk * 16, dst + first * S::kRowBytes);
   }
 }
@@ -229,10 +231,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
 
   // ---- LDS read addresses: K chunk 2 s + half of key l31 (+ 32 u); V^T: keys 4 half +
   // (i >> 2) (+ 16 kk + 8), columns 32 dt + 16 dg + 4 (i & 3)
-  const int xk = lds_swizzle<D>(l31) * 16;
+  int xk = lds_swizzle<D>(l31) * 16;
   const int kaddr = l31 * S::kRowBytes + half * 16;
   const int i16 = lane & 15, dg = (lane >> 4) & 1, vkey = 4 * half + (i16 >> 2);
-  const int xv = lds_swizzle<D>(vkey) * 16;
+  int xv = lds_swizzle<D>(vkey) * 16;
   const int vaddr = vkey * S::kRowBytes + (i16 & 1) * 8;
   const int vcol = (2 * dg + ((i16 & 3) >> 1)) * 16;
 
@@ -256,14 +258,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
 
   // loads of tile `it` of the list: a 16-bit tile on its way into LDS, a 4-bit one into registers
   auto fetch = [&](int it, lds_char* dst) __attribute__((always_inline)) {
-    const int j0 = tiles.tile_index(it) * KT;
+    const int j0 = tiles.tile_start<KT>(it), rows = tiles.tile_end(it, hi_pos, a.sinks) - j0;
     if constexpr (!KV4) {
-      load_rows_to_lds<D>(kb + j0 * a.k_stride[2], a.k_stride[2], span.n - j0, dst, wave, lane);
-      load_rows_to_lds<D>(vb + j0 * a.v_stride[2], a.v_stride[2], span.n - j0, dst + S::kTileBytes, wave, lane);
+      load_rows_to_lds<D>(kb + j0 * a.k_stride[2], a.k_stride[2], rows, dst, wave, lane);
+      load_rows_to_lds<D>(vb + j0 * a.v_stride[2], a.v_stride[2], rows, dst + S::kTileBytes, wave, lane);
     } else {
       const size_t at = row_at + j0;
-      ks.load(static_cast<const uint8_t*>(a.k) + at * (D / 2), a.k_scales + at * (D / 64), span.n - j0, t);
-      vs.load(static_cast<const uint8_t*>(a.v) + at * (D / 2), a.v_scales + at * (D / 64), span.n - j0, t);
+      ks.load(static_cast<const uint8_t*>(a.k) + at * (D / 2), a.k_scales + at * (D / 64), rows, t);
+      vs.load(static_cast<const uint8_t*>(a.v) + at * (D / 2), a.v_scales + at * (D / 64), rows, t);
     }
   };
 
@@ -322,64 +324,71 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
       }
   };
 
-  // A tile that some query sees only in part: hidden scores become -inf.  A product with a
-  // zero p would still carry a hidden value's infinity or NaN into the row, so a tile that
-  // holds any adds them by hand to the rows that see them and zeroes them in LDS.
-  auto masked_tile = [&](lds_char* cur, int j0) __attribute__((always_inline)) {
+  // A tile that some query sees only in part: hidden scores become -inf.  Keys that no query
+  // of the workgroup sees are zeros in LDS.  One that some see may hold an infinity or a NaN,
+  // and a product with a hidden query's zero p would carry it into that row: `careful` adds
+  // such values by hand to the rows that see them and zeroes them in LDS.
+  auto masked_tile = [&](lds_char* cur, int j0, bool sink_tile, bool careful) __attribute__((always_inline)) {
+    const TileMask seen(p, a.window, a.sinks, sink_tile, tiles.joined);
     f32x16_t s[S::kSub];
     u32x4_t pf[2 * S::kSub];
     if (active) {
       scores(cur, s);
+      const auto hide = [&](auto sees) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < S::kSub; ++u)
+        for (int u = 0; u < S::kSub; ++u)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!sees(p, j0 + 32 * u + (r & 3) + 8 * (r >> 2) + 4 * half, a.window, a.sinks)) s[u][r] = -INFINITY;
+          for (int r = 0; r < 16; ++r)
+            s[u][r] = sees(j0 + 4 * half + 32 * u + (r & 3) + 8 * (r >> 2)) ? s[u][r] : -INFINITY;
+      };
+      if (sink_tile || tiles.joined) hide([&](int j) __attribute__((always_inline)) { return seen.sees(j); });
+      else hide([&](int j) __attribute__((always_inline)) { return seen.sees_window(j); });
       softmax(s, pf);
     }
     lds_char* vt = cur + S::kTileBytes;
-    unsigned bad = 0;
-    for (int i = t * 16; i < S::kTileBytes; i += 256 * 16) {
-      const u32x4_t w = lds_b128(vt + i);
-      bad |= nonfinite_pair<CDT>(w[0]) | nonfinite_pair<CDT>(w[1]) | nonfinite_pair<CDT>(w[2]) |
-             nonfinite_pair<CDT>(w[3]);
-    }
-    if (__syncthreads_or(bad != 0)) {
-      for (int j = 0; j < KT; ++j) {
-        if (!active || !sees(p, j0 + j, a.window, a.sinks)) continue;
-#pragma unroll
-        for (int d = 0; d < S::kDims; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int x = 32 * d + (r & 3) + 8 * (r >> 2) + 4 * half;
-            const uint16_t bits = *reinterpret_cast<const __attribute__((address_space(3))) uint16_t*>(
-                vt + j * S::kRowBytes + (((x >> 3) ^ lds_swizzle<D>(j)) * 16) + (x & 7) * 2);
-            o[d][r] += nonfinite_pair<CDT>(bits) ? to_f32<CDT>(bits) : 0.f;
-          }
-      }
-      __syncthreads();
+    if (careful) {
+      unsigned bad = 0;
       for (int i = t * 16; i < S::kTileBytes; i += 256 * 16) {
-        u32x4_t w = lds_b128(vt + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = finite_pair<CDT>(w[e]);
-        *reinterpret_cast<__attribute__((address_space(3))) u32x4_t*>(vt + i) = w;
+        const u32x4_t w = lds_b128(vt + i);
+        bad |= nonfinite_pair<CDT>(w[0]) | nonfinite_pair<CDT>(w[1]) | nonfinite_pair<CDT>(w[2]) |
+               nonfinite_pair<CDT>(w[3]);
       }
-      __syncthreads();
+      if (__syncthreads_or(bad != 0)) {
+        int h = half;
+        asm volatile("" : "+v"(h));  // no address of this rare path is kept in a register elsewhere
+        for (int j = 0; j < KT; ++j) {
+          if (!active || !seen.sees(j0 + j)) continue;
+#pragma unroll
+          for (int d = 0; d < S::kDims; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int x = 32 * d + (r & 3) + 8 * (r >> 2) + 4 * h;
+              const uint16_t bits = *reinterpret_cast<const __attribute__((address_space(3))) uint16_t*>(
+                  vt + j * S::kRowBytes + (((x >> 3) ^ lds_swizzle<D>(j)) * 16) + (x & 7) * 2);
+              o[d][r] += nonfinite_pair<CDT>(bits) ? to_f32<CDT>(bits) : 0.f;
+            }
+        }
+        __syncthreads();
+        for (int i = t * 16; i < S::kTileBytes; i += 256 * 16) {
+          u32x4_t w = lds_b128(vt + i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = finite_pair<CDT>(w[e]);
+          *reinterpret_cast<__attribute__((address_space(3))) u32x4_t*>(vt + i) = w;
+        }
+        __syncthreads();
+      }
     }
     if (active) values(vt, pf);
   };
 
-  if (it0 < it1) {
-    fetch(it0, lds);
-    if constexpr (KV4) {
-      ks.store(lds, t);
-      vs.store(lds + S::kTileBytes, t);
-    }
-  }
-  auto step = [&](lds_char* cur, lds_char* nxt, int it, bool more) __attribute__((always_inline)) {
+  auto step = [&](lds_char* cur, lds_char* nxt, int it, bool more, bool careful) __attribute__((always_inline)) {
     if (more) fetch(it + 1, nxt);
-    const int j0 = tiles.tile_index(it) * KT;
-    if (all_see(lo_pos, hi_pos, j0, j0 + KT, a.window, a.sinks)) {
+    const int j0 = tiles.tile_start<KT>(it);
+    const bool sink_tile = it < tiles.sink_tiles;
+    // 256 columns: the swizzled addresses formed anew for each tile (kept, they spill, and a
+    // reload waits for the tile in flight)
+    if constexpr (D == 256) asm volatile("" : "+v"(xk), "+v"(xv));
+    if (all_see(lo_pos, hi_pos, j0, j0 + KT, a.window, a.sinks, sink_tile)) {
       if (active) {
         f32x16_t s[S::kSub];
         u32x4_t pf[2 * S::kSub];
@@ -388,32 +397,67 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
         values(cur + S::kTileBytes, pf);
       }
     } else {
-      masked_tile(cur, j0);
+      masked_tile(cur, j0, sink_tile, careful);
     }
   };
-  int parity = 0;
-  for (int it = it0; it < it1; ++it) {
-    lds_char* cur = lds + parity * 2 * S::kTileBytes;
-    lds_char* nxt = lds + (parity ^ 1) * 2 * S::kTileBytes;
-    // this tile has arrived (every wave waits for its own loads), and the other buffer's
-    // readers are done
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    const bool more = it + 1 < it1;
-    step(cur, nxt, it, more);
-    if constexpr (KV4) {
-      if (more) {
-        ks.store(nxt, t);
-        vs.store(nxt + S::kTileBytes, t);
+
+  // Once, and again carefully if some row came out infinite or NaN: such a row may have it
+  // from a value that it does not see (and a row that has it by right can wait).
+  bool careful = false;
+  while (true) {
+    if (it0 < it1) {
+      fetch(it0, lds);
+      if constexpr (KV4) {
+        ks.store(lds, t);
+        vs.store(lds + S::kTileBytes, t);
       }
     }
-    parity ^= 1;
+    int parity = 0;
+    for (int it = it0; it < it1; ++it) {
+      lds_char* cur = lds + parity * 2 * S::kTileBytes;
+      lds_char* nxt = lds + (parity ^ 1) * 2 * S::kTileBytes;
+      // this tile has arrived (every wave waits for its own loads), and the other buffer's
+      // readers are done
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      const bool more = it + 1 < it1;
+      int how = careful;
+      asm volatile("" : "+v"(how));  // one copy of the loop serves both rounds
+      how = __builtin_amdgcn_readfirstlane(how);
+      step(cur, nxt, it, more, how != 0);
+      if constexpr (KV4) {
+        if (more) {
+          ks.store(nxt, t);
+          vs.store(nxt + S::kTileBytes, t);
+        }
+      }
+      parity ^= 1;
+    }
+    if (careful) break;
+    float probe = 0.f;
+#pragma unroll
+    for (int d = 0; d < S::kDims; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) probe = __builtin_fmaf(o[d][r], 0.f, probe);
+    if (!__syncthreads_or(!(probe == 0.f))) break;  // also: every wave is done with the tiles
+    careful = true;
+#pragma unroll
+    for (int d = 0; d < S::kDims; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    m = -INFINITY;
+    m_use = l = 0.f;
   }
 
-  if (!active || wave_row + l31 >= rows) return;
+  // ---- out.  (The row's place again: kept through the loop, it would cost the loop registers.)
+  if (!active) return;
+  int own_row = wave_row + l31;
+  asm volatile("" : "+v"(own_row));
+  const bool live = own_row < rows;
   l = half_pair_sum(l);
   if (a.splits > 1) {
-    const size_t slot = (size_t(head) * a.T * a.G + row) * a.splits + split;
+    if (!live) return;
+    const size_t slot = (size_t(head) * a.T * a.G + own_row) * a.splits + split;
     float* po = a.partial + slot * D;
 #pragma unroll
     for (int d = 0; d < S::kDims; ++d)
@@ -434,24 +478,42 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
     }
     return;
   }
-  const float inv = softmax_inverse(l, p);
-  uint16_t* out = a.out + b * a.out_stride[0] + hq * a.out_stride[1] + tok * a.out_stride[2];
+  // rows through LDS (each wave its own 32, the tiles are done with): written as the lanes
+  // hold them, 16 bytes of 32 rows at a time, a prompt's output cost 16 times the requests
+  const float inv = softmax_inverse(l, base_pos + min(own_row, rows - 1) / a.G);
+  lds_char* const mine = lds + wave * 32 * S::kRowBytes;
 #pragma unroll
   for (int d = 0; d < S::kDims; ++d)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
-      const int x = 32 * d + 2 * r + 4 * half;
       float v[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = o[d][r + e] * inv;
+      u32x2_t w;
       if constexpr (!KV4) {
-        const unsigned lo = round_pair_bits<QDT>(v[0], v[1]), hi = round_pair_bits<QDT>(v[2], v[3]);
-        *reinterpret_cast<u32x2_t*>(out + x) = u32x2_t{lo, hi};
+        w = u32x2_t{round_pair_bits<QDT>(v[0], v[1]), round_pair_bits<QDT>(v[2], v[3])};
       } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[kv4_column(x + e)] = from_f32<QDT>(v[e]);
+        // this lane holds columns 0 4 1 5 of a chunk, lane + 32 its 2 6 3 7: trade for 0 1 2 3
+        // and 4 5 6 7
+        w = __builtin_amdgcn_permlane32_swap(round_pair_bits<QDT>(v[0], v[2]), round_pair_bits<QDT>(v[1], v[3]), false,
+                                             false);
       }
+      const int chunk = 4 * d + r / 4;
+      *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(
+          mine + l31 * S::kRowBytes + ((chunk ^ lds_swizzle<D>(l31)) * 16) + half * 8) = w;
     }
+  wave_lds_order();
+#pragma unroll
+  for (int i = 0; i < S::kChunks / 2; ++i) {
+    const int at = i * 64 + lane, r = at / S::kChunks, chunk = at % S::kChunks;
+    const int rr = wave_row + r;
+    const u32x4_t w = lds_b128(mine + r * S::kRowBytes + ((chunk ^ lds_swizzle<D>(r)) * 16));
+    if (rr < rows) {
+      const int tk = rr / a.G, hd = g * a.G + rr - tk * a.G;
+      *reinterpret_cast<u32x4_t*>(a.out + b * a.out_stride[0] + hd * a.out_stride[1] + tk * a.out_stride[2] +
+                                  chunk * 8) = w;
+    }
+  }
 }
 
 template <int DT, int D, bool KV4>

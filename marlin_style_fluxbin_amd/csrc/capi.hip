@@ -1772,12 +1772,6 @@ int validate_attention_sizes(int batch, int n_q_heads, int n_kv_heads, int token
   return FX_OK;
 }
 
-fx::CachedAttentionPlan attention_plan(int batch, int n_q_heads, int n_kv_heads, int tokens, int max_len,
-                                       int head_dim, int window, int sinks, bool kv4) {
-  return fx::plan_cached_attention(batch, n_kv_heads, n_q_heads / n_kv_heads, tokens, max_len, head_dim, window,
-                                   sinks, kv4);
-}
-
 size_t attention_workspace(const fx::CachedAttentionPlan& plan, int batch, int n_q_heads, int tokens, int head_dim) {
   if (plan.splits <= 1) return 0;
   return size_t(batch) * n_q_heads * tokens * plan.splits * (size_t(head_dim) + 2) * sizeof(float);
@@ -1810,7 +1804,7 @@ int run_cached_attention(bool kv4, fx::CachedAttentionArgs& a, const long long* 
   std::copy(out_strides, out_strides + 3, a.out_stride);
   a.G = n_q_heads / a.Hk;
   const fx::CachedAttentionPlan plan =
-      attention_plan(a.B, n_q_heads, a.Hk, a.T, a.L, head_dim, a.window, a.sinks, kv4);
+      fx::plan_cached_attention(dtype, a.B, a.Hk, a.G, a.T, a.L, head_dim, a.window, a.sinks, kv4);
   const size_t need = attention_workspace(plan, a.B, n_q_heads, a.T, head_dim);
   if (need) {
     if (!workspace || workspace_bytes < need)
@@ -1820,7 +1814,8 @@ int run_cached_attention(bool kv4, fx::CachedAttentionArgs& a, const long long* 
   a.partial = static_cast<float*>(workspace);
   a.splits = plan.splits;
   a.row_tiles = plan.row_tiles;
-  fx::launch_cached_attention(dtype, head_dim, kv4, plan.few, a, static_cast<hipStream_t>(stream));
+  a.row_groups = plan.row_groups;
+  fx::launch_cached_attention(dtype, head_dim, kv4, plan, a, static_cast<hipStream_t>(stream));
   return check_launch(kv4 ? "fx_kv4_attention" : "fx_window_attention");
 }
 
@@ -1836,11 +1831,12 @@ int validate_kv4_cache(const void* k_codes, const void* k_scales, const void* v_
 extern "C" {
 
 size_t fx_cached_attention_workspace_bytes(int batch, int n_q_heads, int n_kv_heads, int tokens, int max_len,
-                                           int head_dim, int window, int sinks, int kv4) {
+                                           int head_dim, int window, int sinks, int dtype, int kv4) {
+  if (!is_half_dtype(dtype)) return 0;
   if (validate_attention_sizes(batch, n_q_heads, n_kv_heads, tokens, max_len, head_dim, window, sinks)) return 0;
   if (batch == 0 || tokens == 0) return 0;
-  return attention_workspace(attention_plan(batch, n_q_heads, n_kv_heads, tokens, max_len, head_dim, window, sinks,
-                                            kv4 != 0),
+  return attention_workspace(fx::plan_cached_attention(dtype, batch, n_kv_heads, n_q_heads / n_kv_heads, tokens, max_len,
+                                                       head_dim, window, sinks, kv4 != 0),
                              batch, n_q_heads, tokens, head_dim);
 }
 

@@ -45,7 +45,10 @@ CASES = {
     "verify": (BF, 2, 2, 3, 5, 333, 128, 100, 4, [(333, 5), (97, 3)]),
     "verify_d64": (HF, 2, 2, 1, 16, 130, 64, 33, 2, [(130, 16), (16, 16)]),
     "verify_more_queries_than_keys": (BF, 2, 1, 4, 4, 40, 128, None, 0, [(2, 4), (0, 4)]),
-    # the rows kernel
+    "verify_groups": (BF, 2, 2, 7, 5, 700, 128, 200, 4, [(700, 5), (150, 3)]),
+    # the rows kernel; fp16 over a 4-bit cache: row groups
+    "rows_8_groups": (HF, 1, 1, 8, 40, 300, 128, 90, 3, [(299, 40)]),
+    "rows_8_groups_d256": (HF, 2, 1, 4, 50, 190, 256, None, 0, [(190, 50), (40, 33)]),
     "rows_17": (BF, 1, 1, 1, 17, 90, 128, None, 0, [(90, 17)]),
     "rows_group_7": (HF, 2, 2, 7, 20, 260, 128, 64, 3, [(260, 20), (131, 13)]),
     "prompt": (BF, 1, 2, 4, 130, 130, 128, None, 0, [(130, 130)]),
