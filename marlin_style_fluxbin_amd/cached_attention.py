@@ -40,25 +40,35 @@ def _rows(t: torch.Tensor, copy: bool = True):
     """``t`` (or a copy of it, or None without ``copy``) as the kernels read it, rows of
     contiguous columns at 16-byte boundaries: the tensor, its address and its strides."""
     s, p = t.stride(), t.data_ptr()
-    if s[3] == 1 and not (s[0] | s[1] | s[2]) & 7 and not p & 15:
+    lazy = t.is_neg()
+    if s[3] == 1 and not (s[0] | s[1] | s[2]) & 7 and not p & 15 and not lazy:
         return t, p, s[:3]
     s = _strides(t)
-    if t.stride(3) != 1 or (s[0] | s[1] | s[2]) & 7 or p & 15:
+    if t.stride(3) != 1 or (s[0] | s[1] | s[2]) & 7 or p & 15 or lazy:
         if not copy:
             return None
+        t = t.resolve_neg()
         t = t.contiguous()
         t = t.clone() if t.data_ptr() & 15 else t
         s = _strides(t)
     return t, t.data_ptr(), s
 
 
-def _check_heads(name: str, t: torch.Tensor) -> None:
-    if t.ndim != 4:
-        raise ValueError(f"{name} must have shape [batch, heads, tokens, head_dim]")
-    if not t.is_cuda:
+_BF16, _FP16 = torch.bfloat16, torch.float16
+
+
+def _check_heads(**tensors: torch.Tensor) -> torch.dtype:
+    """Four axes, one GPU, one half dtype (returned); the message names what is not."""
+    first = next(iter(tensors.values()))
+    for name, t in tensors.items():
+        if t.ndim != 4:
+            raise ValueError(f"{name} must have shape [batch, heads, tokens, head_dim]")
         _lib.require_gpu_tensor(t, name)
-    if t.dtype not in _HALF:
-        raise ValueError(f"{name} must be fp16 or bf16")
+        if t.dtype not in _HALF:
+            raise ValueError(f"{name} must be fp16 or bf16")
+        if t.dtype != first.dtype or t.device != first.device:
+            raise ValueError(f"{' and '.join(tensors)} must share dtype and device")
+    return first.dtype
 
 
 def _check_head_dim(dim: int) -> None:
@@ -66,9 +76,7 @@ def _check_head_dim(dim: int) -> None:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {dim}")
 
 
-def _counts(name: str, t: torch.Tensor | None, batch: int, index: int) -> int | None:
-    if t is None:
-        return None
+def _counts(name: str, t: torch.Tensor, batch: int, index: int) -> int:
     if t.dtype is not torch.int32 or t.shape != (batch,) or t.get_device() != index or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 [batch] tensor on the device of the cache")
     return t.data_ptr()
@@ -104,19 +112,19 @@ def _attention(name, q, cache, cache_args, cache_strides, lengths, query_lengths
         raise ValueError(f"query heads ({heads}) must be a positive multiple of KV heads ({kv_heads})")
     if window is None:
         window = 0
-    elif not isinstance(window, int) or isinstance(window, bool) or window < 1:
+    elif type(window) is not int or window < 1:
         raise ValueError("window must be None or a positive integer")
-    if not isinstance(sinks, int) or isinstance(sinks, bool) or sinks < 0:
+    if type(sinks) is not int or sinks < 0:
         raise ValueError("sinks must be a non-negative integer")
     # no key lies beyond max_len, so neither a window nor sinks need to
     window, sinks = min(window, max_len + 1), min(sinks, max_len)
     index = device.index
-    lengths_ptr = _counts("lengths", lengths, batch, index)
-    counts_ptr = _counts("query_lengths", query_lengths, batch, index)
+    lengths_ptr = None if lengths is None else _counts("lengths", lengths, batch, index)
+    counts_ptr = None if query_lengths is None else _counts("query_lengths", query_lengths, batch, index)
     if out is None:
         make = torch.empty if query_lengths is None else torch.zeros
         out = make((batch, tokens, heads, dim), dtype=dtype, device=device).transpose(1, 2)
-    elif out.shape != shape or out.dtype is not dtype or out.device != device:
+    elif out.shape != shape or out.dtype is not dtype or out.get_device() != index:
         raise ValueError("out must have q's shape, dtype and device")
     elif out.requires_grad and torch.is_grad_enabled():
         _no_gradient()
@@ -127,9 +135,12 @@ def _attention(name, q, cache, cache_args, cache_strides, lengths, query_lengths
     q, q_ptr, q_strides = _rows(q)
     code = _lib.dtype_code(dtype)
     nbytes = _workspace_bytes(batch, heads, kv_heads, tokens, max_len, dim, window, sinks, code, kv4)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    workspace = workspace_ptr = None
+    if nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        workspace_ptr = workspace.data_ptr()
     strides = (_Strides6 if kv4 else _Strides12)(*q_strides, *cache_strides, *out_strides)
-    _launch(name, device, q_ptr, *cache_args, out_ptr, strides, lengths_ptr, counts_ptr, _lib.ptr(workspace), nbytes,
+    _launch(name, device, q_ptr, *cache_args, out_ptr, strides, lengths_ptr, counts_ptr, workspace_ptr, nbytes,
             batch, heads, kv_heads, tokens, max_len, dim, window, sinks,
             1.0 / math.sqrt(dim) if scale is None else scale, code)
     return out
@@ -149,15 +160,14 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengt
     ``query_lengths[b]`` stay as they are in ``out`` and are zeros in a new output.  ``scale``
     defaults to ``1 / sqrt(head_dim)``.  fp16 or bf16, head_dim 64, 128 or 256, any strides
     (rows that are not 16-byte aligned are copied first, ``out`` is refused)."""
-    _check_heads("q", q)
-    _check_heads("k", k)
-    _check_heads("v", v)
-    shape, dtype, device = k.shape, q.dtype, q.device
+    dtype, index = q.dtype, q.get_device()
+    if not (q.ndim == k.ndim == v.ndim == 4 and index >= 0 and (dtype is _BF16 or dtype is _FP16)
+            and k.dtype is dtype and v.dtype is dtype and k.get_device() == index and v.get_device() == index):
+        _check_heads(q=q, k=k, v=v)
+    shape = k.shape
     if v.shape != shape or q.shape[3] != shape[3]:
         raise ValueError("k and v must have one shape, with q's head_dim")
     _check_head_dim(shape[3])
-    if not dtype == k.dtype == v.dtype or not device == k.device == v.device:
-        raise ValueError("q, k and v must share dtype and device")
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         _no_gradient()
     k, k_ptr, k_strides = _rows(k)
@@ -208,34 +218,38 @@ class Int4KVCache:
         [batch, kv_heads, tokens, head_dim]`` into positions ``start[b] + t`` (``start`` int32
         ``[batch]`` on the device, or one integer for all).  Positions outside the cache are
         dropped; nothing else of it changes."""
-        _check_heads("k", k)
-        _check_heads("v", v)
-        device = self.device
-        if k.shape != v.shape or k.dtype != v.dtype or not k.device == v.device == device:
-            raise ValueError("k and v must share shape and dtype, on the cache's device")
-        batch, heads, tokens, dim = k.shape
+        dtype, device = k.dtype, self.device
+        index = device.index
+        if not (k.ndim == v.ndim == 4 and k.get_device() == index and v.get_device() == index
+                and (dtype is _BF16 or dtype is _FP16) and v.dtype is dtype):
+            _check_heads(k=k, v=v)
+            raise ValueError("k and v must be on the cache's device")
+        shape = k.shape
+        if v.shape != shape:
+            raise ValueError("k and v must share their shape")
+        batch, heads, tokens, dim = shape
         if (batch, heads, dim) != (self.batch, self.kv_heads, self.head_dim):
             raise ValueError("k and v must be [batch, kv_heads, tokens, head_dim] of the cache")
         if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
             _no_gradient()
         start_ptr, start_all = None, 0
         if isinstance(start, torch.Tensor):
-            start_ptr = _counts("start", start, batch, device.index)
-        elif isinstance(start, int) and not isinstance(start, bool) and 0 <= start <= _LIMIT:
+            start_ptr = _counts("start", start, batch, index)
+        elif type(start) is int and 0 <= start <= _LIMIT:
             start_all = start
         else:
             raise ValueError("start must be a non-negative integer or an int32 [batch] tensor")
-        counts_ptr = _counts("counts", counts, batch, device.index)
+        counts_ptr = None if counts is None else _counts("counts", counts, batch, index)
         k, k_ptr, k_strides = _rows(k)
         v, v_ptr, v_strides = _rows(v)
         _launch("fx_kv4_append", device, k_ptr, v_ptr, _Strides6(*k_strides, *v_strides), start_ptr, start_all,
-                counts_ptr, *self._pointers(), batch, heads, tokens, self.max_len, dim, _lib.dtype_code(k.dtype))
+                counts_ptr, *self._pointers(), batch, heads, tokens, self.max_len, dim, _lib.dtype_code(dtype))
 
     def restore(self, *, length: int | None = None, dtype: torch.dtype = torch.bfloat16):
         """The values that the first ``length`` positions (default all) stand for, as new
         ``k, v [batch, kv_heads, length, head_dim]`` tensors of ``dtype`` (fp16 or bf16)."""
         length = self.max_len if length is None else length
-        if not isinstance(length, int) or isinstance(length, bool) or not 0 <= length <= self.max_len:
+        if type(length) is not int or not 0 <= length <= self.max_len:
             raise ValueError("length must be an integer in [0, max_len]")
         if dtype not in _HALF:
             raise ValueError("dtype must be fp16 or bf16")
@@ -250,9 +264,12 @@ def kv4_attention(q: torch.Tensor, cache: Int4KVCache, *, lengths: torch.Tensor 
                   query_lengths: torch.Tensor | None = None, window: int | None = None, sinks: int = 0,
                   scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`window_attention` over the values that an :class:`Int4KVCache` stands for."""
-    _check_heads("q", q)
-    if q.shape[3] != cache.head_dim or q.device != cache.device:
-        raise ValueError("q must have the cache's head_dim and device")
+    dtype = q.dtype
+    if not (q.ndim == 4 and q.get_device() == cache.device.index and (dtype is _BF16 or dtype is _FP16)):
+        _check_heads(q=q)
+        raise ValueError("q must be on the cache's device")
+    if q.shape[3] != cache.head_dim:
+        raise ValueError("q must have the cache's head_dim")
     if q.requires_grad and torch.is_grad_enabled():
         _no_gradient()
     return _attention("fx_kv4_attention", q, (cache.batch, cache.kv_heads, cache.max_len), cache._pointers(), (),

@@ -13,9 +13,8 @@
 // with S, m, the sum and O in fp32.  O is rescaled only when some query's maximum grew by
 // more than 2^8 (p then stays below 2^8, which fp16 holds too).
 //
-// LDS: rows of D 16-bit values in 16-byte chunks, chunk c of key j at c ^ swizzle(j), so
-// that both the 16-byte reads of 8 consecutive keys (K) and the transposing reads of 4
-// keys x 32 bytes (V) touch every bank once.  16-bit caches load straight into LDS (the
+// LDS: rows of D 16-bit values in 16-byte chunks, chunk c of key j at c ^ swizzle(j), keys
+// and values each for their reads.  16-bit caches load straight into LDS (the
 // swizzle is applied to the global address of each lane), the next tile while this one is
 // multiplied; the 4-bit cache is widened in registers and stored.
 #pragma once
@@ -37,10 +36,17 @@ struct RowsShape {
   static constexpr int kSub = KT / 32;          // 32-key blocks of a tile
 };
 
-// A row of 128 bytes covers half the banks, so two keys share a swizzle there.
+// LDS serves 256 bytes a clock, 64 banks: sixteen lanes of a 16-byte read (keys: 16 rows, one
+// chunk) or 32 of a transposing one (values: 4 rows, 64 bytes), which have to fall into
+// different banks.  Measured 515 and 370 bytes a ns for each CU; with the low three bits of
+// the row for both, 279 and 274.
 template <int D>
-__device__ __forceinline__ int lds_swizzle(int key) {
-  return D == 64 ? ((key >> 1) & 3) << 1 : (key & 7) << 1;
+__device__ __forceinline__ int key_swizzle(int row) {
+  return D == 64 ? (row >> 1) & 7 : row & 15;
+}
+template <int D>
+__device__ __forceinline__ int value_swizzle(int row) {
+  return D == 64 ? (row & 2) << 1 : (row & 3) << 2;
 }
 
 __device__ __forceinline__ u32x4_t lds_b128(const lds_char* p) {
@@ -63,22 +69,23 @@ __device__ __forceinline__ void load_to_lds(const u32x4_t& resource, int offset,
 }
 
 // One tile (rows left of it may be fewer than KT: the others become zero) into LDS.
-template <int D>
+template <int D, bool KEYS>
 __device__ __forceinline__ void load_rows_to_lds(const uint16_t* base, long long stride, int rows, lds_char* dst,
                                                  int wave, int lane) {
   using S = RowsShape<D>;
   constexpr int kRowsPerLoad = 1024 / S::kRowBytes;  // one wave load: 64 lanes x 16 bytes
   constexpr int kLoads = S::KT / kRowsPerLoad / 4;   // per wave
   const int live = min(rows, S::KT);
+  asm volatile("" : "+v"(lane));  // offsets formed here: kept between calls they cost registers
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
-    // the scalar part of the address in the resource, two or four lane offsets for all loads
+    // the scalar part of the address in the resource
     const int first = (wave * kLoads + i) * kRowsPerLoad, left = live - first;
     const size_t address = reinterpret_cast<size_t>(base + first * stride);
     const u32x4_t r = {unsigned(address), unsigned(address >> 32) & 0xffffu,
                        left > 0 ? unsigned(left - 1) * unsigned(stride) * 2u + unsigned(D) * 2u : 0u, 0x00020000u};
     const int row = lane / S::kChunks;
-    const int chunk = (lane % S::kChunks) ^ lds_swizzle<D>(i * kRowsPerLoad + row);  // a wave's rows start at 8 w
+    const int chunk = (lane % S::kChunks) ^ (KEYS ? key_swizzle<D>(first + row) : value_swizzle<D>(first + row));
     load_to_lds(r, row * int(stride) * 2 + chunk * 16, dst + first * S::kRowBytes);
   }
 }
@@ -112,6 +119,7 @@ struct Kv4Stage {
     }
   }
 
+  template <bool KEYS>
   __device__ __forceinline__ void store(lds_char* dst, int t) const {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
     const h2 bias = {_Float16(1024.f), _Float16(1024.f)};
@@ -141,7 +149,7 @@ struct Kv4Stage {
           // columns 64 g + 4 (units of the pieces before + u) .. + 7: chunk 8 g + that / 8
           const int chunk = 8 * g + (piece * kUnits + u) / 2;
           *reinterpret_cast<__attribute__((address_space(3))) u32x4_t*>(
-              dst + key * S::kRowBytes + ((chunk ^ lds_swizzle<D>(key)) * 16)) = w;
+              dst + key * S::kRowBytes + ((chunk ^ (KEYS ? key_swizzle<D>(key) : value_swizzle<D>(key))) * 16)) = w;
         }
       }
     }
@@ -231,10 +239,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
 
   // ---- LDS read addresses: K chunk 2 s + half of key l31 (+ 32 u); V^T: keys 4 half +
   // (i >> 2) (+ 16 kk + 8), columns 32 dt + 16 dg + 4 (i & 3)
-  int xk = lds_swizzle<D>(l31) * 16;
-  const int kaddr = l31 * S::kRowBytes + half * 16;
+  int xk = key_swizzle<D>(l31) * 16;
+  const int kaddr = l31 * S::kRowBytes;
   const int i16 = lane & 15, dg = (lane >> 4) & 1, vkey = 4 * half + (i16 >> 2);
-  int xv = lds_swizzle<D>(vkey) * 16;
+  int xv = value_swizzle<D>(vkey) * 16;
   const int vaddr = vkey * S::kRowBytes + (i16 & 1) * 8;
   const int vcol = (2 * dg + ((i16 & 3) >> 1)) * 16;
 
@@ -256,39 +264,61 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
   }
   Kv4Stage<D> ks, vs;
 
-  // loads of tile `it` of the list: a 16-bit tile on its way into LDS, a 4-bit one into registers
-  auto fetch = [&](int it, lds_char* dst) __attribute__((always_inline)) {
+  // LDS: keys of tile i at (i % 2) tiles, values at 2 + (i % 2) (i from it0)
+  const auto key_tile = [&](int parity) __attribute__((always_inline)) { return lds + parity * S::kTileBytes; };
+  const auto value_tile = [&](int parity) __attribute__((always_inline)) { return lds + (2 + parity) * S::kTileBytes; };
+  // loads of tile `it` of the list (none past the last): 16-bit rows on their way into LDS,
+  // 4-bit ones into registers
+  auto fetch_keys = [&](int it, int parity) __attribute__((always_inline)) {
+    if (it >= it1) return;
     const int j0 = tiles.tile_start<KT>(it), rows = tiles.tile_end(it, hi_pos, a.sinks) - j0;
-    if constexpr (!KV4) {
-      load_rows_to_lds<D>(kb + j0 * a.k_stride[2], a.k_stride[2], rows, dst, wave, lane);
-      load_rows_to_lds<D>(vb + j0 * a.v_stride[2], a.v_stride[2], rows, dst + S::kTileBytes, wave, lane);
-    } else {
-      const size_t at = row_at + j0;
+    const size_t at = row_at + j0;
+    if constexpr (!KV4)
+      load_rows_to_lds<D, true>(kb + j0 * a.k_stride[2], a.k_stride[2], rows, key_tile(parity), wave, lane);
+    else
       ks.load(static_cast<const uint8_t*>(a.k) + at * (D / 2), a.k_scales + at * (D / 64), rows, t);
+  };
+  auto fetch_values = [&](int it, int parity) __attribute__((always_inline)) {
+    if (it >= it1) return;
+    const int j0 = tiles.tile_start<KT>(it), rows = tiles.tile_end(it, hi_pos, a.sinks) - j0;
+    const size_t at = row_at + j0;
+    if constexpr (!KV4)
+      load_rows_to_lds<D, false>(vb + j0 * a.v_stride[2], a.v_stride[2], rows, value_tile(parity), wave, lane);
+    else
       vs.load(static_cast<const uint8_t*>(a.v) + at * (D / 2), a.v_scales + at * (D / 64), rows, t);
-    }
   };
 
+  // operand n of a tile's S^T products (key block n / kSteps, step n % kSteps) and of its O^T
+  // products (16 keys n / kDims, column block n % kDims)
+  constexpr int kKeyOps = S::kSteps * S::kSub, kValueOps = 2 * S::kSub * S::kDims;
+  auto key_operand = [&](const lds_char* kt, int n) __attribute__((always_inline)) {
+    return lds_b128(kt + kaddr + n / S::kSteps * 32 * S::kRowBytes + ((n % S::kSteps * 32 + half * 16) ^ xk));
+  };
+  auto value_operand = [&](const lds_char* vt, int n) __attribute__((always_inline)) {
+    const lds_char* at = vt + vaddr + n / S::kDims * 16 * S::kRowBytes + ((vcol + n % S::kDims * 64) ^ xv);
+    const u32x2_t x = lds_transposed(at), y = lds_transposed(at + 8 * S::kRowBytes);
+    return u32x4_t{x[0], x[1], y[0], y[1]};
+  };
   auto scores = [&](const lds_char* kt, f32x16_t(&s)[S::kSub]) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < S::kSub; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
 #pragma unroll
-    for (int st = 0; st < S::kSteps; ++st)
-#pragma unroll
-      for (int u = 0; u < S::kSub; ++u)
-        s[u] = mfma32<CDT>(lds_b128(kt + kaddr + u * 32 * S::kRowBytes + ((st * 32) ^ xk)), qf[st], s[u]);
+    for (int n = 0; n < kKeyOps; ++n)
+      s[n / S::kSteps] = mfma32<CDT>(key_operand(kt, n), qf[n % S::kSteps], s[n / S::kSteps]);
   };
 
-  // running maximum and sum; s becomes p in the operand layout of P^T
-  auto softmax = [&](f32x16_t(&s)[S::kSub], u32x4_t(&pf)[2 * S::kSub]) __attribute__((always_inline)) {
+  // the largest of a tile's scores; the running maximum takes it in
+  auto largest = [&](const f32x16_t(&s)[S::kSub]) __attribute__((always_inline)) {
     float top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < S::kSub; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-    top = half_pair_max(top) * f;
+    return half_pair_max(top) * f;
+  };
+  auto raise = [&](float top) __attribute__((always_inline)) {
     if (__builtin_amdgcn_ballot_w64(top > m + 8.f)) {
       const float mn = fmaxf(m, top);
       m_use = mn == -INFINITY ? 0.f : mn;
@@ -300,153 +330,215 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
     }
-#pragma unroll
-    for (int u = 0; u < S::kSub; ++u) {
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], f, -m_use));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r + 1], f, -m_use));
-        l += p0 + p1;
-        float c0 = p0, c1 = p1;
-        pf[2 * u + r / 8][(r & 7) / 2] = round_pair_bits<CDT>(c0, c1);
-      }
-    }
   };
 
-  auto values = [&](const lds_char* vt, const u32x4_t(&pf)[2 * S::kSub]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int kk = 0; kk < 2 * S::kSub; ++kk)
-#pragma unroll
-      for (int d = 0; d < S::kDims; ++d) {
-        const lds_char* at = vt + vaddr + kk * 16 * S::kRowBytes + ((vcol + d * 64) ^ xv);
-        const u32x2_t x = lds_transposed(at), y = lds_transposed(at + 8 * S::kRowBytes);
-        o[d] = mfma32<CDT>(u32x4_t{x[0], x[1], y[0], y[1]}, pf[kk], o[d]);
-      }
+  // scores 2 i, 2 i + 1 of the tile: p in the operand layout of P^T, and its sum
+  auto weigh = [&](const f32x16_t(&s)[S::kSub], u32x4_t(&pf)[2 * S::kSub], int i) __attribute__((always_inline)) {
+    const int u = i / 8, r = i % 8 * 2;
+    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], f, -m_use));
+    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r + 1], f, -m_use));
+    l += p0 + p1;
+    asm volatile("" : "+v"(l));  // here, not behind the products with every p kept until then
+    float c0 = p0, c1 = p1;
+    pf[2 * u + r / 8][(r & 7) / 2] = round_pair_bits<CDT>(c0, c1);
   };
 
-  // A tile that some query sees only in part: hidden scores become -inf.  Keys that no query
-  // of the workgroup sees are zeros in LDS.  One that some see may hold an infinity or a NaN,
-  // and a product with a hidden query's zero p would carry it into that row: `careful` adds
-  // such values by hand to the rows that see them and zeroes them in LDS.
-  auto masked_tile = [&](lds_char* cur, int j0, bool sink_tile, bool careful) __attribute__((always_inline)) {
-    const TileMask seen(p, a.window, a.sinks, sink_tile, tiles.joined);
-    f32x16_t s[S::kSub];
-    u32x4_t pf[2 * S::kSub];
-    if (active) {
-      scores(cur, s);
-      const auto hide = [&](auto sees) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < S::kSub; ++u)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s[u][r] = sees(j0 + 4 * half + 32 * u + (r & 3) + 8 * (r >> 2)) ? s[u][r] : -INFINITY;
-      };
-      if (sink_tile || tiles.joined) hide([&](int j) __attribute__((always_inline)) { return seen.sees(j); });
-      else hide([&](int j) __attribute__((always_inline)) { return seen.sees_window(j); });
-      softmax(s, pf);
-    }
-    lds_char* vt = cur + S::kTileBytes;
-    if (careful) {
-      unsigned bad = 0;
-      for (int i = t * 16; i < S::kTileBytes; i += 256 * 16) {
-        const u32x4_t w = lds_b128(vt + i);
-        bad |= nonfinite_pair<CDT>(w[0]) | nonfinite_pair<CDT>(w[1]) | nonfinite_pair<CDT>(w[2]) |
-               nonfinite_pair<CDT>(w[3]);
-      }
-      if (__syncthreads_or(bad != 0)) {
-        int h = half;
-        asm volatile("" : "+v"(h));  // no address of this rare path is kept in a register elsewhere
-        for (int j = 0; j < KT; ++j) {
-          if (!active || !seen.sees(j0 + j)) continue;
-#pragma unroll
-          for (int d = 0; d < S::kDims; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int x = 32 * d + (r & 3) + 8 * (r >> 2) + 4 * h;
-              const uint16_t bits = *reinterpret_cast<const __attribute__((address_space(3))) uint16_t*>(
-                  vt + j * S::kRowBytes + (((x >> 3) ^ lds_swizzle<D>(j)) * 16) + (x & 7) * 2);
-              o[d][r] += nonfinite_pair<CDT>(bits) ? to_f32<CDT>(bits) : 0.f;
-            }
-        }
-        __syncthreads();
-        for (int i = t * 16; i < S::kTileBytes; i += 256 * 16) {
-          u32x4_t w = lds_b128(vt + i);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = finite_pair<CDT>(w[e]);
-          *reinterpret_cast<__attribute__((address_space(3))) u32x4_t*>(vt + i) = w;
-        }
-        __syncthreads();
-      }
-    }
-    if (active) values(vt, pf);
-  };
-
-  auto step = [&](lds_char* cur, lds_char* nxt, int it, bool more, bool careful) __attribute__((always_inline)) {
-    if (more) fetch(it + 1, nxt);
+  // A tile that some query sees only in part: hidden scores become -inf.
+  auto partial = [&](int it) __attribute__((always_inline)) {
     const int j0 = tiles.tile_start<KT>(it);
+    return !all_see(lo_pos, hi_pos, j0, j0 + KT, a.window, a.sinks, it < tiles.sink_tiles);
+  };
+  auto hide = [&](int it, f32x16_t(&s)[S::kSub]) __attribute__((always_inline)) {
     const bool sink_tile = it < tiles.sink_tiles;
-    // 256 columns: the swizzled addresses formed anew for each tile (kept, they spill, and a
-    // reload waits for the tile in flight)
-    if constexpr (D == 256) asm volatile("" : "+v"(xk), "+v"(xv));
-    if (all_see(lo_pos, hi_pos, j0, j0 + KT, a.window, a.sinks, sink_tile)) {
-      if (active) {
-        f32x16_t s[S::kSub];
-        u32x4_t pf[2 * S::kSub];
-        scores(cur, s);
-        softmax(s, pf);
-        values(cur + S::kTileBytes, pf);
-      }
-    } else {
-      masked_tile(cur, j0, sink_tile, careful);
+    const TileMask seen(p, a.window, a.sinks, sink_tile, tiles.joined);
+    const int first = tiles.tile_start<KT>(it) + 4 * half;
+    const auto each = [&](auto sees) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < S::kSub; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[u][r] = sees(first + 32 * u + (r & 3) + 8 * (r >> 2)) ? s[u][r] : -INFINITY;
+    };
+    if (sink_tile || tiles.joined) each([&](int j) __attribute__((always_inline)) { return seen.sees(j); });
+    else each([&](int j) __attribute__((always_inline)) { return seen.sees_window(j); });
+  };
+  // Keys that no query of the workgroup sees are zeros in LDS.  One that some see may hold an
+  // infinity or a NaN, and a product with a hidden query's zero p would carry it into that
+  // row: the careful round adds such values by hand to the rows that see them and zeroes them.
+  auto settle = [&](int it, lds_char* vt) __attribute__((always_inline)) {
+    unsigned bad = 0;
+    for (int i = t * 16; i < S::kTileBytes; i += 256 * 16) {
+      const u32x4_t w = lds_b128(vt + i);
+      bad |= nonfinite_pair<CDT>(w[0]) | nonfinite_pair<CDT>(w[1]) | nonfinite_pair<CDT>(w[2]) |
+             nonfinite_pair<CDT>(w[3]);
     }
+    if (!__syncthreads_or(bad != 0)) return;
+    const TileMask seen(p, a.window, a.sinks, it < tiles.sink_tiles, tiles.joined);
+    const int j0 = tiles.tile_start<KT>(it);
+    int h = half;
+    asm volatile("" : "+v"(h));  // no address of this rare path is kept in a register elsewhere
+    for (int j = 0; j < KT; ++j) {
+      if (!active || !seen.sees(j0 + j)) continue;
+#pragma unroll
+      for (int d = 0; d < S::kDims; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int x = 32 * d + (r & 3) + 8 * (r >> 2) + 4 * h;
+          const uint16_t bits = *reinterpret_cast<const __attribute__((address_space(3))) uint16_t*>(
+              vt + j * S::kRowBytes + (((x >> 3) ^ value_swizzle<D>(j)) * 16) + (x & 7) * 2);
+          o[d][r] += nonfinite_pair<CDT>(bits) ? to_f32<CDT>(bits) : 0.f;
+          if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few values at a time: registers are scarce
+        }
+    }
+    __syncthreads();
+    for (int i = t * 16; i < S::kTileBytes; i += 256 * 16) {
+      u32x4_t w = lds_b128(vt + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = finite_pair<CDT>(w[e]);
+      *reinterpret_cast<__attribute__((address_space(3))) u32x4_t*>(vt + i) = w;
+    }
+    __syncthreads();
+  };
+  // Loads asked for one step ago have arrived (every wave waits for its own), and every wave
+  // is done with what the next ones overwrite.
+  auto arrive = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
   };
 
-  // Once, and again carefully if some row came out infinite or NaN: such a row may have it
-  // from a value that it does not see (and a row that has it by right can wait).
-  bool careful = false;
-  while (true) {
-    if (it0 < it1) {
-      fetch(it0, lds);
-      if constexpr (KV4) {
-        ks.store(lds, t);
-        vs.store(lds + S::kTileBytes, t);
-      }
-    }
-    int parity = 0;
-    for (int it = it0; it < it1; ++it) {
-      lds_char* cur = lds + parity * 2 * S::kTileBytes;
-      lds_char* nxt = lds + (parity ^ 1) * 2 * S::kTileBytes;
-      // this tile has arrived (every wave waits for its own loads), and the other buffer's
-      // readers are done
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      const bool more = it + 1 < it1;
-      int how = careful;
-      asm volatile("" : "+v"(how));  // one copy of the loop serves both rounds
-      how = __builtin_amdgcn_readfirstlane(how);
-      step(cur, nxt, it, more, how != 0);
-      if constexpr (KV4) {
-        if (more) {
-          ks.store(nxt, t);
-          vs.store(nxt + S::kTileBytes, t);
+  // Step `it` (it - it0 = parity mod 2): p of this tile's scores s beside the products of the
+  // next tile's, sn; then O.  In LDS: this tile's values, the next one's keys; on their way:
+  // the next one's values, the keys after.
+  auto step = [&](int it, int parity, f32x16_t(&s)[S::kSub], f32x16_t(&sn)[S::kSub])
+                  __attribute__((always_inline)) {
+    arrive();
+    fetch_keys(it + 2, parity);
+    fetch_values(it + 1, parity ^ 1);
+    // the swizzled addresses are formed anew for each tile (kept, they spill other values, and
+    // a reload waits for the tile in flight)
+    asm volatile("" : "+v"(xk), "+v"(xv));
+    if (active) {
+      // One list of products, S^T of the next tile and then O^T of this one, operands read
+      // from LDS kAhead products early; between the former the exponentials of this tile,
+      // between the latter the maximum of the next.  Fenced product by product: left alone,
+      // the compiler orders for fewest registers, every operand read just before its use and
+      // all exponentials behind all products.
+      const lds_char* kt = key_tile(parity ^ 1);
+      const lds_char* vt = value_tile(parity);
+      constexpr int kAhead = 4, kOps = kKeyOps + kValueOps, kPairs = 8 * S::kSub;
+      u32x4_t pf[2 * S::kSub], ring[kAhead + 1];
+      const auto operand = [&](int n) __attribute__((always_inline)) {
+        return n < kKeyOps ? key_operand(kt, n) : value_operand(vt, n - kKeyOps);
+      };
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) ring[n] = operand(n);
+#pragma unroll
+      for (int u = 0; u < S::kSub; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sn[u][r] = 0.f;
+      float top = -INFINITY;  // as if no score were hidden
+#pragma unroll
+      for (int n = 0; n < kOps; ++n) {
+        if (n + kAhead < kOps) ring[(n + kAhead) % (kAhead + 1)] = operand(n + kAhead);
+        const u32x4_t x = ring[n % (kAhead + 1)];
+        if (n < kKeyOps) {
+          sn[n / S::kSteps] = mfma32<CDT>(x, qf[n % S::kSteps], sn[n / S::kSteps]);
+#pragma unroll
+          for (int i = n * kPairs / kKeyOps; i < (n + 1) * kPairs / kKeyOps; ++i) weigh(s, pf, i);
+        } else {
+          const int v = n - kKeyOps;
+          o[v % S::kDims] = mfma32<CDT>(x, pf[v / S::kDims], o[v % S::kDims]);
+#pragma unroll
+          for (int i = v * kPairs / kValueOps; i < (v + 1) * kPairs / kValueOps; ++i)
+            top = fmaxf(fmaxf(top, sn[i / 8][i % 8 * 2]), sn[i / 8][i % 8 * 2 + 1]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      parity ^= 1;
+      top = half_pair_max(top) * f;
+      if (partial(it + 1)) {
+        hide(it + 1, sn);
+        top = largest(sn);
+      }
+      raise(top);
     }
-    if (careful) break;
+    if constexpr (KV4) {
+      if (it + 2 < it1) ks.template store<true>(key_tile(parity), t);
+      vs.template store<false>(value_tile(parity ^ 1), t);
+    }
+  };
+  auto weigh_values = [&](int parity, f32x16_t(&s)[S::kSub]) __attribute__((always_inline)) {
+    u32x4_t pf[2 * S::kSub];
+#pragma unroll
+    for (int i = 0; i < 8 * S::kSub; ++i) weigh(s, pf, i);
+#pragma unroll
+    for (int n = 0; n < kValueOps; ++n)
+      o[n % S::kDims] = mfma32<CDT>(value_operand(value_tile(parity), n), pf[n / S::kDims], o[n % S::kDims]);
+  };
+
+  if (it0 < it1) {
+    f32x16_t sa[S::kSub], sb[S::kSub];
+    fetch_keys(it0, 0);
+    fetch_values(it0, 0);
+    if constexpr (KV4) {
+      ks.template store<true>(key_tile(0), t);
+      vs.template store<false>(value_tile(0), t);
+    }
+    fetch_keys(it0 + 1, 1);
+    if constexpr (KV4) {
+      if (it0 + 1 < it1) ks.template store<true>(key_tile(1), t);
+    }
+    arrive();
+    if (active) {
+      scores(key_tile(0), sa);
+      if (partial(it0)) hide(it0, sa);
+      raise(largest(sa));
+    }
+    int it = it0;
+    for (; it + 2 < it1; it += 2) {
+      step(it, 0, sa, sb);
+      step(it + 1, 1, sb, sa);
+    }
+    if (it + 1 < it1) {
+      step(it, 0, sa, sb);
+      arrive();
+      if (active) weigh_values(1, sb);
+    } else {
+      arrive();
+      if (active) weigh_values(0, sa);
+    }
+    // If some row came out infinite or NaN, once more and carefully: such a row may have it
+    // from a value that it does not see (and a row that has it by right can wait).
     float probe = 0.f;
 #pragma unroll
     for (int d = 0; d < S::kDims; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) probe = __builtin_fmaf(o[d][r], 0.f, probe);
-    if (!__syncthreads_or(!(probe == 0.f))) break;  // also: every wave is done with the tiles
-    careful = true;
+    // (the barrier: every wave is done with the tiles)
+    if (__builtin_expect(__syncthreads_or(!(probe == 0.f)), 0)) {
 #pragma unroll
-    for (int d = 0; d < S::kDims; ++d)
+      for (int d = 0; d < S::kDims; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-    m = -INFINITY;
-    m_use = l = 0.f;
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+      m = -INFINITY;
+      m_use = l = 0.f;
+      for (it = it0; it < it1; ++it) {
+        fetch_keys(it, 0);
+        fetch_values(it, 0);
+        if constexpr (KV4) {
+          ks.template store<true>(key_tile(0), t);
+          vs.template store<false>(value_tile(0), t);
+        }
+        arrive();
+        if (active) {
+          scores(key_tile(0), sa);
+          if (partial(it)) hide(it, sa);
+          raise(largest(sa));
+        }
+        if (partial(it)) settle(it, value_tile(0));
+        if (active) weigh_values(0, sa);
+        __syncthreads();  // the next tile's loads overwrite this one
+      }
+    }
   }
 
   // ---- out.  (The row's place again: kept through the loop, it would cost the loop registers.)
@@ -500,14 +592,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
       }
       const int chunk = 4 * d + r / 4;
       *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(
-          mine + l31 * S::kRowBytes + ((chunk ^ lds_swizzle<D>(l31)) * 16) + half * 8) = w;
+          mine + l31 * S::kRowBytes + ((chunk ^ key_swizzle<D>(l31)) * 16) + half * 8) = w;
     }
   wave_lds_order();
 #pragma unroll
   for (int i = 0; i < S::kChunks / 2; ++i) {
     const int at = i * 64 + lane, r = at / S::kChunks, chunk = at % S::kChunks;
     const int rr = wave_row + r;
-    const u32x4_t w = lds_b128(mine + r * S::kRowBytes + ((chunk ^ lds_swizzle<D>(r)) * 16));
+    const u32x4_t w = lds_b128(mine + r * S::kRowBytes + ((chunk ^ key_swizzle<D>(r)) * 16));
     if (rr < rows) {
       const int tk = rr / a.G, hd = g * a.G + rr - tk * a.G;
       *reinterpret_cast<u32x4_t*>(a.out + b * a.out_stride[0] + hd * a.out_stride[1] + tk * a.out_stride[2] +
