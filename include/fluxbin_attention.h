@@ -59,7 +59,8 @@ int fx_kv4_attention(const void *q, const void *k_codes, const void *k_scales, c
  *   minimum = fp16(lo), scale = fp16(fp32(hi - lo) * fp32(1 / 15)),
  *   code = clamp(round(fp32(fp32(x - minimum) * fp32(1 / scale))), 0, 15), ties to even
  *   (scale 0: code 0), standing for code * scale + minimum.
- * A group that holds an infinity, a NaN or a magnitude above 32768 stands for NaN.
+ * A group that holds an infinity, a NaN or a magnitude above 32768 stands for NaN (scale 0,
+ * minimum NaN).
  * codes uint16 [batch, n_kv_heads, max_len, 16, head_dim / 64]: word [c, g] holds columns
  * 64 g + 4 c + k, k < 4, in bits 4 k .. 4 k + 3; scales fp16 [batch, n_kv_heads, max_len,
  * head_dim / 64, 2]: (scale, minimum).  All contiguous and 16-byte aligned.

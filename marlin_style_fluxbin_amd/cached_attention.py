@@ -116,6 +116,10 @@ def _attention(name, q, cache, cache_args, cache_strides, lengths, query_lengths
         raise ValueError("window must be None or a positive integer")
     if type(sinks) is not int or sinks < 0:
         raise ValueError("sinks must be a non-negative integer")
+    if scale is None:
+        scale = 1.0 / math.sqrt(dim)
+    elif not 0.0 < float(scale) < 3.4e38:
+        raise ValueError("scale must be positive and finite")
     # no key lies beyond max_len, so neither a window nor sinks need to
     window, sinks = min(window, max_len + 1), min(sinks, max_len)
     index = device.index
@@ -141,8 +145,7 @@ def _attention(name, q, cache, cache_args, cache_strides, lengths, query_lengths
         workspace_ptr = workspace.data_ptr()
     strides = (_Strides6 if kv4 else _Strides12)(*q_strides, *cache_strides, *out_strides)
     _launch(name, device, q_ptr, *cache_args, out_ptr, strides, lengths_ptr, counts_ptr, workspace_ptr, nbytes,
-            batch, heads, kv_heads, tokens, max_len, dim, window, sinks,
-            1.0 / math.sqrt(dim) if scale is None else scale, code)
+            batch, heads, kv_heads, tokens, max_len, dim, window, sinks, scale, code)
     return out
 
 

@@ -1757,6 +1757,9 @@ int validate_cache_sizes(int batch, int n_kv_heads, int tokens, int max_len, int
     return fail(FX_EINVAL, "n_kv_heads must be in [1, 4096], got %d", n_kv_heads);
   if (tokens < 0 || tokens > (1 << 24)) return fail(FX_EINVAL, "tokens must be in [0, 2^24], got %d", tokens);
   if (max_len < 0 || max_len > (1 << 28)) return fail(FX_EINVAL, "max_len must be in [0, 2^28], got %d", max_len);
+  // a launch holds fewer than 2^32 threads: at most a workgroup of 512 for 32 rows of a head
+  if ((long long)(batch) * n_kv_heads * (tokens / 32 + 1) > (1LL << 23))
+    return fail(FX_EINVAL, "batch %d x %d KV heads x %d tokens is too large for one call", batch, n_kv_heads, tokens);
   return FX_OK;
 }
 
@@ -1766,8 +1769,9 @@ int validate_attention_sizes(int batch, int n_q_heads, int n_kv_heads, int token
   if (n_q_heads < 1 || n_q_heads % n_kv_heads != 0)
     return fail(FX_EINVAL, "n_q_heads %d must be a positive multiple of n_kv_heads %d", n_q_heads, n_kv_heads);
   if (window < 0 || sinks < 0) return fail(FX_EINVAL, "window and sinks must be non-negative");
-  // 31 bits hold every row index and the number of workgroups
-  if ((long long)(tokens) * n_q_heads > (1LL << 30) || (long long)(batch) * n_q_heads * (tokens / 8 + 1) > (1LL << 30))
+  if (n_q_heads > (1 << 16)) return fail(FX_EINVAL, "n_q_heads must be at most 65536, got %d", n_q_heads);
+  // the same for query rows (32 a workgroup at least), whose indexes stay within 31 bits
+  if ((long long)(batch) * n_q_heads * (tokens + 31LL) > (1LL << 28))
     return fail(FX_EINVAL, "batch %d x %d heads x %d tokens is too large for one call", batch, n_q_heads, tokens);
   return FX_OK;
 }
@@ -1796,6 +1800,9 @@ int run_cached_attention(bool kv4, fx::CachedAttentionArgs& a, const long long* 
   if (!is_half_dtype(dtype)) return fail(FX_EINVAL, "dtype must be fp16 or bf16");
   if (!(a.scale > 0.f) || a.scale > 3.4e38f) return fail(FX_EINVAL, "scale must be positive and finite");
   if (a.B == 0 || a.T == 0) return FX_OK;
+  // no key lies beyond max_len, so neither a window nor sinks need to
+  a.window = std::min(a.window, a.L + 1);
+  a.sinks = std::min(a.sinks, a.L);
   if (!a.q || !a.out) return fail(FX_EINVAL, "q and out must be non-null");
   if (!aligned16(a.q) || !aligned16(a.out)) return fail(FX_EINVAL, "q and out must be 16-byte aligned");
   if (int rc = validate_strides("q", q_strides, kTokenRowLimit)) return rc;
@@ -1847,7 +1854,8 @@ int fx_window_attention(const void* q, const void* k, const void* v, void* out, 
   if (int rc = validate_attention_sizes(batch, n_q_heads, n_kv_heads, tokens, max_len, head_dim, window, sinks))
     return rc;
   if (!strides) return fail(FX_EINVAL, "strides must be non-null");
-  if (max_len > 0 && (!k || !v)) return fail(FX_EINVAL, "k and v must be non-null");
+  const bool reads = batch > 0 && tokens > 0 && max_len > 0;
+  if (reads && (!k || !v)) return fail(FX_EINVAL, "k and v must be non-null");
   if (!aligned16(k) || !aligned16(v)) return fail(FX_EINVAL, "k and v must be 16-byte aligned");
   if (int rc = validate_strides("k", strides + 3, kCacheRowLimit)) return rc;
   if (int rc = validate_strides("v", strides + 6, kCacheRowLimit)) return rc;
@@ -1879,7 +1887,7 @@ int fx_kv4_attention(const void* q, const void* k_codes, const void* k_scales, c
   if (int rc = validate_attention_sizes(batch, n_q_heads, n_kv_heads, tokens, max_len, head_dim, window, sinks))
     return rc;
   if (!strides) return fail(FX_EINVAL, "strides must be non-null");
-  if (max_len > 0)
+  if (batch > 0 && tokens > 0 && max_len > 0)
     if (int rc = validate_kv4_cache(k_codes, k_scales, v_codes, v_scales)) return rc;
   fx::CachedAttentionArgs a{};
   a.q = static_cast<const uint16_t*>(q);
@@ -1906,8 +1914,6 @@ int fx_kv4_append(const void* k, const void* v, const long long* strides, const 
                   int n_kv_heads, int tokens, int max_len, int head_dim, int dtype, void* stream) {
   if (int rc = validate_cache_sizes(batch, n_kv_heads, tokens, max_len, head_dim)) return rc;
   if (!is_half_dtype(dtype)) return fail(FX_EINVAL, "dtype must be fp16 or bf16");
-  if ((long long)(batch) * n_kv_heads * (tokens / 8 + 1) > (1LL << 30))
-    return fail(FX_EINVAL, "batch %d x %d heads x %d tokens is too large for one call", batch, n_kv_heads, tokens);
   if (!strides) return fail(FX_EINVAL, "strides must be non-null");
   if (int rc = validate_strides("k", strides, kTokenRowLimit)) return rc;
   if (int rc = validate_strides("v", strides + 3, kTokenRowLimit)) return rc;
@@ -1940,8 +1946,6 @@ int fx_kv4_restore(const void* k_codes, const void* k_scales, const void* v_code
   if (int rc = validate_cache_sizes(batch, n_kv_heads, rows, max_len, head_dim)) return rc;
   if (!is_half_dtype(dtype)) return fail(FX_EINVAL, "dtype must be fp16 or bf16");
   if (rows > max_len) return fail(FX_EINVAL, "rows must be in [0, max_len], got %d of %d", rows, max_len);
-  if ((long long)(batch) * n_kv_heads * (rows / 8 + 1) > (1LL << 30))
-    return fail(FX_EINVAL, "batch %d x %d heads x %d rows is too large for one call", batch, n_kv_heads, rows);
   if (batch == 0 || rows == 0) return FX_OK;
   if (int rc = validate_kv4_cache(k_codes, k_scales, v_codes, v_scales)) return rc;
   if (!k_out || !v_out) return fail(FX_EINVAL, "k_out and v_out must be non-null");

@@ -6,7 +6,8 @@
 //   (scale 0: code 0), standing for code * scale + minimum,
 // lo and hi the group's extremes; every step is one fp32 operation, so the codes are the
 // same wherever they are formed.  A group that holds a value beyond 2^15 in magnitude (where
-// code * scale + minimum could leave fp16), an infinity or a NaN stands for NaN.
+// code * scale + minimum could leave fp16), an infinity or a NaN stands for NaN: scale 0,
+// minimum NaN (the attention sizes its running maximum by the scales).
 // Codes: uint16 [16, D / 64] per position; word [c, g] holds columns 64 g + 4 c + k, k < 4,
 // in bits 4 k .. 4 k + 3.  (scale, minimum) fp16 [D / 64, 2].  So a lane that holds one word
 // of 16 neighbouring lanes' contiguous row has four columns of one group, and two words'
@@ -83,7 +84,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4AppendArgs a) 
         words |= unsigned(int(fminf(fmaxf(c, 0.f), 15.f))) << (4 * e);
       }
     }
-    const unsigned stored = bad > 0.f ? 0x7e007e00u : unsigned(scale_bits) | unsigned(min_bits) << 16;
+    const unsigned stored = bad > 0.f ? 0x7e000000u : unsigned(scale_bits) | unsigned(min_bits) << 16;
     // a unit's words of neighbouring groups share a dword: trade with the other group's lane
     unsigned dword = words;
     int at = y;

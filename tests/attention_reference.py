@@ -77,8 +77,8 @@ def quantize(x):
     inverse = torch.where(scale > 0, 1 / scale.float(), torch.zeros_like(lo))
     codes = ((groups - minimum.float()) * inverse).round().clamp(0, 15)
     bad = ~(groups.abs() <= 32768).all(-1, keepdim=True)
-    nan = torch.full_like(scale, float("nan"))
-    scale, minimum = torch.where(bad, nan, scale), torch.where(bad, nan, minimum)
+    scale = torch.where(bad, torch.zeros_like(scale), scale)
+    minimum = torch.where(bad, torch.full_like(minimum, float("nan")), minimum)
     value = codes.double() * scale.double() + minimum.double()
     return codes.flatten(-2).to(torch.uint8), scale[..., 0], minimum[..., 0], value.flatten(-2)
 

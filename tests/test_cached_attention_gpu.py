@@ -172,3 +172,323 @@ def test_new_cache_stands_for_zeros():
     assert cache.nbytes == 2 * 2 * 50 * (64 + 8)
     for x in cache.restore(dtype=HF):
         assert (x == 0).all()
+
+
+# ------------------------------------------------------------------ what a row does not see
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t", [5, 150])  # the few-rows and the rows kernel
+def test_infinities_stay_with_the_rows_that_see_them(dtype, d, t):
+    """One key's value holds +inf, another's -inf, a third's NaN, a fourth key is NaN: rows in
+    front of them are as if they were not there, rows that see a value's infinity have it."""
+    n, window, sinks = t + 60, 40, 2
+    q, k, v = make(dtype, 1, 1, 2, t, n, d)
+    spans = [(n, t)]
+    clean, mass, score = reference(q, k, v, spans, window, sinks, 1 / math.sqrt(d))
+    bound = bound16(clean, mass, score, dtype, n)
+    first = n - t
+    plus, minus, nan, key = first + 1, first + 2, first + 3, first + 4
+    v[0, 0, plus, 3], v[0, 0, minus, 3], v[0, 0, minus, 7], v[0, 0, nan, 9] = (
+        float("inf"), float("-inf"), float("-inf"), float("nan"))
+    k[0, 0, key, 11] = float("nan")
+    got = window_attention(q, k, v, window=window, sinks=sinks).double()
+    p = torch.arange(first, n, device="cuda")
+
+    def seen(j):
+        return ((j <= p) & (j > p - window))[None, :].expand(2, -1)
+
+    want = clean[0].clone()
+    inf = float("inf")
+    want[..., 3] = torch.where(seen(plus), inf, want[..., 3])
+    want[..., 3] = torch.where(seen(minus), want[..., 3] - inf, want[..., 3])  # both: NaN
+    want[..., 7] = torch.where(seen(minus), -inf, want[..., 7])
+    want[..., 9] = torch.where(seen(nan), float("nan"), want[..., 9])
+    want[seen(key)] = float("nan")
+    plain = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got[0]), torch.isnan(want))
+    assert torch.equal(got[0][torch.isinf(want)], want[torch.isinf(want)])
+    assert ((got[0] - want).abs()[plain] <= bound[0][plain]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("t", [4, 90])
+def test_kv4_nan_groups_stay_with_the_rows_that_see_them(dtype, t):
+    n, d = t + 40, 128
+    q, k, v = make(dtype, 1, 1, 2, t, n, d)
+    cache = Int4KVCache(1, 1, n, d)
+    cache.append(k, v, 0)
+    kv, (_, _, v_min, vv) = quantize(k)[3].cuda(), quantize(v)
+    want, _, score = reference(q, kv, vv.cuda(), [(n, t)], None, 0, 1 / math.sqrt(d))
+    bound = bound4(want, score, dtype, n, vv.abs().max().item(), v_min.double().abs().max().item())
+    at = n - t + 2
+    v[0, 0, at, 70] = float("inf")  # columns 64 .. 127 of that position stand for NaN
+    cache.append(k, v, 0)
+    got = kv4_attention(q, cache).double()
+    see = torch.arange(t, device="cuda") >= 2
+    assert torch.isnan(got[:, :, see, 64:]).all()
+    got[:, :, see, 64:] = want[:, :, see, 64:]
+    assert ((got - want).abs() <= bound).all()
+
+
+def test_a_row_of_minus_infinity_has_no_softmax():
+    """Every visible score -inf: NaN, as the formula; a row that sees no key: zeros."""
+    q, k, v = make(BF, 1, 1, 1, 2, 8, 64)
+    q.fill_(1.0)
+    k.fill_(float("-inf"))
+    got = window_attention(q, k, v, lengths=int32([1]))
+    assert (got[0, 0, 0] == 0).all() and torch.isnan(got[0, 0, 1]).all()
+
+
+# ------------------------------------------------------------------ how calls are made
+def test_lengths_are_clamped():
+    q, k, v = make(BF, 3, 2, 2, 6, 50, 64)
+    whole = window_attention(q, k, v, window=9)
+    out = torch.full_like(whole, 5.0)
+    window_attention(q, k, v, window=9, lengths=int32([1000, -4, 50]), query_lengths=int32([99, 6, -1]), out=out)
+    assert torch.equal(out[0], whole[0])
+    assert (out[1] == 0).all()
+    assert (out[2] == 5).all()
+
+
+def test_new_output_has_zeros_behind_the_queries():
+    q, k, v = make(HF, 2, 1, 2, 7, 30, 128)
+    got = window_attention(q, k, v, query_lengths=int32([7, 3]))
+    assert (got[1, :, 3:] == 0).all() and (got[1, :, :3] != 0).any()
+
+
+@pytest.mark.parametrize("layout", ["odd_start", "odd_stride", "column_step", "expanded", "negated"])
+def test_layouts(layout):
+    b, hk, g, t, n, d = 2, 2, 3, 20, 70, 64
+    q, k, v = make(HF, b, hk, g, t, n, d)
+    want = window_attention(q, k, v, window=30, sinks=3)
+
+    def odd(x):
+        if layout == "odd_start":
+            base = torch.empty(x.numel() + 3, dtype=x.dtype, device="cuda")
+            return base[3:].view(x.shape).copy_(x)
+        if layout == "odd_stride":
+            base = torch.empty(*x.shape[:-1], d + 5, dtype=x.dtype, device="cuda")
+            return base[..., :d].copy_(x)
+        base = torch.empty(*x.shape[:-1], 2 * d, dtype=x.dtype, device="cuda")
+        return base[..., ::2].copy_(x)
+
+    if layout == "expanded":  # one sequence's cache for the whole batch
+        k1, v1 = (x[:1].expand(b, -1, -1, -1) for x in (k, v))
+        want = window_attention(q, k1.contiguous(), v1.contiguous(), window=30, sinks=3)
+        assert torch.equal(window_attention(q, k1, v1, window=30, sinks=3), want)
+        return
+    if layout == "negated":
+        lazy = torch.complex(torch.zeros_like(q).contiguous(), -q.contiguous()).conj().imag
+        assert lazy.is_neg() and torch.equal(window_attention(lazy, k, v, window=30, sinks=3), want)
+        return
+    assert torch.equal(window_attention(odd(q), odd(k), odd(v), window=30, sinks=3), want)
+    cache, same = Int4KVCache(b, hk, n, d), Int4KVCache(b, hk, n, d)
+    cache.append(k, v, 0)
+    same.append(odd(k), odd(v), 0)
+    assert all(torch.equal(x, y) for x, y in zip(cache._parts(), same._parts()))
+
+
+def test_output_layouts():
+    q, k, v = make(BF, 2, 2, 2, 9, 40, 128)
+    want = window_attention(q, k, v)
+    heads_major = torch.empty(2, 4, 9, 128, dtype=BF, device="cuda")
+    assert torch.equal(window_attention(q, k, v, out=heads_major), want)
+    wide = torch.zeros(2, 4, 9, 160, dtype=BF, device="cuda")
+    assert torch.equal(window_attention(q, k, v, out=wide[..., :128]), want)
+    assert (wide[..., 128:] == 0).all()
+    for bad in (torch.empty(2, 4, 9, 130, dtype=BF, device="cuda")[..., 1:129],
+                torch.empty(1, 4, 9, 128, dtype=BF, device="cuda").expand(2, -1, -1, -1), heads_major.half(),
+                heads_major[:1], torch.empty(2, 4, 9, 128, dtype=BF)):
+        with pytest.raises(ValueError, match="out must have"):
+            window_attention(q, k, v, out=bad)
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(q=torch.zeros(1, 2, 64)), "shape"), (dict(window=0), "window"), (dict(window=2.0), "window"),
+    (dict(window=True), "window"), (dict(sinks=-1), "sinks"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
+    (dict(lengths=[3]), "lengths"), (dict(query_lengths=[1, 1]), "query_lengths"), (dict(heads=3), "multiple"),
+    (dict(dim=96), "head_dim"), (dict(v_len=9), "one shape"), (dict(k_dtype=HF), "share dtype"),
+    (dict(dtype=torch.float32), "fp16 or bf16"), (dict(batch=2), "batch"), (dict(grad=True), "no backward")])
+def test_refusals(change, message):
+    b, dt, d = 1, change.get("dtype", BF), change.get("dim", 64)
+    heads = change.get("heads", 4)
+    q = torch.zeros(change.get("batch", b), heads, 1, d, dtype=dt, device="cuda")
+    k = torch.zeros(b, 2, 10, d, dtype=change.get("k_dtype", dt), device="cuda")
+    v = torch.zeros(b, 2, change.get("v_len", 10), d, dtype=dt, device="cuda")
+    if "q" in change:
+        q = change["q"].to(dt).cuda()
+    kw = {n: change[n] for n in ("window", "sinks", "scale") if n in change}
+    for n in ("lengths", "query_lengths"):
+        if n in change:
+            kw[n] = torch.tensor(change[n], device="cuda")  # int64
+    if "grad" in change:
+        q.requires_grad_()
+    with pytest.raises((ValueError, TypeError), match=message):
+        window_attention(q, k, v, **kw)
+    if "grad" in change:
+        with torch.no_grad():
+            window_attention(q, k, v)
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(start=-1), "start"), (dict(start=1.5), "start"), (dict(start=[0, 0]), "start"), (dict(counts=[1.0]), "counts"),
+    (dict(heads=3), "of the cache"), (dict(batch=2), "of the cache"), (dict(v_len=3), "share their shape"),
+    (dict(dtype=torch.float32), "fp16 or bf16"), (dict(v_dtype=HF), "share dtype"), (dict(device="cpu"), "GPU"),
+    (dict(grad=True), "no backward")])
+def test_append_refusals(change, message):
+    cache = Int4KVCache(1, 2, 20, 64)
+    kw = dict(device=change.get("device", "cuda"), dtype=change.get("dtype", BF))
+    k = torch.zeros(change.get("batch", 1), change.get("heads", 2), 4, 64, **kw)
+    v = torch.zeros(k.shape[0], k.shape[1], change.get("v_len", 4), 64, **kw).to(change.get("v_dtype", kw["dtype"]))
+    if "grad" in change:
+        k.requires_grad_()
+    start = change.get("start", 0)
+    start = torch.tensor(start, device="cuda") if isinstance(start, list) else start
+    counts = torch.tensor(change["counts"], device="cuda") if "counts" in change else None
+    with pytest.raises(ValueError, match=message):
+        cache.append(k, v, start, counts=counts)
+    assert all((x == 0).all() for x in cache._parts())
+
+
+def test_cache_refusals():
+    cache = Int4KVCache(1, 2, 20, 64)
+    for bad in (dict(length=21), dict(length=-1), dict(length=True), dict(dtype=torch.float32)):
+        with pytest.raises(ValueError):
+            cache.restore(**bad)
+    q = torch.zeros(1, 4, 1, 128, dtype=BF, device="cuda")
+    with pytest.raises(ValueError, match="head_dim"):
+        kv4_attention(q, cache)
+    with pytest.raises(ValueError, match="multiple"):
+        kv4_attention(q[:, :3, :, :64], cache)
+    with pytest.raises(ValueError, match="GPU"):
+        kv4_attention(q.cpu(), cache)
+
+
+def test_empty_batches_and_calls():
+    q, k, v = make(BF, 2, 1, 2, 3, 8, 64)
+    assert window_attention(q[:, :, :0], k, v).shape == (2, 2, 0, 64)
+    assert window_attention(q[:0], k[:0], v[:0]).shape == (0, 2, 3, 64)
+    assert (window_attention(q, k[:, :, :0], v[:, :, :0]) == 0).all()
+
+
+# ------------------------------------------------------------------ large addresses
+def test_offsets_past_four_gib():
+    """A 16-bit cache of 5 GiB and a 4-bit one of 4.7 GB: the last sequence lies past 2^32 bytes."""
+    b, hk, n, d = 10, 8, 131072, 128
+    k = torch.zeros(b, hk, n, d, dtype=BF, device="cuda")
+    v = torch.zeros(b, hk, n, d, dtype=BF, device="cuda")
+    assert k.numel() * 2 > 2**31
+    q, kk, vv = make(BF, 1, hk, 4, 1, 200, d)
+    k[-1:, :, -200:], v[-1:, :, -200:] = kk, vv
+    lengths = torch.full((b,), n, dtype=torch.int32, device="cuda")
+    got = window_attention(q.expand(b, -1, -1, -1), k, v, lengths=lengths, window=200)
+    want, mass, score = reference(q, kk, vv, [(200, 1)], None, 0, 1 / math.sqrt(d))
+    assert ((got[-1:].double() - want).abs() <= bound16(want, mass, score, BF, 200)).all()
+    assert (got[:-1] == 0).all()
+    del k, v
+    b = 30
+    cache = Int4KVCache(b, hk, n, d)
+    assert cache.k_codes.numel() > 2**30 and cache.k_codes[-1].data_ptr() - cache.k_codes.data_ptr() > 1.9e9
+    start = torch.full((b,), n, dtype=torch.int32, device="cuda")
+    start[-1] = n - 200
+    cache.append(kk.expand(b, -1, -1, -1), vv.expand(b, -1, -1, -1), start)  # only the last one's positions exist
+    got = kv4_attention(q.expand(b, -1, -1, -1), cache, window=200)
+    small = Int4KVCache(1, hk, 200, d)
+    small.append(kk, vv, 0)
+    assert all(torch.equal(x[-1:, :, -200:], y) for x, y in zip(cache._parts(), small._parts()))
+    kv, vm = quantize(kk)[3].cuda(), quantize(vv)
+    want, _, score = reference(q, kv, vm[3].cuda(), [(200, 1)], None, 0, 1 / math.sqrt(d))
+    bound = bound4(want, score, BF, 200, vm[3].abs().max().item(), vm[2].double().abs().max().item())
+    assert ((got[-1:].double() - want).abs() <= bound).all()
+    assert (got[:-1] == 0).all()
+
+
+# ------------------------------------------------------------------ streams, graphs, a run of them together
+def test_results_do_not_depend_on_the_stream_or_the_time():
+    q, k, v = make(BF, 4, 2, 4, 1, 3000, 128)
+    want = window_attention(q, k, v)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        outs = [window_attention(q, k, v) for _ in range(20)]
+    here = [window_attention(q, k, v) for _ in range(20)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in outs + here)
+
+
+def _decode(cache, q, k, v, lengths, out, window, sinks):
+    """One step: the new token into the cache at its position, then its attention."""
+    cache.append(k, v, lengths - 1)
+    return kv4_attention(q, cache, lengths=lengths, window=window, sinks=sinks, out=out)
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (64, 4)])
+def test_prompt_then_decode_on_the_cache(window, sinks):
+    """As they are used: a padded batch's prompts are attended in 16 bits and appended, then
+    decode steps append a token and attend to the 4-bit cache; each step eagerly, and as one
+    captured graph that is replayed with other lengths and tokens."""
+    b, hk, g, d, prompt, steps, length = 2, 2, 4, 128, 70, 6, 100
+    q, k, v = make(BF, b, hk, g, prompt, prompt, d)
+    counts = int32([70, 41])
+    first = window_attention(q, k, v, lengths=counts, query_lengths=counts, window=window, sinks=sinks)
+    assert (first[1, :, 41:] == 0).all()
+    cache, replayed = Int4KVCache(b, hk, length, d), Int4KVCache(b, hk, length, d)
+    for c in (cache, replayed):
+        c.append(k, v, 0, counts=counts)
+    tokens = [make(BF, b, hk, g, 1, 1, d, seed=100 + i) for i in range(steps)]
+    values = [[quantize(k)[3][i, :, :n], quantize(v)[3][i, :, :n]] for i, n in enumerate((70, 41))]
+
+    at = counts.clone()
+    sq, sk, sv = (torch.empty_like(x) for x in tokens[0])
+    out = torch.empty(b, hk * g, 1, d, dtype=BF, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        spare = Int4KVCache(b, hk, length, d)
+        _decode(spare, tokens[0][0], tokens[0][1], tokens[0][2], at + 1, out, window, sinks)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _decode(replayed, sq, sk, sv, at, out, window, sinks)
+
+    for i, (nq, nk, nv) in enumerate(tokens):
+        at.add_(1)
+        eager = _decode(cache, nq, nk, nv, at.clone(), None, window, sinks)
+        for dst, src in ((sq, nq), (sk, nk), (sv, nv)):
+            dst.copy_(src)
+        out.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        assert all(torch.equal(x, y) for x, y in zip(cache._parts(), replayed._parts()))
+        for s in range(b):
+            values[s] = [torch.cat((old, quantize(x)[3][s]), 1) for old, x in zip(values[s], (nk, nv))]
+            n = values[s][0].shape[1]
+            kk, vv = (x[None].cuda() for x in values[s])
+            want, _, score = reference(nq[s:s + 1], kk, vv, [(n, 1)], window, sinks, 1 / math.sqrt(d))
+            low = torch.cat([quantize(v)[2][s].flatten()] + [quantize(t[2])[2][s].flatten() for t in tokens])
+            bound = bound4(want, score, BF, n, vv.abs().max().item(), low.double().abs().max().item())
+            assert ((eager[s:s + 1].double() - want).abs() <= bound).all(), (i, s)
+
+
+@pytest.mark.parametrize("t", [1, 40])
+def test_two_captured_calls_share_nothing(t):
+    """Two graphs of split calls, replayed in turn and interleaved with eager work."""
+    ins = [make(BF, 1, 2, 4, t, 2000, 128, seed=s) for s in (0, 50)]
+    want = [window_attention(*x) for x in ins]
+    outs = [torch.empty_like(w) for w in want]
+    graphs = []
+    for x, out in zip(ins, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            window_attention(*x, out=out)
+        graphs.append(graph)
+    for order in ((0, 1), (1, 0), (0, 0, 1, 1), (1, 1, 0)):
+        for out in outs:
+            out.zero_()
+        for i in order:
+            graphs[i].replay()
+        other = window_attention(*ins[order[0]])
+        torch.cuda.synchronize()
+        assert torch.equal(other, want[order[0]])
+        assert all(torch.equal(x, y) for x, y in zip(outs, want))
