@@ -32,7 +32,8 @@ import time
 import torch
 
 from . import _lib
-from .fused_modules import add_rms_norm
+from .cached_attention import Int4KVCache, kv4_attention, window_attention
+from .fused_modules import add_rms_norm, head_norm_rope
 from .static_decode import graph_kernel_count
 from .deployment import HybridSegmentsGemv, PackedHybridLinear
 from .w3_lut_deployment import PackedW3Linear, W3Gemv
@@ -437,7 +438,15 @@ class _ResidualStream:
 
 
 class NativeDecodeSession:
-    def __init__(self, model, input_ids: torch.Tensor, forced_tokens: torch.Tensor, w3_payload: str = "fields"):
+    """``kv_cache="int4"`` holds the keys and values in an :class:`Int4KVCache` per layer (the
+    prefix quantized after its prefill, each token as it is decoded); ``window`` / ``sinks``
+    let a decoded token see the last ``window`` keys and the first ``sinks`` ones only (the
+    prefix is prefilled by the model, over all of its keys).  Either takes the attention of
+    ``cached_attention`` behind one launch for the q/k norms and RoPE, in place of the fused
+    ``fx_decode_attention_rope``."""
+
+    def __init__(self, model, input_ids: torch.Tensor, forced_tokens: torch.Tensor, w3_payload: str = "fields",
+                 kv_cache: str = "16bit", window: int | None = None, sinks: int = 0):
         from transformers import StaticCache
 
         if input_ids.ndim != 2 or input_ids.shape[0] != 1 or input_ids.shape[1] < 2:
@@ -454,7 +463,14 @@ class NativeDecodeSession:
         dtype = model.model.embed_tokens.weight.dtype
         if dtype not in (torch.bfloat16, torch.float16):
             raise ValueError("native decode needs a bf16 or fp16 model")
+        if kv_cache not in ("16bit", "int4"):
+            raise ValueError(f"kv_cache must be '16bit' or 'int4', got {kv_cache!r}")
+        if window is not None and (type(window) is not int or window < 1):
+            raise ValueError("window must be None or a positive integer")
+        if type(sinks) is not int or sinks < 0:
+            raise ValueError("sinks must be a non-negative integer")
         self.model, self.dtype, self.device = model, dtype, input_ids.device
+        self.window, self.sinks = window, sinks
         self.ids = input_ids
         self.tokens = forced_tokens.to(self.device).contiguous()
         self.steps = self.tokens.shape[1]
@@ -473,8 +489,12 @@ class NativeDecodeSession:
             out = model(input_ids=input_ids, past_key_values=cache, use_cache=True, logits_to_keep=1)
             self.prefill_logits = out.logits[:, -1, :].detach().clone()
             shape = (n, self.kv_heads, self.maximum_length, self.head_dim)
-            self.k_cache = torch.zeros(shape, dtype=dtype, device=self.device)
-            self.v_cache = torch.zeros(shape, dtype=dtype, device=self.device)
+            self.int4_cache = self.k_cache = self.v_cache = None
+            if kv_cache == "int4":
+                self.int4_cache = [Int4KVCache(1, *shape[1:], device=self.device) for _ in range(n)]
+            else:
+                self.k_cache = torch.zeros(shape, dtype=dtype, device=self.device)
+                self.v_cache = torch.zeros(shape, dtype=dtype, device=self.device)
             self.prefix_k = torch.stack([l.keys[0, :, :self.prefix_length] for l in cache.layers]).clone()
             self.prefix_v = torch.stack([l.values[0, :, :self.prefix_length] for l in cache.layers]).clone()
             # cos/sin rows for every position, built by the model's own rotary module
@@ -530,8 +550,18 @@ class NativeDecodeSession:
                 and self.hidden % 512 == 0 and self.hidden <= 8192):
             self.lm_ws = torch.empty(lib.fx_lm_head_argmax_workspace_bytes(), dtype=torch.uint8,
                                      device=self.device)  # per-workgroup argmax partials
-        nbytes = lib.fx_decode_attention_workspace_bytes(self.heads, self.maximum_length, self.head_dim)
-        self.attn_ws = torch.empty(nbytes // 4 + 64, dtype=torch.float32, device=self.device)  # split partials
+        self.fused_attention = kv_cache == "16bit" and window is None
+        if self.fused_attention:
+            nbytes = lib.fx_decode_attention_workspace_bytes(self.heads, self.maximum_length, self.head_dim)
+            self.attn_ws = torch.empty(nbytes // 4 + 64, dtype=torch.float32, device=self.device)  # split partials
+        else:
+            # normalised and rotated q and k of the token, and its length in the cache
+            self.q_rope = torch.empty(1, self.heads, 1, self.head_dim, dtype=dtype, device=self.device)
+            self.k_rope = torch.empty(1, self.kv_heads, 1, self.head_dim, dtype=dtype, device=self.device)
+            self.heads_out = torch.empty_like(self.q_rope)
+            self.lengths = torch.arange(1, self.maximum_length + 1, dtype=torch.int32, device=self.device)
+            indexes = self.stream.o_index if self.stream is not None and self.stream.o_index else [None] * n
+            self.o_index_long = [None if index is None else index.long() for index in indexes]
         self.graph = None
         self.kernel_nodes = None
         self.launches_per_step = None
@@ -540,10 +570,40 @@ class NativeDecodeSession:
         self.layer_observer = None
 
     # -- one token -------------------------------------------------------------------
+    def _cached_attention(self, layer, pos, out_index):
+        """The q/k norms and RoPE (one launch, a 16-bit cache's position ``pos`` written by it;
+        a 4-bit cache's by one more), then the windowed or 4-bit attention."""
+        d = self.head_dim
+        heads = (1, -1, 1, d)
+        k, v = self.k.view(heads), self.v.view(heads)
+        k_out, v_out = self.k_rope, v
+        if self.int4_cache is None:
+            k_out, v_out = (x[layer, None, :, pos:pos + 1] for x in (self.k_cache, self.v_cache))
+        rows = [(self.q.view(heads), self.q_rope, self.q_norm[layer], self.heads),
+                (k, k_out, self.k_norm[layer], self.kv_heads)]
+        if self.int4_cache is None:
+            rows.append((v, v_out, None, self.kv_heads))
+        head_norm_rope([{"x": x, "out": out, "weight": weight, "heads": count, "rope": weight is not None,
+                         "in_strides": x.stride()[:3], "out_strides": out.stride()[:3]}
+                        for x, out, weight, count in rows],
+                       cos=self.cos[pos], sin=self.sin[pos], eps=self.eps)
+        out = self.attn.view(heads) if out_index is None else self.heads_out
+        kw = dict(lengths=self.lengths[pos:pos + 1], window=self.window, sinks=self.sinks, scale=self.scale, out=out)
+        if self.int4_cache is not None:
+            cache = self.int4_cache[layer]
+            cache.append(self.k_rope, v, pos)
+            kv4_attention(self.q_rope, cache, **kw)
+        else:
+            window_attention(self.q_rope, self.k_cache[layer, None], self.v_cache[layer, None], **kw)
+        if out_index is not None:
+            self.attn.view(-1).index_copy_(0, self.o_index_long[layer], out.view(-1))
+
     def _attention(self, layer, pos, out_index=None):
         """q/k RMSNorm + RoPE, the KV-cache write of position ``pos`` and the
         attention, from the raw q|k|v projections (one launch at decode lengths);
         ``out_index``: the output in the o projection's sorted column order."""
+        if not self.fused_attention:
+            return self._cached_attention(layer, pos, out_index)
         lib = self.lib
         _lib.check(lib.fx_decode_attention_rope(
             self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), self.q_norm[layer].data_ptr(),
@@ -653,6 +713,10 @@ class NativeDecodeSession:
     # -- session protocol --------------------------------------------------------------
     @torch.inference_mode()
     def reset(self):
+        if self.int4_cache is not None:
+            for cache, k, v in zip(self.int4_cache, self.prefix_k, self.prefix_v):
+                cache.append(k[None], v[None], 0)
+            return
         self.k_cache.zero_()
         self.v_cache.zero_()
         self.k_cache[:, :, :self.prefix_length].copy_(self.prefix_k)
