@@ -47,6 +47,18 @@ __device__ __forceinline__ float half_pair_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The same over the four lanes l, l ^ 16, l ^ 32 and l ^ 48.
+__device__ __forceinline__ float quarter_max(float v) {
+  const unsigned u = __float_as_uint(v);
+  const u32x2_t r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return half_pair_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarter_sum(float v) {
+  const unsigned u = __float_as_uint(v);
+  const u32x2_t r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return half_pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
 // Two 16-bit values of one word: nonzero iff either is an infinity or a NaN (the exponent
 // field, all ones, carries into its sign bit).
 template <int DT>

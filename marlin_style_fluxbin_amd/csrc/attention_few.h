@@ -28,6 +28,8 @@
 
 namespace fx {
 
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+
 // The tile in registers: what this lane's operands need of 32 keys.
 template <int D, bool KV4>
 struct FewTile {
@@ -96,43 +98,53 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) qf[rt][s] = *reinterpret_cast<const u32x4_t*>(q + 32 * s + 8 * h4);
     } else {
-      // columns 64 g + 16 h4 .. + 15 of every group, scaled by a power of two so that the
-      // row's largest magnitude lies in [2^9, 2^10); step (g, half): word r holds nibble r of
-      // units 4 h4 + 2 half and the next, odd nibbles 2^-4 for their place in the byte
-      float v[kGroups][16], mag = 0.f;
+      // columns 64 g + 16 h4 .. + 15 of every group, in fp16 and scaled by a power of two so
+      // that the row's largest magnitude lies in [2^9, 2^10); step (g, half): word r holds
+      // nibble r of units 4 h4 + 2 half and the next, odd nibbles 2^-4 for their place in the
+      // byte.  On packed halves: every wave prepares its rows, and of a short split's time
+      // that is a large part.
+      unsigned w[kGroups][8];
+      u16x2_t big = {0, 0};
 #pragma unroll
       for (int gg = 0; gg < kGroups; ++gg)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const u32x4_t w = *reinterpret_cast<const u32x4_t*>(q + 64 * gg + 16 * h4 + 8 * c);
+          const u32x4_t x = *reinterpret_cast<const u32x4_t*>(q + 64 * gg + 16 * h4 + 8 * c);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v[gg][8 * c + e] = to_f32<QDT>(uint16_t(w[e >> 1] >> (16 * (e & 1))));
-            mag = fmaxf(mag, fabsf(v[gg][8 * c + e]));
+          for (int i = 0; i < 4; ++i) {
+            w[gg][4 * c + i] = x[i];
+            big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2_t, x[i] & 0x7fff7fffu));
           }
         }
-      mag = fmaxf(mag, __shfl_xor(mag, 16, 64));
-      mag = fmaxf(mag, __shfl_xor(mag, 32, 64));
+      const float mag = quarter_max(to_f32<QDT>(max(big[0], big[1])));
       const int shift = mag > 0.f && mag < INFINITY ? 10 - __builtin_amdgcn_frexp_expf(mag) : 0;
       f[rt] = ldexpf(f[rt], -shift);
+      const _Float16 once = _Float16(ldexpf(1.f, shift >> 1)), again = _Float16(ldexpf(1.f, shift - (shift >> 1)));
 #pragma unroll
       for (int gg = 0; gg < kGroups; ++gg) {
         float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          v[gg][e] = f16_bits_to_f32(f32_to_f16_bits(ldexpf(v[gg][e], shift)));
-          sum += v[gg][e];
+        for (int i = 0; i < 8; ++i) {
+          f16x2_t v;
+          if constexpr (QDT == kF16) {  // shift -6 .. 33: in two steps, exact unless down into the subnormals
+            v = __builtin_bit_cast(f16x2_t, w[gg][i]) * once * again;
+          } else {
+            v = __builtin_convertvector(f32x2_t{ldexpf(__uint_as_float(w[gg][i] << 16), shift),
+                                                ldexpf(__uint_as_float(w[gg][i] & 0xffff0000u), shift)},
+                                        f16x2_t);
+          }
+          sum = __builtin_amdgcn_fdot2(v, f16x2_t{1, 1}, sum, false);
+          w[gg][i] = __builtin_bit_cast(unsigned, v);
         }
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        qsum[rt][gg] = sum * f[rt];
+        qsum[rt][gg] = quarter_sum(sum) * f[rt];
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float place = r & 1 ? 0.0625f : 1.f;
+            const unsigned pair = __builtin_amdgcn_perm(w[gg][4 * half + 2 + r / 2], w[gg][4 * half + r / 2],
+                                                        r & 1 ? 0x07060302u : 0x05040100u);
             qf[rt][2 * gg + half][r] =
-                f32x2_to_f16x2_bits(v[gg][8 * half + r] * place, v[gg][8 * half + 4 + r] * place);
+                r & 1 ? __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2_t, pair) * _Float16(0.0625f)) : pair;
           }
       }
       f[rt] = ldexpf(f[rt], 24);  // the codes' 2^-24
@@ -253,13 +265,12 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
 
   auto half_of = [](unsigned w, int i) { return f16_bits_to_f32(uint16_t(i ? w >> 16 : w)); };
 
-  // running maximum of row tile rt: `bound` holds what it runs over
-  auto raise = [&](int rt, const float(&bound)[8]) __attribute__((always_inline)) {
+  // running maximum of row tile rt: over `bound`, all by `less` too large
+  auto raise = [&](int rt, const float(&bound)[8], float less) __attribute__((always_inline)) {
     float top = bound[0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) top = fmaxf(top, bound[e]);
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    top = quarter_max(top) - less;
     if (__builtin_amdgcn_ballot_w64(top > m[rt])) {
       const float before = m[rt];
       m[rt] = fmaxf(before, top);
@@ -278,6 +289,7 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
     return TileMask(p[rt], a.window, a.sinks, sink_tile, tiles.joined);
   };
   auto hide = [&](int rt, int j0, bool sink_tile, float(&s)[8]) __attribute__((always_inline)) {
+    asm volatile("");  // a branch: not worked out for the tiles that every row sees
     const TileMask seen = mask(rt, sink_tile);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e] = seen.sees(j0 + 16 * (e >> 2) + 4 * h4 + (e & 3)) ? s[e] : -INFINITY;
@@ -298,7 +310,7 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
         for (int r = 0; r < 4; ++r) s[4 * u + r] = c[r] * f[rt];
       }
       if (!whole) hide(rt, j0, sink_tile, s);
-      raise(rt, s);
+      raise(rt, s, 0.f);
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         float p0 = __builtin_amdgcn_exp2f(s[e] - m_use[rt]), p1 = __builtin_amdgcn_exp2f(s[e + 1] - m_use[rt]);
@@ -393,9 +405,8 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const unsigned w = ks[r * kGroups + gg];
-            acc[rt][r] = gg == 0 ? half_of(w, 0) * c[r] : __builtin_fmaf(half_of(w, 0), c[r], acc[rt][r]);
-            low[rt][r] = gg == 0 ? half_of(w, 1) * qsum[rt][gg]
-                                 : __builtin_fmaf(half_of(w, 1), qsum[rt][gg], low[rt][r]);
+            acc[rt][r] = __builtin_fmaf(half_of(w, 0), c[r], gg == 0 ? 0.f : acc[rt][r]);
+            low[rt][r] = __builtin_fmaf(half_of(w, 1), qsum[rt][gg], gg == 0 ? 0.f : low[rt][r]);
           }
         }
       }
@@ -405,7 +416,7 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
         for (int r = 0; r < 4; ++r) s[rt][4 * u + r] = __builtin_fmaf(acc[rt][r], f[rt], low[rt][r]);
     }
     unsigned vs[2][4 * kGroups];
-    float size[8];  // log2 of the keys' largest value scales, rounded down, -15 .. 16
+    float size[8];  // 2^10 (15 + log2 of the keys' largest value scales, rounded down)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -416,10 +427,11 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        unsigned big = 0;
+        u16x2_t big = {0, 0};  // of the low halves, all positive
 #pragma unroll
-        for (int gg = 0; gg < kGroups; ++gg) big = max(big, vs[u][r * kGroups + gg] & 0x7fffu);
-        size[4 * u + r] = float(int(big >> 10) - 15);
+        for (int gg = 0; gg < kGroups; ++gg)
+          big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2_t, vs[u][r * kGroups + gg]));
+        size[4 * u + r] = float(__builtin_bit_cast(unsigned, big) & 0x7c00u);
       }
     }
     float pr[RT][8];
@@ -428,46 +440,62 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
       if (!whole) hide(rt, j0, sink_tile, s[rt]);
       float bound[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) bound[e] = s[rt][e] + size[e];
-      raise(rt, bound);
+      for (int e = 0; e < 8; ++e) bound[e] = __builtin_fmaf(size[e], 0x1p-10f, s[rt][e]);
+      raise(rt, bound, 15.f);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         pr[rt][e] = __builtin_amdgcn_exp2f(s[rt][e] - m_use[rt]);
         l[rt] += pr[rt][e];
       }
     }
+    // the groups' weights, of all groups together where registers allow
+    constexpr int kAtOnce = kGroups == 2 ? 2 : 1;
+    u32x4_t pf[RT][kGroups];
+    const auto weigh = [&](int g0, auto all) __attribute__((always_inline)) {
 #pragma unroll
-    for (int gg = 0; gg < kGroups; ++gg) {
-      u32x4_t pf[RT];
-      const auto weigh = [&](auto all) __attribute__((always_inline)) {
+      for (int gg = g0; gg < g0 + kAtOnce; ++gg)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
             const unsigned w0 = vs[e >> 2][(e & 3) * kGroups + gg], w1 = vs[e >> 2][((e & 3) + 1) * kGroups + gg];
             const float p0 = pr[rt][e], p1 = pr[rt][e + 1];
             float s0 = p0 * half_of(w0, 0), s1 = p1 * half_of(w1, 0);
-            float low0 = p0 * half_of(w0, 1), low1 = p1 * half_of(w1, 1);
-            if constexpr (!decltype(all)::value) {  // a hidden key's pair may be anything
+            float low = omin[rt][gg];
+            if constexpr (decltype(all)::value) {
+              low = __builtin_fmaf(p0, half_of(w0, 1), low);
+              low = __builtin_fmaf(p1, half_of(w1, 1), low);
+            } else {  // a hidden key's pair may be anything
               s0 = p0 == 0.f ? 0.f : s0;
-              low0 = p0 == 0.f ? 0.f : low0;
+              low += p0 == 0.f ? 0.f : p0 * half_of(w0, 1);
               s1 = p1 == 0.f ? 0.f : s1;
-              low1 = p1 == 0.f ? 0.f : low1;
+              low += p1 == 0.f ? 0.f : p1 * half_of(w1, 1);
             }
-            pf[rt][e / 2] = f32x2_to_f16x2_bits(s0, s1);
-            omin[rt][gg] += low0 + low1;
+            const unsigned rounded = f32x2_to_f16x2_bits(s0, s1);
             if constexpr (QDT == kF16) {
               // what the rounding of p * scale took away, at the codes' middle: the rounding
               // then weighs codes - 8, the value's own size, in place of codes (0 .. 15).
               // Below a bf16 output's own rounding either way.
-              const float lost = (s0 - half_of(pf[rt][e / 2], 0)) + (s1 - half_of(pf[rt][e / 2], 1));
-              omin[rt][gg] = __builtin_fmaf(8.f, lost, omin[rt][gg]);
+              const float lost = (s0 - half_of(rounded, 0)) + (s1 - half_of(rounded, 1));
+              low = __builtin_fmaf(8.f, lost, low);
             }
+            pf[rt][gg][e / 2] = rounded;
+            omin[rt][gg] = low;
           }
-        }
-      };
-      if (whole || !careful) weigh(std::true_type{});
-      else weigh(std::false_type{});
+    };
+    const auto weigh_from = [&](int g0) __attribute__((always_inline)) {
+      if (whole || !careful) {
+        asm volatile("");  // two paths, neither worked out for the other
+        weigh(g0, std::true_type{});
+      } else {
+        asm volatile("");
+        weigh(g0, std::false_type{});
+      }
+    };
+    if constexpr (kAtOnce > 1) weigh_from(0);
+#pragma unroll
+    for (int gg = 0; gg < kGroups; ++gg) {
+      if constexpr (kAtOnce == 1) weigh_from(gg);
       // this group's four columns of the chunk: nibble i of word gg
       unsigned ab[4], hi[4];
 #pragma unroll
@@ -483,7 +511,7 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
 #pragma unroll
         for (int c = 0; c < 4; ++c) vf[c] = (i & 2 ? hi[c] : ab[c]) & mask;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][4 * gg + i] = mfma16<CDT>(vf, pf[rt], o[rt][4 * gg + i]);
+        for (int rt = 0; rt < RT; ++rt) o[rt][4 * gg + i] = mfma16<CDT>(vf, pf[rt][gg], o[rt][4 * gg + i]);
       }
     }
     wave_lds_order();  // the pairs are read before the next tile's are written
@@ -539,14 +567,10 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
   // ---- the key waves' joins: O^T row 4 h4 + r, index i
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    l[rt] += __shfl_xor(l[rt], 16, 64);
-    l[rt] += __shfl_xor(l[rt], 32, 64);
+    l[rt] = quarter_sum(l[rt]);
     if constexpr (KV4) {
 #pragma unroll
-      for (int gg = 0; gg < kGroups; ++gg) {
-        omin[rt][gg] += __shfl_xor(omin[rt][gg], 16, 64);
-        omin[rt][gg] += __shfl_xor(omin[rt][gg], 32, 64);
-      }
+      for (int gg = 0; gg < kGroups; ++gg) omin[rt][gg] = quarter_sum(omin[rt][gg]);
     }
     if (h4 == 0) {
       red_ml[wave][0][16 * rt + l16] = m[rt];
