@@ -64,6 +64,39 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(const CachedAtte
   }
 }
 
+// How many splits of the keys: more shorten every workgroup's way until the chip is full, and
+// cost the join's launch and the partial results, written and read.  The times (us) are those
+// of 30 sizes measured with 1 .. 64 splits; the choice is within 10% of the best at nearly all
+// of them.  Splits until the chip is full, whatever the join costs, took up to 60% longer: 301
+// tokens of 14 heads of 64 columns, window 257, 18.3 us (2 splits) for 12.6 (1); 300 tokens
+// of 16 heads of 256 columns over 2000 keys 52.6 us (13) for 38.1 (6); 24 sequences' tokens over
+// a window of 4096 keys 83 us (6) for 74 (1).
+struct SplitTimes {
+  long groups, tiles;  // workgroups of a split, key tiles
+  int waves;           // of a workgroup along the keys
+  int slots;           // workgroups that run at once, each at the speed of one alone
+  float tile;          // a wave's key tile
+  float shared;        // 0: further workgroups wait; else they run beside these, `slots` more in `shared` of their time
+  float memory;        // reading the cache once
+  float tail;          // how much of a workgroup's time is waited for at the end (no window: lengths that differ)
+  float join, join_split;
+};
+int best_splits(const SplitTimes& t, long most) {
+  float best = 0.f;
+  int splits = 1;
+  for (int s = 1; s <= most; s += s < 8 ? 1 : s < 16 ? 2 : s < 32 ? 4 : 8) {
+    const float per = std::max(1.f, float(t.tiles) / float(s * t.waves));
+    const long rounds = (t.groups * s + t.slots - 1) / t.slots;
+    const float one = t.tile * per;
+    const float work = one * (rounds == 1 ? 1.f : t.shared > 0.f ? t.shared * rounds : float(rounds));
+    const float time = std::max(work, t.memory) + t.tail * one + (s > 1 ? t.join + t.join_split * s : 0.f) +
+                       (s > 16 ? 1.5f : 0.f);  // the join's four-wave form
+    if (s == 1 || time < best) best = time, splits = s;
+    if (per == 1.f) break;
+  }
+  return splits;
+}
+
 // Which kernel: up to 16 query rows of a KV head fit one operand of the few-rows kernel.  A
 // 4-bit cache keeps it for up to 64 rows (5 tokens of 7 heads over 4101 keys of 8 sequences
 // of 4 KV heads: 23 us, the rows kernel 25 us on half as exact fp16 results), and always for
@@ -89,17 +122,30 @@ CachedAttentionPlan plan_cached_attention(int dt, int B, int Hk, int G, int T, i
   long keys = L;
   if (window > 0) keys = std::min<long>(L, long(sinks) + window + tokens - 1 + 2 * kt);
   const long tiles = (keys + kt - 1) / kt;
-  // Key splits until the chip is full, each with a tile for every wave (four tiles in the
-  // rows kernel, whose first one's latency is not hidden).  Full is, measured over 256 to
-  // 2048 workgroups: 512 of the rows kernel (two a CU, LDS and registers); 1024 of the
-  // few-rows kernel (24 sequences, 4096 keys of 16 bits: 83 us, 512 or 2048 87 us), 2048 over
-  // a 4-bit cache (32 sequences of 32768 keys: 198 us, 1024 226, 512 219: ragged lengths even
-  // out); 256 with several row groups (35 rows: 31 us, 128 39, 512 39 us).
-  const long target = !plan.few ? 512 : rows > 16 ? 256 : kv4 ? 2048 : 1024;
-  const long smallest = plan.few ? plan.waves / plan.row_groups : 4;
   const long groups = heads * plan.row_tiles;
-  const long splits = std::min((target + groups - 1) / groups, (tiles + smallest - 1) / smallest);
-  plan.splits = int(std::max<long>(1, std::min<long>(splits, kMaxAttentionSplits)));
+  SplitTimes t{};
+  t.groups = groups;
+  t.tiles = tiles;
+  t.waves = plan.few ? plan.waves / plan.row_groups : 1;
+  t.join = 3.5f;
+  t.join_split = float(heads * rows) * D * 8 / 4e6f;
+  if (!plan.few) {
+    t.tile = (D == 64 ? 1.f : 1.2f) * (kv4 ? 1.25f : 1.f);
+    t.slots = 256;
+    t.shared = 0.83f;
+    t.join = 5.f;
+  } else if (rows > 16) {
+    t.tile = D == 64 ? 1.5f : 2.4f;
+    t.slots = 256;
+  } else {
+    t.tile = D == 64 ? 0.65f : D == 128 ? 1.f : 2.f;
+    t.slots = kv4 ? 768 : 512;
+    t.memory = float(groups) * tiles * kFewKeys * D * (kv4 ? 1.125f : 4.f) / 4.8e6f;
+    if (window == 0 || window > L / 2) t.tail = 0.25f;
+  }
+  // (workgroups beyond these gained nothing anywhere)
+  const long target = !plan.few ? 1024 : rows > 16 ? 512 : kv4 ? 2048 : 1024;
+  plan.splits = best_splits(t, std::min<long>((target + groups - 1) / groups, kMaxAttentionSplits));
   return plan;
 }
 

@@ -492,3 +492,52 @@ def test_two_captured_calls_share_nothing(t):
         torch.cuda.synchronize()
         assert torch.equal(other, want[order[0]])
         assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+# Joined key splits: few rows (one to 64 splits), the rows kernel (4 to 64), fp16 rows in
+# groups over a 4-bit cache (12 to 48), each with a window that cuts splits short and lengths
+# that leave splits without a key.
+JOINS = {
+    "few_window": (HF, 2, 2, 4, 1, 1500, 128, 700, 5, [(1500, 1), (3, 1)]),
+    "few_window_d64": (BF, 1, 1, 7, 2, 3000, 64, 1400, 3, [(2950, 2)]),
+    "few_most": (BF, 1, 1, 4, 1, 9000, 128, 8000, 0, [(8999, 1)]),
+    "few_heads": (HF, 6, 4, 2, 2, 900, 64, None, 0, [(900, 2), (0, 2), (31, 2), (33, 1), (1, 1), (600, 2)]),
+    "few_d256": (HF, 1, 2, 3, 1, 3000, 256, 1400, 9, [(2999, 1)]),
+    "rows_4": (BF, 2, 8, 5, 70, 900, 128, None, 0, [(900, 70), (71, 64)]),
+    "rows_d256": (BF, 2, 5, 2, 70, 700, 256, None, 0, [(699, 70), (5, 3)]),
+    "rows_d64_window": (HF, 2, 6, 3, 70, 900, 64, 600, 3, [(900, 70), (500, 1)]),
+    "rows_window": (BF, 1, 1, 4, 40, 2500, 64, 1200, 5, [(2400, 40)]),
+    "rows_most": (BF, 1, 1, 4, 33, 6000, 128, None, 0, [(5999, 33)]),
+    "rows_most_window": (HF, 1, 1, 2, 66, 6000, 128, 3000, 7, [(6000, 66)]),
+    "groups_most_window": (HF, 1, 1, 7, 5, 5000, 128, 3000, 3, [(4990, 5)]),
+    "groups_d64": (HF, 1, 2, 9, 12, 1000, 64, None, 0, [(1000, 12)]),
+}
+
+
+@pytest.mark.parametrize("case", JOINS)
+@pytest.mark.parametrize("bits", [16, 4])
+def test_joined_splits(case, bits):
+    dtype, b, hk, g, t, length, d, window, sinks, spans = JOINS[case]
+    kw = dict(lengths=int32([n for n, _ in spans]), query_lengths=int32([m for _, m in spans]), window=window,
+              sinks=sinks)
+    q, k, v = make(dtype, b, hk, g, t, length, d)
+    out = torch.full((b, hk * g, t, d), 7.0, dtype=dtype, device="cuda")
+    if bits == 16:
+        want, mass, score = reference(q, k, v, spans, window, sinks, 1 / math.sqrt(d))
+        bound = bound16(want, mass, score, dtype, length)
+        got = window_attention(q, k, v, out=out, **kw)
+    else:
+        cache = Int4KVCache(b, hk, length, d)
+        cache.append(k, v, 0)
+        (_, _, _, kv), (_, _, v_min, vv) = quantize(k), quantize(v)
+        kv, vv = kv.cuda(), vv.cuda()
+        want, _, score = reference(q, kv, vv, spans, window, sinks, 1 / math.sqrt(d))
+        bound = bound4(want, score, dtype, length, vv.abs().max().item(), v_min.double().abs().max().item())
+        got = kv4_attention(q, cache, out=out, **kw)
+    check(got, want, bound, spans, 7.0)
+    again = torch.full_like(out, 7.0)
+    if bits == 16:
+        window_attention(q, k, v, out=again, **kw)
+    else:
+        kv4_attention(q, cache, out=again, **kw)
+    assert torch.equal(got, again)
