@@ -99,7 +99,7 @@ int best_splits(const SplitTimes& t, long most) {
 
 // Which kernel: up to 16 query rows of a KV head fit one operand of the few-rows kernel.  A
 // 4-bit cache keeps it for up to 64 rows (5 tokens of 7 heads over 4101 keys of 8 sequences
-// of 4 KV heads: 23 us, the rows kernel 25 us on half as exact fp16 results), and always for
+// of 4 KV heads: 21 us, the rows kernel 25 us on half as exact fp16 results), and always for
 // fp16 queries: the rows kernel widens the cache to fp16, which a bf16 output does not show
 // and an fp16 output does (error of the output 1.5 to 2 times its own rounding's).
 CachedAttentionPlan plan_cached_attention(int dt, int B, int Hk, int G, int T, int L, int D, int window, int sinks,

