@@ -102,7 +102,7 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
       for (int s = 0; s < kSteps; ++s) qf[rt][s] = *reinterpret_cast<const u32x4_t*>(q + 32 * s + 8 * h4);
     } else {
       // columns 64 g + 16 h4 .. + 15 of every group, in fp16 and scaled by a power of two so
-      // that the row's largest magnitude lies in [2^9, 2^10); step (g, half): word r holds
+      // that the row's largest magnitude lies in [2^9, 2^10) (of fp16 subnormals in [2^6, 2^10)); step (g, half): word r holds
       // nibble r of units 4 h4 + 2 half and the next, odd nibbles 2^-4 for their place in the
       // byte.  On packed halves: every wave prepares its rows, and of a short split's time
       // that is a large part.
@@ -120,7 +120,8 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
           }
         }
       const float mag = quarter_max(to_f32<QDT>(max(big[0], big[1])));
-      const int shift = mag > 0.f && mag < INFINITY ? 10 - __builtin_amdgcn_frexp_expf(mag) : 0;
+      int shift = mag > 0.f && mag < INFINITY ? 10 - __builtin_amdgcn_frexp_expf(mag) : 0;
+      if constexpr (QDT == kF16) shift = min(shift, 30);  // two factors of fp16; 2^-24 comes to 2^6 by it
       f[rt] = ldexpf(f[rt], -shift);
       const _Float16 once = _Float16(ldexpf(1.f, shift >> 1)), again = _Float16(ldexpf(1.f, shift - (shift >> 1)));
 #pragma unroll
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           f16x2_t v;
-          if constexpr (QDT == kF16) {  // shift -6 .. 33: in two steps, exact unless down into the subnormals
+          if constexpr (QDT == kF16) {  // shift -6 .. 30: in two steps, exact unless down into the subnormals
             v = __builtin_bit_cast(f16x2_t, w[gg][i]) * once * again;
           } else {
             v = __builtin_convertvector(f32x2_t{ldexpf(__uint_as_float(w[gg][i] << 16), shift),

@@ -541,3 +541,28 @@ def test_joined_splits(case, bits):
     else:
         kv4_attention(q, cache, out=again, **kw)
     assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("dtype,power", [(HF, -24), (HF, -22), (HF, -16), (HF, 12), (BF, -120), (BF, -60), (BF, 60)])
+@pytest.mark.parametrize("t", [1, 9, 40])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_queries_of_any_size(dtype, power, t, bits):
+    """Queries times 2^power under a scale times 2^-power (as far as a float holds it); fp16
+    ones at 2^-22 and below are subnormals."""
+    b, hk, g, length, d = 2, 2, 4, 150, 128
+    q, k, v = make(dtype, b, hk, g, t, length, d)
+    q = (q.float() * 2.0**power).to(dtype)
+    scale = 2.0 ** -power / math.sqrt(d)
+    spans = [(150, t), (100, t)]
+    kw = dict(lengths=int32([150, 100]), scale=scale)
+    if bits == 16:
+        want, mass, score = reference(q, k, v, spans, None, 0, scale)
+        check(window_attention(q, k, v, **kw), want, bound16(want, mass, score, dtype, length), spans, 7.0)
+        return
+    cache = Int4KVCache(b, hk, length, d)
+    cache.append(k, v, 0)
+    (_, _, _, kv), (_, _, v_min, vv) = quantize(k), quantize(v)
+    kv, vv = kv.cuda(), vv.cuda()
+    want, _, score = reference(q, kv, vv, spans, None, 0, scale)
+    bound = bound4(want, score, dtype, length, vv.abs().max().item(), v_min.double().abs().max().item())
+    check(kv4_attention(q, cache, **kw), want, bound, spans, 7.0)
