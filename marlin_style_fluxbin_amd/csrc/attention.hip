@@ -81,8 +81,8 @@ struct SplitTimes {
   float tail;          // how much of a workgroup's time is waited for at the end (no window: lengths that differ)
   float join, join_split;
 };
-int best_splits(const SplitTimes& t, long most) {
-  float best = 0.f;
+// (the splits' time to *best)
+int best_splits(const SplitTimes& t, long most, float* best) {
   int splits = 1;
   for (int s = 1; s <= most; s += s < 8 ? 1 : s < 16 ? 2 : s < 32 ? 4 : 8) {
     const float per = std::max(1.f, float(t.tiles) / float(s * t.waves));
@@ -91,7 +91,7 @@ int best_splits(const SplitTimes& t, long most) {
     const float work = one * (rounds == 1 ? 1.f : t.shared > 0.f ? t.shared * rounds : float(rounds));
     const float time = std::max(work, t.memory) + t.tail * one + (s > 1 ? t.join + t.join_split * s : 0.f) +
                        (s > 16 ? 1.5f : 0.f);  // the join's four-wave form
-    if (s == 1 || time < best) best = time, splits = s;
+    if (s == 1 || time < *best) *best = time, splits = s;
     if (per == 1.f) break;
   }
   return splits;
@@ -102,20 +102,26 @@ int best_splits(const SplitTimes& t, long most) {
 // of 4 KV heads: 21 us, the rows kernel 25 us on half as exact fp16 results), and always for
 // fp16 queries: the rows kernel widens the cache to fp16, which a bf16 output does not show
 // and an fp16 output does (error of the output 1.5 to 2 times its own rounding's).
-CachedAttentionPlan plan_cached_attention(int dt, int B, int Hk, int G, int T, int L, int D, int window, int sinks,
-                                          bool kv4) {
+//
+// `wide`: workgroups of eight waves, 256 rows, in the rows kernel over a 4-bit cache, so that
+// half as many of them widen a tile.  1024 tokens of 32 heads over 9000 keys 199 us (four
+// waves 215), 4096 tokens of a prompt 177 (195); but with a window of 1024 keys, where it
+// leaves half the chip empty, 54 (37.5): taken where the estimate of the split times is
+// smaller.
+CachedAttentionPlan plan_with(bool wide, int dt, int B, int Hk, int G, int T, int L, int D, int window, int sinks,
+                              bool kv4, float* time) {
   CachedAttentionPlan plan{};
   const long rows = long(T) * G, heads = long(B) * Hk;
   plan.few = rows <= 16 || (kv4 && (dt == kF16 || rows <= 64));
   const int kt = plan.few ? kFewKeys : rows_key_tile(D);
-  plan.waves = 4;
+  plan.waves = wide ? 8 : 4;
   plan.row_blocks = plan.row_groups = 1;
   if (plan.few && rows > 16) {
     plan.waves = 8;
     plan.row_blocks = D <= 128 ? 2 : 1;
     while (plan.row_groups < plan.waves && plan.row_groups * plan.row_blocks * 16 < rows) plan.row_groups *= 2;
   }
-  const long tile_rows = plan.few ? 16 * plan.row_blocks * plan.row_groups : kRowsTile;
+  const long tile_rows = plan.few ? 16 * plan.row_blocks * plan.row_groups : 32 * plan.waves;
   plan.row_tiles = int((rows + tile_rows - 1) / tile_rows);
   // the most key tiles that a row tile can see
   const long tokens = std::min<long>(T, (tile_rows + G - 1) / G + 1);
@@ -130,9 +136,9 @@ CachedAttentionPlan plan_cached_attention(int dt, int B, int Hk, int G, int T, i
   t.join = 3.5f;
   t.join_split = float(heads * rows) * D * 8 / 4e6f;
   if (!plan.few) {
-    t.tile = (D == 64 ? 1.f : 1.2f) * (kv4 ? 1.25f : 1.f);
+    t.tile = (D == 64 ? 1.f : 1.2f) * (kv4 ? 1.25f : 1.f) * (wide ? 1.5f : 1.f);
     t.slots = 256;
-    t.shared = 0.83f;
+    t.shared = wide ? 0.f : 0.83f;
     t.join = 5.f;
   } else if (rows > 16) {
     t.tile = D == 64 ? 1.5f : 2.4f;
@@ -145,8 +151,16 @@ CachedAttentionPlan plan_cached_attention(int dt, int B, int Hk, int G, int T, i
   }
   // (workgroups beyond these gained nothing anywhere)
   const long target = !plan.few ? 1024 : rows > 16 ? 512 : kv4 ? 2048 : 1024;
-  plan.splits = best_splits(t, std::min<long>((target + groups - 1) / groups, kMaxAttentionSplits));
+  plan.splits = best_splits(t, std::min<long>((target + groups - 1) / groups, kMaxAttentionSplits), time);
   return plan;
+}
+CachedAttentionPlan plan_cached_attention(int dt, int B, int Hk, int G, int T, int L, int D, int window, int sinks,
+                                          bool kv4) {
+  float time = 0.f, wide_time = 0.f;
+  const CachedAttentionPlan plan = plan_with(false, dt, B, Hk, G, T, L, D, window, sinks, kv4, &time);
+  if (plan.few || !kv4 || D > 128) return plan;
+  const CachedAttentionPlan wide = plan_with(true, dt, B, Hk, G, T, L, D, window, sinks, kv4, &wide_time);
+  return wide_time < time ? wide : plan;
 }
 
 template <int DT, int D>
@@ -167,9 +181,9 @@ void launch_for_dim(bool kv4, const CachedAttentionPlan& plan, const CachedAtten
     if (kv4) launch_attention_few<DT, D, true>(plan, a, s);
     else launch_attention_few<DT, D, false>(plan, a, s);
   } else if (!kv4) {
-    launch_attention_rows<DT, D, false>(a, s);
+    launch_attention_rows<DT, D, false>(plan, a, s);
   } else if constexpr (DT == kBF16) {  // fp16 queries of a 4-bit cache always take the few-rows kernel
-    launch_attention_rows<DT, D, true>(a, s);
+    launch_attention_rows<DT, D, true>(plan, a, s);
   }
   if (a.splits > 1) launch_combine<DT, D>(a, s);
 }

@@ -31,15 +31,14 @@ struct CachedAttentionArgs {
 // The kernel and split that a call takes, from its sizes alone.
 struct CachedAttentionPlan {
   bool few;        // attention_few.h, else attention_rows.h
-  int waves;       // few: waves of a workgroup (4, 8),
-  int row_blocks;  //      16-row blocks of a wave (1, 2),
+  int waves;       // of a workgroup (4, 8); each takes 32 rows in the rows kernel
+  int row_blocks;  // few: 16-row blocks of a wave (1, 2),
   int row_groups;  //      waves of a workgroup along the rows; the others take other keys
   int row_tiles;   // workgroups along the T * G query rows of a KV head
   int splits;      // workgroups along the keys
 };
 
 constexpr int kFewKeys = 32;    // keys of a wave step of the few-rows kernel
-constexpr int kRowsTile = 128;  // query rows of a rows-kernel workgroup
 constexpr int kMaxAttentionSplits = 64;
 constexpr int rows_key_tile(int D) { return D == 256 ? 32 : 64; }
 
@@ -50,7 +49,7 @@ bool launch_cached_attention(int dt, int D, bool kv4, const CachedAttentionPlan&
                              hipStream_t s);
 
 template <int DT, int D, bool KV4>
-void launch_attention_rows(const CachedAttentionArgs& a, hipStream_t s);
+void launch_attention_rows(const CachedAttentionPlan& plan, const CachedAttentionArgs& a, hipStream_t s);
 template <int DT, int D, bool KV4>
 void launch_attention_few(const CachedAttentionPlan& plan, const CachedAttentionArgs& a, hipStream_t s);
 

@@ -1,8 +1,8 @@
 // Cached attention of many query rows (a prompt, a chunk, several drafted tokens): one
 // pass over the keys with a running maximum and sum, both products on the matrix cores.
 //
-// A workgroup of four waves takes 128 query rows of one KV head, row = token * G + head
-// of the group, so every head grouping fills the tile and the four waves share each key
+// A workgroup of four (eight) waves takes 128 (256) query rows of one KV head, row = token
+// * G + head of the group, so every head grouping fills the tile and the waves share each key
 // and value tile in LDS.  Per tile of KT keys a wave forms
 //   S^T = K Q^T   (32 x 32 x 16 products: column = query, so a query's scores sit in two
 //                  lanes: its maximum and sum are register work and one lane swap)
@@ -24,10 +24,12 @@
 // which need the vector pipe, beside them.  D = 256 (4096 tokens, 16 heads) 0.78 PFLOP/s and
 // D = 64 (32 heads) 0.70: per score as many exponentials for half the products.  With a window
 // of 1024 keys (4096 tokens, 32 heads) 81 us: three of 18 tiles (the sinks', both ends') are
-// computed whole for a part, and q and the output are 67 MB, 14 us at a copy's rate.  A 4-bit cache (1024 tokens over 9000 keys) 183 us: each of
-// the 32 row tiles of a head widens the keys that it reads, a quarter of its time.
+// computed whole for a part, and q and the output are 67 MB, 14 us at a copy's rate.  A 4-bit cache (1024 tokens over 9000 keys) 180 us: each row
+// tile of a head widens the keys that it reads, a fifth of its time at 128 rows, an eighth
+// at 256.
 // 128 rows, so that a key or value read from LDS meets 32 columns a wave, four waves a
-// tile: two workgroups a CU, one's exponentials beside the other's products.
+// tile: two workgroups a CU, one's exponentials beside the other's products.  256 rows and one
+// workgroup where that halves the widening (a 4-bit cache, D <= 128).
 #pragma once
 #include "attention_core.h"
 
@@ -170,11 +172,12 @@ struct Kv4Stage {
 // Column of position x of a widened 4-bit row.
 __device__ __forceinline__ int kv4_column(int x) { return (x & ~7) | ((x & 1) << 2) | ((x >> 1) & 3); }
 
-template <int QDT, int D, bool KV4>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(const CachedAttentionArgs a) {
+template <int QDT, int D, bool KV4, int NW>
+__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attention_rows_kernel(const CachedAttentionArgs a) {
   using S = RowsShape<D>;
   constexpr int CDT = KV4 ? kF16 : QDT;  // the products' type
-  constexpr int KT = S::KT;
+  constexpr int KT = S::KT, kRows = 32 * NW, kThreads = 64 * NW;
+  static_assert(NW == 4 || (NW == 8 && KV4 && kRows <= 4 * KT), "loads by four waves; the output through the tiles' memory");
   __shared__ __attribute__((aligned(1024))) char lds_memory[4 * S::kTileBytes];
   lds_char* const lds = (lds_char*)lds_memory;
   const int t = threadIdx.x, lane = t & 63, wave = wave_index();
@@ -198,10 +201,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
   const int tile = a.row_tiles - 1 - item / a.splits, split = item % a.splits;
   const int b = head / a.Hk, g = head - b * a.Hk;
   const SequenceSpan span = sequence_span(a, b);
-  const int rows = span.m * a.G, r0 = tile * kRowsTile;
+  const int rows = span.m * a.G, r0 = tile * kRows;
   if (r0 >= rows) return;
   const int base_pos = span.n - span.m;
-  const int lo_pos = base_pos + r0 / a.G, hi_pos = base_pos + (min(r0 + kRowsTile, rows) - 1) / a.G;
+  const int lo_pos = base_pos + r0 / a.G, hi_pos = base_pos + (min(r0 + kRows, rows) - 1) / a.G;
   const KeyTiles tiles = key_tiles<KT>(lo_pos, hi_pos, a.window, a.sinks);
   const int per = (tiles.count + a.splits - 1) / a.splits;
   const int it0 = split * per, it1 = min(tiles.count, it0 + per);
@@ -273,7 +276,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
   } else {
     row_at = size_t(head) * a.L;
   }
-  Kv4Stage<D> ks, vs;
+  // four waves: each stages keys and values; eight: four stage keys, four values
+  Kv4Stage<D> ks, other;
+  Kv4Stage<D>& vs = NW == 8 ? ks : other;
+  const bool keys_here = NW == 4 || wave < 4, values_here = NW == 4 || wave >= 4;
+  const int ts = t & 255;
 
   // LDS: keys of tile i at (i % 2) tiles, values at 2 + (i % 2) (i from it0)
   const auto key_tile = [&](int parity) __attribute__((always_inline)) { return lds + parity * S::kTileBytes; };
@@ -286,8 +293,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
     const size_t at = row_at + j0;
     if constexpr (!KV4)
       load_rows_to_lds<D, true>(kb + j0 * a.k_stride[2], a.k_stride[2], rows, key_tile(parity), wave, lane);
-    else
-      ks.load(static_cast<const uint8_t*>(a.k) + at * (D / 2), a.k_scales + at * (D / 64), rows, t);
+    else if (keys_here)
+      ks.load(static_cast<const uint8_t*>(a.k) + at * (D / 2), a.k_scales + at * (D / 64), rows, ts);
   };
   auto fetch_values = [&](int it, int parity) __attribute__((always_inline)) {
     if (it >= it1) return;
@@ -295,8 +302,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
     const size_t at = row_at + j0;
     if constexpr (!KV4)
       load_rows_to_lds<D, false>(vb + j0 * a.v_stride[2], a.v_stride[2], rows, value_tile(parity), wave, lane);
-    else
-      vs.load(static_cast<const uint8_t*>(a.v) + at * (D / 2), a.v_scales + at * (D / 64), rows, t);
+    else if (values_here)
+      vs.load(static_cast<const uint8_t*>(a.v) + at * (D / 2), a.v_scales + at * (D / 64), rows, ts);
   };
 
   // operand n of a tile's S^T products (key block n / kSteps, step n % kSteps) and of its O^T
@@ -378,7 +385,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
   // row: the careful round adds such values by hand to the rows that see them and zeroes them.
   auto settle = [&](int it, lds_char* vt) __attribute__((always_inline)) {
     unsigned bad = 0;
-    for (int i = t * 16; i < S::kTileBytes; i += 256 * 16) {
+    for (int i = t * 16; i < S::kTileBytes; i += kThreads * 16) {
       const u32x4_t w = lds_b128(vt + i);
       bad |= nonfinite_pair<CDT>(w[0]) | nonfinite_pair<CDT>(w[1]) | nonfinite_pair<CDT>(w[2]) |
              nonfinite_pair<CDT>(w[3]);
@@ -402,7 +409,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
         }
     }
     __syncthreads();
-    for (int i = t * 16; i < S::kTileBytes; i += 256 * 16) {
+    for (int i = t * 16; i < S::kTileBytes; i += kThreads * 16) {
       u32x4_t w = lds_b128(vt + i);
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = finite_pair<CDT>(w[e]);
@@ -473,8 +480,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
       raise(top);
     }
     if constexpr (KV4) {
-      if (it + 2 < it1) ks.template store<true>(key_tile(parity), t);
-      vs.template store<false>(value_tile(parity ^ 1), t);
+      if (keys_here && it + 2 < it1) ks.template store<true>(key_tile(parity), ts);
+      if (values_here) vs.template store<false>(value_tile(parity ^ 1), ts);
     }
   };
   auto weigh_values = [&](int parity, f32x16_t(&s)[S::kSub]) __attribute__((always_inline)) {
@@ -491,12 +498,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
     fetch_keys(it0, 0);
     fetch_values(it0, 0);
     if constexpr (KV4) {
-      ks.template store<true>(key_tile(0), t);
-      vs.template store<false>(value_tile(0), t);
+      if (keys_here) ks.template store<true>(key_tile(0), ts);
+      if (values_here) vs.template store<false>(value_tile(0), ts);
     }
     fetch_keys(it0 + 1, 1);
     if constexpr (KV4) {
-      if (it0 + 1 < it1) ks.template store<true>(key_tile(1), t);
+      if (keys_here && it0 + 1 < it1) ks.template store<true>(key_tile(1), ts);
     }
     arrive();
     if (active) {
@@ -536,8 +543,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
         fetch_keys(it, 0);
         fetch_values(it, 0);
         if constexpr (KV4) {
-          ks.template store<true>(key_tile(0), t);
-          vs.template store<false>(value_tile(0), t);
+          if (keys_here) ks.template store<true>(key_tile(0), ts);
+          if (values_here) vs.template store<false>(value_tile(0), ts);
         }
         arrive();
         if (active) {
@@ -620,9 +627,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_rows_kernel(c
 }
 
 template <int DT, int D, bool KV4>
-void launch_attention_rows(const CachedAttentionArgs& a, hipStream_t s) {
-  const unsigned blocks = unsigned(a.B) * a.Hk * a.row_tiles * a.splits;
-  hipLaunchKernelGGL((attention_rows_kernel<DT, D, KV4>), dim3(blocks), dim3(256), 0, s, a);
+void launch_attention_rows(const CachedAttentionPlan& plan, const CachedAttentionArgs& a, hipStream_t s) {
+  const dim3 blocks(unsigned(a.B) * a.Hk * a.row_tiles * a.splits);
+  if constexpr (KV4 && D <= 128) {
+    if (plan.waves == 8) {
+      hipLaunchKernelGGL((attention_rows_kernel<DT, D, KV4, 8>), blocks, dim3(512), 0, s, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((attention_rows_kernel<DT, D, KV4, 4>), blocks, dim3(256), 0, s, a);
 }
 
 }  // namespace fx

@@ -2,7 +2,7 @@
 #include "attention_rows.h"
 
 namespace fx {
-template void launch_attention_rows<kBF16, 64, false>(const CachedAttentionArgs&, hipStream_t);
-template void launch_attention_rows<kBF16, 128, false>(const CachedAttentionArgs&, hipStream_t);
-template void launch_attention_rows<kBF16, 256, false>(const CachedAttentionArgs&, hipStream_t);
+template void launch_attention_rows<kBF16, 64, false>(const CachedAttentionPlan&, const CachedAttentionArgs&, hipStream_t);
+template void launch_attention_rows<kBF16, 128, false>(const CachedAttentionPlan&, const CachedAttentionArgs&, hipStream_t);
+template void launch_attention_rows<kBF16, 256, false>(const CachedAttentionPlan&, const CachedAttentionArgs&, hipStream_t);
 }  // namespace fx

@@ -566,3 +566,41 @@ def test_queries_of_any_size(dtype, power, t, bits):
     want, _, score = reference(q, kv, vv, spans, None, 0, scale)
     bound = bound4(want, score, dtype, length, vv.abs().max().item(), v_min.double().abs().max().item())
     check(kv4_attention(q, cache, **kw), want, bound, spans, 7.0)
+
+
+@pytest.mark.parametrize("case", [
+    (BF, 5, 8, 4, 200, 600, 128, None, 0, [(600, 200), (200, 200), (31, 40), (0, 200), (599, 1)]),
+    (BF, 3, 14, 3, 270, 700, 64, 600, 5, [(700, 270), (270, 270), (423, 111)])])
+def test_kv4_wide_row_tiles(case):
+    """Enough row tiles of a 4-bit cache for workgroups of 256 rows."""
+    dtype, b, hk, g, t, length, d, window, sinks, spans = case
+    q, k, v = make(dtype, b, hk, g, t, length, d)
+    cache = Int4KVCache(b, hk, length, d)
+    cache.append(k, v, 0)
+    (_, _, _, kv), (_, _, v_min, vv) = quantize(k), quantize(v)
+    kv, vv = kv.cuda(), vv.cuda()
+    scale = 1 / math.sqrt(d)
+    want, _, score = reference(q, kv, vv, spans, window, sinks, scale)
+    bound = bound4(want, score, dtype, length, vv.abs().max().item(), v_min.double().abs().max().item())
+    for i, (n, m) in enumerate(spans):  # poison
+        for x in (cache.k_scales, cache.v_scales):
+            x[i, :, n:] = float("nan")
+    out = torch.full((b, hk * g, t, d), 7.0, dtype=dtype, device="cuda")
+    kw = dict(lengths=int32([n for n, _ in spans]), query_lengths=int32([m for _, m in spans]), window=window,
+              sinks=sinks)
+    check(kv4_attention(q, cache, out=out, **kw), want, bound, spans, 7.0)
+
+
+def test_kv4_wide_row_tiles_nan_groups():
+    """A NaN group reaches the rows that see it and no other, there too."""
+    b, hk, g, t, length, d = 5, 8, 4, 200, 600, 128
+    q, k, v = make(BF, b, hk, g, t, length, d)
+    bad = 450  # queries sit at 400 .. 599
+    v[1, 3, bad, 70] = float("inf")
+    cache = Int4KVCache(b, hk, length, d)
+    cache.append(k, v, 0)
+    out = kv4_attention(q, cache)
+    nan = torch.isnan(out)
+    assert nan[1, 12:16, 50:, 64:].all()
+    nan[1, 12:16, 50:, 64:] = False
+    assert not nan.any()
