@@ -24,7 +24,7 @@
 // which need the vector pipe, beside them.  D = 256 (4096 tokens, 16 heads) 0.78 PFLOP/s and
 // D = 64 (32 heads) 0.70: per score as many exponentials for half the products.  With a window
 // of 1024 keys (4096 tokens, 32 heads) 81 us: three of 18 tiles (the sinks', both ends') are
-// computed whole for a part, and q and the output are 67 MB, 14 us at a copy's rate.  A 4-bit cache (1024 tokens over 9000 keys) 180 us: each row
+// computed whole for a part, and q and the output are 67 MB, 14 us at a copy's rate.  A 4-bit cache (1024 tokens over 9000 keys) 170 us: each row
 // tile of a head widens the keys that it reads, a fifth of its time at 128 rows, an eighth
 // at 256.
 // 128 rows, so that a key or value read from LDS meets 32 columns a wave, four waves a
