@@ -604,3 +604,45 @@ def test_kv4_wide_row_tiles_nan_groups():
     assert nan[1, 12:16, 50:, 64:].all()
     nan[1, 12:16, 50:, 64:] = False
     assert not nan.any()
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (HF, 128), (BF, 128), (BF, 256)])
+@pytest.mark.parametrize("sinks", [1, 4, 8, 9, 24, 33, 64, 65])
+@pytest.mark.parametrize("window,t,length", [(64, 150, 701), (100, 150, 690), (257, 33, 683), (5, 300, 640), (130, 257, 663)])
+def test_sinks_and_window_in_every_place(dtype, d, sinks, window, t, length):
+    """Sinks in tiles of their own and joining the window's."""
+    b, hk, g = 2, 1, 2
+    spans = [(length, t), (length - 61, t - 7)]
+    q, k, v = make(dtype, b, hk, g, t, length, d)
+    want, mass, score = reference(q, k, v, spans, window, sinks, 1 / math.sqrt(d))
+    bound = bound16(want, mass, score, dtype, length)
+    for i, (n, m) in enumerate(spans):  # what no query of a sequence sees is poison
+        k[i, :, n:], v[i, :, n:] = float("nan"), float("inf")
+        first = max(0, n - m - window + 1)
+        k[i, :, min(sinks, first):first], v[i, :, min(sinks, first):first] = float("inf"), float("nan")
+    kw = dict(lengths=int32([n for n, _ in spans]), query_lengths=int32([m for _, m in spans]), window=window,
+              sinks=sinks)
+    out = torch.full((b, hk * g, t, d), 7.0, dtype=dtype, device="cuda")
+    check(window_attention(q, k, v, out=out, **kw), want, bound, spans, 7.0)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (HF, 128), (BF, 256)])
+@pytest.mark.parametrize("sinks", [3, 8])
+def test_infinities_among_sinks_and_window(dtype, d, sinks):
+    """An infinite sink reaches every row, a NaN of the window the rows that see it alone."""
+    b, hk, g, t, length, window = 1, 1, 2, 70, 400, 40
+    spans = [(length, t)]
+    q, k, v = make(dtype, b, hk, g, t, length, d)
+    want, mass, score = reference(q, k, v, spans, window, sinks, 1 / math.sqrt(d))
+    bound = bound16(want, mass, score, dtype, length)
+    v[0, 0, sinks - 1, 5] = float("inf")
+    v[0, 0, 395, 9] = float("nan")   # queries sit at 330 .. 399: the last five see it
+    v[0, 0, 300, 11] = float("-inf")  # seen by 330 .. 339
+    out = window_attention(q, k, v, window=window, sinks=sinks)
+    assert (out[..., 5] == float("inf")).all()
+    assert torch.isnan(out[:, :, 65:, 9]).all() and torch.isfinite(out[:, :, :65, 9]).all()
+    assert (out[:, :, :10, 11] == float("-inf")).all() and torch.isfinite(out[:, :, 10:, 11]).all()
+    keep = [c for c in range(d) if c not in (5, 9, 11)]
+    check(out[..., keep], want[..., keep], bound[..., keep], spans, 7.0)
+    error = (out[:, :, :65, 9].double() - want[:, :, :65, 9]).abs()
+    assert (error <= bound[:, :, :65, 9]).all()
