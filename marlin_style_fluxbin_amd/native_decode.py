@@ -32,7 +32,7 @@ import time
 import torch
 
 from . import _lib
-from .cached_attention import Int4KVCache, kv4_attention, window_attention
+from .cached_attention import HEAD_DIMS, Int4KVCache, kv4_attention, window_attention
 from .fused_modules import add_rms_norm, head_norm_rope
 from .static_decode import graph_kernel_count
 from .deployment import HybridSegmentsGemv, PackedHybridLinear
@@ -469,6 +469,8 @@ class NativeDecodeSession:
             raise ValueError("window must be None or a positive integer")
         if type(sinks) is not int or sinks < 0:
             raise ValueError("sinks must be a non-negative integer")
+        if (kv_cache == "int4" or window is not None) and cfg.head_dim not in HEAD_DIMS:
+            raise ValueError(f"kv_cache='int4' and window need a head_dim of {HEAD_DIMS}, got {cfg.head_dim}")
         self.model, self.dtype, self.device = model, dtype, input_ids.device
         self.window, self.sinks = window, sinks
         self.ids = input_ids

@@ -82,3 +82,13 @@ def test_session_refusals(gpu):
                         (dict(sinks=-1), "sinks")):
         with pytest.raises(ValueError, match=message):
             NativeDecodeSession(model, ids, forced, **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(kv_cache="int4"), dict(window=40)])
+def test_session_refuses_other_head_dims(gpu, kw):
+    config = qwen3_config(hidden_size=256, intermediate_size=512, num_hidden_layers=1, num_attention_heads=4,
+                          num_key_value_heads=2, head_dim=32, vocab_size=512, max_position_embeddings=512)
+    model = random_qwen3_model(config, device=gpu, dtype=torch.bfloat16, seed=2)
+    ids = torch.zeros(1, 9, dtype=torch.long, device=gpu)
+    with pytest.raises(ValueError, match="head_dim"):
+        NativeDecodeSession(model, ids, ids[:, :3], **kw)
