@@ -102,10 +102,10 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
       for (int s = 0; s < kSteps; ++s) qf[rt][s] = *reinterpret_cast<const u32x4_t*>(q + 32 * s + 8 * h4);
     } else {
       // columns 64 g + 16 h4 .. + 15 of every group, in fp16 and scaled by a power of two so
-      // that the row's largest magnitude lies in [2^9, 2^10) (of fp16 subnormals in [2^6, 2^10)); step (g, half): word r holds
-      // nibble r of units 4 h4 + 2 half and the next, odd nibbles 2^-4 for their place in the
-      // byte.  On packed halves: every wave prepares its rows, and of a short split's time
-      // that is a large part.
+      // that the row's largest magnitude lies in [2^9, 2^10) (of fp16 subnormals in [2^6,
+      // 2^10)); step (g, half): word r holds nibble r of units 4 h4 + 2 half and the next, odd
+      // nibbles 2^-4 for their place in the byte.  On packed halves: every wave prepares its
+      // rows, and of a short split's time that is a large part.
       unsigned w[kGroups][8];
       u16x2_t big = {0, 0};
 #pragma unroll
