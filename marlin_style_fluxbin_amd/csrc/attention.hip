@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(const CachedAtte
   const float* po = a.partial + first * D + lane * kCols;
   cols_t v[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i)  // splits past the last: the last again, with weight 0
+  for (int i = 0; i < N; ++i)  // splits past the last: the last again, not counted below
     v[i] = *reinterpret_cast<const cols_t*>(po + size_t(min(part + W * i, a.splits - 1)) * D);
   const bool live = lane < a.splits;
   const float m = live ? ml[lane * 2] : -INFINITY, ls = live ? ml[lane * 2 + 1] : 0.f;
@@ -40,9 +40,11 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(const CachedAtte
   for (int c = 0; c < kCols; ++c) o[c] = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), min(part + W * i, 63)));
+    const int s = part + W * i;
+    const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), min(s, 63)));
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) o[c] += ws * v[i][c];
+    for (int c = 0; c < kCols; ++c)  // (a weight of 0 would make NaN of an infinity)
+      o[c] = s < a.splits ? __builtin_fmaf(ws, v[i][c], o[c]) : o[c];
   }
   const int tok = row / a.G;
   const float inv = softmax_inverse(l, span.n - span.m + tok);

@@ -1,0 +1,43 @@
+"""window_attention, kv4_attention and Int4KVCache where they can go wrong: infinities in joined
+splits, weights far below a row's largest, the ends of the types' ranges, addresses past 2^32
+bytes, calls that cannot be recorded."""
+import math
+
+import pytest
+import torch
+
+from marlin_style_fluxbin_amd import Int4KVCache, _lib, kv4_attention, window_attention
+from tests.attention_bounds import Cache, reference_and_bound
+from tests.test_cached_attention_gpu import BF, HF, check, int32, make
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+
+def splits_of(dtype, b, hk, g, t, length, d, window=0, sinks=0, kv4=0):
+    nbytes = _lib.library().fx_cached_attention_workspace_bytes(b, hk * g, hk, t, length, d, window, sinks,
+                                                                _lib.dtype_code(dtype), kv4)
+    return max(1, nbytes // (b * hk * g * t * (d + 2) * 4))
+
+
+# ------------------------------------------------------------------ visible infinities
+@pytest.mark.parametrize("dtype,b,hk,g,t,length,d", [
+    (BF, 24, 8, 4, 1, 300, 128),   # one split
+    (BF, 1, 8, 4, 1, 700, 128), (BF, 1, 8, 4, 1, 1500, 128), (HF, 1, 2, 3, 2, 1700, 64),  # joined by one wave a row
+    (HF, 1, 4, 2, 1, 1800, 256), (BF, 1, 2, 4, 1, 5000, 128),  # 16; 40, joined by four
+    (BF, 2, 2, 5, 70, 900, 128), (BF, 2, 5, 2, 70, 700, 256), (HF, 1, 1, 4, 33, 6000, 128)])  # the rows kernel
+def test_infinities_in_every_split(dtype, b, hk, g, t, length, d):
+    """Every 64 keys one value's column holds an infinity that every row sees: it reaches each
+    of them, whichever split it lies in, and nothing else changes."""
+    q, k, v = make(dtype, b, hk, g, t, length, d)
+    scale = 1 / math.sqrt(d)
+    want, bound = reference_and_bound(q, Cache(k, v, 16), [(length, t)] * b, None, 0, scale)
+    keys = range(5, length - t, 64)
+    assert len(keys) <= d - 8
+    for c, j in enumerate(keys):
+        v[:, :, j, c] = -INF if c % 3 == 0 else INF
+    out = window_attention(q, k, v)
+    for c in range(len(keys)):
+        assert (out[..., c] == (-INF if c % 3 == 0 else INF)).all(), (c, splits_of(dtype, b, hk, g, t, length, d))
+    rest = slice(len(keys), None)
+    check(out[..., rest], want[..., rest], bound[..., rest], [(length, t)] * b, 7.0)
