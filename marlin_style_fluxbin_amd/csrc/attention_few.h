@@ -322,9 +322,10 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
         pf[rt][e / 2] = round_pair_bits<CDT>(p0, p1);
       }
     }
-    if (!whole && careful) {
-      // a hidden key's infinity or NaN must not meet its zero p: rows that see one take it
-      // by hand (every lane reads the rows it needs again), then it counts as zero
+    if (careful) {
+      // an infinity or NaN must not meet a zero p, a hidden key's or one too small for 16 bits:
+      // rows that see one take it by hand (every lane reads the rows it needs again), then it
+      // counts as zero
       unsigned bad = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e)

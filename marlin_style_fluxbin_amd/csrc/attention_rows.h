@@ -381,8 +381,9 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attention_rows_kern
     else each([&](int j) __attribute__((always_inline)) { return seen.sees_window(j); });
   };
   // Keys that no query of the workgroup sees are zeros in LDS.  One that some see may hold an
-  // infinity or a NaN, and a product with a hidden query's zero p would carry it into that
-  // row: the careful round adds such values by hand to the rows that see them and zeroes them.
+  // infinity or a NaN, and a product with a zero p, a hidden query's or one too small for 16
+  // bits, would make NaN of it: the careful round adds such values by hand to the rows that
+  // see them and zeroes them.
   auto settle = [&](int it, lds_char* vt) __attribute__((always_inline)) {
     unsigned bad = 0;
     for (int i = t * 16; i < S::kTileBytes; i += kThreads * 16) {
@@ -552,7 +553,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attention_rows_kern
           if (partial(it)) hide(it, sa);
           raise(largest(sa));
         }
-        if (partial(it)) settle(it, value_tile(0));
+        settle(it, value_tile(0));
         if (active) weigh_values(0, sa);
         __syncthreads();  // the next tile's loads overwrite this one
       }

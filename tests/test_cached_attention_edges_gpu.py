@@ -41,3 +41,22 @@ def test_infinities_in_every_split(dtype, b, hk, g, t, length, d):
         assert (out[..., c] == (-INF if c % 3 == 0 else INF)).all(), (c, splits_of(dtype, b, hk, g, t, length, d))
     rest = slice(len(keys), None)
     check(out[..., rest], want[..., rest], bound[..., rest], [(length, t)] * b, 7.0)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t,length", [(1, 300), (1, 2000), (150, 400), (60, 3000)])
+@pytest.mark.parametrize("top,at", [(70, 10), (10, 70), (130, 200), (20, 10), (20, 40), (40, 20)])
+def test_an_infinity_of_little_weight(dtype, d, t, length, top, at):
+    """One key outweighs the others by e^40 (their p is no fp16 number): their infinite values
+    still reach the rows that see them."""
+    q, k, v = make(dtype, 1, 1, 2, t, length, d)
+    q.fill_(1.0)
+    k.zero_()
+    k[:, :, top] = 40.0
+    v[:, :, at, 3], v[:, :, at + 1, 5] = INF, -INF
+    got = window_attention(q, k, v, scale=1 / d)
+    see = torch.arange(length - t, length, device="cuda") >= max(top, at + 1)  # rows that see all three
+    assert (got[:, :, see, 3] == INF).all() and (got[:, :, see, 5] == -INF).all()
+    rest = [c for c in range(d) if c not in (3, 5)]
+    assert torch.equal(got[:, :, see][..., rest], v[:, :, top, None][..., rest].expand(-1, 2, int(see.sum()), -1))
