@@ -35,6 +35,13 @@ __device__ __forceinline__ f32x4_t mfma16(const u32x4_t& a, const u32x4_t& b, co
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// 16-bit p reach 2^room and not 1 at a row's largest score (log2 units), the running maximum
+// being that much less: fp16 then holds what lies up to 2^-(14 + room) below it in full and
+// loses what lies below 2^-(25 + room), in place of 2^-14 and 2^-25 (a key whose value is small
+// may outweigh all that make the output).  Scores so large that a difference of `room` is
+// rounded get none: p could leave fp16.
+__device__ __forceinline__ float p_room(float top, float room) { return fabsf(top) < 0x1p20f ? room : 0.f; }
+
 // The sum / maximum over the two lanes l and l ^ 32 (every lane gets it).
 __device__ __forceinline__ float half_pair_max(float v) {
   const unsigned u = __float_as_uint(v);

@@ -269,12 +269,13 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
 
   auto half_of = [](unsigned w, int i) { return f16_bits_to_f32(uint16_t(i ? w >> 16 : w)); };
 
-  // running maximum of row tile rt: over `bound`, all by `less` too large
-  auto raise = [&](int rt, const float(&bound)[8], float less) __attribute__((always_inline)) {
+  // running maximum of row tile rt: over `bound`, all by `less` too large; p up to 2^room
+  auto raise = [&](int rt, const float(&bound)[8], float less, float room) __attribute__((always_inline)) {
     float top = bound[0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) top = fmaxf(top, bound[e]);
-    top = quarter_max(top) - less;
+    top = quarter_max(top);
+    top -= less + (room > 0.f ? p_room(top, room) : 0.f);
     if (__builtin_amdgcn_ballot_w64(top > m[rt])) {
       const float before = m[rt];
       m[rt] = fmaxf(before, top);
@@ -314,7 +315,7 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
         for (int r = 0; r < 4; ++r) s[4 * u + r] = c[r] * f[rt];
       }
       if (!whole) hide(rt, j0, sink_tile, s);
-      raise(rt, s, 0.f);
+      raise(rt, s, 0.f, CDT == kF16 ? 15.f : 0.f);
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         float p0 = __builtin_amdgcn_exp2f(s[e] - m_use[rt]), p1 = __builtin_amdgcn_exp2f(s[e + 1] - m_use[rt]);
@@ -446,7 +447,7 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
       float bound[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) bound[e] = __builtin_fmaf(size[e], 0x1p-10f, s[rt][e]);
-      raise(rt, bound, 15.f);
+      raise(rt, bound, 15.f, 0.f);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         pr[rt][e] = __builtin_amdgcn_exp2f(s[rt][e] - m_use[rt]);

@@ -11,7 +11,8 @@
 //                  free as long as both operands use the same, and V^T is read from LDS
 //                  by the transposing read in the order that S^T has left P^T in)
 // with S, m, the sum and O in fp32.  O is rescaled only when some query's maximum grew by
-// more than 2^8 (p then stays below 2^8, which fp16 holds too).
+// more than 2^8, so that p stays below that (fp16: within 2^7 .. 2^15 at the row's largest,
+// p_room).
 //
 // LDS: rows of D 16-bit values in 16-byte chunks, chunk c of key j at c ^ swizzle(j), keys
 // and values each for their reads.  16-bit caches load straight into LDS (the
@@ -337,8 +338,9 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attention_rows_kern
     return half_pair_max(top) * f;
   };
   auto raise = [&](float top) __attribute__((always_inline)) {
-    if (__builtin_amdgcn_ballot_w64(top > m + 8.f)) {
-      const float mn = fmaxf(m, top);
+    constexpr bool kF16P = CDT == kF16;
+    if (__builtin_amdgcn_ballot_w64(top > m + (kF16P ? p_room(top, 15.f) : 8.f))) {
+      const float mn = fmaxf(m, kF16P ? top - p_room(top, 7.f) : top);
       m_use = mn == -INFINITY ? 0.f : mn;
       const float alpha = __builtin_amdgcn_exp2f(m - m_use);  // 0 before the first visible key
       m = mn;

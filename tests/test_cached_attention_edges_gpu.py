@@ -60,3 +60,54 @@ def test_an_infinity_of_little_weight(dtype, d, t, length, top, at):
     assert (got[:, :, see, 3] == INF).all() and (got[:, :, see, 5] == -INF).all()
     rest = [c for c in range(d) if c not in (3, 5)]
     assert torch.equal(got[:, :, see][..., rest], v[:, :, top, None][..., rest].expand(-1, 2, int(see.sum()), -1))
+
+
+# ------------------------------------------------------------------ weights far below the largest
+@pytest.mark.parametrize("gap", [18.3, 22.6, 28.7])
+@pytest.mark.parametrize("b,hk,t,length,d", [(32, 16, 1, 1000, 128), (1, 1, 1, 3000, 64), (16, 16, 1, 900, 256),
+                                             (2, 1, 150, 1000, 128), (2, 1, 150, 1000, 256)])
+def test_small_fp16_weights_count(gap, b, hk, t, length, d):
+    """A key of value zero outweighs the others by 2^gap; what they hold is the output.  p is
+    fp16: 2^15 at the row's largest in the few-rows kernel, 2^7 at least in the rows kernel, so
+    that it is off by half a step, 2^-11 of itself or 2^-40 (2^-32) of the largest."""
+    q, k, v = make(HF, b, hk, 1, t, length, d)
+    q.fill_(1.0)
+    k.zero_()
+    k[:, :, 37] = gap * math.log(2)
+    v.abs_().add_(1).mul_(50)
+    v[:, :, 37] = 0
+    got = window_attention(q, k, v, scale=1 / d).double()
+    score = k[0, 0, 37, 0].double()  # as fp16 holds it
+    p = torch.arange(length - t, length, device="cuda")
+    weight = torch.exp(-score) / (1 + p * torch.exp(-score))
+    sums = v.double().cumsum(2)[:, :, p]
+    want = sums * weight[:, None]
+    step = 2.0**-40 if t == 1 else 2.0**-32
+    bound = want * (2.0**-10 + 2.0**-16) + step * sums + 2.0**-25
+    error = (got - want).abs()
+    assert (error <= bound).all(), (error / bound).max().item()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("power", range(0, 16, 3))
+@pytest.mark.parametrize("t,length,d", [(1, 700, 128), (20, 300, 64), (150, 400, 128), (70, 300, 256)])
+def test_scores_of_any_size(dtype, bits, power, t, length, d):
+    """Queries of 2^power, keys of 0 and 2^power, scores up to 2^37 and more: the mean of the
+    values whose keys are largest (of all of them where the scores are 1 apart)."""
+    q, k, v = make(dtype, 1, 1, 2, t, length, d)
+    q.fill_(2.0**power)
+    k.zero_()
+    g = torch.Generator().manual_seed(power)
+    k[:, :, torch.randperm(length, generator=g)[:length // 2]] = 2.0**power
+    k[:, :, 0] = 2.0**power
+    scale = 1 / d if power == 0 else 1.0
+    spans = [(length, t)]
+    want, bound = reference_and_bound(q, Cache(k, v, bits), spans, None, 0, scale)
+    if bits == 16:
+        got = window_attention(q, k, v, scale=scale)
+    else:
+        cache = Int4KVCache(1, 1, length, d)
+        cache.append(k, v, 0)
+        got = kv4_attention(q, cache, scale=scale)
+    check(got, want, bound, spans, 7.0)
