@@ -3,7 +3,8 @@
 With w_j the softmax weights, o = sum_j w_j v_j the output and, over a 4-bit cache, v_j = a_j +
 minimum_j (a_j = code * scale; over a 16-bit one a_j = v_j):
 
-* the output's rounding, half a step of |o|, is counted whole;
+* the output's rounding, half a step of |o|, is counted whole; fp16's steps stay 2^-24 below
+  2^-14, so half a step is 2^-25 = 2^-11 2^-14 there;
 * everything else is a sum of many roundings that have nothing to do with each other, each
   at most h of what it rounds, so of variance at most h^2 / 3 of its square.  Their sum is
   counted as Z = 8 times its standard deviation (10^6 elements exceed that once in 10^9 runs):
@@ -15,6 +16,14 @@ minimum_j (a_j = code * scale; over a 16-bit one a_j = v_j):
     - the fp32 sums over the keys and their joins, sqrt(n + 128) 2^-24 of sum_j w_j |terms|;
     - 16-bit weights that sink into the subnormals: at most `step` of the row's largest
       (fp16 alone).
+
+The few-rows kernel multiplies 4-bit codes as fp16 subnormals, code * 2^-24.  The matrix unit
+aligns the eight terms of a step to the largest exponent among them, where a subnormal counts
+as 2^-14, and cuts them 24 bits below (measured: 2^14 * 8 * 2^-24 beside 2^-1 * 2^-24 loses the
+latter; beside 2^0 * 2^-24 both are held).  So a term is off by less than 2^-24 2^-14 / 2^-24 =
+2^-14 of the largest p * scale of its eight, one code's worth, always towards the same side:
+7 2^-14 sum_j w_j scale_j in all, counted whole; and a score by 2^-14 of the row's largest |q|
+times the key's scale for each of its D terms, of either sign.
 
 fp16 queries over a 4-bit cache weigh the rounding of p * scale at the codes' middle, so that
 a_j is (code - 8) * scale there.
@@ -73,10 +82,11 @@ class Cache:
 
         codes, scales, minima, self.k = parts(k)
         self.k_terms = codes * scales + minima.abs()
+        self.k_unit = scales.amax(-1)  # [B, Hk, L]
         codes, scales, minima, self.v = parts(v)
         self.v_part, self.v_mid = codes * scales, (codes - 8) * scales
         self.v_terms = self.v_part + minima.abs()
-        self.v_scale = scales.amax(-1)  # [B, Hk, L]
+        self.v_unit, self.v_scale = scales, scales.amax(-1)
 
 
 def reference_and_bound(q, cache, spans, window, sinks, scale):
@@ -113,6 +123,9 @@ def reference_and_bound(q, cache, spans, window, sinks, scale):
                 delta += (2.0**-23 * (terms / math.log(2) + 4)).square()
                 if h_kv:
                     delta += h_kv**2 / 3 * scale**2 * torch.matmul(qq.square(), k.square().t().contiguous())
+                if cache.bits == 4 and few:
+                    cut = 2.0**-14 * scale * qq.abs().amax(-1, keepdim=True) * cache.k_unit[i, h, :n]
+                    delta += d / 3 * cut.square()
                 w2 = w.square()
                 wd = w2 * delta
                 var = torch.matmul(wd, v.square()) - 2 * o * torch.matmul(wd, v) + o.square() * wd.sum(-1, keepdim=True)
@@ -127,5 +140,8 @@ def reference_and_bound(q, cache, spans, window, sinks, scale):
                     lost = step * largest.amax(-1, keepdim=True)
                     var += lost.square() / 3 * torch.matmul(see.double(), size.square())
                 out[i, heads, t0:t1] = o
-                bound[i, heads, t0:t1] = half_step(dtype) * o.abs() + Z * var.sqrt()
+                smallest = 2.0**-14 if dtype == torch.float16 else 0.0
+                bound[i, heads, t0:t1] = half_step(dtype) * o.abs().clamp_min(smallest) + Z * var.sqrt()
+                if cache.bits == 4 and few:
+                    bound[i, heads, t0:t1] += 7 * 2.0**-14 * torch.matmul(w, cache.v_unit[i, h, :n])
     return out, bound

@@ -111,3 +111,22 @@ def test_scores_of_any_size(dtype, bits, power, t, length, d):
         cache.append(k, v, 0)
         got = kv4_attention(q, cache, scale=scale)
     check(got, want, bound, spans, 7.0)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("power", [0, -6, -10, -14])
+@pytest.mark.parametrize("b,hk,t,length,d", [(16, 8, 1, 2000, 128), (1, 1, 1, 5000, 128), (8, 8, 1, 900, 256),
+                                             (1, 1, 20, 700, 128), (1, 1, 150, 700, 128)])
+def test_kv4_groups_of_mixed_size(dtype, power, b, hk, t, length, d):
+    """A strong key, and value groups 2^power as large as their neighbours: each group is as
+    exact as if it were alone."""
+    q, k, v = make(dtype, b, hk, 1, t, length, d)
+    q.fill_(1.0)
+    k.zero_()
+    k[:, :, 37] = 12 * math.log(2)
+    v[..., 64:128] *= 2.0**power
+    cache = Int4KVCache(b, hk, length, d)
+    cache.append(k, v, 0)
+    spans = [(length, t)] * b
+    want, bound = reference_and_bound(q, Cache(k, v, 4), spans, None, 0, 1 / d)
+    check(kv4_attention(q, cache, scale=1 / d), want, bound, spans, 7.0)
