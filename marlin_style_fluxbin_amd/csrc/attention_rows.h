@@ -246,6 +246,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attention_rows_kern
       }
       f = ldexpf(f, -shift);
     }
+    f = fmaxf(f, 0x1p-126f);  // scores that vanish: not 0, which a hidden score's -inf makes NaN
     // the loads end here: a first use inside the loop would wait, every time round, for
     // the tiles in flight too
 #pragma unroll

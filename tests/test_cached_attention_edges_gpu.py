@@ -130,3 +130,23 @@ def test_kv4_groups_of_mixed_size(dtype, power, b, hk, t, length, d):
     spans = [(length, t)] * b
     want, bound = reference_and_bound(q, Cache(k, v, 4), spans, None, 0, 1 / d)
     check(kv4_attention(q, cache, scale=1 / d), want, bound, spans, 7.0)
+
+
+# ------------------------------------------------------------------ the ends of the ranges
+@pytest.mark.parametrize("bits,q_value,scale", [(4, 2.0**-133, 1e-3), (4, 2.0**-126, 1e-6), (16, 1.0, 1e-42),
+                                                (4, 1.0, 1e-42)])
+@pytest.mark.parametrize("t", [1, 150])
+def test_scores_that_vanish(bits, q_value, scale, t):
+    """Queries and scales so small that every score is zero: the mean of the visible values."""
+    b, hk, g, length, d = 1, 2, 2, 260, 128
+    q, k, v = make(BF, b, hk, g, t, length, d)
+    q.fill_(q_value)
+    spans = [(length, t)]
+    want, bound = reference_and_bound(q, Cache(k, v, bits), spans, None, 0, scale)
+    if bits == 16:
+        got = window_attention(q, k, v, scale=scale)
+    else:
+        cache = Int4KVCache(b, hk, length, d)
+        cache.append(k, v, 0)
+        got = kv4_attention(q, cache, scale=scale)
+    check(got, want, bound, spans, 7.0)
