@@ -7,7 +7,8 @@ ragged lengths, prompts and chunks of any number of tokens, a window of the last
 with a few first tokens that stay visible, and an :class:`Int4KVCache` in a quarter of the
 bytes (4.5 bits a value).  Every call goes to the HIP kernels behind
 ``include/fluxbin_attention.h`` on the current stream of the tensors' device; there is no
-CPU substitute and no backward pass.  Lengths stay on the device, so calls can be captured
+CPU substitute, no backward pass and no forward-mode derivative, and calls are not traced
+(what would need one of them is refused).  Lengths stay on the device, so calls can be captured
 into a HIP graph and follow the lengths of each replay.
 """
 from __future__ import annotations
@@ -17,6 +18,7 @@ import math
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -84,6 +86,39 @@ def _counts(name: str, t: torch.Tensor, batch: int, index: int) -> int:
 
 def _no_gradient() -> None:
     raise ValueError("cached attention has no backward pass; call it under torch.no_grad()")
+
+
+# torch's own queries; they are internal, and a torch without one has nothing in force
+_jit_tracer = getattr(torch._C, "_get_tracing_state", lambda: None)
+_dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 0)
+
+
+def _fx_tracer() -> bool:
+    """True while make_fx records, in either of its forms."""
+    keys = getattr(torch._C, "_TorchDispatchModeKey", None)
+    if _dispatch_modes() and keys is not None and torch._C._get_dispatch_mode(keys.PROXY) is not None:
+        return True
+    return _key_included(_PRE_DISPATCH)
+
+
+_PRE_DISPATCH = getattr(getattr(torch._C, "DispatchKey", None), "PreDispatch", None)
+_key_included = getattr(torch._C, "_dispatch_tls_is_dispatch_key_included", None)
+if _PRE_DISPATCH is None or _key_included is None:
+    def _key_included(key) -> bool:
+        return False
+
+
+def _refuse_records(*tensors: torch.Tensor | None) -> None:
+    """What a kernel called by address writes carries no tangent, and a tracer's record of the
+    call would hold its output's allocation alone.  (torch.compile breaks its graph at the call
+    and runs it as it is.)"""
+    if torch.compiler.is_dynamo_compiling():
+        return
+    if _jit_tracer() is not None or _fx_tracer():
+        raise ValueError("cached attention cannot be traced: its kernels would be missing from the record")
+    if getattr(forward_ad, "_current_level", -1) >= 0:
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise ValueError("cached attention has no forward-mode derivative: an argument carries a tangent")
 
 
 def _launch(name: str, device: torch.device, *args) -> None:
@@ -173,6 +208,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengt
     _check_head_dim(shape[3])
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         _no_gradient()
+    _refuse_records(q, k, v, out)
     k, k_ptr, k_strides = _rows(k)
     v, v_ptr, v_strides = _rows(v)
     return _attention("fx_window_attention", q, shape[:3], (k_ptr, v_ptr), (*k_strides, *v_strides), lengths,
@@ -235,6 +271,7 @@ class Int4KVCache:
             raise ValueError("k and v must be [batch, kv_heads, tokens, head_dim] of the cache")
         if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
             _no_gradient()
+        _refuse_records(k, v)
         start_ptr, start_all = None, 0
         if isinstance(start, torch.Tensor):
             start_ptr = _counts("start", start, batch, index)
@@ -256,6 +293,7 @@ class Int4KVCache:
             raise ValueError("length must be an integer in [0, max_len]")
         if dtype not in _HALF:
             raise ValueError("dtype must be fp16 or bf16")
+        _refuse_records()
         shape = (self.batch, self.kv_heads, length, self.head_dim)
         k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
         _launch("fx_kv4_restore", self.device, *self._pointers(), k.data_ptr(), v.data_ptr(), self.batch, self.kv_heads,
@@ -275,5 +313,6 @@ def kv4_attention(q: torch.Tensor, cache: Int4KVCache, *, lengths: torch.Tensor 
         raise ValueError("q must have the cache's head_dim")
     if q.requires_grad and torch.is_grad_enabled():
         _no_gradient()
+    _refuse_records(q, out)
     return _attention("fx_kv4_attention", q, (cache.batch, cache.kv_heads, cache.max_len), cache._pointers(), (),
                       lengths, query_lengths, window, sinks, scale, out, 1)

@@ -150,3 +150,56 @@ def test_scores_that_vanish(bits, q_value, scale, t):
         cache.append(k, v, 0)
         got = kv4_attention(q, cache, scale=scale)
     check(got, want, bound, spans, 7.0)
+
+
+# ------------------------------------------------------------------ calls that are refused
+def test_what_a_kernel_cannot_record_is_refused():
+    """Forward-mode tangents and tracers: the kernels would drop the one and leave no trace of
+    themselves in the other's record."""
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    q, k, v = make(BF, 1, 2, 2, 3, 40, 64)
+    want = window_attention(q, k, v)
+    cache = Int4KVCache(1, 2, 40, 64)
+    cache.append(k, v, 0)
+    want4 = kv4_attention(q, cache)
+    out = torch.zeros_like(q)
+    before = [x.clone() for x in cache._parts()]
+    with forward_ad.dual_level():
+        dual = lambda x: forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: window_attention(dual(q), k, v), lambda: window_attention(q, dual(k), v),
+                     lambda: window_attention(q, k, dual(v)), lambda: window_attention(q, k, v, out=dual(out)),
+                     lambda: kv4_attention(dual(q), cache), lambda: kv4_attention(q, cache, out=dual(out)),
+                     lambda: cache.append(dual(k), v, 0), lambda: cache.append(k, dual(v), 0)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        assert torch.equal(window_attention(q, k, v), want)  # no tangent: as ever
+        assert torch.equal(kv4_attention(q, cache), want4)
+        cache.append(k, v, 0)
+    for call in (lambda x: window_attention(x, k, v), lambda x: kv4_attention(x, cache),
+                 lambda x: cache.append(k, v, 0) or x + 1, lambda x: cache.restore()[0]):
+        with pytest.raises(ValueError, match="trac"):
+            torch.jit.trace(call, (q,))
+        with pytest.raises(ValueError, match="trac"):
+            make_fx(call)(q)
+    for call in (lambda x: window_attention(x, k, v), lambda x: kv4_attention(x, cache)):
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.func.jvp(call, (q,), (torch.ones_like(q),))
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.func.vmap(call)(torch.stack((q, q)))
+    assert (out == 0).all() and all(torch.equal(x, y) for x, y in zip(before, cache._parts()))
+    assert torch.equal(window_attention(q, k, v), want)
+
+
+def test_a_compiled_caller_runs_the_call_as_it_is():
+    q, k, v = make(BF, 1, 2, 2, 3, 40, 64)
+    cache = Int4KVCache(1, 2, 40, 64)
+
+    def step(q, k, v):
+        cache.append(k * 1, v, 0)
+        return window_attention(q * 1, k, v, window=9), kv4_attention(q, cache) * 1, cache.restore()[0]
+
+    want = step(q, k, v)
+    got = torch.compile(step, backend="eager")(q, k, v)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
