@@ -56,6 +56,28 @@ def _rows(t: torch.Tensor, copy: bool = True):
     return t, t.data_ptr(), s
 
 
+def _disjoint(shape, strides) -> bool:
+    """No element of the rows at these (batch, head, row) strides is another's memory."""
+    b, h, t, dim = shape
+    s0, s1, s2 = strides
+    if dim <= s1 and h * s1 <= s2 and t * s2 <= s0 or dim <= s2 and t * s2 <= s1 and h * s1 <= s0:
+        return True  # in the order of the axes, either way
+    axes = sorted((s, n) for s, n in ((s0, b), (s1, h), (s2, t)) if n != 1)
+    extent = dim
+    for s, n in axes:  # each axis behind all that lies within its step
+        if s < extent:
+            break
+        extent += s * (n - 1)
+    else:
+        return True
+    if any(n == 0 for _, n in axes):
+        return True
+    starts = torch.zeros(1, dtype=torch.int64, device="cpu")
+    for s, n in axes:  # rows in each other's gaps: every one of them
+        starts = (starts[:, None] + s * torch.arange(n, dtype=torch.int64, device="cpu")).flatten()
+    return bool((starts.sort().values.diff() >= dim).all())
+
+
 _BF16, _FP16 = torch.bfloat16, torch.float16
 
 
@@ -168,7 +190,7 @@ def _attention(name, q, cache, cache_args, cache_strides, lengths, query_lengths
     elif out.requires_grad and torch.is_grad_enabled():
         _no_gradient()
     rows = _rows(out, copy=False)
-    if rows is None or (0 in rows[2] and any(s == 0 and n > 1 for n, s in zip(shape, rows[2]))):
+    if rows is None or not _disjoint(shape, rows[2]):
         raise ValueError("out must have contiguous 16-byte aligned rows, each its own memory")
     _, out_ptr, out_strides = rows
     q, q_ptr, q_strides = _rows(q)

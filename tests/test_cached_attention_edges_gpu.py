@@ -203,3 +203,15 @@ def test_a_compiled_caller_runs_the_call_as_it_is():
     want = step(q, k, v)
     got = torch.compile(step, backend="eager")(q, k, v)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_an_output_whose_rows_overlap_is_refused():
+    q, k, v = make(BF, 2, 2, 2, 5, 40, 64)
+    want = window_attention(q, k, v)
+    memory = torch.zeros(2 * 4 * 5 * 64, dtype=BF, device="cuda")
+    for bad in ((1280, 320, 32, 1), (1280, 64, 64, 1), (640, 320, 64, 1), (8, 320, 64, 1), (1280, 0, 64, 1)):
+        with pytest.raises(ValueError, match="its own memory"):
+            window_attention(q, k, v, out=memory.as_strided(q.shape, bad))
+    assert (memory == 0).all()
+    for good in ((1280, 320, 64, 1), (1280, 64, 256, 1), (320, 640, 64, 1), (64, 128, 512, 1), (256, 64, 512, 1)):
+        assert torch.equal(window_attention(q, k, v, out=memory.as_strided(q.shape, good)), want)
