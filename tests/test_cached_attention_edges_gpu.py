@@ -215,3 +215,53 @@ def test_an_output_whose_rows_overlap_is_refused():
     assert (memory == 0).all()
     for good in ((1280, 320, 64, 1), (1280, 64, 256, 1), (320, 640, 64, 1), (64, 128, 512, 1), (256, 64, 512, 1)):
         assert torch.equal(window_attention(q, k, v, out=memory.as_strided(q.shape, good)), want)
+
+
+# ------------------------------------------------------------------ large addresses
+def test_16_bit_caches_past_2_to_32_bytes():
+    """Keys, values, queries and outputs beyond 2^32 bytes of their tensors' starts, in both
+    kernels, and read by append."""
+    b, hk, g, n, d, tail, window = 18, 8, 4, 131072, 128, 300, 200
+    k, v = (torch.zeros(b, hk, n, d, dtype=BF, device="cuda") for _ in range(2))
+    assert k[-1].data_ptr() - k.data_ptr() > 2**32
+    for t in (1, 100):
+        q, kk, vv = make(BF, 1, hk, g, t, tail, d)
+        k[-1:, :, -tail:], v[-1:, :, -tail:] = kk, vv
+        want, bound = reference_and_bound(q, Cache(kk, vv, 16), [(tail, t)], window, 0, 1 / math.sqrt(d))
+        got = window_attention(q.expand(b, -1, -1, -1), k, v, window=window)
+        check(got[-1:], want, bound, [(tail, t)], 7.0)
+        assert (got[:-1] == 0).all()
+        # two sequences' q and out 2^32 bytes apart
+        apart = (2**31, d, hk * g * d, 1)
+        far = [torch.zeros(2**31 + t * hk * g * d, dtype=BF, device="cuda").as_strided((2, hk * g, t, d), apart)
+               for _ in range(2)]
+        far[0][1:] = q
+        got = window_attention(far[0], k[-2:], v[-2:], window=window, out=far[1])
+        check(got[1:], want, bound, [(tail, t)], 7.0)
+        assert (got[0] == 0).all()
+    cache, small = Int4KVCache(b, hk, n, d), Int4KVCache(1, hk, tail, d)
+    cache.append(k, v, 0)
+    small.append(kk, vv, 0)
+    assert all(torch.equal(x[-1:, :, -tail:], y) for x, y in zip(cache._parts(), small._parts()))
+    assert all((x[:-1] == 0).all() for x in cache._parts())
+
+
+def test_4_bit_caches_past_2_to_32_bytes():
+    b, hk, g, n, d, tail, window = 68, 8, 4, 131072, 128, 300, 200
+    cache = Int4KVCache(b, hk, n, d)
+    assert cache.k_codes[-1].data_ptr() - cache.k_codes.data_ptr() > 2**32
+    start = torch.full((b,), n, dtype=torch.int32, device="cuda")
+    start[-1] = n - tail
+    for dtype, t in ((BF, 1), (BF, 100), (HF, 100)):  # the rows kernel: bf16's 100 tokens
+        q, kk, vv = make(dtype, 1, hk, g, t, tail, d)
+        small = Int4KVCache(1, hk, tail, d)
+        small.append(kk, vv, 0)
+        cache.append(kk.expand(b, -1, -1, -1), vv.expand(b, -1, -1, -1), start)  # the other positions do not exist
+        assert all(torch.equal(x[-1:, :, -tail:], y) for x, y in zip(cache._parts(), small._parts()))
+        want, bound = reference_and_bound(q, Cache(kk, vv, 4), [(tail, t)], window, 0, 1 / math.sqrt(d))
+        got = kv4_attention(q.expand(b, -1, -1, -1), cache, window=window)
+        check(got[-1:], want, bound, [(tail, t)], 7.0)
+        assert (got[:-1] == 0).all()
+    for x, y in zip(cache.restore(dtype=HF), small.restore(dtype=HF)):
+        assert x[-1].data_ptr() - x.data_ptr() > 2**34
+        assert torch.equal(x[-1:, :, -tail:], y) and (x[-1, :, :-tail] == 0).all() and not x[:-1].any()
