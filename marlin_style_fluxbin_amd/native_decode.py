@@ -492,13 +492,20 @@ class NativeDecodeSession:
             self.prefill_logits = out.logits[:, -1, :].detach().clone()
             shape = (n, self.kv_heads, self.maximum_length, self.head_dim)
             self.int4_cache = self.k_cache = self.v_cache = None
+            prefix = [(l.keys[:, :, :self.prefix_length], l.values[:, :, :self.prefix_length]) for l in cache.layers]
+            self.prefix_k = self.prefix_v = None
             if kv_cache == "int4":
+                # quantized once: no step writes in front of its own position, so reset() has
+                # nothing to restore and no 16-bit copy of the prefix stays
                 self.int4_cache = [Int4KVCache(1, *shape[1:], device=self.device) for _ in range(n)]
+                for packed, (k, v) in zip(self.int4_cache, prefix):
+                    packed.append(k, v, 0)
             else:
                 self.k_cache = torch.zeros(shape, dtype=dtype, device=self.device)
                 self.v_cache = torch.zeros(shape, dtype=dtype, device=self.device)
-            self.prefix_k = torch.stack([l.keys[0, :, :self.prefix_length] for l in cache.layers]).clone()
-            self.prefix_v = torch.stack([l.values[0, :, :self.prefix_length] for l in cache.layers]).clone()
+                self.prefix_k = torch.stack([k[0] for k, _ in prefix])
+                self.prefix_v = torch.stack([v[0] for _, v in prefix])
+            del prefix
             # cos/sin rows for every position, built by the model's own rotary module
             positions = torch.arange(self.maximum_length, device=self.device)[None]
             cos, sin = model.model.rotary_emb(self.prefill_logits.to(dtype), positions)
@@ -716,9 +723,7 @@ class NativeDecodeSession:
     @torch.inference_mode()
     def reset(self):
         if self.int4_cache is not None:
-            for cache, k, v in zip(self.int4_cache, self.prefix_k, self.prefix_v):
-                cache.append(k[None], v[None], 0)
-            return
+            return  # the prefix is still there; lengths hide the positions behind each step's own
         self.k_cache.zero_()
         self.v_cache.zero_()
         self.k_cache[:, :, :self.prefix_length].copy_(self.prefix_k)
