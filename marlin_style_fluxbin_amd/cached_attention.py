@@ -110,24 +110,14 @@ def _no_gradient() -> None:
     raise ValueError("cached attention has no backward pass; call it under torch.no_grad()")
 
 
-# torch's own queries; they are internal, and a torch without one has nothing in force
-_jit_tracer = getattr(torch._C, "_get_tracing_state", lambda: None)
-_dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 0)
-
-
-def _fx_tracer() -> bool:
-    """True while make_fx records, in either of its forms."""
-    keys = getattr(torch._C, "_TorchDispatchModeKey", None)
-    if _dispatch_modes() and keys is not None and torch._C._get_dispatch_mode(keys.PROXY) is not None:
-        return True
-    return _key_included(_PRE_DISPATCH)
-
-
+# torch's own queries of what records a call: jit.trace, make_fx and its pre-dispatch form.
+# They are internal; a torch without one has nothing of its kind in force.
+_PROXY = getattr(getattr(torch._C, "_TorchDispatchModeKey", None), "PROXY", None)
 _PRE_DISPATCH = getattr(getattr(torch._C, "DispatchKey", None), "PreDispatch", None)
-_key_included = getattr(torch._C, "_dispatch_tls_is_dispatch_key_included", None)
-if _PRE_DISPATCH is None or _key_included is None:
-    def _key_included(key) -> bool:
-        return False
+_jit_tracer = getattr(torch._C, "_get_tracing_state", lambda: None)
+_mode_count = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 0)
+_mode_of = getattr(torch._C, "_get_dispatch_mode", lambda key: None)
+_key_included = getattr(torch._C, "_dispatch_tls_is_dispatch_key_included", lambda key: False)
 
 
 def _refuse_records(*tensors: torch.Tensor | None) -> None:
@@ -136,17 +126,22 @@ def _refuse_records(*tensors: torch.Tensor | None) -> None:
     and runs it as it is.)"""
     if torch.compiler.is_dynamo_compiling():
         return
-    if _jit_tracer() is not None or _fx_tracer():
+    if (_jit_tracer() is not None or (_mode_count() and _mode_of(_PROXY) is not None)
+            or _key_included(_PRE_DISPATCH)):
         raise ValueError("cached attention cannot be traced: its kernels would be missing from the record")
     if getattr(forward_ad, "_current_level", -1) >= 0:
         if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
             raise ValueError("cached attention has no forward-mode derivative: an argument carries a tangent")
 
 
+# (the arguments are on a GPU, so torch has initialised it)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _launch(name: str, device: torch.device, *args) -> None:
     """The library call with ``device`` current (kernels launch on the current device)."""
     call = getattr(_lib.library(), name)
-    if torch.cuda.current_device() == device.index:
+    if _current_device() == device.index:
         rc = call(*args, _lib.stream_handle(device))
     else:
         with torch.cuda.device(device):
@@ -271,7 +266,7 @@ class Int4KVCache:
         return self.k_codes, self.k_scales, self.v_codes, self.v_scales
 
     def _pointers(self):
-        return tuple(t.data_ptr() for t in self._parts())
+        return (self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(), self.v_scales.data_ptr())
 
     def append(self, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor | int, *,
                counts: torch.Tensor | None = None) -> None:
