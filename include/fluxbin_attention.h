@@ -10,9 +10,10 @@
  * h / (n_q_heads / n_kv_heads):
  *   out = sum_j softmax_j(scale q . k_j) v_j
  * with fp32 scores, softmax and accumulation, p rounded to 16 bits as the matrix cores take
- * it, out rounded once.  A query that sees no key (p < 0) gives zeros; rows t >= m of out
- * are left as they are.  Keys that a query does not see never reach its row, whatever they
- * hold.  lengths and query_lengths are int32 arrays in device memory, read by the kernels:
+ * it (fp16: weights below 2^-32 of a row's largest count as zero), out rounded once.  A query
+ * that sees no key (p < 0) gives zeros; rows t >= m of out are left as they are.  Keys that a
+ * query does not see never reach its row, whatever they hold; an infinity or NaN that it sees
+ * does.  lengths and query_lengths are int32 arrays in device memory, read by the kernels:
  * a captured call follows their contents on every replay.
  *
  * The launches are chosen from the sizes alone (never from the lengths); a call takes one or

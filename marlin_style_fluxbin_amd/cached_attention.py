@@ -214,7 +214,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengt
     None: all) or ``j < sinks``.  A query in front of the first key gives zeros; rows behind
     ``query_lengths[b]`` stay as they are in ``out`` and are zeros in a new output.  ``scale``
     defaults to ``1 / sqrt(head_dim)``.  fp16 or bf16, head_dim 64, 128 or 256, any strides
-    (rows that are not 16-byte aligned are copied first, ``out`` is refused)."""
+    (rows that are not 16-byte aligned are copied first, ``out`` is refused; positions of a cache
+    at most 2^22 elements apart)."""
     dtype, index = q.dtype, q.get_device()
     if not (q.ndim == k.ndim == v.ndim == 4 and index >= 0 and (dtype is _BF16 or dtype is _FP16)
             and k.dtype is dtype and v.dtype is dtype and k.get_device() == index and v.get_device() == index):

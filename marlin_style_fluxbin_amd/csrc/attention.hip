@@ -8,8 +8,8 @@ namespace fx {
 // The join of a row's key splits: o = sum_s w_s o_s / sum_s w_s l_s, w_s = 2^(m_s - max m).
 // W waves a row (every wave forms the weights: lane s holds split s, splits <= 64), each
 // with its share of at most N splits loaded at once; four rows (W = 1) or one a workgroup.
-// Bound by the launch and one round trip: 64 splits of 32 rows 4.7 us, with one wave looping
-// over them 17.7; many rows by the partials: 2 splits of 32768 rows of 128 columns 13 us.
+// Bound by the launch and one round trip: 64 splits of 32 rows 4.0 us, with one wave looping
+// over them 17.7; many rows by the partials: 2 splits of 32768 rows of 128 columns 14 us.
 template <int DT, int D, int N, int W>
 __global__ __launch_bounds__(256) void attention_combine_kernel(const CachedAttentionArgs a) {
   constexpr int kRows = 4 / W, kCols = D / 64;
@@ -68,12 +68,12 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(const CachedAtte
 }
 
 // How many splits of the keys: more shorten every workgroup's way until the chip is full, and
-// cost the join's launch and the partial results, written and read.  The times (us) are those
-// of 30 sizes measured with 1 .. 64 splits; the choice is within 10% of the best at nearly all
-// of them.  Splits until the chip is full, whatever the join costs, took up to 60% longer: 301
-// tokens of 14 heads of 64 columns, window 257, 18.3 us (2 splits) for 12.6 (1); 300 tokens
-// of 16 heads of 256 columns over 2000 keys 52.6 us (13) for 38.1 (6); 24 sequences' tokens over
-// a window of 4096 keys 83 us (6) for 74 (1).
+// cost the join's launch and the partial results, written and read.  The constants below (us)
+// are fits; of 36 sizes measured with 1 .. 64 splits the choice is within 5% of the best at 30
+// and within 17% at all.  Splits until the chip is full, whatever the join costs, take longer:
+// 3 x 301 tokens of 14 heads of 64 columns, window 257, 19.1 us (2 splits) for 12.5 (1); 1000
+// tokens of 32 heads over their own keys 36.7 (2) for 27.9 (1); 2 x 300 tokens of 16 heads of
+// 256 columns over 2000 keys 86 (12) for 46 (3).
 struct SplitTimes {
   long groups, tiles;  // workgroups of a split, key tiles
   int waves;           // of a workgroup along the keys
@@ -102,14 +102,14 @@ int best_splits(const SplitTimes& t, long most, float* best) {
 
 // Which kernel: up to 16 query rows of a KV head fit one operand of the few-rows kernel.  A
 // 4-bit cache keeps it for up to 64 rows (5 tokens of 7 heads over 4101 keys of 8 sequences
-// of 4 KV heads: 21 us, the rows kernel 25 us on half as exact fp16 results), and always for
+// of 4 KV heads: 20 us, the rows kernel 25 us on half as exact fp16 results), and always for
 // fp16 queries: the rows kernel widens the cache to fp16, which a bf16 output does not show
 // and an fp16 output does (error of the output 1.5 to 2 times its own rounding's).
 //
 // `wide`: workgroups of eight waves, 256 rows, in the rows kernel over a 4-bit cache, so that
-// half as many of them widen a tile.  1024 tokens of 32 heads over 9000 keys 199 us (four
-// waves 215), 4096 tokens of a prompt 177 (195); but with a window of 1024 keys, where it
-// leaves half the chip empty, 54 (37.5): taken where the estimate of the split times is
+// half as many of them widen a tile.  1024 tokens of 32 heads over 9000 keys 186 us (four
+// waves 201), 4096 tokens of a prompt 169 (188); but 1024 tokens over a window of 1024 keys,
+// where it leaves half the chip empty, 54 (39): taken where the estimate of the split times is
 // smaller.
 CachedAttentionPlan plan_with(bool wide, int dt, int B, int Hk, int G, int T, int L, int D, int window, int sinks,
                               bool kv4, float* time) {

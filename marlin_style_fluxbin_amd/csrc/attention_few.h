@@ -2,10 +2,11 @@
 // decode step, or a few drafted tokens; over a 4-bit cache with fp16 queries any number of
 // them.  Bound by reading the cache once: 24 sequences x 4100 keys x 8 heads of 128 16-bit
 // columns 74 us (5.4 TB/s; a large copy moves 4.8), 32 x 16384..32768 in 4 bits 190 us
-// (4.8 TB/s).  Short calls are bound by the two launches and their chain of loads: 2000 keys
-// of one sequence 9.5 us.  Several row groups (5 tokens of 7 heads over 4101 keys of 8
-// sequences of 4 KV heads in 4 bits: 21 us, 7 of them for one key alone) are bound by the
-// vector work on the codes, ~600 instructions for 32 keys and 32 rows.
+// (4.8 TB/s).  D = 256 on a 16-bit cache spills 33 registers and asks for no tile ahead: 8 x
+// 8192 keys of 8 heads 129 us (4.2 TB/s).  Short calls are bound by the two launches and their
+// chain of loads: 2000 keys of one sequence 9.5 us.  Several row groups (5 tokens of 7 heads
+// over 4101 keys of 8 sequences of 4 KV heads in 4 bits: 20 us, 10 of them for 5 keys too) are
+// bound by the vector work on the codes, ~600 instructions for 32 keys and 32 rows.
 //
 // A wave takes 32 keys at a time straight from memory into operand registers, with the
 // next 32 on their way: S^T = K Q^T and O^T += V^T P^T on 16 x 16 x 32 products, column =

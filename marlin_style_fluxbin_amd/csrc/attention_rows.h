@@ -20,14 +20,17 @@
 // multiplied; the 4-bit cache is widened in registers and stored.
 //
 // Bound by the matrix cores, at the clock that their power leaves: 16384 tokens of 32 heads
-// on 8 KV heads, D = 128, causal: 2034 us, 1.08 PFLOP/s, where a library product of 8192^3
-// reaches 1.26; the products are issued 59% of the time, the exponentials and the maxima,
-// which need the vector pipe, beside them.  D = 256 (4096 tokens, 16 heads) 0.78 PFLOP/s and
-// D = 64 (32 heads) 0.70: per score as many exponentials for half the products.  With a window
-// of 1024 keys (4096 tokens, 32 heads) 81 us: three of 18 tiles (the sinks', both ends') are
-// computed whole for a part, and q and the output are 67 MB, 14 us at a copy's rate.  A 4-bit cache (1024 tokens over 9000 keys) 170 us: each row
-// tile of a head widens the keys that it reads, a fifth of its time at 128 rows, an eighth
-// at 256.
+// on 8 KV heads, D = 128, causal: 2000 to 2130 us on different cards, 1.03 to 1.10 PFLOP/s,
+// where a library product of 8192^3 reaches 1.26; the products are issued 59% of the time, the
+// exponentials and the maxima, which need the vector pipe, beside them.  D = 256 (4096 tokens,
+// 16 heads) 174 us, 0.79 PFLOP/s, and D = 64 (32 heads) 100 us, 0.69: per score as many
+// exponentials for half the products.  With a window of 1024 keys (4096 tokens, 32 heads) 80 to
+// 91 us: three of 18 tiles (the sinks', both ends') are computed whole for a part, and q and
+// the output are 67 MB, 14 us at a copy's rate.  A 4-bit cache (1024 tokens over 9000 keys; two
+// splits) 186 us, the join's 14 among them: each row tile of a head widens the keys that it
+// reads, a fifth of its time at 128 rows, an eighth at 256.
+// Registers: spilled are 13 (D = 128, outside the loop over the tiles), over a 4-bit cache 26 to 30
+// (D = 128, a few of them in each tile) and 9 (D = 256); the others fit.
 // 128 rows, so that a key or value read from LDS meets 32 columns a wave, four waves a
 // tile: two workgroups a CU, one's exponentials beside the other's products.  256 rows and one
 // workgroup where that halves the widening (a 4-bit cache, D <= 128).
