@@ -81,6 +81,13 @@ __device__ __forceinline__ unsigned finite_pair(unsigned w) {
   return w & ~((bad >> 15) * 0xffffu);
 }
 
+// The least score (log2 units) whose p is not zero in 16 bits beside the running maximum m.  A
+// visible infinity must not meet a zero p: where one lies in a tile, lower scores are raised to
+// it (beside a row's largest, 2^7 and more in fp16, what that adds to others is nothing).  A row
+// without a score yet keeps its -inf.
+template <int DT>
+__device__ __forceinline__ float least_score(float m) { return m - (DT == kF16 ? 24.f : 125.f); }
+
 // A sequence's share of the call, and the keys that its query rows see.
 struct SequenceSpan {
   int n, m;  // keys, queries

@@ -321,6 +321,12 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
       }
       if (!whole) hide(rt, j0, sink_tile, s);
       raise(rt, s, 0.f, CDT == kF16 ? 15.f : 0.f);
+      if (whole && careful) {
+        asm volatile("");
+        const float least = least_score<CDT>(m[rt]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = s[e] < least ? least : s[e];
+      }
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         float p0 = __builtin_amdgcn_exp2f(s[e] - m_use[rt]), p1 = __builtin_amdgcn_exp2f(s[e + 1] - m_use[rt]);
@@ -328,10 +334,9 @@ __global__ __launch_bounds__(64 * NW, KV4 && RT == 1 && D <= 128 ? 3 : 2) void a
         pf[rt][e / 2] = round_pair_bits<CDT>(p0, p1);
       }
     }
-    if (careful) {
-      // an infinity or NaN must not meet a zero p, a hidden key's or one too small for 16 bits:
-      // rows that see one take it by hand (every lane reads the rows it needs again), then it
-      // counts as zero
+    if (!whole && careful) {
+      // a hidden key's infinity or NaN must not meet its zero p: rows that see one take it
+      // by hand (every lane reads the rows it needs again), then it counts as zero
       unsigned bad = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e)

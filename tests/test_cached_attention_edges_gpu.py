@@ -265,3 +265,41 @@ def test_4_bit_caches_past_2_to_32_bytes():
     for x, y in zip(cache.restore(dtype=HF), small.restore(dtype=HF)):
         assert x[-1].data_ptr() - x.data_ptr() > 2**34
         assert torch.equal(x[-1:, :, -tail:], y) and (x[-1, :, :-tail] == 0).all() and not x[:-1].any()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t,length", [(1, 300), (4, 700), (150, 400)])
+def test_rows_of_minus_infinity_beside_infinite_values(dtype, d, t, length):
+    """A head whose scores are all -inf is NaN, beside one that sees an infinite value."""
+    q, k, v = make(dtype, 1, 1, 2, t, length, d)
+    q[:, 0], q[:, 1] = -1.0, 0.0
+    k.fill_(1.0)
+    k[..., 0] = INF
+    q[:, 1, :, 0] = 1.0  # +inf against +inf
+    k2 = k.clone()
+    k2[..., 0] = 1.0
+    v[:, :, 20, 3] = INF
+    got = window_attention(q, k, v)
+    assert torch.isnan(got).all()
+    got = window_attention(q, k2, v)
+    assert (got[..., 3] == INF).all() and torch.isfinite(got[..., 4:]).all()
+    q[:, 1] = 0.0
+    k3 = torch.zeros_like(k)
+    k3[..., 1] = -INF
+    q[:, 0], q[:, 1] = 1.0, 0.0  # the second: 0 times -inf, NaN
+    assert torch.isnan(window_attention(q, k3, v)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("t,length,d", [(1, 3000, 128), (150, 1000, 128), (150, 1000, 256)])
+def test_finite_columns_beside_infinite_ones(dtype, t, length, d):
+    """What an infinity in one column costs the others' exactness: nothing."""
+    q, k, v = make(dtype, 1, 2, 2, t, length, d)
+    spans = [(length, t)]
+    want, bound = reference_and_bound(q, Cache(k, v, 16), spans, None, 0, 1 / math.sqrt(d))
+    v[:, :, ::50, 3] = INF
+    v[:, :, 7::50, 4] = float("nan")
+    got = window_attention(q, k, v)
+    assert (got[..., 3] == INF).all() and torch.isnan(got[..., 4]).all()
+    check(got[..., 5:], want[..., 5:], bound[..., 5:], spans, 7.0)
