@@ -29,8 +29,9 @@
 // the output are 67 MB, 14 us at a copy's rate.  A 4-bit cache (1024 tokens over 9000 keys; two
 // splits) 186 us, the join's 14 among them: each row tile of a head widens the keys that it
 // reads, a fifth of its time at 128 rows, an eighth at 256.
-// Registers: spilled are 13 (D = 128, outside the loop over the tiles), over a 4-bit cache 26 to 30
-// (D = 128, a few of them in each tile) and 9 (D = 256); the others fit.
+// Registers: spilled are 13 (D = 128) and, in fp16, 17 to memory (D = 256), outside the loop over
+// the tiles; over a 4-bit cache 26 to 30 (D = 128, a few of them in each tile) and 10 (D = 256).
+// The others fit.
 // 128 rows, so that a key or value read from LDS meets 32 columns a wave, four waves a
 // tile: two workgroups a CU, one's exponentials beside the other's products.  256 rows and one
 // workgroup where that halves the widening (a 4-bit cache, D <= 128).
