@@ -535,5 +535,7 @@ int fx_hybrid_restore(const uint8_t *codes, const float *rows, const float *colu
 
 /* Cached attention with a sliding window and sinks, and the 4-bit key/value cache. */
 #include "fluxbin_attention.h"
+/* Products in 8-bit integers, and the rows that feed them. */
+#include "fluxbin_int8.h"
 
 #endif /* FLUXBIN_AMD_H */

@@ -6,7 +6,8 @@ LUT Linear (``w3_lut_deployment``), fused RMSNorm / RoPE (``fused_modules``) and
 the static-KV decode session (``static_decode``), and the two-base binary-basis
 formats (``packing``, ``evaluation``, ``deployment``, ``engine_interface``; the
 benchmark's rank-one variant in ``two_base``), and attention over long caches
-(``cached_attention``: sliding window with sinks, 4-bit key/value cache).  GPU work runs in hand-written
+(``cached_attention``: sliding window with sinks, 4-bit key/value cache), and Linears with 8-bit
+weights and activations (``int8_linear``).  GPU work runs in hand-written
 HIP kernels behind the C ABI of ``libfluxbin_amd.so`` (``include/fluxbin_amd.h``).
 """
 from .gptq_deployment import (  # noqa: F401
@@ -52,6 +53,17 @@ from .fused_modules import (  # noqa: F401
 )
 
 from .cached_attention import Int4KVCache, kv4_attention, window_attention  # noqa: F401
+from .int8_linear import (  # noqa: F401
+    PackedInt8Linear,
+    add_rms_norm_int8,
+    dequantize_int8,
+    int8_matmul,
+    quantize_int8,
+    quantize_weight_int8,
+    replace_int8_block_linears,
+    rms_norm_int8,
+    silu_mul_int8,
+)
 from .packing import pack_two_bases, unpack_two_bases  # noqa: F401
 from .evaluation import materialize_global_two_base_weight, materialize_hybrid_s8_weight  # noqa: F401
 from .deployment import PackedHybridLinear  # noqa: F401

@@ -91,6 +91,17 @@ ATTENTION_SIGNATURES: dict[str, tuple] = {
     "fx_kv4_restore": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p]),
 }
 
+# mirrors include/fluxbin_int8.h
+_l = ctypes.c_longlong
+INT8_SIGNATURES: dict[str, tuple] = {
+    "fx_int8_quantize": (_i, [_p, _l, _p, _l, _p, _i, _i, _i, _i, _p]),
+    "fx_int8_rmsnorm": (_i, [_p, _l, _p, _l, _p, _l, _p, _p, _l, _p, _i, _i, _i, _f, _i, _p]),
+    "fx_int8_silu_mul": (_i, [_p, _l, _p, _l, _p, _l, _p, _i, _i, _i, _i, _p]),
+    "fx_int8_restore": (_i, [_p, _l, _p, _p, _l, _i, _i, _i, _p]),
+    "fx_int8_gemm_workspace_bytes": (_sz, [_i, _i, _i]),
+    "fx_int8_gemm": (_i, [_p, _l, _p, _p, _l, _p, _p, _p, _l, _p, _sz, _i, _i, _i, _i, _p]),
+}
+
 _lock = threading.Lock()
 _library = None
 
@@ -109,7 +120,7 @@ def library():
                 "(or __graft_entry__.build()). There is no CPU substitute for the HIP kernels."
             )
         lib = ctypes.CDLL(str(LIBRARY_PATH))
-        for name, (restype, argtypes) in (SIGNATURES | ATTENTION_SIGNATURES).items():
+        for name, (restype, argtypes) in (SIGNATURES | ATTENTION_SIGNATURES | INT8_SIGNATURES).items():
             fn = getattr(lib, name)
             fn.restype = restype
             fn.argtypes = argtypes

@@ -120,7 +120,7 @@ _mode_of = getattr(torch._C, "_get_dispatch_mode", lambda key: None)
 _key_included = getattr(torch._C, "_dispatch_tls_is_dispatch_key_included", lambda key: False)
 
 
-def _refuse_records(*tensors: torch.Tensor | None) -> None:
+def _refuse_records(*tensors: torch.Tensor | None, what: str = "cached attention") -> None:
     """What a kernel called by address writes carries no tangent, and a tracer's record of the
     call would hold its output's allocation alone.  (torch.compile breaks its graph at the call
     and runs it as it is.)"""
@@ -128,10 +128,10 @@ def _refuse_records(*tensors: torch.Tensor | None) -> None:
         return
     if (_jit_tracer() is not None or (_mode_count() and _mode_of(_PROXY) is not None)
             or _key_included(_PRE_DISPATCH)):
-        raise ValueError("cached attention cannot be traced: its kernels would be missing from the record")
+        raise ValueError(f"{what} cannot be traced: its kernels would be missing from the record")
     if getattr(forward_ad, "_current_level", -1) >= 0:
         if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
-            raise ValueError("cached attention has no forward-mode derivative: an argument carries a tangent")
+            raise ValueError(f"{what} has no forward-mode derivative: an argument carries a tangent")
 
 
 # (the arguments are on a GPU, so torch has initialised it)

@@ -17,6 +17,7 @@
 #include "decode_launch.h"
 #include "lm_head_launch.h"
 #include "two_base_launch.h"
+#include "int8_launch.h"
 #include "w3_gemm_launch.h"
 #include "w3_restore_launch.h"
 #include "w3_split_launch.h"
@@ -1963,6 +1964,203 @@ int fx_kv4_restore(const void* k_codes, const void* k_scales, const void* v_code
   a.rows = rows;
   fx::launch_kv4_restore(dtype, head_dim, a, static_cast<hipStream_t>(stream));
   return check_launch("fx_kv4_restore");
+}
+
+}  // extern "C"
+
+namespace {
+
+bool aligned_to(const void* p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+int validate_int8_rows(const int8_t* codes, long long code_stride, const float* scales, int rows, int columns,
+                       int code_columns) {
+  if (rows < 0 || rows > (1 << 21)) return fail(FX_EINVAL, "rows must be in [0, 2^21], got %d", rows);
+  if (columns < 1 || columns > (1 << 20)) return fail(FX_EINVAL, "columns must be in [1, 2^20], got %d", columns);
+  if (code_columns < columns || code_columns > columns + 127)
+    return fail(FX_EINVAL, "code_columns must be in [%d, %d], got %d", columns, columns + 127, code_columns);
+  if (rows == 0) return FX_OK;
+  if (!codes || !scales) return fail(FX_EINVAL, "codes and scales must be non-null");
+  if (!aligned_to(scales, 4)) return fail(FX_EINVAL, "scales must be 4-byte aligned");
+  if (code_stride < code_columns && rows > 1)
+    return fail(FX_EINVAL, "codes stride %lld is shorter than a row of %d", code_stride, code_columns);
+  return FX_OK;
+}
+
+int validate_half_rows(const char* name, const void* p, long long stride) {
+  if (!p) return fail(FX_EINVAL, "%s must be non-null", name);
+  if (!aligned_to(p, 2)) return fail(FX_EINVAL, "%s must be 2-byte aligned", name);
+  if (stride < 0) return fail(FX_EINVAL, "%s stride must be non-negative, got %lld", name, stride);
+  return FX_OK;
+}
+
+int run_int8_rows(int mode, const fx::Int8RowsArgs& a, int dtype, void* stream, const char* what) {
+  fx::launch_int8_rows(dtype, mode, a, static_cast<hipStream_t>(stream));
+  return check_launch(what);
+}
+
+int validate_int8_gemm_sizes(int M, int N, int K) {
+  if (M < 0 || M > (1 << 21)) return fail(FX_EINVAL, "M must be in [0, 2^21], got %d", M);
+  if (N < 1 || N > (1 << 20)) return fail(FX_EINVAL, "N must be in [1, 2^20], got %d", N);
+  if (K < 16 || K % 16 != 0 || K > fx::kInt8MaxK)
+    return fail(FX_EINVAL, "K must be a positive multiple of 16 up to %d, got %d", fx::kInt8MaxK / 16 * 16, K);
+  return FX_OK;
+}
+
+size_t int8_gemm_workspace(const fx::Int8GemmPlan& plan, int M, int N) {
+  return plan.splits > 1 ? size_t(plan.splits) * M * N * sizeof(int) : 0;
+}
+
+int validate_code_rows(const char* name, const int8_t* p, long long stride, int rows, int K) {
+  if (!p) return fail(FX_EINVAL, "%s must be non-null", name);
+  if (!aligned_to(p, 16) || stride % 16 != 0) return fail(FX_EINVAL, "%s must have 16-byte aligned rows", name);
+  if (stride < 0 || stride > fx::kInt8RowLimit || (rows > 1 && stride != 0 && stride < K))
+    return fail(FX_EINVAL, "%s stride must be 0 or in [%d, 2^22], got %lld", name, K, stride);
+  return FX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fx_int8_quantize(const void* x, long long x_stride, int8_t* codes, long long code_stride, float* scales, int rows,
+                     int columns, int code_columns, int dtype, void* stream) {
+  if (int rc = validate_int8_rows(codes, code_stride, scales, rows, columns, code_columns)) return rc;
+  if (!is_half_dtype(dtype)) return fail(FX_EINVAL, "dtype must be fp16 or bf16");
+  if (rows == 0) return FX_OK;
+  if (int rc = validate_half_rows("x", x, x_stride)) return rc;
+  fx::Int8RowsArgs a{};
+  a.x = static_cast<const uint16_t*>(x);
+  a.codes = codes;
+  a.scales = scales;
+  a.x_stride = x_stride;
+  a.code_stride = code_stride;
+  a.rows = rows;
+  a.columns = columns;
+  a.code_columns = code_columns;
+  return run_int8_rows(fx::kRowsPlain, a, dtype, stream, "fx_int8_quantize");
+}
+
+int fx_int8_rmsnorm(const void* x, long long x_stride, const void* residual, long long residual_stride,
+                    void* residual_out, long long residual_out_stride, const void* weight, int8_t* codes,
+                    long long code_stride, float* scales, int rows, int columns, int code_columns, float eps, int dtype,
+                    void* stream) {
+  if (int rc = validate_int8_rows(codes, code_stride, scales, rows, columns, code_columns)) return rc;
+  if (!is_half_dtype(dtype)) return fail(FX_EINVAL, "dtype must be fp16 or bf16");
+  if (!(eps >= 0.f) || !(eps < INFINITY)) return fail(FX_EINVAL, "eps must be non-negative and finite");
+  if (rows == 0) return FX_OK;
+  if (int rc = validate_half_rows("x", x, x_stride)) return rc;
+  if (int rc = validate_half_rows("weight", weight, 0)) return rc;
+  if (residual) {
+    if (int rc = validate_half_rows("residual", residual, residual_stride)) return rc;
+    if (int rc = validate_half_rows("residual_out", residual_out, residual_out_stride)) return rc;
+    if (residual_out_stride < columns && rows > 1)
+      return fail(FX_EINVAL, "residual_out stride %lld is shorter than a row of %d", residual_out_stride, columns);
+  }
+  fx::Int8RowsArgs a{};
+  a.x = static_cast<const uint16_t*>(x);
+  a.second = static_cast<const uint16_t*>(residual);
+  a.sum = residual ? static_cast<uint16_t*>(residual_out) : nullptr;
+  a.weight = static_cast<const uint16_t*>(weight);
+  a.codes = codes;
+  a.scales = scales;
+  a.x_stride = x_stride;
+  a.second_stride = residual_stride;
+  a.sum_stride = residual_out_stride;
+  a.code_stride = code_stride;
+  a.rows = rows;
+  a.columns = columns;
+  a.code_columns = code_columns;
+  a.eps = eps;
+  return run_int8_rows(fx::kRowsNorm, a, dtype, stream, "fx_int8_rmsnorm");
+}
+
+int fx_int8_silu_mul(const void* gate, long long gate_stride, const void* up, long long up_stride, int8_t* codes,
+                     long long code_stride, float* scales, int rows, int columns, int code_columns, int dtype,
+                     void* stream) {
+  if (int rc = validate_int8_rows(codes, code_stride, scales, rows, columns, code_columns)) return rc;
+  if (!is_half_dtype(dtype)) return fail(FX_EINVAL, "dtype must be fp16 or bf16");
+  if (rows == 0) return FX_OK;
+  if (int rc = validate_half_rows("gate", gate, gate_stride)) return rc;
+  if (int rc = validate_half_rows("up", up, up_stride)) return rc;
+  fx::Int8RowsArgs a{};
+  a.x = static_cast<const uint16_t*>(gate);
+  a.second = static_cast<const uint16_t*>(up);
+  a.codes = codes;
+  a.scales = scales;
+  a.x_stride = gate_stride;
+  a.second_stride = up_stride;
+  a.code_stride = code_stride;
+  a.rows = rows;
+  a.columns = columns;
+  a.code_columns = code_columns;
+  return run_int8_rows(fx::kRowsSwiglu, a, dtype, stream, "fx_int8_silu_mul");
+}
+
+int fx_int8_restore(const int8_t* codes, long long code_stride, const float* scales, void* out, long long out_stride,
+                    int rows, int columns, int dtype, void* stream) {
+  if (rows < 0 || rows > (1 << 21)) return fail(FX_EINVAL, "rows must be in [0, 2^21], got %d", rows);
+  if (columns < 1 || columns > (1 << 20)) return fail(FX_EINVAL, "columns must be in [1, 2^20], got %d", columns);
+  // a launch holds fewer than 2^32 threads, of 16 columns each
+  if ((long long)(rows) * ((columns + 15) / 16) > (1LL << 31))
+    return fail(FX_EINVAL, "%d rows of %d columns are too large for one call", rows, columns);
+  if (!is_half_dtype(dtype) && dtype != FX_F32) return fail(FX_EINVAL, "dtype must be fp32, fp16 or bf16");
+  if (rows == 0) return FX_OK;
+  if (!codes || !scales || !out) return fail(FX_EINVAL, "codes, scales and out must be non-null");
+  if (!aligned_to(scales, 4) || !aligned_to(out, dtype == FX_F32 ? 4 : 2))
+    return fail(FX_EINVAL, "scales and out must be aligned to their elements");
+  if (code_stride < 0 || (out_stride < columns && rows > 1))
+    return fail(FX_EINVAL, "strides %lld and %lld do not fit rows of %d", code_stride, out_stride, columns);
+  const fx::Int8RestoreArgs a{codes, scales, out, code_stride, out_stride, rows, columns};
+  fx::launch_int8_restore(dtype, a, static_cast<hipStream_t>(stream));
+  return check_launch("fx_int8_restore");
+}
+
+size_t fx_int8_gemm_workspace_bytes(int M, int N, int K) {
+  if (validate_int8_gemm_sizes(M, N, K) || M == 0) return 0;
+  return int8_gemm_workspace(fx::plan_int8_gemm(M, N, K), M, N);
+}
+
+int fx_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales, const int8_t* w, long long w_stride,
+                 const float* w_scales, const void* bias, void* out, long long out_stride, void* workspace,
+                 size_t workspace_bytes, int M, int N, int K, int dtype, void* stream) {
+  if (int rc = validate_int8_gemm_sizes(M, N, K)) return rc;
+  if (!is_half_dtype(dtype) && dtype != FX_F32) return fail(FX_EINVAL, "dtype must be fp32, fp16 or bf16");
+  if (M == 0) return FX_OK;
+  if (int rc = validate_code_rows("a", a, a_stride, M, K)) return rc;
+  if (int rc = validate_code_rows("w", w, w_stride, N, K)) return rc;
+  if (!a_scales || !w_scales || !out) return fail(FX_EINVAL, "scales and out must be non-null");
+  const unsigned size = dtype == FX_F32 ? 4 : 2;
+  if (!aligned_to(a_scales, 4) || !aligned_to(w_scales, 4) || !aligned_to(out, size) || !aligned_to(bias, size))
+    return fail(FX_EINVAL, "scales, bias and out must be aligned to their elements");
+  if (out_stride < 0 || (out_stride < N && M > 1))
+    return fail(FX_EINVAL, "out stride %lld is shorter than a row of %d", out_stride, N);
+  const fx::Int8GemmPlan plan = fx::plan_int8_gemm(M, N, K);
+  const size_t need = int8_gemm_workspace(plan, M, N);
+  if (need) {
+    if (!workspace || workspace_bytes < need)
+      return fail(FX_EINVAL, "gemm workspace needs %zu bytes, got %zu", need, workspace_bytes);
+    if (!aligned16(workspace)) return fail(FX_EINVAL, "workspace must be 16-byte aligned");
+  }
+  fx::Int8GemmArgs g{};
+  g.a = a;
+  g.w = w;
+  g.a_scales = a_scales;
+  g.w_scales = w_scales;
+  g.bias = bias;
+  g.out = out;
+  g.partial = need ? static_cast<int*>(workspace) : nullptr;
+  g.a_stride = a_stride;
+  g.w_stride = w_stride;
+  g.out_stride = out_stride;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.dt = dtype;
+  g.k_per_split = plan.k_per_split;
+  g.vec = aligned_to(out, 4 * size) && out_stride % 4 == 0;
+  if (!fx::launch_int8_gemm(plan, g, static_cast<hipStream_t>(stream)))
+    return fail(FX_EINVAL, "no kernel for a product of %d x %d x %d", M, N, K);
+  return check_launch("fx_int8_gemm");
 }
 
 }  // extern "C"

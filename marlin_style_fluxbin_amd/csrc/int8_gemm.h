@@ -1,0 +1,60 @@
+// Products of 8-bit rows: what the kernels share.
+#pragma once
+#include "int8_launch.h"
+
+namespace fx {
+
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+
+// D[i, j] += sum_k A[i, k] B[j, k] over 64 bytes of k: lane l gives bytes 16 (l / 16) .. of row
+// l % 16 of A and of B, and holds D[4 (l / 16) + r, l % 16].  A is the weight, so that a lane's
+// four results are neighbours in a row of the output.
+__device__ __forceinline__ i32x4_t mfma_i8_16(const u32x4_t& a, const u32x4_t& b, const i32x4_t& c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
+}
+
+template <int DT>
+__device__ __forceinline__ float load_value(const void* p, long long i) {
+  if constexpr (DT == kF32) return static_cast<const float*>(p)[i];
+  else return to_f32<DT>(static_cast<const uint16_t*>(p)[i]);
+}
+
+// Columns n .. n + 3 (those below N) of row m: one rounding of (acc a_scale) w_scale + bias in fp32.
+// acc's own float is rounded once beyond 2^24 (2^-24 of it).
+template <int DT>
+__device__ __forceinline__ void store4_as(const Int8GemmArgs& g, int m, int n, const i32x4_t& acc) {
+  const float sa = g.a_scales[m];
+  float y[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int c = min(n + r, g.N - 1);
+    y[r] = fmaf(float(acc[r]) * sa, g.w_scales[c], g.bias ? load_value<DT>(g.bias, c) : 0.f);
+  }
+  const long long at = m * g.out_stride + n;
+  const bool whole = g.vec && n + 4 <= g.N;
+  if constexpr (DT == kF32) {
+    float* out = static_cast<float*>(g.out) + at;
+    if (whole) *reinterpret_cast<float4*>(out) = float4{y[0], y[1], y[2], y[3]};
+    else
+      for (int r = 0; r < 4; ++r)
+        if (n + r < g.N) out[r] = y[r];
+  } else {
+    uint16_t* out = static_cast<uint16_t*>(g.out) + at;
+    if (whole) {
+      uint2 v;
+      v.x = round_pair_bits<DT>(y[0], y[1]);
+      v.y = round_pair_bits<DT>(y[2], y[3]);
+      *reinterpret_cast<uint2*>(out) = v;
+    } else {
+      for (int r = 0; r < 4; ++r)
+        if (n + r < g.N) out[r] = from_f32<DT>(y[r]);
+    }
+  }
+}
+__device__ __forceinline__ void store4(const Int8GemmArgs& g, int m, int n, const i32x4_t& acc) {
+  if (g.dt == kBF16) store4_as<kBF16>(g, m, n, acc);
+  else if (g.dt == kF16) store4_as<kF16>(g, m, n, acc);
+  else store4_as<kF32>(g, m, n, acc);
+}
+
+}  // namespace fx

@@ -1,0 +1,395 @@
+"""Linears whose activations and weights are 8-bit integers, and the rows that feed them.
+
+No reference counterpart: the reference's Linears keep 16-bit activations
+(``w3_lut_deployment.py:190-359``, ``deployment.py:182-297``).  Here a row of activations (a
+token) and a row of the weight (an output channel) are 8-bit codes with an fp32 scale each, the
+products run on the int8 matrix cores with exact sums, and what produces a Linear's input
+writes it as codes at once: :func:`add_rms_norm_int8` in front of q|k|v and gate|up,
+:func:`silu_mul_int8` in front of down, :func:`quantize_int8` elsewhere.
+:class:`PackedInt8Linear` is the module; ``include/fluxbin_int8.h`` has the format.
+
+Every call goes to the HIP kernels on the current stream of the tensors' device; there is no
+CPU substitute, no backward pass and no forward-mode derivative, and calls are not traced.
+Nothing synchronises, so calls can be captured into a HIP graph.
+"""
+from __future__ import annotations
+
+import torch
+from torch import nn
+from torch.nn import functional as F
+
+from . import _lib
+from .cached_attention import _launch, _refuse_records
+from .packed_linear import PACKED_M1, PACKED_SMALL_M, DENSE_FALLBACK, PackedLinearBase, replace_linears_atomically
+
+_HALF = (torch.float16, torch.bfloat16)
+_OUT = (torch.float16, torch.bfloat16, torch.float32)
+MAX_IN_FEATURES = 131056  # sums of so many products of codes stay within 32 bits
+_STEP = 16                # columns of the products' rows come in whole 16 bytes
+_ROW_LIMIT = 1 << 22      # bytes between two rows of codes that the products take
+_WHAT = "an 8-bit operator"
+
+_workspaces: dict[tuple[int, int, int], int] = {}
+
+
+def _workspace_bytes(m: int, n: int, k: int) -> int:
+    """The library's answer, kept: it depends on the sizes alone."""
+    key = (m, n, k)
+    found = _workspaces.get(key)
+    if found is None:
+        if len(_workspaces) > 4096:
+            _workspaces.clear()
+        found = _workspaces[key] = _lib.library().fx_int8_gemm_workspace_bytes(m, n, k)
+    return found
+
+
+def _refuse(*tensors: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("8-bit operators have no backward pass; call them under torch.no_grad()")
+    _refuse_records(*tensors, what=_WHAT)
+
+
+def _rows_of(t: torch.Tensor) -> tuple[int, int] | None:
+    """(rows, elements between rows) of ``t [..., columns]`` where its rows lie evenly in memory
+    with contiguous columns, else None."""
+    shape, columns = t.shape, t.shape[-1]
+    if t.is_contiguous():
+        return t.numel() // columns, columns
+    if t.stride(-1) != 1 and columns > 1:
+        return None
+    rows, step = 1, columns
+    for n, s in zip(reversed(shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if rows == 1:
+            step = s
+        elif s != rows * step:
+            return None
+        rows *= n
+    return rows, step
+
+
+def _half_input(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> tuple[torch.Tensor, int, int]:
+    """``t`` or a copy of it as the kernels read it, its row count and row stride."""
+    if not t.is_cuda or t.dtype not in _HALF:
+        _lib.require_gpu_tensor(t, name)
+        raise ValueError(f"{name} must be fp16 or bf16")
+    if t.ndim < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{name} must have shape [..., columns] with columns to hold")
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name} must have the input's shape, dtype and device")
+    if t.is_neg():
+        t = t.resolve_neg()
+    found = _rows_of(t)
+    if found is None:
+        t = t.contiguous()
+        found = _rows_of(t)
+    return t, *found
+
+
+def _code_outputs(x: torch.Tensor, out) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """codes, scales and the codes' row stride: new ones, or the caller's checked."""
+    shape = x.shape
+    if out is None:
+        codes = torch.empty(shape, dtype=torch.int8, device=x.device)
+        return codes, torch.empty(shape[:-1], dtype=torch.float32, device=x.device), shape[-1]
+    codes, scales = out
+    if codes.shape != shape or codes.dtype is not torch.int8 or codes.device != x.device:
+        raise ValueError("out's codes must be int8 of the input's shape on its device")
+    if (scales.shape != shape[:-1] or scales.dtype is not torch.float32 or scales.device != x.device
+            or not scales.is_contiguous()):
+        raise ValueError("out's scales must be contiguous fp32 of the input's leading shape on its device")
+    found = _rows_of(codes)
+    if found is None or (found[0] > 1 and found[1] < shape[-1]):
+        raise ValueError("out's codes must have contiguous rows, each its own memory")
+    return codes, scales, found[1]
+
+
+def _quantize_into(x2: torch.Tensor, rows: int, stride: int, columns: int, codes: torch.Tensor, code_stride: int,
+                   code_columns: int, scales: torch.Tensor) -> None:
+    _launch("fx_int8_quantize", x2.device, x2.data_ptr(), stride, codes.data_ptr(), code_stride, scales.data_ptr(), rows,
+            columns, code_columns, _lib.dtype_code(x2.dtype))
+
+
+def quantize_int8(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """Each row of ``x [..., columns]`` (fp16 or bf16) as ``codes`` (int8, x's shape) and ``scales``
+    (fp32, x's leading shape): with a the row's largest magnitude, code = round(127 x / a), ties to
+    even, scale = a / 127.  A row with an infinity or NaN stands for NaN (its scale is NaN)."""
+    _refuse(x)
+    x, rows, stride = _half_input(x, "x")
+    codes, scales, code_stride = _code_outputs(x, out)
+    columns = x.shape[-1]
+    _quantize_into(x, rows, stride, columns, codes, code_stride, columns, scales)
+    return codes, scales
+
+
+def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values that rows of codes stand for: ``codes * scales[..., None]`` as a new ``dtype`` (fp16,
+    bf16 or fp32) tensor."""
+    _check_codes(codes, scales, "codes", "scales")
+    if dtype not in _OUT:
+        raise ValueError("dtype must be fp16, bf16 or fp32")
+    _refuse_records(codes, scales, what=_WHAT)
+    if codes.shape[-1] < 1:
+        raise ValueError("codes must have shape [..., columns] with columns to hold")
+    found = _rows_of(codes)
+    if found is None:
+        codes = codes.contiguous()
+        found = _rows_of(codes)
+    scales = scales.contiguous()
+    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    columns = codes.shape[-1]
+    _launch("fx_int8_restore", codes.device, codes.data_ptr(), found[1], scales.data_ptr(), out.data_ptr(), columns,
+            found[0], columns, _lib.dtype_code(dtype))
+    return out
+
+
+def _norm(x, residual, weight, eps, residual_out, out, padded: int | None = None):
+    _refuse(x, residual, weight, residual_out)
+    x, rows, stride = _half_input(x, "hidden_states")
+    columns = x.shape[-1]
+    if weight.shape != (columns,) or weight.dtype != x.dtype or weight.device != x.device:
+        raise ValueError("weight must have shape [hidden] and the input's dtype and device")
+    weight = weight.resolve_neg().contiguous()
+    r_ptr = r_stride = s_ptr = s_stride = None
+    if residual is not None:
+        residual, _, r_stride = _half_input(residual, "residual", x)
+        if residual_out is None:
+            residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif residual_out.shape != x.shape or residual_out.dtype != x.dtype or residual_out.device != x.device:
+            raise ValueError("residual_out must have the input's shape, dtype and device")
+        found = None if residual_out.is_neg() else _rows_of(residual_out)
+        if found is None or (found[0] > 1 and found[1] < columns):
+            raise ValueError("residual_out must have contiguous rows, each its own memory")
+        r_ptr, s_ptr, s_stride = residual.data_ptr(), residual_out.data_ptr(), found[1]
+    codes, scales, code_stride = _code_outputs(x, out)
+    _launch("fx_int8_rmsnorm", x.device, x.data_ptr(), stride, r_ptr, r_stride or 0, s_ptr, s_stride or 0,
+            weight.data_ptr(), codes.data_ptr(), code_stride, scales.data_ptr(), rows, columns, columns, float(eps),
+            _lib.dtype_code(x.dtype))
+    return codes, scales, residual_out
+
+
+def rms_norm_int8(hidden_states: torch.Tensor, weight: torch.Tensor, eps: float, *,
+                  out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """:func:`quantize_int8` of ``weight * x * rsqrt(mean(x^2) + eps)`` over the last axis, in one launch
+    and without the rounding to 16 bits between the two: ``(codes, scales)``."""
+    return _norm(hidden_states, None, weight, eps, None, out)[:2]
+
+
+def add_rms_norm_int8(hidden_states: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float, *,
+                      residual_out: torch.Tensor | None = None,
+                      out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """:func:`rms_norm_int8` of ``residual_out = round(hidden_states + residual)``, which is written too:
+    ``(codes, scales, residual_out)``.  ``residual_out`` may be ``hidden_states`` or ``residual`` itself;
+    otherwise it shares no memory with them."""
+    if residual is None:
+        raise ValueError("residual must be a tensor")
+    return _norm(hidden_states, residual, weight, eps, residual_out, out)
+
+
+def silu_mul_int8(gate: torch.Tensor, up: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """:func:`quantize_int8` of ``silu(gate) * up`` (formed in fp32), in one launch.  ``gate`` and ``up``
+    may be the halves of one product's output."""
+    _refuse(gate, up)
+    gate, rows, stride = _half_input(gate, "gate")
+    up, _, up_stride = _half_input(up, "up", gate)
+    codes, scales, code_stride = _code_outputs(gate, out)
+    columns = gate.shape[-1]
+    _launch("fx_int8_silu_mul", gate.device, gate.data_ptr(), stride, up.data_ptr(), up_stride, codes.data_ptr(),
+            code_stride, scales.data_ptr(), rows, columns, columns, _lib.dtype_code(gate.dtype))
+    return codes, scales
+
+
+def _check_codes(codes: torch.Tensor, scales: torch.Tensor, name: str, scales_name: str) -> None:
+    if not codes.is_cuda or codes.dtype is not torch.int8 or codes.ndim < 1:
+        _lib.require_gpu_tensor(codes, name)
+        raise ValueError(f"{name} must be int8 [..., columns]")
+    if scales.dtype is not torch.float32 or scales.shape != codes.shape[:-1] or scales.device != codes.device:
+        raise ValueError(f"{scales_name} must be fp32, one for each row of {name}, on its device")
+
+
+def _code_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """Rows as the products read them (whole 16 bytes at 16-byte boundaries): ``t`` or a padded
+    copy of it, rows, row stride and columns."""
+    columns = t.shape[-1]
+    if columns % _STEP == 0:
+        found = _rows_of(t)
+        if found is not None:
+            rows, stride = found
+            if not t.data_ptr() % 16 and (rows == 1 or (not stride % 16 and (stride >= columns or stride == 0)
+                                                        and stride <= _ROW_LIMIT)):
+                return t, rows, stride if rows > 1 else columns, columns
+    width = -(-columns // _STEP) * _STEP
+    t = F.pad(t, (0, width - columns)) if width != columns else t.clone(memory_format=torch.contiguous_format)
+    return t, t.numel() // width, width, width
+
+
+def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, *,
+                bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[..., n] = (sum_k a[..., k] weight[n, k]) * a_scales[...] * weight_scales[n] + bias[n]``.
+
+    ``a [..., K]`` and ``weight [N, K]`` int8, their scales fp32 (one per row), ``bias [N]`` and the
+    result of ``dtype`` (fp16, bf16 or fp32).  The sum is exact (K up to 131056); scales and bias are
+    applied in fp32, rounded once.  Rows are read in place where they are 16-byte aligned and K is a
+    multiple of 16; others are copied first."""
+    _check_codes(a, a_scales, "a", "a_scales")
+    _check_codes(weight, weight_scales, "weight", "weight_scales")
+    if weight.ndim != 2 or a.shape[-1] != weight.shape[1] or a.device != weight.device:
+        raise ValueError("weight must be [N, K] with a's K, on a's device")
+    k, n = a.shape[-1], weight.shape[0]
+    if not 1 <= k <= MAX_IN_FEATURES or n < 1:
+        raise ValueError(f"K must be in [1, {MAX_IN_FEATURES}] and N positive, got {k} and {n}")
+    if dtype not in _OUT:
+        raise ValueError("dtype must be fp16, bf16 or fp32")
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype != dtype or bias.device != a.device:
+            raise ValueError("bias must have shape [N], the result's dtype and a's device")
+        bias = bias.resolve_neg().contiguous()
+    _refuse(a_scales, weight_scales, bias, out)
+    shape = (*a.shape[:-1], n)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=a.device)
+        out_stride = n
+    else:
+        if out.shape != shape or out.dtype != dtype or out.device != a.device or out.is_neg():
+            raise ValueError("out must have shape [..., N], the result's dtype and a's device")
+        found = _rows_of(out)
+        if found is None or (found[0] > 1 and found[1] < n):
+            raise ValueError("out must have contiguous rows, each its own memory")
+        out_stride = found[1]
+    a, rows, a_stride, width = _code_rows(a)
+    weight, _, w_stride, _ = _code_rows(weight)
+    a_scales, weight_scales = a_scales.contiguous(), weight_scales.contiguous()
+    _product(a, a_stride, a_scales, weight, w_stride, weight_scales, bias, out, out_stride, rows, n, width)
+    return out
+
+
+def _product(a, a_stride, a_scales, weight, w_stride, weight_scales, bias, out, out_stride, m, n, k, workspace=None):
+    nbytes = _workspace_bytes(m, n, k)
+    if nbytes and workspace is None:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=out.device)
+    _launch("fx_int8_gemm", out.device, a.data_ptr(), a_stride, a_scales.data_ptr(), weight.data_ptr(), w_stride,
+            weight_scales.data_ptr(), _lib.ptr(bias), out.data_ptr(), out_stride, _lib.ptr(workspace), nbytes, m, n, k,
+            _lib.dtype_code(out.dtype))
+
+
+def quantize_weight_int8(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """A Linear's weight ``[O, K]`` as codes and scales, one scale per output channel: the kernel's
+    codes for a 16-bit weight on a GPU, the same formula in 64 bits elsewhere."""
+    if weight.ndim != 2:
+        raise ValueError("weight must have shape [O, K]")
+    weight = weight.detach()
+    if weight.is_cuda and weight.dtype in _HALF:
+        return quantize_int8(weight)
+    wide = weight.double()
+    top = wide.abs().amax(1, keepdim=True)
+    if not bool(torch.isfinite(top).all()):
+        raise ValueError("weight must be finite")
+    codes = torch.round(wide * 127 / torch.where(top > 0, top, torch.ones_like(top))).to(torch.int8)
+    return codes, (top[:, 0] / 127).float()
+
+
+class PackedInt8Linear(PackedLinearBase):
+    """Linear with 8-bit weights (a scale per output channel) and activations (a scale per row,
+    formed in the call).
+
+    ``codes [O, K]`` int8 and ``scales [O]`` fp32 stand for the weight ``codes * scales[:, None]``.
+    Any number of fp16 or bf16 rows on the GPU take the kernels; other inputs are refused unless
+    ``fallback='dense'`` (``F.linear`` with the weight that the codes stand for).  Routes, counters
+    and the bound one-row decode call are those of ``packed_linear.PackedLinearBase``."""
+
+    max_packed_rows = 1 << 21
+    bias_in_kernel = True
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, *, bias: torch.Tensor | None = None,
+                 fallback: str = "error"):
+        super().__init__()
+        if codes.ndim != 2 or codes.dtype is not torch.int8 or not 1 <= codes.shape[1] <= MAX_IN_FEATURES or (
+                codes.shape[0] < 1):
+            raise ValueError(f"codes must be int8 [O, K], K at most {MAX_IN_FEATURES}")
+        self.out_features, self.in_features = codes.shape
+        if scales.shape != (self.out_features,) or scales.dtype is not torch.float32 or scales.device != codes.device:
+            raise ValueError("scales must be fp32 [O] on the codes' device")
+        if bias is not None and (bias.shape != (self.out_features,) or bias.device != codes.device):
+            raise ValueError("bias must have shape [O] on the codes' device")
+        self._init_protocol(fallback=fallback, bias=bias)
+        # rows of whole 16 bytes, the columns behind K zero, as the kernels read them
+        self._width = -(-self.in_features // _STEP) * _STEP
+        codes = codes.detach()
+        self.register_buffer("codes", F.pad(codes, (0, self._width - self.in_features)).contiguous()
+                             if self._width != self.in_features else codes.clone(memory_format=torch.contiguous_format))
+        self.register_buffer("scales", scales.detach().clone())
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, *, fallback: str = "error") -> "PackedInt8Linear":
+        """The Linear with its weight quantized per output channel."""
+        if not isinstance(linear, nn.Linear):
+            raise ValueError("from_linear takes an nn.Linear")
+        codes, scales = quantize_weight_int8(linear.weight)
+        return cls(codes, scales, bias=linear.bias, fallback=fallback)
+
+    def _payload_device(self) -> torch.device:
+        return self.codes.device
+
+    def _dense_weight(self, dtype: torch.dtype) -> torch.Tensor:
+        return (self.codes[:, :self.in_features].float() * self.scales[:, None]).to(dtype)
+
+    def _check_before_call(self) -> None:
+        if self._tensor("scales").dtype is not torch.float32 or self._tensor("codes").dtype is not torch.int8:
+            raise ValueError("codes or scales were cast; move devices without dtype conversion")
+
+    def _check_before_bind(self, device: torch.device) -> None:
+        if self.scales.device != device or not self.codes.is_contiguous():
+            raise ValueError("contiguous same-device codes and scales required")
+        self._check_before_call()
+
+    def _packed_kernel(self, rows: int, device: torch.device):
+        """The rows quantized and multiplied, through buffers of this callable's own."""
+        codes, scales, bias = self._tensor("codes"), self._tensor("scales"), self._tensor("bias")
+        width, k, o = self._width, self.in_features, self.out_features
+        a = torch.empty((rows, width), dtype=torch.int8, device=device)
+        a_scales = torch.empty(rows, dtype=torch.float32, device=device)
+        nbytes = _workspace_bytes(rows, o, width)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+        def run(x2: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+            _quantize_into(x2, rows, k, k, a, width, width, a_scales)
+            added = bias if bias is None or bias.dtype == out.dtype else bias.to(out.dtype)
+            _product(a, width, a_scales, codes, width, scales, added, out, o, rows, o, width, workspace)
+            return out
+        return run
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self._decode_binding is not None:
+            return self._decode_binding(x)
+        if torch.is_grad_enabled():
+            raise RuntimeError("packed inference requires no_grad/inference_mode")
+        shape, k = x.shape, self.in_features
+        if len(shape) < 2 or shape[-1] != k:
+            raise ValueError("expected [...,K] input")
+        self._check_before_call()
+        device = self._tensor("codes").device
+        rows = x.numel() // k
+        if x.dtype not in _HALF or x.device != device or not x.is_cuda or rows > self.max_packed_rows:
+            if self.fallback != "dense":
+                raise ValueError("unsupported input; enable explicit dense fallback if needed")
+            self._count(DENSE_FALLBACK)
+            return self._dense_linear(x)
+        _refuse_records(x, what=_WHAT)
+        self._count(PACKED_M1 if rows == 1 else PACKED_SMALL_M)
+        out = torch.empty((*shape[:-1], self.out_features), device=device, dtype=x.dtype)
+        if rows:
+            x = x.resolve_neg() if x.is_neg() else x
+            self._packed_kernel(rows, device)(x.reshape(rows, k).contiguous(), out)
+        return out
+
+
+def replace_int8_block_linears(block: nn.Module, *, fallback: str = "error") -> list[str]:
+    """Replace the seven Qwen3 Linears of one block by :class:`PackedInt8Linear` of their weights;
+    every replacement is built before the block is touched.  Returns their names."""
+    from .qwen3 import QWEN3_LINEAR_MODULES
+
+    return replace_linears_atomically(
+        block, [(name, PackedInt8Linear.from_linear(block.get_submodule(name), fallback=fallback))
+                for name in QWEN3_LINEAR_MODULES])

@@ -97,6 +97,7 @@ class PackedLinearBase(nn.Module):
     # w3_lut_deployment.py:357-358) or out of place (type promotion: the hybrid
     # Linear, deployment.py:295-296); the bound decode route adds in place for both
     bias_in_place = True
+    bias_in_kernel = False  # the packed kernel adds the bias itself
 
     def _init_protocol(self, *, fallback: str, bias: torch.Tensor | None) -> None:
         if fallback not in ("error", "dense"):
@@ -180,7 +181,7 @@ class PackedLinearBase(nn.Module):
         view = output.view(1, 1, self.out_features)
         flat_in = (1, self.in_features)
         expected = (1, 1, self.in_features)
-        bias = self.bias
+        bias = None if self.bias_in_kernel else self.bias
 
         def prepared(x: torch.Tensor) -> torch.Tensor:
             if torch.is_grad_enabled():

@@ -195,6 +195,14 @@ def w3_quantize_qwen3_model(model, *, fallback: str = "dense", row_tile_by_shape
     return count
 
 
+def int8_quantize_qwen3_model(model, *, fallback: str = "error") -> int:
+    """Replace every decoder block's seven Linears by ``PackedInt8Linear`` of their weights (in
+    place); returns the count."""
+    from .int8_linear import replace_int8_block_linears
+
+    return sum(len(replace_int8_block_linears(block, fallback=fallback)) for block in model.model.layers)
+
+
 def random_hybrid_payload(out_features: int, in_features: int, *, device, generator, row_scale: float = 0.01) -> dict:
     """A random hybrid g128/s8 two-base payload of one Linear (the seven fields of
     ``deployment.FIELDS``): uniform random signs, row scales ~ N(0, row_scale),
