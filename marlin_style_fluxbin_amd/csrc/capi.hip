@@ -2157,7 +2157,7 @@ int fx_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales, con
   g.K = K;
   g.dt = dtype;
   g.k_per_split = plan.k_per_split;
-  g.vec = aligned_to(out, 4 * size) && out_stride % 4 == 0;
+  g.vec = aligned16(out) && out_stride * size % 16 == 0;
   if (!fx::launch_int8_gemm(plan, g, static_cast<hipStream_t>(stream)))
     return fail(FX_EINVAL, "no kernel for a product of %d x %d x %d", M, N, K);
   return check_launch("fx_int8_gemm");

@@ -19,23 +19,37 @@ __device__ __forceinline__ float load_value(const void* p, long long i) {
   else return to_f32<DT>(static_cast<const uint16_t*>(p)[i]);
 }
 
+typedef float f32x4v_t __attribute__((ext_vector_type(4)));
+
+// The scales of columns n .. n + 3 (0 past the last).
+__device__ __forceinline__ f32x4v_t column_scales(const Int8GemmArgs& g, int n) {
+  return __builtin_bit_cast(f32x4v_t, load_b128(buffer_resource(g.w_scales, size_t(g.N) * 4), n * 4, 0));
+}
+template <int DT>
+__device__ __forceinline__ f32x4v_t column_bias(const Int8GemmArgs& g, int n) {
+  f32x4v_t b = {0.f, 0.f, 0.f, 0.f};
+  if (g.bias)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) b[r] = load_value<DT>(g.bias, min(n + r, g.N - 1));
+  return b;
+}
+
 // Columns n .. n + 3 (those below N) of row m: one rounding of (acc a_scale) w_scale + bias in fp32.
 // acc's own float is rounded once beyond 2^24 (2^-24 of it).
 template <int DT>
 __device__ __forceinline__ void store4_as(const Int8GemmArgs& g, int m, int n, const i32x4_t& acc) {
   const float sa = g.a_scales[m];
+  const f32x4v_t ws = column_scales(g, n), bias = column_bias<DT>(g, n);
   float y[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int c = min(n + r, g.N - 1);
-    y[r] = fmaf(float(acc[r]) * sa, g.w_scales[c], g.bias ? load_value<DT>(g.bias, c) : 0.f);
-  }
+  for (int r = 0; r < 4; ++r) y[r] = fmaf(float(acc[r]) * sa, ws[r], bias[r]);
   const long long at = m * g.out_stride + n;
   const bool whole = g.vec && n + 4 <= g.N;
   if constexpr (DT == kF32) {
     float* out = static_cast<float*>(g.out) + at;
     if (whole) *reinterpret_cast<float4*>(out) = float4{y[0], y[1], y[2], y[3]};
     else
+#pragma unroll
       for (int r = 0; r < 4; ++r)
         if (n + r < g.N) out[r] = y[r];
   } else {
@@ -46,6 +60,7 @@ __device__ __forceinline__ void store4_as(const Int8GemmArgs& g, int m, int n, c
       v.y = round_pair_bits<DT>(y[2], y[3]);
       *reinterpret_cast<uint2*>(out) = v;
     } else {
+#pragma unroll
       for (int r = 0; r < 4; ++r)
         if (n + r < g.N) out[r] = from_f32<DT>(y[r]);
     }
@@ -55,6 +70,15 @@ __device__ __forceinline__ void store4(const Int8GemmArgs& g, int m, int n, cons
   if (g.dt == kBF16) store4_as<kBF16>(g, m, n, acc);
   else if (g.dt == kF16) store4_as<kF16>(g, m, n, acc);
   else store4_as<kF32>(g, m, n, acc);
+}
+
+// The same columns of one K split's sums, [splits, M, N].
+__device__ __forceinline__ void store4_partial(const Int8GemmArgs& g, int split, int m, int n, const i32x4_t& acc) {
+  int* out = g.partial + (size_t(split) * g.M + m) * g.N + n;
+  if (g.N % 4 == 0) *reinterpret_cast<i32x4_t*>(out) = acc;
+  else
+    for (int r = 0; r < 4; ++r)
+      if (n + r < g.N) out[r] = acc[r];
 }
 
 }  // namespace fx

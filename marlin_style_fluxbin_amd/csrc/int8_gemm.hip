@@ -1,56 +1,82 @@
 // Products of 8-bit rows (int8_launch.h): the sums in whole numbers on the int8 matrix cores, exact
-// in any order, the scales and the bias in fp32, one rounding.
-#include "int8_gemm.h"
+// in any order, the scales and the bias in fp32, one rounding.  Here: which kernel a product takes,
+// and the join of K splits.
+#include <algorithm>
+
+#include "int8_gemm_few.h"
+#include "int8_gemm_tile_launch.h"
 
 namespace fx {
 namespace {
 
-// Four waves, each 32 rows of the weight by 32 of the activations, operands straight from memory.
-__global__ __launch_bounds__(256) void int8_gemm_direct_kernel(const Int8GemmArgs g) {
-  const int lane = threadIdx.x & 63, wave = wave_index();
-  const int r = lane & 15, k16 = (lane >> 4) * 16;
-  const int n0 = int(blockIdx.x) * 64 + (wave & 1) * 32, m0 = int(blockIdx.y) * 64 + (wave >> 1) * 32;
-  const int8_t *pw[2], *pa[2];
+// The sums of the K splits, scaled: 4 columns a thread.  Bound by the launch and the partial sums.
+__global__ __launch_bounds__(256) void int8_gemm_join_kernel(const Int8GemmArgs g, int splits) {
+  const unsigned quads = unsigned(g.N + 3) / 4;
+  const unsigned unit = blockIdx.x * 256u + threadIdx.x;
+  const int m = int(unit / quads), n = int(unit - unsigned(m) * quads) * 4;
+  if (m >= g.M) return;
+  const size_t plane = size_t(g.M) * g.N;
+  const int* p = g.partial + size_t(m) * g.N + n;
+  i32x4_t total = {0, 0, 0, 0};
+  if (g.N % 4 == 0) {
+    for (int s = 0; s < splits; ++s) total += *reinterpret_cast<const i32x4_t*>(p + s * plane);
+  } else {
+    for (int s = 0; s < splits; ++s)
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {  // rows past the last: the last again, not stored
-    pw[t] = g.w + min(n0 + 16 * t + r, g.N - 1) * g.w_stride;
-    pa[t] = g.a + min(m0 + 16 * t + r, g.M - 1) * g.a_stride;
+      for (int r = 0; r < 4; ++r)
+        if (n + r < g.N) total[r] += p[s * plane + r];
   }
-  i32x4_t acc[2][2];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = i32x4_t{0, 0, 0, 0};
-  for (int k = k16; k - k16 < g.K; k += 64) {
-    const u32x4_t zero = {0u, 0u, 0u, 0u};
-    u32x4_t w[2], a[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      w[t] = k < g.K ? *reinterpret_cast<const u32x4_t*>(pw[t] + k) : zero;
-      a[t] = k < g.K ? *reinterpret_cast<const u32x4_t*>(pa[t] + k) : zero;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mfma_i8_16(w[i], a[j], acc[i][j]);
-  }
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int m = m0 + 16 * j + r;
-    if (m >= g.M) continue;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int n = n0 + 16 * i + (lane >> 4) * 4;
-      if (n < g.N) store4(g, m, n, acc[i][j]);
-    }
-  }
+  store4(g, m, n, total);
 }
+
+constexpr int kFewRows = 16;
+constexpr int kMaxSplits = 16;
 
 }  // namespace
 
-Int8GemmPlan plan_int8_gemm(int M, int N, int K) { return {0, 1, K}; }
+// Which kernel, and how many workgroups along K, by an estimate of the time (us): rounds of
+// workgroups, each its stages of 128 columns at what a stage takes (with the chip's other places of
+// the same compute unit empty, and full), or the bytes; and for splits the join's launch and the
+// partial sums written and read.
+Int8GemmPlan plan_int8_gemm(int M, int N, int K) {
+  const int stages = (K + 127) / 128;
+  const float bytes = (float(M) + N) * K / 4.8e6f;
+  Int8GemmPlan best{kInt8Few, 1, K};
+  float least = M <= kFewRows ? 3.f + float(N) * K / 4.9e6f * (1.f + 0.016f * M) : 1e30f;
+  for (int tile = 0; tile < kInt8Tiles; ++tile) {
+    const Int8Tile& t = kInt8Tile[tile];
+    const long tiles = long((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+    for (int splits = 1; splits <= std::min(stages, kMaxSplits); ++splits) {
+      if (splits > 1 && tiles * (splits - 1) >= 256 * t.places) break;  // the chip was full
+      const int per = (stages + splits - 1) / splits;
+      if ((stages + per - 1) / per != splits) continue;  // a last split would be empty
+      const long groups = tiles * splits, slots = 256 * t.places, rounds = (groups + slots - 1) / slots;
+      const float last = float(groups - (rounds - 1) * slots) / 256.f;  // workgroups of a unit in the last round
+      const float stage = (rounds - 1) * t.full + (last <= 1.f ? t.alone : t.alone + (t.full - t.alone) * (last - 1.f));
+      float time = 3.f + std::max(per * stage + rounds * t.ends, bytes);
+      if (splits > 1) time += 2.5f + 2.f * splits * float(M) * N * 4.f / 5e6f;
+      if (time < least) least = time, best = {tile, splits, splits == 1 ? K : per * 128};
+    }
+  }
+  return best;
+}
 
 bool launch_int8_gemm(const Int8GemmPlan& plan, const Int8GemmArgs& g, hipStream_t s) {
-  const dim3 grid(unsigned(g.N + 63) / 64, unsigned(g.M + 63) / 64);
-  hipLaunchKernelGGL(int8_gemm_direct_kernel, grid, dim3(256), 0, s, g);
+  if (plan.tile == kInt8Few) {
+    const dim3 grid(unsigned(g.N + 15) / 16);
+    // long rows: more of them in flight (4096 x 12288 11.8 us, with eight waves 12.5; 24576 x 4096 20.4 and 19.7)
+    if (g.K > 8192) hipLaunchKernelGGL((int8_gemm_few_kernel<16, 2>), grid, dim3(1024), 0, s, g);
+    else hipLaunchKernelGGL((int8_gemm_few_kernel<8, 4>), grid, dim3(512), 0, s, g);
+    return true;
+  }
+  const Int8Tile& t = kInt8Tile[plan.tile];
+  const long groups = long((g.M + t.bm - 1) / t.bm) * ((g.N + t.bn - 1) / t.bn) * plan.splits;
+  if (groups >= 1L << 22) return false;  // a launch holds fewer than 2^32 threads
+  t.launch(g, unsigned(groups), s);
+  if (plan.splits > 1) {
+    const unsigned long long units = (unsigned long long)(g.M) * ((g.N + 3) / 4);
+    hipLaunchKernelGGL(int8_gemm_join_kernel, dim3(unsigned((units + 255) / 256)), dim3(256), 0, s, g, plan.splits);
+  }
   return true;
 }
 

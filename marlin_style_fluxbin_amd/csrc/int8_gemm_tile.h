@@ -1,0 +1,234 @@
+// Products of 8-bit rows, BM rows of the activations by BN of the weight a workgroup: both in LDS in
+// a ring of S stages of 64 columns, filled from memory without passing through registers.
+#pragma once
+#include "int8_gemm.h"
+
+namespace fx {
+
+typedef int i32x16_t __attribute__((ext_vector_type(16)));
+typedef unsigned u32x2v_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) char lds8_t;
+
+// D[i, j] += sum_k A[i, k] B[j, k] over 32 bytes of k: lane l gives bytes 16 (l / 32) .. of row
+// l % 32 of both and holds D[8 (r / 4) + 4 (l / 32) + r % 4, l % 32], r < 16.
+__device__ __forceinline__ i32x16_t mfma_i8_32(const u32x4_t& a, const u32x4_t& b, const i32x16_t& c) {
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
+}
+
+// 16 bytes per lane from `resource` at the lane's offset to lds + 16 * lane, asynchronously
+// (vmcnt).  The instruction has no result register; written as the builtin, every later LDS
+// read of the kernel waits for it, whichever buffer it fills.
+__device__ __forceinline__ void fill_lds(const u32x4_t& resource, int offset, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset),
+               "s"(resource)
+               : "memory", "m0");
+}
+
+template <int N>
+__device__ __forceinline__ void tile_wait() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));
+  __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void tile_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// A wave's results to memory, 32 rows of them at a time through LDS of its own, so that eight lanes
+// and more write a row's neighbours: written from the registers (8 bytes a lane and 32 rows at a time)
+// the results of a 256 x 256 tile took 20 us.
+// OUT: kBF16, kF16, kF32, or -1 for the sums of a K split.
+template <int OUT, int NT, int MT>
+__device__ __forceinline__ void tile_store_as(const Int8GemmArgs& g, const i32x16_t (&acc)[NT][MT], int m0, int n0,
+                                              int split, lds8_t* lds, int lane) {
+  constexpr int kSize = OUT == kBF16 || OUT == kF16 ? 2 : 4, kRow = NT * 32 * kSize + 16;
+  constexpr int kLanes = NT * 32 * kSize / 16, kPass = 64 / kLanes;  // lanes of a row, rows of a wave store
+  const int half = lane >> 5, low = lane & 31;
+  char* out = OUT < 0 ? reinterpret_cast<char*>(g.partial + size_t(split) * g.M * g.N) : static_cast<char*>(g.out);
+  const long long stride = OUT < 0 ? g.N : g.out_stride;
+  const bool vec = OUT < 0 ? g.N % 4 == 0 : g.vec;
+  f32x4v_t ws[NT * 4], bias[NT * 4];
+  if constexpr (OUT >= 0) {
+#pragma unroll
+    for (int q = 0; q < NT * 4; ++q) {
+      const int n = n0 + q * 8 + half * 4;
+      ws[q] = column_scales(g, n);
+      bias[q] = column_bias<OUT>(g, n);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    const int m = m0 + j * 32;
+    const float sa = OUT < 0 ? 0.f : g.a_scales[min(m + low, g.M - 1)];
+    wave_lds_order();
+#pragma unroll
+    for (int q = 0; q < NT * 4; ++q) {
+      lds8_t* at = lds + low * kRow + (q * 8 + half * 4) * kSize;
+      const i32x16_t& v = acc[q / 4][j];
+      const int r0 = (q & 3) * 4;
+      if constexpr (OUT < 0) {
+        *reinterpret_cast<__attribute__((address_space(3))) i32x4_t*>(at) = i32x4_t{v[r0], v[r0 + 1], v[r0 + 2], v[r0 + 3]};
+      } else {
+        float y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = fmaf(float(v[r0 + r]) * sa, ws[q][r], bias[q][r]);
+        if constexpr (OUT == kF32) {
+          *reinterpret_cast<__attribute__((address_space(3))) f32x4v_t*>(at) = f32x4v_t{y[0], y[1], y[2], y[3]};
+        } else {
+          u32x2v_t p = {round_pair_bits<OUT>(y[0], y[1]), round_pair_bits<OUT>(y[2], y[3])};
+          *reinterpret_cast<__attribute__((address_space(3))) u32x2v_t*>(at) = p;
+        }
+      }
+    }
+    wave_lds_order();
+    if (vec && n0 + NT * 32 <= g.N) {
+#pragma unroll
+      for (int p = 0; p < 32 / kPass; ++p) {
+        const int row = p * kPass + lane / kLanes, place = (lane % kLanes) * 16;
+        const u32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(lds + row * kRow + place);
+        if (m + row < g.M)
+          *reinterpret_cast<u32x4_t*>(out + ((m + row) * stride + n0) * kSize + place) = v;
+      }
+    } else {
+      for (int u = lane; u < 32 * NT * 32; u += 64) {
+        const int row = u / (NT * 32), col = u % (NT * 32);
+        if (m + row < g.M && n0 + col < g.N) {
+          const lds8_t* at = lds + row * kRow + col * kSize;
+          char* to = out + ((m + row) * stride + n0 + col) * kSize;
+          if constexpr (kSize == 2) *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const __attribute__((address_space(3))) uint16_t*>(at);
+          else *reinterpret_cast<unsigned*>(to) = *reinterpret_cast<const __attribute__((address_space(3))) unsigned*>(at);
+        }
+      }
+    }
+  }
+}
+template <int NT, int MT>
+__device__ __forceinline__ void tile_store(const Int8GemmArgs& g, const i32x16_t (&acc)[NT][MT], int m0, int n0,
+                                           int split, lds8_t* lds, int lane) {
+  if (g.partial) tile_store_as<-1>(g, acc, m0, n0, split, lds, lane);
+  else if (g.dt == kBF16) tile_store_as<kBF16>(g, acc, m0, n0, split, lds, lane);
+  else if (g.dt == kF16) tile_store_as<kF16>(g, acc, m0, n0, split, lds, lane);
+  else tile_store_as<kF32>(g, acc, m0, n0, split, lds, lane);
+}
+constexpr int tile_store_bytes(int NT) { return 32 * (NT * 32 * 4 + 16); }  // of LDS, a wave
+
+template <int BM, int BN, int WM, int WN, int BK, int S>
+__global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8GemmArgs g) {
+  constexpr int kWaves = WM * WN, TM = BM / WM, TN = BN / WN, MT = TM / 32, NT = TN / 32;
+  constexpr int kStage = (BM + BN) * BK, kRows = 1024 / BK, kPlaces = BK / 16, kSteps = BK / 32;
+  constexpr int P = (BM + BN) / kRows / kWaves;  // wave loads of kRows rows a stage
+  static_assert((BM + BN) / kRows % kWaves == 0 && S >= 2, "waves share a stage's loads evenly");
+  constexpr int kResults = kWaves * tile_store_bytes(NT);
+  __shared__ __attribute__((aligned(1024))) char ring[S * kStage > kResults ? S * kStage : kResults];
+  const int lane = threadIdx.x & 63, wave = wave_index();
+  const unsigned lds0 = unsigned(size_t((lds8_t*)ring));
+
+  // the tile: those that one XCD runs at a time are neighbours, eight along M
+  const int tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.N + BN - 1) / BN, tiles = tiles_m * tiles_n;
+  const int linear = xcd_local_index8(blockIdx.x, gridDim.x);
+  const int split = linear / tiles, tile = linear - split * tiles;
+  constexpr int kGroup = 8;
+  const int group = tile / (kGroup * tiles_n), first = group * kGroup, high = min(kGroup, tiles_m - first);
+  const int in_group = tile - group * kGroup * tiles_n;
+  const int tn = in_group / high, tm = first + in_group - tn * high;
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int k_begin = split * g.k_per_split, k_end = min(g.K, k_begin + g.k_per_split);
+  const int stages = (k_end - k_begin + BK - 1) / BK;
+
+  // This wave's loads: kRows rows of BK bytes each, lane l bytes 16 c .. of row l / kPlaces, where it
+  // fills place l % kPlaces: c is that place with swizzle(row) applied, so that 16 lanes that read one c
+  // of 16 rows in a row meet 16 places of 16 bytes within 256 bytes (64 banks).
+  const auto swizzle = [](int row) { return BK == 64 ? (row >> 2) & 3 : (row >> 1) & 7; };
+  int chunk[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) chunk[i] = ((lane % kPlaces) ^ swizzle(i * kRows + lane / kPlaces)) * 16;
+  size_t base[P];
+  int records[P], offset[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int piece = wave * P + i;
+    const bool is_w = piece < BN / kRows;
+    const int row = is_w ? n0 + piece * kRows : m0 + (piece - BN / kRows) * kRows;
+    const int left = min(kRows, (is_w ? g.N : g.M) - row);
+    const long long stride = is_w ? g.w_stride : g.a_stride;
+    base[i] = reinterpret_cast<size_t>(is_w ? g.w : g.a) + row * stride + k_begin;
+    records[i] = left > 0 ? (left - 1) * int(stride) + k_end - k_begin : 0;
+    offset[i] = (lane / kPlaces) * int(stride) + chunk[piece & 1];
+  }
+  // The XCDs begin at different columns: they read the same rows at different times, and rows of a
+  // power of two apart meet more of the memory's channels at any one.
+  int issued = 0, next = int(blockIdx.x % kXcdCount) * stages / kXcdCount;  // stages
+  auto issue = [&]() __attribute__((always_inline)) {
+    const int k = next * BK, left = issued < stages ? k_end - k_begin - k : 0;
+    const unsigned dst = lds0 + unsigned(issued % S) * kStage + wave * (P * 1024);
+    next = next + 1 == stages ? 0 : next + 1;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const size_t at = base[i] + k;
+      const u32x4_t r = {unsigned(at), unsigned(at >> 32) & 0xffffu, left > 0 ? unsigned(max(records[i] - k, 0)) : 0u,
+                         0x00020000u};
+      fill_lds(r, chunk[(wave * P + i) & 1] < left ? offset[i] : kOutOfRange, dst + i * 1024);
+    }
+    ++issued;
+  };
+
+  const int wm = wave / WN, wn = wave % WN;
+  const char* w_at = ring + (wn * TN + (lane & 31)) * BK;
+  const char* a_at = ring + (BN + wm * TM + (lane & 31)) * BK;
+  const int place = ((lane >> 5) ^ swizzle(lane & 31)) * 16;
+
+  i32x16_t acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+  u32x4_t w[2][NT], a[2][MT];
+  auto read = [&](int h, int step, int stage) __attribute__((always_inline)) {
+    const int at = stage * kStage + (place ^ (step * 32));
+#pragma unroll
+    for (int i = 0; i < NT; ++i) w[h][i] = *reinterpret_cast<const u32x4_t*>(w_at + at + i * 32 * BK);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) a[h][j] = *reinterpret_cast<const u32x4_t*>(a_at + at + j * 32 * BK);
+  };
+  auto multiply = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[i][j] = mfma_i8_32(w[h][i], a[h][j], acc[i][j]);
+  };
+
+#pragma unroll
+  for (int s = 0; s < S; ++s) issue();
+  tile_wait<(S - 1) * P>();
+  tile_barrier();
+  read(0, 0, 0);
+  int here = 0;
+  for (int s = 0; s < stages; ++s) {
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+      if (t < kSteps - 1) {
+        read((t + 1) & 1, t + 1, here);
+      } else {
+        // stage s is in every wave's registers, and stage s + 1 is there
+        tile_wait<(S - 2) * P>();
+        tile_barrier();
+        issue();
+        here = here + 1 == S ? 0 : here + 1;
+        read(0, 0, here);
+      }
+      multiply(t & 1);
+    }
+  }
+  tile_wait<0>();  // nothing fills this workgroup's LDS after its last wave has left
+
+  tile_barrier();  // nor does a wave read it any more
+  tile_store(g, acc, m0 + wm * TM, n0 + wn * TN, split, (lds8_t*)ring + wave * tile_store_bytes(NT), lane);
+}
+
+}  // namespace fx
