@@ -62,6 +62,17 @@ int fx_int8_gemm(const int8_t *a, long long a_stride, const float *a_scales, con
                  const float *w_scales, const void *bias, void *out, long long out_stride, void *workspace,
                  size_t workspace_bytes, int M, int N, int K, int dtype, void *stream);
 
+/*
+ * A Linear in one call: rows x [M, K] of x_dtype (fp16 or bf16) quantized (fx_int8_quantize) and
+ * multiplied (fx_int8_gemm) with w [N, K padded to whole 16, zeros behind K] to out of out_dtype.
+ * `workspace`: fx_int8_linear_workspace_bytes bytes, 16-byte aligned, no initial contents; it
+ * holds the codes, their scales and the product's partial sums.
+ */
+size_t fx_int8_linear_workspace_bytes(int M, int N, int K);
+int fx_int8_linear(const void *x, long long x_stride, int x_dtype, const int8_t *w, long long w_stride,
+                   const float *w_scales, const void *bias, void *out, long long out_stride, void *workspace,
+                   size_t workspace_bytes, int M, int N, int K, int out_dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2120,12 +2120,14 @@ size_t fx_int8_gemm_workspace_bytes(int M, int N, int K) {
   return int8_gemm_workspace(fx::plan_int8_gemm(M, N, K), M, N);
 }
 
-int fx_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales, const int8_t* w, long long w_stride,
-                 const float* w_scales, const void* bias, void* out, long long out_stride, void* workspace,
-                 size_t workspace_bytes, int M, int N, int K, int dtype, void* stream) {
-  if (int rc = validate_int8_gemm_sizes(M, N, K)) return rc;
+namespace {
+
+// The checks of a product, its arguments and its plan.
+int prepare_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales, const int8_t* w, long long w_stride,
+                      const float* w_scales, const void* bias, void* out, long long out_stride, void* workspace,
+                      size_t workspace_bytes, int M, int N, int K, int dtype, fx::Int8GemmArgs* args,
+                      fx::Int8GemmPlan* planned) {
   if (!is_half_dtype(dtype) && dtype != FX_F32) return fail(FX_EINVAL, "dtype must be fp32, fp16 or bf16");
-  if (M == 0) return FX_OK;
   if (int rc = validate_code_rows("a", a, a_stride, M, K)) return rc;
   if (int rc = validate_code_rows("w", w, w_stride, N, K)) return rc;
   if (!a_scales || !w_scales || !out) return fail(FX_EINVAL, "scales and out must be non-null");
@@ -2141,7 +2143,9 @@ int fx_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales, con
       return fail(FX_EINVAL, "gemm workspace needs %zu bytes, got %zu", need, workspace_bytes);
     if (!aligned16(workspace)) return fail(FX_EINVAL, "workspace must be 16-byte aligned");
   }
-  fx::Int8GemmArgs g{};
+  *planned = plan;
+  fx::Int8GemmArgs& g = *args;
+  g = {};
   g.a = a;
   g.w = w;
   g.a_scales = a_scales;
@@ -2158,9 +2162,86 @@ int fx_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales, con
   g.dt = dtype;
   g.k_per_split = plan.k_per_split;
   g.vec = aligned16(out) && out_stride * size % 16 == 0;
+  return FX_OK;
+}
+
+int run_int8_gemm(const fx::Int8GemmArgs& g, const fx::Int8GemmPlan& plan, void* stream) {
   if (!fx::launch_int8_gemm(plan, g, static_cast<hipStream_t>(stream)))
-    return fail(FX_EINVAL, "no kernel for a product of %d x %d x %d", M, N, K);
+    return fail(FX_EINVAL, "a product of %d x %d x %d is too large for one call", g.M, g.N, g.K);
   return check_launch("fx_int8_gemm");
+}
+
+}  // namespace
+
+int fx_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales, const int8_t* w, long long w_stride,
+                 const float* w_scales, const void* bias, void* out, long long out_stride, void* workspace,
+                 size_t workspace_bytes, int M, int N, int K, int dtype, void* stream) {
+  if (int rc = validate_int8_gemm_sizes(M, N, K)) return rc;
+  if (!is_half_dtype(dtype) && dtype != FX_F32) return fail(FX_EINVAL, "dtype must be fp32, fp16 or bf16");
+  if (M == 0) return FX_OK;
+  fx::Int8GemmArgs g{};
+  fx::Int8GemmPlan plan{};
+  if (int rc = prepare_int8_gemm(a, a_stride, a_scales, w, w_stride, w_scales, bias, out, out_stride, workspace,
+                                 workspace_bytes, M, N, K, dtype, &g, &plan))
+    return rc;
+  return run_int8_gemm(g, plan, stream);
+}
+
+namespace {
+// The parts of a Linear's workspace: codes, scales, partial sums.
+struct Int8LinearParts {
+  int width;  // of a row of codes
+  size_t scales, partial, bytes;
+};
+Int8LinearParts int8_linear_parts(int M, int N, int K) {
+  Int8LinearParts p;
+  p.width = (K + 15) / 16 * 16;
+  p.scales = align_up(size_t(M) * p.width, 256);
+  p.partial = align_up(p.scales + size_t(M) * sizeof(float), 256);
+  p.bytes = p.partial + fx_int8_gemm_workspace_bytes(M, N, p.width);
+  return p;
+}
+}  // namespace
+
+size_t fx_int8_linear_workspace_bytes(int M, int N, int K) {
+  if (K < 1 || K > fx::kInt8MaxK / 16 * 16 || validate_int8_gemm_sizes(M, N, 16) || M == 0) return 0;
+  return int8_linear_parts(M, N, K).bytes;
+}
+
+int fx_int8_linear(const void* x, long long x_stride, int x_dtype, const int8_t* w, long long w_stride,
+                   const float* w_scales, const void* bias, void* out, long long out_stride, void* workspace,
+                   size_t workspace_bytes, int M, int N, int K, int out_dtype, void* stream) {
+  if (K < 1 || K > fx::kInt8MaxK / 16 * 16)
+    return fail(FX_EINVAL, "K must be in [1, %d], got %d", fx::kInt8MaxK / 16 * 16, K);
+  if (int rc = validate_int8_gemm_sizes(M, N, 16)) return rc;
+  if (!is_half_dtype(x_dtype)) return fail(FX_EINVAL, "x dtype must be fp16 or bf16");
+  if (!is_half_dtype(out_dtype) && out_dtype != FX_F32) return fail(FX_EINVAL, "out dtype must be fp32, fp16 or bf16");
+  if (M == 0) return FX_OK;
+  const Int8LinearParts p = int8_linear_parts(M, N, K);
+  if (!workspace || workspace_bytes < p.bytes)
+    return fail(FX_EINVAL, "linear workspace needs %zu bytes, got %zu", p.bytes, workspace_bytes);
+  if (!aligned16(workspace)) return fail(FX_EINVAL, "workspace must be 16-byte aligned");
+  char* base = static_cast<char*>(workspace);
+  int8_t* codes = reinterpret_cast<int8_t*>(base);
+  float* scales = reinterpret_cast<float*>(base + p.scales);
+  if (int rc = validate_half_rows("x", x, x_stride)) return rc;
+  fx::Int8GemmArgs g{};
+  fx::Int8GemmPlan plan{};
+  if (int rc = prepare_int8_gemm(codes, p.width, scales, w, w_stride, w_scales, bias, out, out_stride,
+                                 base + p.partial, workspace_bytes - p.partial, M, N, p.width, out_dtype, &g, &plan))
+    return rc;
+  if (fx::int8_linear_fuses(plan, M, p.width)) {
+    fx::Int8RowsArgs rows{};
+    rows.x = static_cast<const uint16_t*>(x);
+    rows.x_stride = x_stride;
+    rows.rows = M;
+    rows.columns = K;
+    rows.code_columns = p.width;
+    fx::launch_int8_linear_few(x_dtype, rows, g, static_cast<hipStream_t>(stream));
+    return check_launch("fx_int8_linear");
+  }
+  if (int rc = fx_int8_quantize(x, x_stride, codes, p.width, scales, M, K, p.width, x_dtype, stream)) return rc;
+  return run_int8_gemm(g, plan, stream);
 }
 
 }  // extern "C"

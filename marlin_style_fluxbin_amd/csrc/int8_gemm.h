@@ -35,10 +35,9 @@ __device__ __forceinline__ f32x4v_t column_bias(const Int8GemmArgs& g, int n) {
 }
 
 // Columns n .. n + 3 (those below N) of row m: one rounding of (acc a_scale) w_scale + bias in fp32.
-// acc's own float is rounded once beyond 2^24 (2^-24 of it).
+// (sa: the row's scale.)  acc's own float is rounded once beyond 2^24 (2^-24 of it).
 template <int DT>
-__device__ __forceinline__ void store4_as(const Int8GemmArgs& g, int m, int n, const i32x4_t& acc) {
-  const float sa = g.a_scales[m];
+__device__ __forceinline__ void store4_as(const Int8GemmArgs& g, int m, int n, const i32x4_t& acc, float sa) {
   const f32x4v_t ws = column_scales(g, n), bias = column_bias<DT>(g, n);
   float y[4];
 #pragma unroll
@@ -66,10 +65,10 @@ __device__ __forceinline__ void store4_as(const Int8GemmArgs& g, int m, int n, c
     }
   }
 }
-__device__ __forceinline__ void store4(const Int8GemmArgs& g, int m, int n, const i32x4_t& acc) {
-  if (g.dt == kBF16) store4_as<kBF16>(g, m, n, acc);
-  else if (g.dt == kF16) store4_as<kF16>(g, m, n, acc);
-  else store4_as<kF32>(g, m, n, acc);
+__device__ __forceinline__ void store4(const Int8GemmArgs& g, int m, int n, const i32x4_t& acc, float sa) {
+  if (g.dt == kBF16) store4_as<kBF16>(g, m, n, acc, sa);
+  else if (g.dt == kF16) store4_as<kF16>(g, m, n, acc, sa);
+  else store4_as<kF32>(g, m, n, acc, sa);
 }
 
 // The same columns of one K split's sums, [splits, M, N].

@@ -26,10 +26,10 @@ __global__ __launch_bounds__(256) void int8_gemm_join_kernel(const Int8GemmArgs 
       for (int r = 0; r < 4; ++r)
         if (n + r < g.N) total[r] += p[s * plane + r];
   }
-  store4(g, m, n, total);
+  store4(g, m, n, total, g.a_scales[m]);
 }
 
-constexpr int kFewRows = 16;
+constexpr int kFewRows = 32;
 constexpr int kMaxSplits = 16;
 
 }  // namespace
@@ -42,7 +42,7 @@ Int8GemmPlan plan_int8_gemm(int M, int N, int K) {
   const int stages = (K + 127) / 128;
   const float bytes = (float(M) + N) * K / 4.8e6f;
   Int8GemmPlan best{kInt8Few, 1, K};
-  float least = M <= kFewRows ? 3.f + float(N) * K / 4.9e6f * (1.f + 0.016f * M) : 1e30f;
+  float least = M <= kFewRows ? 3.f + float(N) * K / 4.9e6f * (M <= 16 ? 1.f + 0.016f * M : 1.45f) : 1e30f;
   for (int tile = 0; tile < kInt8Tiles; ++tile) {
     const Int8Tile& t = kInt8Tile[tile];
     const long tiles = long((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
@@ -54,19 +54,43 @@ Int8GemmPlan plan_int8_gemm(int M, int N, int K) {
       const float last = float(groups - (rounds - 1) * slots) / 256.f;  // workgroups of a unit in the last round
       const float stage = (rounds - 1) * t.full + (last <= 1.f ? t.alone : t.alone + (t.full - t.alone) * (last - 1.f));
       float time = 3.f + std::max(per * stage + rounds * t.ends, bytes);
-      if (splits > 1) time += 2.5f + 2.f * splits * float(M) * N * 4.f / 5e6f;
+      if (splits > 1) time += 3.5f + 2.f * splits * float(M) * N * 4.f / 5e6f;
       if (time < least) least = time, best = {tile, splits, splits == 1 ? K : per * 128};
     }
   }
   return best;
 }
 
+template <int XDT>
+void launch_few(const Int8GemmArgs& g, const Int8RowsArgs& rows, int vec, hipStream_t s) {
+  const dim3 grid(unsigned(g.N + 15) / 16);
+  // long rows: more of them in flight (4096 x 12288 11.8 us, with eight waves 12.5; 24576 x 4096 20.4 and 19.7)
+  if (g.K > 8192) hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, 1, 1, 16, 2>), grid, dim3(1024), 0, s, g, rows, vec);
+  else hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, 1, 1, 8, 4>), grid, dim3(512), 0, s, g, rows, vec);
+}
+
+// Rows that every workgroup of the few-rows kernel had better quantize for itself.
+bool int8_linear_fuses(const Int8GemmPlan& plan, int M, int K) {
+  return plan.tile == kInt8Few && M <= 16 && long(M) * K <= kFewCodes;
+}
+
+void launch_int8_linear_few(int x_dt, const Int8RowsArgs& rows, const Int8GemmArgs& g, hipStream_t s) {
+  const int vec = reinterpret_cast<uintptr_t>(rows.x) % 16 == 0 && rows.x_stride % 8 == 0;
+  if (x_dt == kBF16) launch_few<kBF16>(g, rows, vec, s);
+  else launch_few<kF16>(g, rows, vec, s);
+}
+
 bool launch_int8_gemm(const Int8GemmPlan& plan, const Int8GemmArgs& g, hipStream_t s) {
   if (plan.tile == kInt8Few) {
-    const dim3 grid(unsigned(g.N + 15) / 16);
-    // long rows: more of them in flight (4096 x 12288 11.8 us, with eight waves 12.5; 24576 x 4096 20.4 and 19.7)
-    if (g.K > 8192) hipLaunchKernelGGL((int8_gemm_few_kernel<16, 2>), grid, dim3(1024), 0, s, g);
-    else hipLaunchKernelGGL((int8_gemm_few_kernel<8, 4>), grid, dim3(512), 0, s, g);
+    if (g.M <= 16) {
+      launch_few<-1>(g, {}, 0, s);
+    } else if (g.N <= 4096) {  // one workgroup a compute unit at most: 32 rows by 4096 x 4096 8.9 us, 11.1 with 32 columns
+      hipLaunchKernelGGL((int8_gemm_few_kernel<-1, 2, 1, 8, 4>), dim3(unsigned(g.N + 15) / 16), dim3(512), 0, s, g,
+                         Int8RowsArgs{}, 0);
+    } else {  // 24 rows by 6144 x 4096 10.8 us, 13.4 with 16 columns
+      hipLaunchKernelGGL((int8_gemm_few_kernel<-1, 2, 2, 8, 4>), dim3(unsigned(g.N + 31) / 32), dim3(512), 0, s, g,
+                         Int8RowsArgs{}, 0);
+    }
     return true;
   }
   const Int8Tile& t = kInt8Tile[plan.tile];

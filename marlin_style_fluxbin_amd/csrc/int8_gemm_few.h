@@ -2,53 +2,107 @@
 // the matrix cores' operands.
 #pragma once
 #include "int8_gemm.h"
+#include "int8_row.h"
 
 namespace fx {
 
-// 16 rows of the weight by at most 16 of the activations a workgroup, its W waves dealing the
+constexpr int kFewCodes = 16384;  // bytes of codes that a workgroup quantizes for itself
+
+// RT x 16 rows of the weight by MT x 16 of the activations a workgroup, its W waves dealing the
 // columns in pieces of 128: a wave's sums are over its own columns and are added through LDS, so that
 // one launch has a burst of the whole weight in flight.  Bound by the weight's bytes (24576 x 4096 at
 // one row 19.7 us, 5.1 TB/s; 4096 x 4096 5.1 us, of which a launch is 4): every wave issues UN pieces'
-// loads in front of its first product (left to the compiler's order, 20.4).  32 rows of the weight a
-// workgroup took 7.2 us for 5.1, two tiles of activations more than int8_gemm_tile.h.
-template <int W, int UN>
-__global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(1, 4))) void int8_gemm_few_kernel(const Int8GemmArgs g) {
-  __shared__ i32x4_t sums[W][64];
+// loads in front of its first product (left to the compiler's order, 20.4).
+//
+// XDT kBF16 or kF16: the rows come unquantized, and every workgroup quantizes them for itself while
+// its part of the weight is on the way: a launch less than codes that another kernel leaves.
+template <int XDT, int MT, int RT, int W, int UN>
+__global__ __launch_bounds__(W * 64) void int8_gemm_few_kernel(const Int8GemmArgs g, const Int8RowsArgs rows, int vec) {
+  constexpr bool kQuantize = XDT >= 0;
+  constexpr int kTiles = MT * RT;
+  static_assert(!kQuantize || MT == 1, "sixteen rows of codes at most in LDS");
+  __shared__ i32x4_t sums[W][kTiles][64];
+  __shared__ __attribute__((aligned(16))) int8_t codes[kQuantize ? kFewCodes : 16];
+  __shared__ double red[W];
+  __shared__ float row_scales[16];
   const int lane = threadIdx.x & 63, wave = wave_index();
   const int r = lane & 15, k16 = (lane >> 4) * 16;
-  const int n0 = xcd_local_index8(blockIdx.x, gridDim.x) * 16;
+  const int n0 = xcd_local_index8(blockIdx.x, gridDim.x) * (16 * RT);
   const int w_stride = int(g.w_stride), a_stride = int(g.a_stride);
   // rows past the last: no access, zeros
-  const auto rw = buffer_resource_2g(g.w + n0 * g.w_stride, unsigned(min(16, g.N - n0) - 1) * w_stride + g.K);
-  const auto ra = buffer_resource_2g(g.a, unsigned(g.M - 1) * a_stride + g.K);
-  const int w_at = n0 + r < g.N ? r * w_stride + k16 : kOutOfRange;
-  const int a_at = r < g.M ? r * a_stride + k16 : kOutOfRange;
-  i32x4_t acc = {0, 0, 0, 0};
-  for (int k0 = wave * 128; k0 < g.K; k0 += W * 128 * UN) {
-    u32x4_t w[UN][2], a[UN][2];
+  const auto rw = buffer_resource_2g(g.w + n0 * g.w_stride, unsigned(min(16 * RT, g.N - n0) - 1) * w_stride + g.K);
+  const auto ra = buffer_resource_2g(g.a, kQuantize ? 0u : unsigned(g.M - 1) * a_stride + g.K);
+  int w_at[RT], a_at[MT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) w_at[t] = n0 + 16 * t + r < g.N ? (16 * t + r) * w_stride + k16 : kOutOfRange;
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    if (kQuantize) a_at[t] = min(r, g.M - 1) * g.K + k16;  // (a column past M is not stored)
+    else a_at[t] = 16 * t + r < g.M ? (16 * t + r) * a_stride + k16 : kOutOfRange;
+  }
+  i32x4_t acc[RT][MT];
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) acc[i / MT][i % MT] = i32x4_t{0, 0, 0, 0};
+  u32x4_t w[UN][2][RT], a[UN][2][MT];
+  // (an offset with kOutOfRange's bit is past every range)
+  auto past = [&](int k) __attribute__((always_inline)) { return k + k16 < g.K ? 0 : kOutOfRange; };
+  auto load_w = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < UN; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int k = k0 + u * W * 128 + h * 64;
-        const int out = k + k16 < g.K ? 0 : kOutOfRange;  // (an offset with this bit is past every range)
-        w[u][h] = load_b128_stream(rw, (w_at + k) | out, 0);
-        a[u][h] = load_b128(ra, (a_at + k) | out, 0);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) w[u][h][t] = load_b128_stream(rw, (w_at[t] + k) | past(k), 0);
+        if constexpr (!kQuantize) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t) a[u][h][t] = load_b128(ra, (a_at[t] + k) | past(k), 0);
+        }
       }
     __builtin_amdgcn_sched_barrier(0);
+  };
+  int k0 = wave * 128;
+  load_w(k0);
+  if constexpr (kQuantize) {
+    RowPointers p{};
+    for (int m = 0; m < g.M; ++m) {
+      p.x = rows.x + m * rows.x_stride;
+      p.codes = codes + m * g.K;
+      quantize_row<XDT, kRowsPlain, W * 64, 2>(rows, p, row_scales + m, threadIdx.x, vec, true, red);
+    }
+    __syncthreads();
+  }
+  while (true) {
+    if constexpr (kQuantize) {
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int k = k0 + u * W * 128 + h * 64;
+          a[u][h][0] = *reinterpret_cast<const u32x4_t*>(codes + (past(k) ? k16 : a_at[0] + k));
+        }
+    }
 #pragma unroll
     for (int u = 0; u < UN; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) acc = mfma_i8_16(w[u][h], a[u][h], acc);
-  }
-  sums[wave][lane] = acc;
-  __syncthreads();
-  if (wave == 0) {
-    i32x4_t total = sums[0][lane];
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int v = 1; v < W; ++v) total += sums[v][lane];
-    const int m = r, n = n0 + (lane >> 4) * 4;
-    if (m < g.M && n < g.N) store4(g, m, n, total);
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < MT; ++j) acc[i][j] = mfma_i8_16(w[u][h][i], a[u][h][j], acc[i][j]);
+    k0 += W * 128 * UN;
+    if (k0 >= g.K) break;
+    load_w(k0);
+  }
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) sums[wave][i][lane] = acc[i / MT][i % MT];
+  __syncthreads();
+  for (int tile = wave; tile < kTiles; tile += W) {
+    i32x4_t total = sums[0][tile][lane];
+#pragma unroll
+    for (int v = 1; v < W; ++v) total += sums[v][tile][lane];
+    const int m = (tile % MT) * 16 + r, n = n0 + (tile / MT) * 16 + (lane >> 4) * 4;
+    if (m < g.M && n < g.N) store4(g, m, n, total, kQuantize ? row_scales[m & 15] : g.a_scales[m]);
   }
 }
 

@@ -54,6 +54,9 @@ struct Int8GemmPlan {
   int k_per_split;
 };
 Int8GemmPlan plan_int8_gemm(int M, int N, int K);
+// Whether a Linear's rows are quantized in the product's own launch, and that launch.
+bool int8_linear_fuses(const Int8GemmPlan& plan, int M, int K);
+void launch_int8_linear_few(int x_dt, const Int8RowsArgs& rows, const Int8GemmArgs& g, hipStream_t s);
 bool launch_int8_gemm(const Int8GemmPlan& plan, const Int8GemmArgs& a, hipStream_t s);
 
 }  // namespace fx

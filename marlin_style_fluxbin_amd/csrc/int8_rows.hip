@@ -4,142 +4,12 @@
 //
 // One pass: a row's values stay in registers between its maximum and its codes.  Bound by the bytes
 // of the rows.
-#include "int8_launch.h"
+#include "int8_row.h"
 
 namespace fx {
 namespace {
 
-constexpr float kSmall = 0x1p-100f;  // 127 / a and the codes' products are normal floats from here on
-constexpr float kRounder = 12582912.f;  // 1.5 * 2^23: adding it rounds to a whole number, ties to even
-
-template <int TPR, class T, class F>
-__device__ __forceinline__ T row_reduce(T v, F f, T* red) {
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) v = f(v, __shfl_xor(v, offset, 64));
-  if constexpr (TPR > 64) {
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int i = 1; i < TPR / 64; ++i) v = f(v, red[i]);
-  }
-  return v;
-}
-
-// Eight 16-bit values from p, n of them there (the others 0).
-__device__ __forceinline__ u32x4_t load8(const uint16_t* p, int n, bool vec) {
-  if (vec && n >= 8) return *reinterpret_cast<const u32x4_t*>(p);
-  u32x4_t v = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < n) v[e >> 1] |= unsigned(p[e]) << (16 * (e & 1));
-  return v;
-}
-__device__ __forceinline__ void store8(uint16_t* p, const u32x4_t& v, int n, bool vec) {
-  if (vec && n >= 8) {
-    *reinterpret_cast<u32x4_t*>(p) = v;
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < n) p[e] = uint16_t(v[e >> 1] >> (16 * (e & 1)));
-}
-// Eight codes, each in the low byte of c, n of them there.
-__device__ __forceinline__ void store_codes(int8_t* p, const unsigned (&c)[8], int n, bool vec) {
-  if (vec && n >= 8) {
-    uint2 v;
-    v.x = (c[0] & 255u) | (c[1] & 255u) << 8 | (c[2] & 255u) << 16 | c[3] << 24;
-    v.y = (c[4] & 255u) | (c[5] & 255u) << 8 | (c[6] & 255u) << 16 | c[7] << 24;
-    *reinterpret_cast<uint2*>(p) = v;
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < n) p[e] = int8_t(c[e]);
-}
-template <int DT>
-__device__ __forceinline__ float at8(const u32x4_t& v, int e) {
-  return to_f32<DT>(uint16_t(v[e >> 1] >> (16 * (e & 1))));
-}
-template <int DT>
-__device__ __forceinline__ u32x4_t add8(const u32x4_t& x, const u32x4_t& r) {
-  u32x4_t s;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    float lo = to_f32<DT>(uint16_t(x[w])) + to_f32<DT>(uint16_t(r[w]));
-    float hi = to_f32<DT>(uint16_t(x[w] >> 16)) + to_f32<DT>(uint16_t(r[w] >> 16));
-    s[w] = round_pair_bits<DT>(lo, hi);
-  }
-  return s;
-}
-
-struct RowPointers {
-  const uint16_t *x, *second;
-  uint16_t* sum;
-  int8_t* codes;
-};
-
-// A row in 64 bits, read anew: rows of any length, and those whose values leave the range that the
-// floats of the fast way hold (a row of zeros, magnitudes below 2^-100, sums of squares or products
-// beyond 2^128, infinities, NaN).
-template <int DT, int MODE, int TPR>
-__device__ void row_in_64_bits(const Int8RowsArgs& a, const RowPointers& p, float* scale_out, int tl, bool vec,
-                               bool code_vec, bool added, double* red) {
-  const auto value = [&](int c, int e, const u32x4_t& xv, const u32x4_t& yv) __attribute__((always_inline)) {
-    const double x = at8<DT>(xv, e);
-    if constexpr (MODE == kRowsNorm) return x * double(at8<DT>(yv, e));
-    else if constexpr (MODE == kRowsSwiglu) return x / (1. + exp(-x)) * double(at8<DT>(yv, e));
-    else return x;
-  };
-  const auto load = [&](int c, u32x4_t& xv, u32x4_t& yv) __attribute__((always_inline)) {
-    const int n = a.columns - 8 * c;
-    yv = u32x4_t{0u, 0u, 0u, 0u};
-    if (MODE == kRowsNorm && p.second) xv = load8(p.sum + 8 * c, n, vec);
-    else xv = load8(p.x + 8 * c, n, vec);
-    if constexpr (MODE == kRowsNorm) yv = load8(a.weight + 8 * c, n, vec);
-    if constexpr (MODE == kRowsSwiglu) yv = load8(p.second + 8 * c, n, vec);
-  };
-  const int chunks = (a.columns + 7) / 8;
-  double top = 0., squares = 0.;
-  for (int c = tl; c < chunks; c += TPR) {
-    if (MODE == kRowsNorm && p.second && !added) {  // each thread reads what it wrote itself
-      const int n = a.columns - 8 * c;
-      store8(p.sum + 8 * c, add8<DT>(load8(p.x + 8 * c, n, vec), load8(p.second + 8 * c, n, vec)), n, vec);
-    }
-    u32x4_t xv, yv;
-    load(c, xv, yv);
-#pragma unroll 1
-    for (int e = 0; e < 8; ++e) {
-      const double v = fabs(value(c, e, xv, yv)), x = at8<DT>(xv, e);
-      top = v >= top || v != v ? v : top;  // a NaN stays: no later value is >= it, and v == v
-      if constexpr (MODE == kRowsNorm) squares += x * x;
-    }
-  }
-  const auto larger = [](double u, double v) { return u != u || u >= v ? u : v; };  // a NaN is the largest
-  const auto plus = [](double u, double v) { return u + v; };
-  top = row_reduce<TPR>(top, larger, red);
-  double inverse = 1.;
-  if constexpr (MODE == kRowsNorm) {
-    squares = row_reduce<TPR>(squares, plus, red);
-    inverse = top > 0. ? 1. / sqrt(squares / a.columns + double(a.eps)) : 0.;
-  }
-  float scale = float(top * inverse / 127.);
-  const bool held = scale < INFINITY;  // a row that no float scale stands for is NaN
-  if (!held) scale = __uint_as_float(0x7fc00000u);
-  if (tl == 0) *scale_out = scale;
-  for (int c = tl; 8 * c < a.code_columns; c += TPR) {
-    u32x4_t xv = {0u, 0u, 0u, 0u}, yv = xv;
-    if (c < chunks) load(c, xv, yv);
-    unsigned code[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      code[e] = held && top > 0. ? unsigned(int(rint(value(c, e, xv, yv) * 127. / top))) : 0u;
-    store_codes(p.codes + 8 * c, code, a.code_columns - 8 * c, code_vec);
-  }
-}
-
-// TPR threads a row, CH chunks of 8 columns a thread in registers (0: rows of any length).
+// TPR threads a row.
 template <int DT, int MODE, int TPR, int CH>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void int8_rows_kernel(const Int8RowsArgs a, int vec, int code_vec) {
   constexpr int kBlock = TPR < 256 ? 256 : TPR;
@@ -152,78 +22,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void int8_rows_kernel(const 
   p.second = a.second ? a.second + row * a.second_stride : nullptr;
   p.sum = a.sum ? a.sum + row * a.sum_stride : nullptr;
   p.codes = a.codes + row * a.code_stride;
-  if constexpr (CH == 0) {
-    row_in_64_bits<DT, MODE, TPR>(a, p, a.scales + row, tl, vec, code_vec, false, red);
-  } else {
-    u32x4_t xv[CH], yv[CH], wv[CH];
-#pragma unroll
-    for (int q = 0; q < CH; ++q) {
-      const int c = tl + q * TPR, n = a.columns - 8 * c;
-      xv[q] = load8(p.x + 8 * c, n, vec);
-      if (MODE != kRowsPlain && p.second) yv[q] = load8(p.second + 8 * c, n, vec);
-      if constexpr (MODE == kRowsNorm) wv[q] = load8(a.weight + 8 * c, n, vec);
-    }
-    float v[CH][8], squares = 0.f;
-    unsigned top_bits = 0u;
-#pragma unroll
-    for (int q = 0; q < CH; ++q) {
-      if (MODE == kRowsNorm && p.second) {
-        const int c = tl + q * TPR;
-        xv[q] = add8<DT>(xv[q], yv[q]);
-        store8(p.sum + 8 * c, xv[q], a.columns - 8 * c, vec);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = at8<DT>(xv[q], e);
-        if constexpr (MODE == kRowsNorm) {
-          squares = fmaf(x, x, squares);
-          v[q][e] = x * at8<DT>(wv[q], e);  // exact: 22 bits at most
-        } else if constexpr (MODE == kRowsSwiglu) {
-          v[q][e] = x / (1.f + expf(-x)) * at8<DT>(yv[q], e);
-        } else {
-          v[q][e] = x;
-        }
-        top_bits = max(top_bits, __float_as_uint(v[q][e]) & 0x7fffffffu);
-      }
-    }
-    // (as bits, so that an infinity or NaN is the largest)
-    top_bits = row_reduce<TPR>(top_bits, [](unsigned u, unsigned w) { return max(u, w); }, reinterpret_cast<unsigned*>(red));
-    const float top = __uint_as_float(top_bits);
-    float inverse = 1.f;
-    bool plain = top_bits < 0x7f800000u && top >= kSmall;
-    if constexpr (MODE == kRowsNorm) {
-      squares = row_reduce<TPR>(squares, [](float u, float w) { return u + w; }, reinterpret_cast<float*>(red));
-      plain = plain && squares < INFINITY && squares >= kSmall;
-      inverse = rsqrtf(squares / float(a.columns) + a.eps);
-    }
-    const float scale = top * inverse / 127.f;
-    if (!plain || !(scale < INFINITY)) {
-      row_in_64_bits<DT, MODE, TPR>(a, p, a.scales + row, tl, vec, code_vec, true, red);
-      return;
-    }
-    if (tl == 0) a.scales[row] = scale;
-    const float r = 127.f / top;
-#pragma unroll
-    for (int q = 0; q < CH; ++q) {
-      const int c = tl + q * TPR, n = a.code_columns - 8 * c;
-      unsigned code[8];
-      bool near = false;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float t = v[q][e] * r, whole = t + kRounder;
-        code[e] = __float_as_uint(whole);
-        // within the rounding of t (2^-15) of a border between two codes
-        near = near || fabsf(t - (whole - kRounder)) > 0.4999f;
-      }
-      // The products w s and x are exact, so their codes can be: the quotient again in 64 bits,
-      // where one of 22-bit numbers that is no border differs from every border.
-      if (MODE != kRowsSwiglu && near) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) code[e] = unsigned(int(rint(double(v[q][e]) * 127. / double(top))));
-      }
-      if (n > 0) store_codes(p.codes + 8 * c, code, n, code_vec);
-    }
-  }
+  quantize_row<DT, MODE, TPR, CH>(a, p, a.scales + row, tl, vec, code_vec, red);
 }
 
 template <int DT, int MODE>

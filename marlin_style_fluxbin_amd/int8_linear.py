@@ -14,6 +14,8 @@ Nothing synchronises, so calls can be captured into a HIP graph.
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 from torch import nn
 from torch.nn import functional as F
@@ -29,36 +31,42 @@ _STEP = 16                # columns of the products' rows come in whole 16 bytes
 _ROW_LIMIT = 1 << 22      # bytes between two rows of codes that the products take
 _WHAT = "an 8-bit operator"
 
-_workspaces: dict[tuple[int, int, int], int] = {}
+_BF16, _FP16, _INT8, _FP32 = torch.bfloat16, torch.float16, torch.int8, torch.float32
+_CODES = {dtype: _lib.dtype_code(dtype) for dtype in _OUT}
 
 
+@lru_cache(maxsize=4096)
 def _workspace_bytes(m: int, n: int, k: int) -> int:
-    """The library's answer, kept: it depends on the sizes alone."""
-    key = (m, n, k)
-    found = _workspaces.get(key)
-    if found is None:
-        if len(_workspaces) > 4096:
-            _workspaces.clear()
-        found = _workspaces[key] = _lib.library().fx_int8_gemm_workspace_bytes(m, n, k)
-    return found
+    return _lib.library().fx_int8_gemm_workspace_bytes(m, n, k)
+
+
+@lru_cache(maxsize=4096)
+def _linear_workspace_bytes(m: int, n: int, k: int) -> int:
+    return _lib.library().fx_int8_linear_workspace_bytes(m, n, k)
 
 
 def _refuse(*tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("8-bit operators have no backward pass; call them under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("8-bit operators have no backward pass; call them under torch.no_grad()")
     _refuse_records(*tensors, what=_WHAT)
 
 
 def _rows_of(t: torch.Tensor) -> tuple[int, int] | None:
     """(rows, elements between rows) of ``t [..., columns]`` where its rows lie evenly in memory
     with contiguous columns, else None."""
-    shape, columns = t.shape, t.shape[-1]
+    shape = t.shape
+    columns = shape[-1]
     if t.is_contiguous():
         return t.numel() // columns, columns
-    if t.stride(-1) != 1 and columns > 1:
+    strides = t.stride()
+    if strides[-1] != 1 and columns > 1:
         return None
+    if len(shape) == 2:
+        return shape[0], strides[0]
     rows, step = 1, columns
-    for n, s in zip(reversed(shape[:-1]), reversed(t.stride()[:-1])):
+    for n, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         if n == 1:
             continue
         if rows == 1:
@@ -71,12 +79,13 @@ def _rows_of(t: torch.Tensor) -> tuple[int, int] | None:
 
 def _half_input(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> tuple[torch.Tensor, int, int]:
     """``t`` or a copy of it as the kernels read it, its row count and row stride."""
-    if not t.is_cuda or t.dtype not in _HALF:
+    dtype, shape = t.dtype, t.shape
+    if not t.is_cuda or (dtype is not _BF16 and dtype is not _FP16):
         _lib.require_gpu_tensor(t, name)
         raise ValueError(f"{name} must be fp16 or bf16")
-    if t.ndim < 1 or t.shape[-1] < 1:
+    if not shape or shape[-1] < 1:
         raise ValueError(f"{name} must have shape [..., columns] with columns to hold")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+    if like is not None and (shape != like.shape or dtype is not like.dtype or t.get_device() != like.get_device()):
         raise ValueError(f"{name} must have the input's shape, dtype and device")
     if t.is_neg():
         t = t.resolve_neg()
@@ -87,16 +96,15 @@ def _half_input(t: torch.Tensor, name: str, like: torch.Tensor | None = None) ->
     return t, *found
 
 
-def _code_outputs(x: torch.Tensor, out) -> tuple[torch.Tensor, torch.Tensor, int]:
+def _code_outputs(shape: torch.Size, device: torch.device, out) -> tuple[torch.Tensor, torch.Tensor, int]:
     """codes, scales and the codes' row stride: new ones, or the caller's checked."""
-    shape = x.shape
     if out is None:
-        codes = torch.empty(shape, dtype=torch.int8, device=x.device)
-        return codes, torch.empty(shape[:-1], dtype=torch.float32, device=x.device), shape[-1]
+        return (torch.empty(shape, dtype=_INT8, device=device), torch.empty(shape[:-1], dtype=_FP32, device=device),
+                shape[-1])
     codes, scales = out
-    if codes.shape != shape or codes.dtype is not torch.int8 or codes.device != x.device:
+    if codes.shape != shape or codes.dtype is not _INT8 or codes.device != device:
         raise ValueError("out's codes must be int8 of the input's shape on its device")
-    if (scales.shape != shape[:-1] or scales.dtype is not torch.float32 or scales.device != x.device
+    if (scales.shape != shape[:-1] or scales.dtype is not _FP32 or scales.device != device
             or not scales.is_contiguous()):
         raise ValueError("out's scales must be contiguous fp32 of the input's leading shape on its device")
     found = _rows_of(codes)
@@ -105,21 +113,17 @@ def _code_outputs(x: torch.Tensor, out) -> tuple[torch.Tensor, torch.Tensor, int
     return codes, scales, found[1]
 
 
-def _quantize_into(x2: torch.Tensor, rows: int, stride: int, columns: int, codes: torch.Tensor, code_stride: int,
-                   code_columns: int, scales: torch.Tensor) -> None:
-    _launch("fx_int8_quantize", x2.device, x2.data_ptr(), stride, codes.data_ptr(), code_stride, scales.data_ptr(), rows,
-            columns, code_columns, _lib.dtype_code(x2.dtype))
-
-
 def quantize_int8(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | None = None):
     """Each row of ``x [..., columns]`` (fp16 or bf16) as ``codes`` (int8, x's shape) and ``scales``
     (fp32, x's leading shape): with a the row's largest magnitude, code = round(127 x / a), ties to
     even, scale = a / 127.  A row with an infinity or NaN stands for NaN (its scale is NaN)."""
     _refuse(x)
     x, rows, stride = _half_input(x, "x")
-    codes, scales, code_stride = _code_outputs(x, out)
-    columns = x.shape[-1]
-    _quantize_into(x, rows, stride, columns, codes, code_stride, columns, scales)
+    shape, device = x.shape, x.device
+    codes, scales, code_stride = _code_outputs(shape, device, out)
+    columns = shape[-1]
+    _launch("fx_int8_quantize", device, x.data_ptr(), stride, codes.data_ptr(), code_stride, scales.data_ptr(), rows,
+            columns, columns, _CODES[x.dtype])
     return codes, scales
 
 
@@ -144,28 +148,32 @@ def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, *, dtype: torch.d
     return out
 
 
-def _norm(x, residual, weight, eps, residual_out, out, padded: int | None = None):
+def _norm(x, residual, weight, eps, residual_out, out):
     _refuse(x, residual, weight, residual_out)
     x, rows, stride = _half_input(x, "hidden_states")
-    columns = x.shape[-1]
-    if weight.shape != (columns,) or weight.dtype != x.dtype or weight.device != x.device:
+    shape, dtype, device = x.shape, x.dtype, x.device
+    columns = shape[-1]
+    if weight.shape != (columns,) or weight.dtype is not dtype or weight.get_device() != device.index:
         raise ValueError("weight must have shape [hidden] and the input's dtype and device")
-    weight = weight.resolve_neg().contiguous()
-    r_ptr = r_stride = s_ptr = s_stride = None
+    if weight.is_neg() or not weight.is_contiguous():
+        weight = weight.resolve_neg().contiguous()
+    r_ptr = s_ptr = None
+    r_stride = s_stride = 0
     if residual is not None:
         residual, _, r_stride = _half_input(residual, "residual", x)
         if residual_out is None:
-            residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        elif residual_out.shape != x.shape or residual_out.dtype != x.dtype or residual_out.device != x.device:
-            raise ValueError("residual_out must have the input's shape, dtype and device")
-        found = None if residual_out.is_neg() else _rows_of(residual_out)
-        if found is None or (found[0] > 1 and found[1] < columns):
-            raise ValueError("residual_out must have contiguous rows, each its own memory")
-        r_ptr, s_ptr, s_stride = residual.data_ptr(), residual_out.data_ptr(), found[1]
-    codes, scales, code_stride = _code_outputs(x, out)
-    _launch("fx_int8_rmsnorm", x.device, x.data_ptr(), stride, r_ptr, r_stride or 0, s_ptr, s_stride or 0,
-            weight.data_ptr(), codes.data_ptr(), code_stride, scales.data_ptr(), rows, columns, columns, float(eps),
-            _lib.dtype_code(x.dtype))
+            residual_out, s_stride = torch.empty(shape, dtype=dtype, device=device), columns
+        else:
+            if residual_out.shape != shape or residual_out.dtype is not dtype or residual_out.device != device:
+                raise ValueError("residual_out must have the input's shape, dtype and device")
+            found = None if residual_out.is_neg() else _rows_of(residual_out)
+            if found is None or (found[0] > 1 and found[1] < columns):
+                raise ValueError("residual_out must have contiguous rows, each its own memory")
+            s_stride = found[1]
+        r_ptr, s_ptr = residual.data_ptr(), residual_out.data_ptr()
+    codes, scales, code_stride = _code_outputs(shape, device, out)
+    _launch("fx_int8_rmsnorm", device, x.data_ptr(), stride, r_ptr, r_stride, s_ptr, s_stride, weight.data_ptr(),
+            codes.data_ptr(), code_stride, scales.data_ptr(), rows, columns, columns, eps, _CODES[dtype])
     return codes, scales, residual_out
 
 
@@ -193,18 +201,19 @@ def silu_mul_int8(gate: torch.Tensor, up: torch.Tensor, *, out: tuple[torch.Tens
     _refuse(gate, up)
     gate, rows, stride = _half_input(gate, "gate")
     up, _, up_stride = _half_input(up, "up", gate)
-    codes, scales, code_stride = _code_outputs(gate, out)
-    columns = gate.shape[-1]
-    _launch("fx_int8_silu_mul", gate.device, gate.data_ptr(), stride, up.data_ptr(), up_stride, codes.data_ptr(),
-            code_stride, scales.data_ptr(), rows, columns, columns, _lib.dtype_code(gate.dtype))
+    shape, device = gate.shape, gate.device
+    codes, scales, code_stride = _code_outputs(shape, device, out)
+    columns = shape[-1]
+    _launch("fx_int8_silu_mul", device, gate.data_ptr(), stride, up.data_ptr(), up_stride, codes.data_ptr(), code_stride,
+            scales.data_ptr(), rows, columns, columns, _CODES[gate.dtype])
     return codes, scales
 
 
 def _check_codes(codes: torch.Tensor, scales: torch.Tensor, name: str, scales_name: str) -> None:
-    if not codes.is_cuda or codes.dtype is not torch.int8 or codes.ndim < 1:
+    if codes.dtype is not _INT8 or not codes.is_cuda or not codes.shape:
         _lib.require_gpu_tensor(codes, name)
         raise ValueError(f"{name} must be int8 [..., columns]")
-    if scales.dtype is not torch.float32 or scales.shape != codes.shape[:-1] or scales.device != codes.device:
+    if scales.dtype is not _FP32 or scales.shape != codes.shape[:-1] or scales.get_device() != codes.get_device():
         raise ValueError(f"{scales_name} must be fp32, one for each row of {name}, on its device")
 
 
@@ -235,24 +244,27 @@ def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, w
     multiple of 16; others are copied first."""
     _check_codes(a, a_scales, "a", "a_scales")
     _check_codes(weight, weight_scales, "weight", "weight_scales")
-    if weight.ndim != 2 or a.shape[-1] != weight.shape[1] or a.device != weight.device:
+    shape, wide, device = a.shape, weight.shape, a.device
+    index, k = device.index, shape[-1]
+    if len(wide) != 2 or k != wide[1] or weight.get_device() != index:
         raise ValueError("weight must be [N, K] with a's K, on a's device")
-    k, n = a.shape[-1], weight.shape[0]
+    n = wide[0]
     if not 1 <= k <= MAX_IN_FEATURES or n < 1:
         raise ValueError(f"K must be in [1, {MAX_IN_FEATURES}] and N positive, got {k} and {n}")
-    if dtype not in _OUT:
+    code = _CODES.get(dtype)
+    if code is None:
         raise ValueError("dtype must be fp16, bf16 or fp32")
     if bias is not None:
-        if bias.shape != (n,) or bias.dtype != dtype or bias.device != a.device:
+        if bias.shape != (n,) or bias.dtype is not dtype or bias.get_device() != index:
             raise ValueError("bias must have shape [N], the result's dtype and a's device")
         bias = bias.resolve_neg().contiguous()
     _refuse(a_scales, weight_scales, bias, out)
-    shape = (*a.shape[:-1], n)
+    shape = (*shape[:-1], n)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=a.device)
+        out = torch.empty(shape, dtype=dtype, device=device)
         out_stride = n
     else:
-        if out.shape != shape or out.dtype != dtype or out.device != a.device or out.is_neg():
+        if out.shape != shape or out.dtype is not dtype or out.get_device() != index or out.is_neg():
             raise ValueError("out must have shape [..., N], the result's dtype and a's device")
         found = _rows_of(out)
         if found is None or (found[0] > 1 and found[1] < n):
@@ -261,17 +273,12 @@ def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, w
     a, rows, a_stride, width = _code_rows(a)
     weight, _, w_stride, _ = _code_rows(weight)
     a_scales, weight_scales = a_scales.contiguous(), weight_scales.contiguous()
-    _product(a, a_stride, a_scales, weight, w_stride, weight_scales, bias, out, out_stride, rows, n, width)
+    nbytes = _workspace_bytes(rows, n, width)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _launch("fx_int8_gemm", device, a.data_ptr(), a_stride, a_scales.data_ptr(), weight.data_ptr(), w_stride,
+            weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), out_stride,
+            None if workspace is None else workspace.data_ptr(), nbytes, rows, n, width, code)
     return out
-
-
-def _product(a, a_stride, a_scales, weight, w_stride, weight_scales, bias, out, out_stride, m, n, k, workspace=None):
-    nbytes = _workspace_bytes(m, n, k)
-    if nbytes and workspace is None:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=out.device)
-    _launch("fx_int8_gemm", out.device, a.data_ptr(), a_stride, a_scales.data_ptr(), weight.data_ptr(), w_stride,
-            weight_scales.data_ptr(), _lib.ptr(bias), out.data_ptr(), out_stride, _lib.ptr(workspace), nbytes, m, n, k,
-            _lib.dtype_code(out.dtype))
 
 
 def quantize_weight_int8(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -345,18 +352,18 @@ class PackedInt8Linear(PackedLinearBase):
         self._check_before_call()
 
     def _packed_kernel(self, rows: int, device: torch.device):
-        """The rows quantized and multiplied, through buffers of this callable's own."""
+        """The rows quantized and multiplied, through a workspace of this callable's own."""
         codes, scales, bias = self._tensor("codes"), self._tensor("scales"), self._tensor("bias")
         width, k, o = self._width, self.in_features, self.out_features
-        a = torch.empty((rows, width), dtype=torch.int8, device=device)
-        a_scales = torch.empty(rows, dtype=torch.float32, device=device)
-        nbytes = _workspace_bytes(rows, o, width)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        nbytes = _linear_workspace_bytes(rows, o, k)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
 
         def run(x2: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
-            _quantize_into(x2, rows, k, k, a, width, width, a_scales)
+            code = _CODES[x2.dtype]
             added = bias if bias is None or bias.dtype == out.dtype else bias.to(out.dtype)
-            _product(a, width, a_scales, codes, width, scales, added, out, o, rows, o, width, workspace)
+            _launch("fx_int8_linear", device, x2.data_ptr(), x2.stride(0), code, codes.data_ptr(), width,
+                    scales.data_ptr(), None if added is None else added.data_ptr(), out.data_ptr(), o,
+                    workspace.data_ptr(), nbytes, rows, o, k, _CODES[out.dtype])
             return out
         return run
 
@@ -365,23 +372,27 @@ class PackedInt8Linear(PackedLinearBase):
             return self._decode_binding(x)
         if torch.is_grad_enabled():
             raise RuntimeError("packed inference requires no_grad/inference_mode")
-        shape, k = x.shape, self.in_features
+        shape, k, dtype = x.shape, self.in_features, x.dtype
         if len(shape) < 2 or shape[-1] != k:
             raise ValueError("expected [...,K] input")
         self._check_before_call()
         device = self._tensor("codes").device
         rows = x.numel() // k
-        if x.dtype not in _HALF or x.device != device or not x.is_cuda or rows > self.max_packed_rows:
+        if (not x.is_cuda or (dtype is not _BF16 and dtype is not _FP16) or x.get_device() != device.index
+                or rows > self.max_packed_rows):
             if self.fallback != "dense":
                 raise ValueError("unsupported input; enable explicit dense fallback if needed")
             self._count(DENSE_FALLBACK)
             return self._dense_linear(x)
         _refuse_records(x, what=_WHAT)
         self._count(PACKED_M1 if rows == 1 else PACKED_SMALL_M)
-        out = torch.empty((*shape[:-1], self.out_features), device=device, dtype=x.dtype)
+        out = torch.empty((*shape[:-1], self.out_features), device=device, dtype=dtype)
         if rows:
-            x = x.resolve_neg() if x.is_neg() else x
-            self._packed_kernel(rows, device)(x.reshape(rows, k).contiguous(), out)
+            if x.is_neg():
+                x = x.resolve_neg()
+            if len(shape) != 2 or not x.is_contiguous():
+                x = x.reshape(rows, k).contiguous()
+            self._packed_kernel(rows, device)(x, out)
         return out
 
 

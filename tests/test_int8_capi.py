@@ -36,6 +36,9 @@ DEFAULTS = {
     "fx_int8_restore": dict(codes=D, code_stride=112, scales=D, out=D, out_stride=100, rows=3, columns=100, dtype=2,
                             stream=None),
     "fx_int8_gemm_workspace_bytes": dict(M=1, N=1, K=16),
+    "fx_int8_linear_workspace_bytes": dict(M=1, N=1, K=16),
+    "fx_int8_linear": dict(x=D, x_stride=60, x_dtype=2, w=D, w_stride=64, w_scales=D, bias=D, out=D, out_stride=8,
+                           workspace=D, workspace_bytes=1 << 20, M=3, N=8, K=60, out_dtype=2, stream=None),
     "fx_int8_gemm": dict(a=D, a_stride=64, a_scales=D, w=D, w_stride=64, w_scales=D, bias=D, out=D, out_stride=8,
                          workspace=None, workspace_bytes=0, M=3, N=8, K=64, dtype=2, stream=None),
 }
@@ -103,6 +106,14 @@ CASES += [("fx_int8_gemm", *c) for c in [
     (dict(out=None), "scales and out must be non-null"), (dict(w_scales=D + 2), "aligned to their elements"),
     (dict(bias=D + 2, dtype=0), "aligned to their elements"), (dict(out=D + 1), "aligned to their elements"),
     (dict(out_stride=7), "out stride")]]
+CASES += [("fx_int8_linear", *c) for c in [
+    (dict(M=-1), "M must be in"), (dict(N=0), "N must be in"), (dict(K=0), "K must be in"),
+    (dict(K=131057), "K must be in"), (dict(x_dtype=0), "x dtype must be"), (dict(out_dtype=3), "dtype must be fp32"),
+    (dict(workspace=None), "workspace needs"), (dict(workspace_bytes=511), "workspace needs"),
+    (dict(workspace=D + 8), "workspace must be 16-byte aligned"), (dict(x=None), "x must be non-null"),
+    (dict(x_stride=-2), "x stride"), (dict(w=None), "w must be non-null"), (dict(w_stride=48), "w stride"),
+    (dict(w=D + 8), "w must have 16-byte aligned rows"), (dict(w_scales=None), "scales and out must be non-null"),
+    (dict(bias=D + 1), "aligned to their elements"), (dict(out_stride=7), "out stride")]]
 
 
 @pytest.mark.parametrize("name,over,message", CASES, ids=lambda x: x if isinstance(x, str) else None)
@@ -111,16 +122,21 @@ def test_refusals(name, over, message):
     assert rc == 1 and message in error, (rc, error)
 
 
-@pytest.mark.parametrize("name", [n for n in DEFAULTS if n not in ("fx_int8_gemm", "fx_int8_gemm_workspace_bytes")])
+@pytest.mark.parametrize("name", [n for n in DEFAULTS if "gemm" not in n and "linear" not in n])
 def test_no_rows_do_nothing(name):
     assert call(name, rows=0, codes=None, scales=None, out=None)[0] == 0 if name == "fx_int8_restore" else (
         call(name, rows=0)[0] == 0)
     assert call("fx_int8_gemm", M=0, a=None, out=None)[0] == 0
+    assert call("fx_int8_linear", M=0, x=None, workspace=None)[0] == 0
 
 
 def test_workspace_query_refuses_bad_sizes():
     size = _lib.library().fx_int8_gemm_workspace_bytes
     assert size(-1, 8, 64) == size(1, 0, 64) == size(1, 8, 65) == size(0, 8, 64) == 0
+    whole = _lib.library().fx_int8_linear_workspace_bytes
+    assert whole(-1, 8, 64) == whole(1, 0, 64) == whole(1, 8, 0) == whole(0, 8, 64) == whole(1, 8, 131057) == 0
+    # codes padded to whole 16 columns, a scale for each row, the product's own
+    assert whole(3, 8, 60) == 256 + 256 + size(3, 8, 64)
 
 
 def test_a_split_products_workspace_is_checked():

@@ -256,3 +256,30 @@ def test_a_layers_mlp(gpu, m, dtype):
     size = smooth.abs() + slack
     assert bool(((both.double() - smooth).abs() <= slack + product_bound(size, size, dtype)).all())
     assert quantize_int8(both)[0].shape == both.shape
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("m,n,k", [(1, 33, 16), (1, 4096, 4096), (2, 1000, 8192), (3, 100, 5000), (4, 64, 4096), (5, 64, 4096),
+                                   (1, 50, 16384), (1, 50, 16400), (16, 100, 1000), (17, 5000, 1024), (32, 300, 640), (33, 300, 640)])
+def test_module_is_quantize_and_matmul(gpu, m, n, k, dtype):
+    """Whichever launches a Linear takes, bit for bit the two operators, rows that no code holds among them."""
+    w, sw = codes(n, k, gpu, 1, -127), scales(n, gpu, 2)
+    bias = torch.randn(n, generator=torch.Generator(device=gpu).manual_seed(3), device=gpu).to(dtype)
+    module = PackedInt8Linear(w, sw, bias=bias)
+    x = torch.randn(m, k, generator=torch.Generator(device=gpu).manual_seed(4), device=gpu).to(dtype)
+    with torch.no_grad():
+        for change in range(4):
+            if change == 1:
+                x[m // 2] = 0
+            if change == 2:
+                x[m // 2, -1] = float("inf")
+            if change == 3:
+                x[0] = (x[0].double() * 2.0**-120).to(dtype)
+            a, sa = quantize_int8(x)
+            want = int8_matmul(a, sa, w, sw, bias=bias, dtype=dtype)
+            got = module(x)
+            assert torch.equal(got.view(torch.int16)[~torch.isnan(want)], want.view(torch.int16)[~torch.isnan(want)])
+            assert torch.equal(torch.isnan(got), torch.isnan(want)), change
+        odd = torch.randn(m, k + 1, device=gpu).to(dtype)[:, 1:]
+        a, sa = quantize_int8(odd)
+        assert torch.equal(module(odd), int8_matmul(a, sa, w, sw, bias=bias, dtype=dtype))
