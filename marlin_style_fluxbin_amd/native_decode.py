@@ -21,7 +21,7 @@ same with the hybrid GEMV's normalising prologue and residual epilogue
 (``fx_hybrid_gemv_segments_rmsnormed``, ``fx_hybrid_gemv_residual``), the
 SwiGLU formed in the down GEMV's prologue (6 per layer).  Other Linears (dense bf16, the bf16
 arm, ``torch.matmul``) run between add+RMSNorm kernels and the same attention
-launches.  The arithmetic and rounding points are the stock HF Qwen3 modules'
+launches; with 8-bit Linears (``PackedInt8Linear``) the norms and the SwiGLU write codes.  The arithmetic and rounding points are the stock HF Qwen3 modules'
 (RMSNorm, RoPE, SDPA with fp32 softmax, SwiGLU).
 """
 from __future__ import annotations
@@ -34,6 +34,7 @@ import torch
 from . import _lib
 from .cached_attention import HEAD_DIMS, Int4KVCache, kv4_attention, window_attention
 from .fused_modules import add_rms_norm, head_norm_rope
+from .int8_linear import PackedInt8Linear, add_rms_norm_int8, int8_matmul, rms_norm_int8, silu_mul_int8
 from .static_decode import graph_kernel_count
 from .deployment import HybridSegmentsGemv, PackedHybridLinear
 from .w3_lut_deployment import PackedW3Linear, W3Gemv
@@ -71,7 +72,7 @@ class _Linear:
         elif isinstance(module, PackedW3Linear):
             self.gemv = W3Gemv(module.layout(), arithmetic=module.arithmetic)
             self.call = self.gemv
-        elif isinstance(module, PackedHybridLinear):
+        elif isinstance(module, (PackedHybridLinear, PackedInt8Linear)):
             self.call = module._packed_kernel(1, module.codes.device)
         elif isinstance(module, torch.nn.Linear):
             weight = module.weight
@@ -79,7 +80,7 @@ class _Linear:
         else:
             raise TypeError(f"unsupported Linear type {type(module).__name__}")
         self.packed = not isinstance(module, torch.nn.Linear)
-        self.bias = module.bias
+        self.bias = None if getattr(module, "bias_in_kernel", False) else module.bias
 
     def __call__(self, x, out):
         self.call(x, out)
@@ -126,6 +127,13 @@ class _FusedLinear:
             except ValueError:
                 return None
             return _FusedLinear(gemv, [m.out_features for m in modules])
+        if all(isinstance(m, PackedInt8Linear) for m in modules):
+            # each output row as its own call gives it: one quantization of the input for all
+            if any(m.bias is not None for m in modules) or len({m.in_features for m in modules}) != 1:
+                return None
+            fused = PackedInt8Linear(torch.cat([m.codes[:, :m.in_features] for m in modules]),
+                                     torch.cat([m.scales for m in modules]))
+            return _FusedLinear(fused._packed_kernel(1, fused.codes.device), [m.out_features for m in modules])
         if all(type(m) is torch.nn.Linear for m in modules) and all(m.bias is None for m in modules):
             weight = torch.cat([m.weight for m in modules], dim=0).contiguous()
             return _FusedLinear(lambda x, out: torch.matmul(x, weight.t(), out=out),
@@ -437,6 +445,59 @@ class _ResidualStream:
                       x_sorted=True)
 
 
+class _Int8Chain:
+    """The decode step on 8-bit Linears: the norms and the SwiGLU write the codes that q|k|v, gate|up
+    and down read (``add_rms_norm_int8``, ``silu_mul_int8``, ``int8_matmul`` on the modules' codes
+    joined along O), o quantizes the attention's output in its own launch.  For sessions whose
+    Linears all are ``PackedInt8Linear`` of whole 16 in_features."""
+
+    def __init__(self, session):
+        def joined(block, names):
+            modules = [block.get_submodule(n) for n in names]
+            for m in modules:
+                m._check_before_bind(session.device)
+            bias = None
+            if any(m.bias is not None for m in modules):
+                bias = torch.cat([torch.zeros(m.out_features, dtype=session.dtype, device=session.device)
+                                  if m.bias is None else m.bias.to(session.dtype) for m in modules])
+            if len(modules) == 1:  # its own buffers, no copy
+                return modules[0].codes, modules[0].scales, bias
+            return torch.cat([m.codes for m in modules]), torch.cat([m.scales for m in modules]), bias
+
+        self.qkv = [joined(b, _ATTN[:3]) for b in session.layers]
+        self.gate_up = [joined(b, _MLP[:2]) for b in session.layers]
+        self.down = [joined(b, _MLP[2:]) for b in session.layers]
+
+        def codes(width):
+            return (torch.empty((1, width), dtype=torch.int8, device=session.device),
+                    torch.empty(1, dtype=torch.float32, device=session.device))
+
+        self.hidden, self.act = codes(session.hidden), codes(session.act.shape[1])
+
+    def product(self, rows, joined, out):
+        codes, scales, bias = joined
+        int8_matmul(*rows, codes, scales, bias=bias, dtype=out.dtype, out=out)
+
+    def step(self, session, pos):
+        """The layers of one token, from its embedding in ``session.residual`` to the last down
+        product in ``session.down`` (not yet added)."""
+        rows, eps = self.hidden, session.eps
+        for l, lin in enumerate(session.lin):
+            if l == 0:
+                rms_norm_int8(session.residual, session.in_norm[0], eps, out=rows)
+            else:
+                add_rms_norm_int8(session.down, session.residual, session.in_norm[l], eps,
+                                  residual_out=session.residual, out=rows)
+            self.product(rows, self.qkv[l], session.qkv_out)
+            session._attention(l, pos)
+            lin["self_attn.o_proj"](session.attn, session.o)
+            add_rms_norm_int8(session.o, session.residual, session.post_norm[l], eps, residual_out=session.residual,
+                              out=rows)
+            self.product(rows, self.gate_up[l], session.gate_up_out)
+            silu_mul_int8(session.gate, session.up, out=self.act)
+            self.product(self.act, self.down[l], session.down)
+
+
 class NativeDecodeSession:
     """``kv_cache="int4"`` holds the keys and values in an :class:`Int4KVCache` per layer (the
     prefix quantized after its prefill, each token as it is decoded); ``window`` / ``sinks``
@@ -519,11 +580,13 @@ class NativeDecodeSession:
         self.lm_head = model.lm_head.weight
         self.lin = [{name: _Linear(block.get_submodule(name)) for name in _ATTN + _MLP} for block in self.layers]
         # q|k|v and gate|up as one GEMV each where the payloads allow it
-        self.qkv = [_FusedLinear.build([b.get_submodule(n) for n in _ATTN[:3]]) for b in self.layers]
+        int8 = all(isinstance(b.get_submodule(n), PackedInt8Linear) and b.get_submodule(n).in_features % 16 == 0
+                   for b in self.layers for n in _ATTN + _MLP)
+        self.qkv = [None if int8 else _FusedLinear.build([b.get_submodule(n) for n in _ATTN[:3]]) for b in self.layers]
         # gate|up + SwiGLU as one launch where both are structural W3; else gate|up
         # (fused where possible) and the SwiGLU kernel
         self.swiglu = [_GateUpSwiGLU.build(*(b.get_submodule(n) for n in _MLP[:2])) for b in self.layers]
-        self.gate_up = [None if f is not None else _FusedLinear.build([b.get_submodule(n) for n in _MLP[:2]])
+        self.gate_up = [None if f is not None or int8 else _FusedLinear.build([b.get_submodule(n) for n in _MLP[:2]])
                         for f, b in zip(self.swiglu, self.layers)]
         if w3_payload not in ("fields", "planar", "fp6"):
             raise ValueError(f"w3_payload must be 'fields', 'planar' or 'fp6', got {w3_payload!r}")
@@ -550,6 +613,7 @@ class NativeDecodeSession:
         self.predictions = torch.empty((self.steps, 1), dtype=torch.int64, device=self.device)
         self.stream = _ResidualStream.build(
             self, {"fields": _lib.PAYLOAD_FIELDS, "planar": _lib.PAYLOAD_PLANAR, "fp6": _lib.PAYLOAD_FP6}[w3_payload])
+        self.int8 = _Int8Chain(self) if int8 else None
         lib = _lib.library()
         self.lib = lib
         # the final RMSNorm, LM head and argmax as one launch where the head allows it
@@ -688,6 +752,11 @@ class NativeDecodeSession:
             return self._step_residual_stream(i)
         pos = self.prefix_length + i
         torch.index_select(self.embed, 0, self.tokens[0, i:i + 1], out=self.residual)
+        if self.int8 is not None:
+            self.int8.step(self, pos)
+            add_rms_norm(self.down, self.residual, self.final_norm, self.eps, out=self.normed,
+                         residual_out=self.residual)
+            return self._lm_head(i, self.normed, None)
         from .fused_modules import rms_norm
 
         rms_norm(self.residual, self.in_norm[0], self.eps, out=self.normed)
