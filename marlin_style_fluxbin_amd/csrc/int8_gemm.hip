@@ -62,11 +62,11 @@ Int8GemmPlan plan_int8_gemm(int M, int N, int K) {
 }
 
 template <int XDT>
-void launch_few(const Int8GemmArgs& g, const Int8RowsArgs& rows, int vec, hipStream_t s) {
+void launch_few(const Int8GemmArgs& g, const Int8RowsArgs& rows, hipStream_t s) {
   const dim3 grid(unsigned(g.N + 15) / 16);
   // long rows: more of them in flight (4096 x 12288 11.8 us, with eight waves 12.5; 24576 x 4096 20.4 and 19.7)
-  if (g.K > 8192) hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, 1, 1, 16, 2>), grid, dim3(1024), 0, s, g, rows, vec);
-  else hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, 1, 1, 8, 4>), grid, dim3(512), 0, s, g, rows, vec);
+  if (g.K > 8192) hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, 1, 1, 16, 2>), grid, dim3(1024), 0, s, g, rows);
+  else hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, 1, 1, 8, 4>), grid, dim3(512), 0, s, g, rows);
 }
 
 // Rows that every workgroup of the few-rows kernel had better quantize for itself.
@@ -75,21 +75,20 @@ bool int8_linear_fuses(const Int8GemmPlan& plan, int M, int K) {
 }
 
 void launch_int8_linear_few(int x_dt, const Int8RowsArgs& rows, const Int8GemmArgs& g, hipStream_t s) {
-  const int vec = reinterpret_cast<uintptr_t>(rows.x) % 16 == 0 && rows.x_stride % 8 == 0;
-  if (x_dt == kBF16) launch_few<kBF16>(g, rows, vec, s);
-  else launch_few<kF16>(g, rows, vec, s);
+  if (x_dt == kBF16) launch_few<kBF16>(g, rows, s);
+  else launch_few<kF16>(g, rows, s);
 }
 
 bool launch_int8_gemm(const Int8GemmPlan& plan, const Int8GemmArgs& g, hipStream_t s) {
   if (plan.tile == kInt8Few) {
     if (g.M <= 16) {
-      launch_few<-1>(g, {}, 0, s);
+      launch_few<-1>(g, {}, s);
     } else if (g.N <= 4096) {  // one workgroup a compute unit at most: 32 rows by 4096 x 4096 8.9 us, 11.1 with 32 columns
       hipLaunchKernelGGL((int8_gemm_few_kernel<-1, 2, 1, 8, 4>), dim3(unsigned(g.N + 15) / 16), dim3(512), 0, s, g,
-                         Int8RowsArgs{}, 0);
+                         Int8RowsArgs{});
     } else {  // 24 rows by 6144 x 4096 10.8 us, 13.4 with 16 columns
       hipLaunchKernelGGL((int8_gemm_few_kernel<-1, 2, 2, 8, 4>), dim3(unsigned(g.N + 31) / 32), dim3(512), 0, s, g,
-                         Int8RowsArgs{}, 0);
+                         Int8RowsArgs{});
     }
     return true;
   }

@@ -17,7 +17,7 @@ constexpr int kFewCodes = 16384;  // bytes of codes that a workgroup quantizes f
 // XDT kBF16 or kF16: the rows come unquantized, and every workgroup quantizes them for itself while
 // its part of the weight is on the way: a launch less than codes that another kernel leaves.
 template <int XDT, int MT, int RT, int W, int UN>
-__global__ __launch_bounds__(W * 64) void int8_gemm_few_kernel(const Int8GemmArgs g, const Int8RowsArgs rows, int vec) {
+__global__ __launch_bounds__(W * 64) void int8_gemm_few_kernel(const Int8GemmArgs g, const Int8RowsArgs rows) {
   constexpr bool kQuantize = XDT >= 0;
   constexpr int kTiles = MT * RT;
   static_assert(!kQuantize || MT == 1, "sixteen rows of codes at most in LDS");
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(W * 64) void int8_gemm_few_kernel(const Int8GemmArg
     for (int m = 0; m < g.M; ++m) {
       p.x = rows.x + m * rows.x_stride;
       p.codes = codes + m * g.K;
-      quantize_row<XDT, kRowsPlain, W * 64, 2>(rows, p, row_scales + m, threadIdx.x, vec, true, red);
+      quantize_row<XDT, kRowsPlain, W * 64, 2>(rows, p, row_scales + m, threadIdx.x, red);
     }
     __syncthreads();
   }

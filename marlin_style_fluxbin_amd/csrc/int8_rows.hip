@@ -11,7 +11,7 @@ namespace {
 
 // TPR threads a row.
 template <int DT, int MODE, int TPR, int CH>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void int8_rows_kernel(const Int8RowsArgs a, int vec, int code_vec) {
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void int8_rows_kernel(const Int8RowsArgs a) {
   constexpr int kBlock = TPR < 256 ? 256 : TPR;
   __shared__ double red[kBlock / 64];
   const int tl = threadIdx.x % TPR;
@@ -22,75 +22,73 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void int8_rows_kernel(const 
   p.second = a.second ? a.second + row * a.second_stride : nullptr;
   p.sum = a.sum ? a.sum + row * a.sum_stride : nullptr;
   p.codes = a.codes + row * a.code_stride;
-  quantize_row<DT, MODE, TPR, CH>(a, p, a.scales + row, tl, vec, code_vec, red);
+  quantize_row<DT, MODE, TPR, CH>(a, p, a.scales + row, tl, red);
 }
 
 template <int DT, int MODE>
-void launch_rows(const Int8RowsArgs& a, int vec, int code_vec, hipStream_t s) {
+void launch_rows(const Int8RowsArgs& a, hipStream_t s) {
   const int width = a.code_columns > a.columns ? a.code_columns : a.columns;
   const auto go = [&](auto kernel, int threads, int rows_per_block) {
-    hipLaunchKernelGGL(kernel, dim3(unsigned(a.rows + rows_per_block - 1) / rows_per_block), dim3(threads), 0, s, a, vec,
-                       code_vec);
+    hipLaunchKernelGGL(kernel, dim3(unsigned(a.rows + rows_per_block - 1) / rows_per_block), dim3(threads), 0, s, a);
   };
   if (width <= 512) go(int8_rows_kernel<DT, MODE, 64, 1>, 256, 4);
   else if (width <= 1024) go(int8_rows_kernel<DT, MODE, 64, 2>, 256, 4);
   else if (width <= 2048) go(int8_rows_kernel<DT, MODE, 256, 1>, 256, 1);
-  else if (width <= 4096) go(int8_rows_kernel<DT, MODE, 256, 2>, 256, 1);
-  else if (width <= 8192) go(int8_rows_kernel<DT, MODE, 512, 2>, 512, 1);
+  else if (width <= 4096) {
+    if (a.rows <= 256) go(int8_rows_kernel<DT, MODE, 512, 1>, 512, 1);
+    else go(int8_rows_kernel<DT, MODE, 256, 2>, 256, 1);
+  }
+  else if (width <= 8192) {
+    if (a.rows <= 256) go(int8_rows_kernel<DT, MODE, 1024, 1>, 1024, 1);
+    else go(int8_rows_kernel<DT, MODE, 512, 2>, 512, 1);
+  }
+  else if (width <= 12288 && a.rows > 256) go(int8_rows_kernel<DT, MODE, 512, 3>, 512, 1);
   else if (width <= 16384) go(int8_rows_kernel<DT, MODE, 1024, 2>, 1024, 1);
   else go(int8_rows_kernel<DT, MODE, 1024, 0>, 1024, 1);
 }
 
-// 16 codes a thread.
+// 16 codes a thread, at whatever address (int8_row.h).
 template <int DT>
-__global__ __launch_bounds__(256) void int8_restore_kernel(const Int8RestoreArgs a, int pieces, int vec) {
+__global__ __launch_bounds__(256) void int8_restore_kernel(const Int8RestoreArgs a, int pieces) {
   const long long unit = (long long)(blockIdx.x) * 256 + threadIdx.x;
   const long long row = unit / pieces;
   if (row >= a.rows) return;
   const int first = int(unit - row * pieces) * 16, n = a.columns - first;
   const int8_t* src = a.codes + row * a.code_stride + first;
   const float scale = a.scales[row];
-  if (vec && n >= 16) {
-    const u32x4_t c = *reinterpret_cast<const u32x4_t*>(src);
+  constexpr int kSize = DT == kF32 ? 4 : 2;
+  char* out = static_cast<char*>(a.out) + (row * a.out_stride + first) * kSize;
+  if (n >= 16) {
+    unsigned c[4];
+    __builtin_memcpy(c, src, 16);
     float v[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = float(int(c[e >> 2] << (24 - 8 * (e & 3))) >> 24) * scale;
     if constexpr (DT == kF32) {
-      float* out = static_cast<float*>(a.out) + row * a.out_stride + first;
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(out + e) = float4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+      __builtin_memcpy(out, v, 64);
     } else {
-      uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.out_stride + first;
+      unsigned o[8];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u32x4_t o;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) o[w] = round_pair_bits<DT>(v[8 * h + 2 * w], v[8 * h + 2 * w + 1]);
-        *reinterpret_cast<u32x4_t*>(out + 8 * h) = o;
-      }
+      for (int w = 0; w < 8; ++w) o[w] = round_pair_bits<DT>(v[2 * w], v[2 * w + 1]);
+      __builtin_memcpy(out, o, 32);
     }
     return;
   }
-  for (int e = 0; e < 16 && e < n; ++e) {
+  for (int e = 0; e < n; ++e) {
     const float v = float(src[e]) * scale;
-    if constexpr (DT == kF32) static_cast<float*>(a.out)[row * a.out_stride + first + e] = v;
-    else static_cast<uint16_t*>(a.out)[row * a.out_stride + first + e] = from_f32<DT>(v);
+    if constexpr (DT == kF32) reinterpret_cast<float*>(out)[e] = v;
+    else reinterpret_cast<uint16_t*>(out)[e] = from_f32<DT>(v);
   }
 }
-
-bool at16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
 
 bool launch_int8_rows(int dt, int mode, const Int8RowsArgs& a, hipStream_t s) {
-  const int vec = at16(a.x) && a.x_stride % 8 == 0 && (!a.second || (at16(a.second) && a.second_stride % 8 == 0)) &&
-                  (!a.weight || at16(a.weight)) && (!a.sum || (at16(a.sum) && a.sum_stride % 8 == 0));
-  const int code_vec = reinterpret_cast<uintptr_t>(a.codes) % 8 == 0 && a.code_stride % 8 == 0;
   const auto pick = [&](auto type) {
     constexpr int DT = decltype(type)::value;
-    if (mode == kRowsPlain) launch_rows<DT, kRowsPlain>(a, vec, code_vec, s);
-    else if (mode == kRowsNorm) launch_rows<DT, kRowsNorm>(a, vec, code_vec, s);
-    else launch_rows<DT, kRowsSwiglu>(a, vec, code_vec, s);
+    if (mode == kRowsPlain) launch_rows<DT, kRowsPlain>(a, s);
+    else if (mode == kRowsNorm) launch_rows<DT, kRowsNorm>(a, s);
+    else launch_rows<DT, kRowsSwiglu>(a, s);
   };
   if (dt == kBF16) pick(std::integral_constant<int, kBF16>{});
   else if (dt == kF16) pick(std::integral_constant<int, kF16>{});
@@ -99,12 +97,11 @@ bool launch_int8_rows(int dt, int mode, const Int8RowsArgs& a, hipStream_t s) {
 }
 
 bool launch_int8_restore(int dt, const Int8RestoreArgs& a, hipStream_t s) {
-  const int pieces = (a.columns + 15) / 16, width = dt == kF32 ? 4 : 2;
-  const int vec = at16(a.codes) && a.code_stride % 16 == 0 && at16(a.out) && a.out_stride * width % 16 == 0;
+  const int pieces = (a.columns + 15) / 16;
   const dim3 grid(unsigned(((long long)(a.rows) * pieces + 255) / 256));
-  if (dt == kBF16) hipLaunchKernelGGL(int8_restore_kernel<kBF16>, grid, dim3(256), 0, s, a, pieces, vec);
-  else if (dt == kF16) hipLaunchKernelGGL(int8_restore_kernel<kF16>, grid, dim3(256), 0, s, a, pieces, vec);
-  else if (dt == kF32) hipLaunchKernelGGL(int8_restore_kernel<kF32>, grid, dim3(256), 0, s, a, pieces, vec);
+  if (dt == kBF16) hipLaunchKernelGGL(int8_restore_kernel<kBF16>, grid, dim3(256), 0, s, a, pieces);
+  else if (dt == kF16) hipLaunchKernelGGL(int8_restore_kernel<kF16>, grid, dim3(256), 0, s, a, pieces);
+  else if (dt == kF32) hipLaunchKernelGGL(int8_restore_kernel<kF32>, grid, dim3(256), 0, s, a, pieces);
   else return false;
   return true;
 }

@@ -21,9 +21,10 @@ import torch
 
 from .acceleration_checks import numerical_gate, stepwise_nrmse
 from .deployment import PackedHybridLinear
+from .int8_linear import PackedInt8Linear
 from .w3_lut_deployment import PackedW3Linear
 
-PACKED_TYPES = (PackedHybridLinear, PackedW3Linear)
+PACKED_TYPES = (PackedHybridLinear, PackedW3Linear, PackedInt8Linear)
 
 
 def packed_modules(model) -> dict:

@@ -13,6 +13,7 @@ from marlin_style_fluxbin_amd import PackedInt8Linear, native_decode
 from marlin_style_fluxbin_amd.full_model_trial import compare_trace
 from marlin_style_fluxbin_amd.native_decode import NativeDecodeSession
 from marlin_style_fluxbin_amd.qwen3 import int8_quantize_qwen3_model, qwen3_config, random_qwen3_model
+from marlin_style_fluxbin_amd.static_decode import StaticDecodeSession, prepared_linears
 from tests.int8_reference import held, norm_rows, product, swiglu_rows
 
 pytestmark = pytest.mark.gpu
@@ -138,3 +139,17 @@ def test_prefill_is_the_quantized_models(gpu):
     # a row of normal values has its largest near 3 to 4 and a step of 1/36 and less: 0.8% of the
     # row's norm (step / sqrt(12)) for each of the 12 inputs in turn, 5% with all against each other
     assert float((got - want).norm() / want.norm()) <= 0.05
+
+
+def test_module_tree_session_with_bound_linears(gpu):
+    """The HF module tree's own session, its Linears bound: the same as unbound, and in a graph."""
+    model, ids, forced = setup(gpu)
+    int8_quantize_qwen3_model(model)
+    session = StaticDecodeSession(model, ids, forced)
+    want = session.audit()
+    with prepared_linears(model, torch.bfloat16) as modules:
+        assert len(modules) == 21
+        got = session.audit()
+        assert torch.equal(got["logits"], want["logits"])
+        assert torch.equal(session.capture()["logits"], want["logits"])
+    assert all(m._decode_binding is None for m in modules.values())
