@@ -35,9 +35,8 @@ constexpr int kMaxSplits = 16;
 }  // namespace
 
 // Which kernel, and how many workgroups along K, by an estimate of the time (us): rounds of
-// workgroups, each its stages of 128 columns at what a stage takes (with the chip's other places of
-// the same compute unit empty, and full), or the bytes; and for splits the join's launch and the
-// partial sums written and read.
+// workgroups, each its stages of 128 columns at what a stage takes, and the operands' bytes, of which
+// the shorter hides but in part; for splits the join's launch and the partial sums written and read.
 Int8GemmPlan plan_int8_gemm(int M, int N, int K) {
   const int stages = (K + 127) / 128;
   const float bytes = (float(M) + N) * K / 4.8e6f;
@@ -45,15 +44,16 @@ Int8GemmPlan plan_int8_gemm(int M, int N, int K) {
   float least = M <= kFewRows ? 3.f + float(N) * K / 4.9e6f * (M <= 16 ? 1.f + 0.016f * M : 1.45f) : 1e30f;
   for (int tile = 0; tile < kInt8Tiles; ++tile) {
     const Int8Tile& t = kInt8Tile[tile];
-    const long tiles = long((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+    const long tiles = long((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn), slots = 256 * t.places;
     for (int splits = 1; splits <= std::min(stages, kMaxSplits); ++splits) {
-      if (splits > 1 && tiles * (splits - 1) >= 256 * t.places) break;  // the chip was full
+      if (splits > 1 && tiles * (splits - 1) >= slots) break;  // the chip was full
       const int per = (stages + splits - 1) / splits;
       if ((stages + per - 1) / per != splits) continue;  // a last split would be empty
-      const long groups = tiles * splits, slots = 256 * t.places, rounds = (groups + slots - 1) / slots;
-      const float last = float(groups - (rounds - 1) * slots) / 256.f;  // workgroups of a unit in the last round
-      const float stage = (rounds - 1) * t.full + (last <= 1.f ? t.alone : t.alone + (t.full - t.alone) * (last - 1.f));
-      float time = 3.f + std::max(per * stage + rounds * t.ends, bytes);
+      const long groups = tiles * splits, rounds = (groups + slots - 1) / slots;
+      const float filled = std::max(2.f * float(groups - (rounds - 1) * slots) / float(slots) - 1.f, 0.f);
+      const float stage = (rounds - 1) * t.full + t.half + (t.full - t.half) * filled;
+      const float work = per * stage + rounds * t.ends;
+      float time = 3.f + std::max(work, bytes) + 0.3f * std::min(work, bytes);
       if (splits > 1) time += 3.5f + 2.f * splits * float(M) * N * 4.f / 5e6f;
       if (time < least) least = time, best = {tile, splits, splits == 1 ? K : per * 128};
     }

@@ -6,21 +6,24 @@ namespace fx {
 
 void launch_int8_tile_64(const Int8GemmArgs& g, unsigned groups, hipStream_t s);
 void launch_int8_tile_128(const Int8GemmArgs& g, unsigned groups, hipStream_t s);
-void launch_int8_tile_128_deep(const Int8GemmArgs& g, unsigned groups, hipStream_t s);
+void launch_int8_tile_128x256(const Int8GemmArgs& g, unsigned groups, hipStream_t s);
 void launch_int8_tile_256(const Int8GemmArgs& g, unsigned groups, hipStream_t s);
 
-// Times in us, fits (plan_int8_gemm): a stage of 128 columns with one workgroup on its compute unit,
-// with `places` of them; a workgroup's first loads and its results.
+// `places`: workgroups that share a compute unit.  Times in us, fits (plan_int8_gemm): a stage of 128
+// columns with half the chip's places taken and with all of them; a workgroup's first loads and its
+// results.
 struct Int8Tile {
   int bm, bn, places;
-  float alone, full, ends;
+  float half, full, ends;
   void (*launch)(const Int8GemmArgs& g, unsigned groups, hipStream_t s);
 };
+// (of 2048 x 4096 x 4096 the four take 63, 43.7, 37.6 and 45.5 us; of 1024 x 4096 x 4096 34, 22.6, 32 and 44;
+// 128 x 128 tiles with two stages, two workgroups a compute unit: 39.4 and 25.7)
 constexpr Int8Tile kInt8Tile[] = {
-    {64, 64, 2, 0.27f, 0.45f, 1.5f, launch_int8_tile_64},
-    {128, 128, 2, 0.75f, 1.15f, 3.f, launch_int8_tile_128},
-    {128, 128, 1, 0.58f, 0.58f, 3.f, launch_int8_tile_128_deep},
-    {256, 256, 1, 1.55f, 1.55f, 8.f, launch_int8_tile_256},
+    {64, 64, 2, 0.28f, 0.43f, 1.5f, launch_int8_tile_64},
+    {128, 128, 1, 0.48f, 0.58f, 3.f, launch_int8_tile_128},
+    {128, 256, 1, 0.8f, 1.f, 5.f, launch_int8_tile_128x256},
+    {256, 256, 1, 1.2f, 1.6f, 8.f, launch_int8_tile_256},
 };
 constexpr int kInt8Tiles = sizeof(kInt8Tile) / sizeof(kInt8Tile[0]);
 constexpr int kInt8Few = -1;  // int8_gemm_few.h

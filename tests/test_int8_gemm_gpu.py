@@ -42,7 +42,7 @@ def test_products(gpu, m):
 
 @pytest.mark.parametrize("m,n,k", [(1, 6144, 4096), (1, 4096, 12288), (5, 24576, 4096), (24, 4096, 12288), (64, 512, 16384),
                                    (96, 300, 8192), (700, 1000, 5120), (1024, 2048, 4096), (2000, 4096, 1024),
-                                   (4100, 1280, 256), (33, 12288, 512), (3, 64, 131056), (130, 64, 131056)])
+                                   (4100, 1280, 256), (33, 12288, 512), (4000, 4100, 272), (2000, 4090, 528), (1000, 4001, 1040), (3, 64, 131056), (130, 64, 131056)])
 def test_larger_products(gpu, m, n, k):
     args, b = case(m, n, k, gpu, torch.bfloat16, True, seed=7)
     assert_product(int8_matmul(*args, bias=b), *args, b, context=(m, n, k))
