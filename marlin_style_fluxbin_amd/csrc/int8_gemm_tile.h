@@ -90,8 +90,12 @@ __device__ __forceinline__ void tile_store_as(const Int8GemmArgs& g, const i32x1
       for (int p = 0; p < 32 / kPass; ++p) {
         const int row = p * kPass + lane / kLanes, place = (lane % kLanes) * 16;
         const u32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(lds + row * kRow + place);
-        if (m + row < g.M)
-          *reinterpret_cast<u32x4_t*>(out + ((m + row) * stride + n0) * kSize + place) = v;
+        if (m + row < g.M) {
+          u32x4_t* to = reinterpret_cast<u32x4_t*>(out + ((m + row) * stride + n0) * kSize + place);
+          // (a result is not read again here: 8192 x 12288 x 4096 356 us, with plain stores 371)
+          if constexpr (OUT >= 0) __builtin_nontemporal_store(v, to);
+          else *to = v;
+        }
       }
     } else {
       for (int u = lane; u < 32 * NT * 32; u += 64) {
@@ -120,8 +124,8 @@ template <int BM, int BN, int WM, int WN, int BK, int S>
 __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8GemmArgs g) {
   constexpr int kWaves = WM * WN, TM = BM / WM, TN = BN / WN, MT = TM / 32, NT = TN / 32;
   constexpr int kStage = (BM + BN) * BK, kRows = 1024 / BK, kPlaces = BK / 16, kSteps = BK / 32;
-  constexpr int P = (BM + BN) / kRows / kWaves;  // wave loads of kRows rows a stage
-  static_assert((BM + BN) / kRows % kWaves == 0 && S >= 2, "waves share a stage's loads evenly");
+  constexpr int PW = BN / kRows / kWaves, PA = BM / kRows / kWaves, P = PW + PA;  // wave loads of kRows rows a stage
+  static_assert(BN % (2 * kRows * kWaves) == 0 && BM % (2 * kRows * kWaves) == 0 && S >= 2, "waves share a stage's loads evenly");
   constexpr int kResults = kWaves * tile_store_bytes(NT);
   __shared__ __attribute__((aligned(1024))) char ring[S * kStage > kResults ? S * kStage : kResults];
   const int lane = threadIdx.x & 63, wave = wave_index();
@@ -143,37 +147,46 @@ __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8G
   // fills place l % kPlaces: c is that place with swizzle(row) applied, so that 16 lanes that read one c
   // of 16 rows in a row meet 16 places of 16 bytes within 256 bytes (64 banks).
   const auto swizzle = [](int row) { return BK == 64 ? (row >> 2) & 3 : (row >> 1) & 7; };
-  int chunk[2];
+  int chunk[2], w_off[PW], a_off[PA];
 #pragma unroll
   for (int i = 0; i < 2; ++i) chunk[i] = ((lane % kPlaces) ^ swizzle(i * kRows + lane / kPlaces)) * 16;
-  size_t base[P];
-  int records[P], offset[P];
+  const int w_stride = int(g.w_stride), a_stride = int(g.a_stride);
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const int piece = wave * P + i;
-    const bool is_w = piece < BN / kRows;
-    const int row = is_w ? n0 + piece * kRows : m0 + (piece - BN / kRows) * kRows;
-    const int left = min(kRows, (is_w ? g.N : g.M) - row);
-    const long long stride = is_w ? g.w_stride : g.a_stride;
-    base[i] = reinterpret_cast<size_t>(is_w ? g.w : g.a) + row * stride + k_begin;
-    records[i] = left > 0 ? (left - 1) * int(stride) + k_end - k_begin : 0;
-    offset[i] = (lane / kPlaces) * int(stride) + chunk[piece & 1];
-  }
+  for (int i = 0; i < PW; ++i) w_off[i] = (i * kRows + lane / kPlaces) * w_stride + chunk[i & 1];
+#pragma unroll
+  for (int i = 0; i < PA; ++i) a_off[i] = (i * kRows + lane / kPlaces) * a_stride + chunk[i & 1];
+  const int w_row = n0 + wave * (PW * kRows), a_row = m0 + wave * (PA * kRows);
+  const int w_left = min(PW * kRows, g.N - w_row), a_left = min(PA * kRows, g.M - a_row);
+  const size_t w_base = reinterpret_cast<size_t>(g.w) + w_row * g.w_stride + k_begin;
+  const size_t a_base = reinterpret_cast<size_t>(g.a) + a_row * g.a_stride + k_begin;
+  const int columns = k_end - k_begin;
+  const int w_bytes = w_left > 0 ? (w_left - 1) * w_stride + columns : 0;
+  const int a_bytes = a_left > 0 ? (a_left - 1) * a_stride + columns : 0;
   // The XCDs begin at different columns: they read the same rows at different times, and rows of a
   // power of two apart meet more of the memory's channels at any one.
-  int issued = 0, next = int(blockIdx.x % kXcdCount) * stages / kXcdCount;  // stages
+  int issued = 0, next = int(blockIdx.x % kXcdCount) * stages / kXcdCount, slot = 0;  // stages
   auto issue = [&]() __attribute__((always_inline)) {
-    const int k = next * BK, left = issued < stages ? k_end - k_begin - k : 0;
-    const unsigned dst = lds0 + unsigned(issued % S) * kStage + wave * (P * 1024);
-    next = next + 1 == stages ? 0 : next + 1;
+    const int k = next * BK, left = issued < stages ? columns - k : 0;
+    const unsigned w_dst = lds0 + unsigned(slot) * kStage + wave * (PW * 1024);
+    const unsigned a_dst = lds0 + unsigned(slot) * kStage + BN * BK + wave * (PA * 1024);
+    const size_t wp = w_base + k, ap = a_base + k;
+    // (past the last stage, and for rows past the last: no access, zeros)
+    const u32x4_t rw = {unsigned(wp), unsigned(wp >> 32) & 0xffffu, left > 0 ? unsigned(max(w_bytes - k, 0)) : 0u, 0x00020000u};
+    const u32x4_t ra = {unsigned(ap), unsigned(ap >> 32) & 0xffffu, left > 0 ? unsigned(max(a_bytes - k, 0)) : 0u, 0x00020000u};
+    if (left >= BK || left <= 0) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const size_t at = base[i] + k;
-      const u32x4_t r = {unsigned(at), unsigned(at >> 32) & 0xffffu, left > 0 ? unsigned(max(records[i] - k, 0)) : 0u,
-                         0x00020000u};
-      fill_lds(r, chunk[(wave * P + i) & 1] < left ? offset[i] : kOutOfRange, dst + i * 1024);
+      for (int i = 0; i < PW; ++i) fill_lds(rw, w_off[i], w_dst + i * 1024);
+#pragma unroll
+      for (int i = 0; i < PA; ++i) fill_lds(ra, a_off[i], a_dst + i * 1024);
+    } else {  // the last columns, not a whole stage of them
+#pragma unroll
+      for (int i = 0; i < PW; ++i) fill_lds(rw, chunk[i & 1] < left ? w_off[i] : kOutOfRange, w_dst + i * 1024);
+#pragma unroll
+      for (int i = 0; i < PA; ++i) fill_lds(ra, chunk[i & 1] < left ? a_off[i] : kOutOfRange, a_dst + i * 1024);
     }
     ++issued;
+    next = next + 1 == stages ? 0 : next + 1;
+    slot = slot + 1 == S ? 0 : slot + 1;
   };
 
   const int wm = wave / WN, wn = wave % WN;
@@ -195,12 +208,15 @@ __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8G
     for (int i = 0; i < NT; ++i) w[h][i] = *reinterpret_cast<const u32x4_t*>(w_at + at + i * 32 * BK);
 #pragma unroll
     for (int j = 0; j < MT; ++j) a[h][j] = *reinterpret_cast<const u32x4_t*>(a_at + at + j * 32 * BK);
+    // (the compiler otherwise reads a step's operands just in front of its products)
+    __builtin_amdgcn_sched_barrier(0);
   };
   auto multiply = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int j = 0; j < MT; ++j) acc[i][j] = mfma_i8_32(w[h][i], a[h][j], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
   };
 
 #pragma unroll
