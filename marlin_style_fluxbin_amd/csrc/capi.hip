@@ -2161,7 +2161,6 @@ int prepare_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales
   g.K = K;
   g.dt = dtype;
   g.k_per_split = plan.k_per_split;
-  g.vec = aligned16(out) && out_stride * size % 16 == 0;
   return FX_OK;
 }
 

@@ -43,24 +43,21 @@ __device__ __forceinline__ void store4_as(const Int8GemmArgs& g, int m, int n, c
 #pragma unroll
   for (int r = 0; r < 4; ++r) y[r] = fmaf(float(acc[r]) * sa, ws[r], bias[r]);
   const long long at = m * g.out_stride + n;
-  const bool whole = g.vec && n + 4 <= g.N;
   if constexpr (DT == kF32) {
     float* out = static_cast<float*>(g.out) + at;
-    if (whole) *reinterpret_cast<float4*>(out) = float4{y[0], y[1], y[2], y[3]};
+    if (n + 4 <= g.N) __builtin_memcpy(out, y, 16);
     else
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 3; ++r)
         if (n + r < g.N) out[r] = y[r];
   } else {
     uint16_t* out = static_cast<uint16_t*>(g.out) + at;
-    if (whole) {
-      uint2 v;
-      v.x = round_pair_bits<DT>(y[0], y[1]);
-      v.y = round_pair_bits<DT>(y[2], y[3]);
-      *reinterpret_cast<uint2*>(out) = v;
+    if (n + 4 <= g.N) {
+      const unsigned v[2] = {round_pair_bits<DT>(y[0], y[1]), round_pair_bits<DT>(y[2], y[3])};
+      __builtin_memcpy(out, v, 8);
     } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 3; ++r)
         if (n + r < g.N) out[r] = from_f32<DT>(y[r]);
     }
   }
@@ -69,15 +66,6 @@ __device__ __forceinline__ void store4(const Int8GemmArgs& g, int m, int n, cons
   if (g.dt == kBF16) store4_as<kBF16>(g, m, n, acc, sa);
   else if (g.dt == kF16) store4_as<kF16>(g, m, n, acc, sa);
   else store4_as<kF32>(g, m, n, acc, sa);
-}
-
-// The same columns of one K split's sums, [splits, M, N].
-__device__ __forceinline__ void store4_partial(const Int8GemmArgs& g, int split, int m, int n, const i32x4_t& acc) {
-  int* out = g.partial + (size_t(split) * g.M + m) * g.N + n;
-  if (g.N % 4 == 0) *reinterpret_cast<i32x4_t*>(out) = acc;
-  else
-    for (int r = 0; r < 4; ++r)
-      if (n + r < g.N) out[r] = acc[r];
 }
 
 }  // namespace fx

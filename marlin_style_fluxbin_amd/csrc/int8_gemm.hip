@@ -18,8 +18,12 @@ __global__ __launch_bounds__(256) void int8_gemm_join_kernel(const Int8GemmArgs 
   const size_t plane = size_t(g.M) * g.N;
   const int* p = g.partial + size_t(m) * g.N + n;
   i32x4_t total = {0, 0, 0, 0};
-  if (g.N % 4 == 0) {
-    for (int s = 0; s < splits; ++s) total += *reinterpret_cast<const i32x4_t*>(p + s * plane);
+  if (n + 4 <= g.N) {
+    for (int s = 0; s < splits; ++s) {
+      i32x4_t v;
+      __builtin_memcpy(&v, p + s * plane, 16);
+      total += v;
+    }
   } else {
     for (int s = 0; s < splits; ++s)
 #pragma unroll

@@ -1,5 +1,5 @@
 // Products of 8-bit rows, BM rows of the activations by BN of the weight a workgroup: both in LDS in
-// a ring of S stages of 64 columns, filled from memory without passing through registers.
+// a ring of S stages of 128 columns, filled from memory without passing through registers.
 #pragma once
 #include "int8_gemm.h"
 
@@ -8,6 +8,7 @@ namespace fx {
 typedef int i32x16_t __attribute__((ext_vector_type(16)));
 typedef unsigned u32x2v_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) char lds8_t;
+typedef unsigned any16_t __attribute__((ext_vector_type(4), aligned(2)));
 
 // D[i, j] += sum_k A[i, k] B[j, k] over 32 bytes of k: lane l gives bytes 16 (l / 32) .. of row
 // l % 32 of both and holds D[8 (r / 4) + 4 (l / 32) + r % 4, l % 32], r < 16.
@@ -50,7 +51,6 @@ __device__ __forceinline__ void tile_store_as(const Int8GemmArgs& g, const i32x1
   const int half = lane >> 5, low = lane & 31;
   char* out = OUT < 0 ? reinterpret_cast<char*>(g.partial + size_t(split) * g.M * g.N) : static_cast<char*>(g.out);
   const long long stride = OUT < 0 ? g.N : g.out_stride;
-  const bool vec = OUT < 0 ? g.N % 4 == 0 : g.vec;
   f32x4v_t ws[NT * 4], bias[NT * 4];
   if constexpr (OUT >= 0) {
 #pragma unroll
@@ -85,26 +85,24 @@ __device__ __forceinline__ void tile_store_as(const Int8GemmArgs& g, const i32x1
       }
     }
     wave_lds_order();
-    if (vec && n0 + NT * 32 <= g.N) {
 #pragma unroll
-      for (int p = 0; p < 32 / kPass; ++p) {
-        const int row = p * kPass + lane / kLanes, place = (lane % kLanes) * 16;
-        const u32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(lds + row * kRow + place);
-        if (m + row < g.M) {
-          u32x4_t* to = reinterpret_cast<u32x4_t*>(out + ((m + row) * stride + n0) * kSize + place);
-          // (a result is not read again here: 8192 x 12288 x 4096 356 us, with plain stores 371)
-          if constexpr (OUT >= 0) __builtin_nontemporal_store(v, to);
-          else *to = v;
-        }
-      }
-    } else {
-      for (int u = lane; u < 32 * NT * 32; u += 64) {
-        const int row = u / (NT * 32), col = u % (NT * 32);
-        if (m + row < g.M && n0 + col < g.N) {
-          const lds8_t* at = lds + row * kRow + col * kSize;
-          char* to = out + ((m + row) * stride + n0 + col) * kSize;
-          if constexpr (kSize == 2) *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const __attribute__((address_space(3))) uint16_t*>(at);
-          else *reinterpret_cast<unsigned*>(to) = *reinterpret_cast<const __attribute__((address_space(3))) unsigned*>(at);
+    for (int p = 0; p < 32 / kPass; ++p) {
+      constexpr int kEach = 16 / kSize;
+      const int row = p * kPass + lane / kLanes, col = lane % kLanes * kEach, left = g.N - n0 - col;
+      if (m + row >= g.M || left <= 0) continue;
+      const u32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(lds + row * kRow + col * kSize);
+      char* to = out + ((m + row) * stride + n0 + col) * kSize;
+      if (left >= kEach) {
+        // at whatever address the row begins (301 x 1001 x 2000 8.2 us, element by element 10.6); a result is
+        // not read again here (8192 x 12288 x 4096 356 us, with plain stores 371)
+        if constexpr (OUT < 0) __builtin_memcpy(to, &v, 16);
+        else __builtin_nontemporal_store(v, reinterpret_cast<any16_t*>(to));
+      } else {
+#pragma unroll
+        for (int e = 0; e < kEach - 1; ++e) {
+          if (e >= left) break;
+          if constexpr (kSize == 2) reinterpret_cast<uint16_t*>(to)[e] = uint16_t(v[e >> 1] >> (16 * (e & 1)));
+          else reinterpret_cast<unsigned*>(to)[e] = v[e];
         }
       }
     }
@@ -120,10 +118,14 @@ __device__ __forceinline__ void tile_store(const Int8GemmArgs& g, const i32x16_t
 }
 constexpr int tile_store_bytes(int NT) { return 32 * (NT * 32 * 4 + 16); }  // of LDS, a wave
 
-template <int BM, int BN, int WM, int WN, int BK, int S>
+// A stage's rows are whole 128-byte lines: pieces of 64 bytes cost the L2 twice the requests (256 x 256
+// tiles of 4096 x 4096 x 16384 with as many bytes in flight 243 us, 228 with 128).
+constexpr int kTileK = 128;
+
+template <int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8GemmArgs g) {
   constexpr int kWaves = WM * WN, TM = BM / WM, TN = BN / WN, MT = TM / 32, NT = TN / 32;
-  constexpr int kStage = (BM + BN) * BK, kRows = 1024 / BK, kPlaces = BK / 16, kSteps = BK / 32;
+  constexpr int kStage = (BM + BN) * kTileK, kRows = 1024 / kTileK, kPlaces = kTileK / 16, kSteps = kTileK / 32;
   constexpr int PW = BN / kRows / kWaves, PA = BM / kRows / kWaves, P = PW + PA;  // wave loads of kRows rows a stage
   static_assert(BN % (2 * kRows * kWaves) == 0 && BM % (2 * kRows * kWaves) == 0 && S >= 2, "waves share a stage's loads evenly");
   constexpr int kResults = kWaves * tile_store_bytes(NT);
@@ -141,12 +143,12 @@ __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8G
   const int tn = in_group / high, tm = first + in_group - tn * high;
   const int m0 = tm * BM, n0 = tn * BN;
   const int k_begin = split * g.k_per_split, k_end = min(g.K, k_begin + g.k_per_split);
-  const int stages = (k_end - k_begin + BK - 1) / BK;
+  const int stages = (k_end - k_begin + kTileK - 1) / kTileK;
 
-  // This wave's loads: kRows rows of BK bytes each, lane l bytes 16 c .. of row l / kPlaces, where it
+  // This wave's loads: kRows rows of kTileK bytes each, lane l bytes 16 c .. of row l / kPlaces, where it
   // fills place l % kPlaces: c is that place with swizzle(row) applied, so that 16 lanes that read one c
   // of 16 rows in a row meet 16 places of 16 bytes within 256 bytes (64 banks).
-  const auto swizzle = [](int row) { return BK == 64 ? (row >> 2) & 3 : (row >> 1) & 7; };
+  const auto swizzle = [](int row) { return (row >> 1) & 7; };
   int chunk[2], w_off[PW], a_off[PA];
 #pragma unroll
   for (int i = 0; i < 2; ++i) chunk[i] = ((lane % kPlaces) ^ swizzle(i * kRows + lane / kPlaces)) * 16;
@@ -166,14 +168,14 @@ __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8G
   // power of two apart meet more of the memory's channels at any one.
   int issued = 0, next = int(blockIdx.x % kXcdCount) * stages / kXcdCount, slot = 0;  // stages
   auto issue = [&]() __attribute__((always_inline)) {
-    const int k = next * BK, left = issued < stages ? columns - k : 0;
+    const int k = next * kTileK, left = issued < stages ? columns - k : 0;
     const unsigned w_dst = lds0 + unsigned(slot) * kStage + wave * (PW * 1024);
-    const unsigned a_dst = lds0 + unsigned(slot) * kStage + BN * BK + wave * (PA * 1024);
+    const unsigned a_dst = lds0 + unsigned(slot) * kStage + BN * kTileK + wave * (PA * 1024);
     const size_t wp = w_base + k, ap = a_base + k;
     // (past the last stage, and for rows past the last: no access, zeros)
     const u32x4_t rw = {unsigned(wp), unsigned(wp >> 32) & 0xffffu, left > 0 ? unsigned(max(w_bytes - k, 0)) : 0u, 0x00020000u};
     const u32x4_t ra = {unsigned(ap), unsigned(ap >> 32) & 0xffffu, left > 0 ? unsigned(max(a_bytes - k, 0)) : 0u, 0x00020000u};
-    if (left >= BK || left <= 0) {
+    if (left >= kTileK || left <= 0) {
 #pragma unroll
       for (int i = 0; i < PW; ++i) fill_lds(rw, w_off[i], w_dst + i * 1024);
 #pragma unroll
@@ -190,8 +192,8 @@ __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8G
   };
 
   const int wm = wave / WN, wn = wave % WN;
-  const char* w_at = ring + (wn * TN + (lane & 31)) * BK;
-  const char* a_at = ring + (BN + wm * TM + (lane & 31)) * BK;
+  const char* w_at = ring + (wn * TN + (lane & 31)) * kTileK;
+  const char* a_at = ring + (BN + wm * TM + (lane & 31)) * kTileK;
   const int place = ((lane >> 5) ^ swizzle(lane & 31)) * 16;
 
   i32x16_t acc[NT][MT];
@@ -205,9 +207,9 @@ __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8G
   auto read = [&](int h, int step, int stage) __attribute__((always_inline)) {
     const int at = stage * kStage + (place ^ (step * 32));
 #pragma unroll
-    for (int i = 0; i < NT; ++i) w[h][i] = *reinterpret_cast<const u32x4_t*>(w_at + at + i * 32 * BK);
+    for (int i = 0; i < NT; ++i) w[h][i] = *reinterpret_cast<const u32x4_t*>(w_at + at + i * 32 * kTileK);
 #pragma unroll
-    for (int j = 0; j < MT; ++j) a[h][j] = *reinterpret_cast<const u32x4_t*>(a_at + at + j * 32 * BK);
+    for (int j = 0; j < MT; ++j) a[h][j] = *reinterpret_cast<const u32x4_t*>(a_at + at + j * 32 * kTileK);
     // (the compiler otherwise reads a step's operands just in front of its products)
     __builtin_amdgcn_sched_barrier(0);
   };

@@ -3,6 +3,6 @@
 
 namespace fx {
 void launch_int8_tile_64(const Int8GemmArgs& g, unsigned groups, hipStream_t s) {
-  hipLaunchKernelGGL((int8_gemm_tile_kernel<64, 64, 2, 2, 128, 4>), dim3(groups), dim3(256), 0, s, g);
+  hipLaunchKernelGGL((int8_gemm_tile_kernel<64, 64, 2, 2, 4>), dim3(groups), dim3(256), 0, s, g);
 }
 }  // namespace fx

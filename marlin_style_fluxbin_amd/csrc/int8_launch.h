@@ -43,7 +43,6 @@ struct Int8GemmArgs {
   int M, N, K;
   int dt;            // of out and bias
   int k_per_split;   // a multiple of the kernel's K step
-  int vec;           // out's rows lie at 16-byte boundaries
 };
 constexpr long long kInt8RowLimit = 1LL << 22;  // bytes between rows: 256 rows stay within 31 bits
 constexpr int kInt8MaxK = 131071;               // 2^14 * 131071 < 2^31: the sums are exact
