@@ -2125,8 +2125,8 @@ namespace {
 // The checks of a product, its arguments and its plan.
 int prepare_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales, const int8_t* w, long long w_stride,
                       const float* w_scales, const void* bias, void* out, long long out_stride, void* workspace,
-                      size_t workspace_bytes, int M, int N, int K, int dtype, fx::Int8GemmArgs* args,
-                      fx::Int8GemmPlan* planned) {
+                      size_t workspace_bytes, int M, int N, int K, int dtype, const fx::Int8GemmPlan& plan,
+                      fx::Int8GemmArgs* args) {
   if (!is_half_dtype(dtype) && dtype != FX_F32) return fail(FX_EINVAL, "dtype must be fp32, fp16 or bf16");
   if (int rc = validate_code_rows("a", a, a_stride, M, K)) return rc;
   if (int rc = validate_code_rows("w", w, w_stride, N, K)) return rc;
@@ -2136,14 +2136,12 @@ int prepare_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales
     return fail(FX_EINVAL, "scales, bias and out must be aligned to their elements");
   if (out_stride < 0 || (out_stride < N && M > 1))
     return fail(FX_EINVAL, "out stride %lld is shorter than a row of %d", out_stride, N);
-  const fx::Int8GemmPlan plan = fx::plan_int8_gemm(M, N, K);
   const size_t need = int8_gemm_workspace(plan, M, N);
   if (need) {
     if (!workspace || workspace_bytes < need)
       return fail(FX_EINVAL, "gemm workspace needs %zu bytes, got %zu", need, workspace_bytes);
     if (!aligned16(workspace)) return fail(FX_EINVAL, "workspace must be 16-byte aligned");
   }
-  *planned = plan;
   fx::Int8GemmArgs& g = *args;
   g = {};
   g.a = a;
@@ -2179,9 +2177,9 @@ int fx_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales, con
   if (!is_half_dtype(dtype) && dtype != FX_F32) return fail(FX_EINVAL, "dtype must be fp32, fp16 or bf16");
   if (M == 0) return FX_OK;
   fx::Int8GemmArgs g{};
-  fx::Int8GemmPlan plan{};
+  const fx::Int8GemmPlan plan = fx::plan_int8_gemm(M, N, K);
   if (int rc = prepare_int8_gemm(a, a_stride, a_scales, w, w_stride, w_scales, bias, out, out_stride, workspace,
-                                 workspace_bytes, M, N, K, dtype, &g, &plan))
+                                 workspace_bytes, M, N, K, dtype, plan, &g))
     return rc;
   return run_int8_gemm(g, plan, stream);
 }
@@ -2192,19 +2190,19 @@ struct Int8LinearParts {
   int width;  // of a row of codes
   size_t scales, partial, bytes;
 };
-Int8LinearParts int8_linear_parts(int M, int N, int K) {
+Int8LinearParts int8_linear_parts(const fx::Int8GemmPlan& plan, int M, int N, int K) {
   Int8LinearParts p;
   p.width = (K + 15) / 16 * 16;
   p.scales = align_up(size_t(M) * p.width, 256);
   p.partial = align_up(p.scales + size_t(M) * sizeof(float), 256);
-  p.bytes = p.partial + fx_int8_gemm_workspace_bytes(M, N, p.width);
+  p.bytes = p.partial + int8_gemm_workspace(plan, M, N);
   return p;
 }
 }  // namespace
 
 size_t fx_int8_linear_workspace_bytes(int M, int N, int K) {
   if (K < 1 || K > fx::kInt8MaxK / 16 * 16 || validate_int8_gemm_sizes(M, N, 16) || M == 0) return 0;
-  return int8_linear_parts(M, N, K).bytes;
+  return int8_linear_parts(fx::plan_int8_gemm(M, N, (K + 15) / 16 * 16), M, N, K).bytes;
 }
 
 int fx_int8_linear(const void* x, long long x_stride, int x_dtype, const int8_t* w, long long w_stride,
@@ -2216,7 +2214,8 @@ int fx_int8_linear(const void* x, long long x_stride, int x_dtype, const int8_t*
   if (!is_half_dtype(x_dtype)) return fail(FX_EINVAL, "x dtype must be fp16 or bf16");
   if (!is_half_dtype(out_dtype) && out_dtype != FX_F32) return fail(FX_EINVAL, "out dtype must be fp32, fp16 or bf16");
   if (M == 0) return FX_OK;
-  const Int8LinearParts p = int8_linear_parts(M, N, K);
+  const fx::Int8GemmPlan plan = fx::plan_int8_gemm(M, N, (K + 15) / 16 * 16);
+  const Int8LinearParts p = int8_linear_parts(plan, M, N, K);
   if (!workspace || workspace_bytes < p.bytes)
     return fail(FX_EINVAL, "linear workspace needs %zu bytes, got %zu", p.bytes, workspace_bytes);
   if (!aligned16(workspace)) return fail(FX_EINVAL, "workspace must be 16-byte aligned");
@@ -2225,9 +2224,8 @@ int fx_int8_linear(const void* x, long long x_stride, int x_dtype, const int8_t*
   float* scales = reinterpret_cast<float*>(base + p.scales);
   if (int rc = validate_half_rows("x", x, x_stride)) return rc;
   fx::Int8GemmArgs g{};
-  fx::Int8GemmPlan plan{};
   if (int rc = prepare_int8_gemm(codes, p.width, scales, w, w_stride, w_scales, bias, out, out_stride,
-                                 base + p.partial, workspace_bytes - p.partial, M, N, p.width, out_dtype, &g, &plan))
+                                 base + p.partial, workspace_bytes - p.partial, M, N, p.width, out_dtype, plan, &g))
     return rc;
   if (fx::int8_linear_fuses(plan, M, p.width)) {
     fx::Int8RowsArgs rows{};

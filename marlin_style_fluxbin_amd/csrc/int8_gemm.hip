@@ -46,7 +46,8 @@ Int8GemmPlan plan_int8_gemm(int M, int N, int K) {
   const float bytes = (float(M) + N) * K / 4.8e6f;
   Int8GemmPlan best{kInt8Few, 1, K};
   float least = M <= kFewRows ? 3.f + float(N) * K / 4.9e6f * (M <= 16 ? 1.f + 0.016f * M : 1.45f) : 1e30f;
-  for (int tile = 0; tile < kInt8Tiles; ++tile) {
+  // (32 rows fill half of the smallest tile; the plan itself is then 0.2 us of a call, and 0.7 of a search)
+  for (int tile = 0; tile < (M <= kFewRows ? 1 : kInt8Tiles); ++tile) {
     const Int8Tile& t = kInt8Tile[tile];
     const long tiles = long((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn), slots = 256 * t.places;
     for (int splits = 1; splits <= std::min(stages, kMaxSplits); ++splits) {
