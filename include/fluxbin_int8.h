@@ -51,13 +51,15 @@ int fx_int8_restore(const int8_t *codes, long long code_stride, const float *sca
 /*
  * out[m, n] = (sum_k a[m, k] w[n, k]) a_scales[m] w_scales[n] + bias[n]: the sum exact, then
  * fp32, rounded once to dtype (out's and bias's; bias may be NULL).  a [M, K], w [N, K] and
- * out [M, N]; K a multiple of 16 up to 131056, a and w 16-byte aligned with strides of whole 16
- * bytes up to 2^22.  M up to 2^21, N up to 2^20.  out overlaps no input.
- * `workspace` (fx_int8_gemm_workspace_bytes bytes, 16-byte aligned, no initial contents; NULL
- * when 0) holds the partial sums of a product that is split along K; calls that share one must
- * be ordered on one stream.
+ * out [M, N]; K up to 131056, M up to 2^21, N up to 2^20; strides of a and w 0 or at least K.  out
+ * overlaps no input.  Rows of whole 16 bytes (K a multiple of 16) at 16-byte boundaries, at most
+ * 2^22 bytes apart, are read where they are, and so are those of a product of up to 32 rows; others
+ * are copied into the workspace first.
+ * `workspace` (16-byte aligned, no initial contents, NULL when 0 bytes) also holds the partial sums
+ * of a product that is split along K; calls that share one must be ordered on one stream.  `loose`: 1
+ * when a's rows do not lie so, plus 2 when w's do not (3 by itself where K is no multiple of 16).
  */
-size_t fx_int8_gemm_workspace_bytes(int M, int N, int K);
+size_t fx_int8_gemm_workspace_bytes(int M, int N, int K, int loose);
 int fx_int8_gemm(const int8_t *a, long long a_stride, const float *a_scales, const int8_t *w, long long w_stride,
                  const float *w_scales, const void *bias, void *out, long long out_stride, void *workspace,
                  size_t workspace_bytes, int M, int N, int K, int dtype, void *stream);

@@ -98,7 +98,7 @@ INT8_SIGNATURES: dict[str, tuple] = {
     "fx_int8_rmsnorm": (_i, [_p, _l, _p, _l, _p, _l, _p, _p, _l, _p, _i, _i, _i, _f, _i, _p]),
     "fx_int8_silu_mul": (_i, [_p, _l, _p, _l, _p, _l, _p, _i, _i, _i, _i, _p]),
     "fx_int8_restore": (_i, [_p, _l, _p, _p, _l, _i, _i, _i, _p]),
-    "fx_int8_gemm_workspace_bytes": (_sz, [_i, _i, _i]),
+    "fx_int8_gemm_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "fx_int8_linear_workspace_bytes": (_sz, [_i, _i, _i]),
     "fx_int8_linear": (_i, [_p, _l, _i, _p, _l, _p, _p, _p, _l, _p, _sz, _i, _i, _i, _i, _p]),
     "fx_int8_gemm": (_i, [_p, _l, _p, _p, _l, _p, _p, _p, _l, _p, _sz, _i, _i, _i, _i, _p]),

@@ -2001,20 +2001,37 @@ int run_int8_rows(int mode, const fx::Int8RowsArgs& a, int dtype, void* stream, 
 int validate_int8_gemm_sizes(int M, int N, int K) {
   if (M < 0 || M > (1 << 21)) return fail(FX_EINVAL, "M must be in [0, 2^21], got %d", M);
   if (N < 1 || N > (1 << 20)) return fail(FX_EINVAL, "N must be in [1, 2^20], got %d", N);
-  if (K < 16 || K % 16 != 0 || K > fx::kInt8MaxK)
-    return fail(FX_EINVAL, "K must be a positive multiple of 16 up to %d, got %d", fx::kInt8MaxK / 16 * 16, K);
+  if (K < 1 || K > fx::kInt8MaxK / 16 * 16)
+    return fail(FX_EINVAL, "K must be in [1, %d], got %d", fx::kInt8MaxK / 16 * 16, K);
   return FX_OK;
 }
 
-size_t int8_gemm_workspace(const fx::Int8GemmPlan& plan, int M, int N) {
-  return plan.splits > 1 ? size_t(plan.splits) * M * N * sizeof(int) : 0;
+int whole16(int k) { return (k + 15) / 16 * 16; }
+
+// What a product's workspace holds: partial sums, and the rows of a (bit 1 of `loose`) and w (bit 2)
+// that a kernel of many rows cannot read where they are.
+struct Int8GemmParts {
+  size_t a, w, bytes;  // (partial sums first)
+};
+Int8GemmParts int8_gemm_parts(const fx::Int8GemmPlan& plan, int M, int N, int K, int loose) {
+  Int8GemmParts p{};
+  p.bytes = plan.splits > 1 ? align_up(size_t(plan.splits) * M * N * sizeof(int), 16) : 0;
+  if (plan.tile == fx::kInt8Few) return p;
+  p.a = p.bytes;
+  if (loose & 1) p.bytes += size_t(M) * whole16(K);
+  p.w = p.bytes;
+  if (loose & 2) p.bytes += size_t(N) * whole16(K);
+  return p;
+}
+
+bool loose_rows(const int8_t* p, long long stride, int rows, int K) {
+  return K % 16 != 0 || !aligned_to(p, 16) || (rows > 1 && (stride % 16 != 0 || stride > fx::kInt8RowLimit));
 }
 
 int validate_code_rows(const char* name, const int8_t* p, long long stride, int rows, int K) {
   if (!p) return fail(FX_EINVAL, "%s must be non-null", name);
-  if (!aligned_to(p, 16) || stride % 16 != 0) return fail(FX_EINVAL, "%s must have 16-byte aligned rows", name);
-  if (stride < 0 || stride > fx::kInt8RowLimit || (rows > 1 && stride != 0 && stride < K))
-    return fail(FX_EINVAL, "%s stride must be 0 or in [%d, 2^22], got %lld", name, K, stride);
+  if (stride < 0 || (rows > 1 && stride != 0 && stride < K))
+    return fail(FX_EINVAL, "%s stride must be 0 or at least %d, got %lld", name, K, stride);
   return FX_OK;
 }
 
@@ -2115,18 +2132,18 @@ int fx_int8_restore(const int8_t* codes, long long code_stride, const float* sca
   return check_launch("fx_int8_restore");
 }
 
-size_t fx_int8_gemm_workspace_bytes(int M, int N, int K) {
+size_t fx_int8_gemm_workspace_bytes(int M, int N, int K, int loose) {
   if (validate_int8_gemm_sizes(M, N, K) || M == 0) return 0;
-  return int8_gemm_workspace(fx::plan_int8_gemm(M, N, K), M, N);
+  if (K % 16 != 0) loose = 3;
+  return int8_gemm_parts(fx::plan_int8_gemm(M, N, whole16(K), loose != 0), M, N, K, loose).bytes;
 }
 
 namespace {
 
 // The checks of a product, its arguments and its plan.
 int prepare_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales, const int8_t* w, long long w_stride,
-                      const float* w_scales, const void* bias, void* out, long long out_stride, void* workspace,
-                      size_t workspace_bytes, int M, int N, int K, int dtype, const fx::Int8GemmPlan& plan,
-                      fx::Int8GemmArgs* args) {
+                      const float* w_scales, const void* bias, void* out, long long out_stride, int M, int N, int K,
+                      int dtype, fx::Int8GemmArgs* args) {
   if (!is_half_dtype(dtype) && dtype != FX_F32) return fail(FX_EINVAL, "dtype must be fp32, fp16 or bf16");
   if (int rc = validate_code_rows("a", a, a_stride, M, K)) return rc;
   if (int rc = validate_code_rows("w", w, w_stride, N, K)) return rc;
@@ -2136,12 +2153,6 @@ int prepare_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales
     return fail(FX_EINVAL, "scales, bias and out must be aligned to their elements");
   if (out_stride < 0 || (out_stride < N && M > 1))
     return fail(FX_EINVAL, "out stride %lld is shorter than a row of %d", out_stride, N);
-  const size_t need = int8_gemm_workspace(plan, M, N);
-  if (need) {
-    if (!workspace || workspace_bytes < need)
-      return fail(FX_EINVAL, "gemm workspace needs %zu bytes, got %zu", need, workspace_bytes);
-    if (!aligned16(workspace)) return fail(FX_EINVAL, "workspace must be 16-byte aligned");
-  }
   fx::Int8GemmArgs& g = *args;
   g = {};
   g.a = a;
@@ -2150,15 +2161,13 @@ int prepare_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales
   g.w_scales = w_scales;
   g.bias = bias;
   g.out = out;
-  g.partial = need ? static_cast<int*>(workspace) : nullptr;
-  g.a_stride = a_stride;
-  g.w_stride = w_stride;
+  g.a_stride = M > 1 ? a_stride : 0;
+  g.w_stride = N > 1 ? w_stride : 0;
   g.out_stride = out_stride;
   g.M = M;
   g.N = N;
   g.K = K;
   g.dt = dtype;
-  g.k_per_split = plan.k_per_split;
   return FX_OK;
 }
 
@@ -2177,10 +2186,43 @@ int fx_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales, con
   if (!is_half_dtype(dtype) && dtype != FX_F32) return fail(FX_EINVAL, "dtype must be fp32, fp16 or bf16");
   if (M == 0) return FX_OK;
   fx::Int8GemmArgs g{};
-  const fx::Int8GemmPlan plan = fx::plan_int8_gemm(M, N, K);
-  if (int rc = prepare_int8_gemm(a, a_stride, a_scales, w, w_stride, w_scales, bias, out, out_stride, workspace,
-                                 workspace_bytes, M, N, K, dtype, plan, &g))
+  if (int rc = prepare_int8_gemm(a, a_stride, a_scales, w, w_stride, w_scales, bias, out, out_stride, M, N, K, dtype, &g))
     return rc;
+  const int loose = loose_rows(a, a_stride, M, K) + 2 * loose_rows(w, w_stride, N, K);
+  const fx::Int8GemmPlan plan = fx::plan_int8_gemm(M, N, whole16(K), loose != 0);
+  const Int8GemmParts parts = int8_gemm_parts(plan, M, N, K, loose);
+  if (parts.bytes) {
+    if (!workspace || workspace_bytes < parts.bytes)
+      return fail(FX_EINVAL, "gemm workspace needs %zu bytes, got %zu", parts.bytes, workspace_bytes);
+    if (!aligned16(workspace)) return fail(FX_EINVAL, "workspace must be 16-byte aligned");
+  }
+  char* base = static_cast<char*>(workspace);
+  if (plan.splits > 1) g.partial = reinterpret_cast<int*>(base);
+  g.k_per_split = plan.k_per_split;
+  g.any = loose != 0;
+  if (loose && plan.tile != fx::kInt8Few) {
+    const int width = whole16(K);
+    fx::Int8AlignArgs c{};
+    c.columns = K;
+    c.width = width;
+    if (loose & 1) {
+      c.from[0] = a;
+      c.stride[0] = g.a_stride;
+      c.rows[0] = M;
+      g.a = c.to[0] = reinterpret_cast<int8_t*>(base + parts.a);
+      g.a_stride = width;
+    }
+    if (loose & 2) {
+      c.from[1] = w;
+      c.stride[1] = g.w_stride;
+      c.rows[1] = N;
+      g.w = c.to[1] = reinterpret_cast<int8_t*>(base + parts.w);
+      g.w_stride = width;
+    }
+    g.K = width;
+    fx::launch_int8_align(c, static_cast<hipStream_t>(stream));
+    if (int rc = check_launch("fx_int8_gemm")) return rc;
+  }
   return run_int8_gemm(g, plan, stream);
 }
 
@@ -2192,29 +2234,27 @@ struct Int8LinearParts {
 };
 Int8LinearParts int8_linear_parts(const fx::Int8GemmPlan& plan, int M, int N, int K) {
   Int8LinearParts p;
-  p.width = (K + 15) / 16 * 16;
+  p.width = whole16(K);
   p.scales = align_up(size_t(M) * p.width, 256);
   p.partial = align_up(p.scales + size_t(M) * sizeof(float), 256);
-  p.bytes = p.partial + int8_gemm_workspace(plan, M, N);
+  p.bytes = p.partial + int8_gemm_parts(plan, M, N, p.width, 0).bytes;
   return p;
 }
 }  // namespace
 
 size_t fx_int8_linear_workspace_bytes(int M, int N, int K) {
-  if (K < 1 || K > fx::kInt8MaxK / 16 * 16 || validate_int8_gemm_sizes(M, N, 16) || M == 0) return 0;
-  return int8_linear_parts(fx::plan_int8_gemm(M, N, (K + 15) / 16 * 16), M, N, K).bytes;
+  if (validate_int8_gemm_sizes(M, N, K) || M == 0) return 0;
+  return int8_linear_parts(fx::plan_int8_gemm(M, N, whole16(K), false), M, N, K).bytes;
 }
 
 int fx_int8_linear(const void* x, long long x_stride, int x_dtype, const int8_t* w, long long w_stride,
                    const float* w_scales, const void* bias, void* out, long long out_stride, void* workspace,
                    size_t workspace_bytes, int M, int N, int K, int out_dtype, void* stream) {
-  if (K < 1 || K > fx::kInt8MaxK / 16 * 16)
-    return fail(FX_EINVAL, "K must be in [1, %d], got %d", fx::kInt8MaxK / 16 * 16, K);
-  if (int rc = validate_int8_gemm_sizes(M, N, 16)) return rc;
+  if (int rc = validate_int8_gemm_sizes(M, N, K)) return rc;
   if (!is_half_dtype(x_dtype)) return fail(FX_EINVAL, "x dtype must be fp16 or bf16");
   if (!is_half_dtype(out_dtype) && out_dtype != FX_F32) return fail(FX_EINVAL, "out dtype must be fp32, fp16 or bf16");
   if (M == 0) return FX_OK;
-  const fx::Int8GemmPlan plan = fx::plan_int8_gemm(M, N, (K + 15) / 16 * 16);
+  const fx::Int8GemmPlan plan = fx::plan_int8_gemm(M, N, whole16(K), false);
   const Int8LinearParts p = int8_linear_parts(plan, M, N, K);
   if (!workspace || workspace_bytes < p.bytes)
     return fail(FX_EINVAL, "linear workspace needs %zu bytes, got %zu", p.bytes, workspace_bytes);
@@ -2224,9 +2264,12 @@ int fx_int8_linear(const void* x, long long x_stride, int x_dtype, const int8_t*
   float* scales = reinterpret_cast<float*>(base + p.scales);
   if (int rc = validate_half_rows("x", x, x_stride)) return rc;
   fx::Int8GemmArgs g{};
-  if (int rc = prepare_int8_gemm(codes, p.width, scales, w, w_stride, w_scales, bias, out, out_stride,
-                                 base + p.partial, workspace_bytes - p.partial, M, N, p.width, out_dtype, plan, &g))
+  if (int rc = prepare_int8_gemm(codes, p.width, scales, w, w_stride, w_scales, bias, out, out_stride, M, N, p.width,
+                                 out_dtype, &g))
     return rc;
+  if (loose_rows(w, w_stride, N, p.width)) return fail(FX_EINVAL, "w must have rows of whole 16 bytes at 16-byte boundaries");
+  if (plan.splits > 1) g.partial = reinterpret_cast<int*>(base + p.partial);
+  g.k_per_split = plan.k_per_split;
   if (fx::int8_linear_fuses(plan, M, p.width)) {
     fx::Int8RowsArgs rows{};
     rows.x = static_cast<const uint16_t*>(x);

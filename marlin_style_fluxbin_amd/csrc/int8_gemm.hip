@@ -33,6 +33,20 @@ __global__ __launch_bounds__(256) void int8_gemm_join_kernel(const Int8GemmArgs 
   store4(g, m, n, total, g.a_scales[m]);
 }
 
+// Rows at whatever address copied to whole 16 bytes at 16-byte boundaries, zeros behind them: those of
+// the activations, then those of the weight (rows 0: none), a thread 16 bytes at a time.
+__global__ __launch_bounds__(256) void int8_align_kernel(const Int8AlignArgs a) {
+  const int pieces = a.width / 16;
+  const long long first = (long long)(a.rows[0]) * pieces, all = first + (long long)(a.rows[1]) * pieces;
+  for (long long unit = (long long)(blockIdx.x) * 256 + threadIdx.x; unit < all; unit += (long long)(gridDim.x) * 256) {
+    const int which = unit >= first;
+    const long long at = unit - (which ? first : 0), row = at / pieces;
+    const int column = int(at - row * pieces) * 16;
+    *reinterpret_cast<u32x4_t*>(a.to[which] + row * a.width + column) =
+        part_b128(a.from[which] + row * a.stride[which] + column, a.columns - column);
+  }
+}
+
 constexpr int kFewRows = 32;
 constexpr int kMaxSplits = 16;
 
@@ -41,7 +55,8 @@ constexpr int kMaxSplits = 16;
 // Which kernel, and how many workgroups along K, by an estimate of the time (us): rounds of
 // workgroups, each its stages of 128 columns at what a stage takes, and the operands' bytes, of which
 // the shorter hides but in part; for splits the join's launch and the partial sums written and read.
-Int8GemmPlan plan_int8_gemm(int M, int N, int K) {
+Int8GemmPlan plan_int8_gemm(int M, int N, int K, bool any) {
+  if (any && M <= kFewRows) return {kInt8Few, 1, K};
   const int stages = (K + 127) / 128;
   const float bytes = (float(M) + N) * K / 4.8e6f;
   Int8GemmPlan best{kInt8Few, 1, K};
@@ -66,12 +81,25 @@ Int8GemmPlan plan_int8_gemm(int M, int N, int K) {
   return best;
 }
 
-template <int XDT>
+template <int XDT, bool ANY>
 void launch_few(const Int8GemmArgs& g, const Int8RowsArgs& rows, hipStream_t s) {
   const dim3 grid(unsigned(g.N + 15) / 16);
   // long rows: more of them in flight (4096 x 12288 11.8 us, with eight waves 12.5; 24576 x 4096 20.4 and 19.7)
-  if (g.K > 8192) hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, 1, 1, 16, 2>), grid, dim3(1024), 0, s, g, rows);
-  else hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, 1, 1, 8, 4>), grid, dim3(512), 0, s, g, rows);
+  if (g.K > 8192) hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, ANY, 1, 1, 16, 2>), grid, dim3(1024), 0, s, g, rows);
+  else hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, ANY, 1, 1, 8, 4>), grid, dim3(512), 0, s, g, rows);
+}
+
+template <bool ANY>
+void launch_few_rows(const Int8GemmArgs& g, hipStream_t s) {
+  if (g.M <= 16) {
+    launch_few<-1, ANY>(g, {}, s);
+  } else if (g.N <= 4096) {  // one workgroup a compute unit at most: 32 rows by 4096 x 4096 8.9 us, 11.1 with 32 columns
+    hipLaunchKernelGGL((int8_gemm_few_kernel<-1, ANY, 2, 1, 8, 4>), dim3(unsigned(g.N + 15) / 16), dim3(512), 0, s, g,
+                       Int8RowsArgs{});
+  } else {  // 24 rows by 6144 x 4096 10.8 us, 13.4 with 16 columns
+    hipLaunchKernelGGL((int8_gemm_few_kernel<-1, ANY, 2, 2, 8, 4>), dim3(unsigned(g.N + 31) / 32), dim3(512), 0, s, g,
+                       Int8RowsArgs{});
+  }
 }
 
 // Rows that every workgroup of the few-rows kernel had better quantize for itself.
@@ -80,21 +108,14 @@ bool int8_linear_fuses(const Int8GemmPlan& plan, int M, int K) {
 }
 
 void launch_int8_linear_few(int x_dt, const Int8RowsArgs& rows, const Int8GemmArgs& g, hipStream_t s) {
-  if (x_dt == kBF16) launch_few<kBF16>(g, rows, s);
-  else launch_few<kF16>(g, rows, s);
+  if (x_dt == kBF16) launch_few<kBF16, false>(g, rows, s);
+  else launch_few<kF16, false>(g, rows, s);
 }
 
 bool launch_int8_gemm(const Int8GemmPlan& plan, const Int8GemmArgs& g, hipStream_t s) {
   if (plan.tile == kInt8Few) {
-    if (g.M <= 16) {
-      launch_few<-1>(g, {}, s);
-    } else if (g.N <= 4096) {  // one workgroup a compute unit at most: 32 rows by 4096 x 4096 8.9 us, 11.1 with 32 columns
-      hipLaunchKernelGGL((int8_gemm_few_kernel<-1, 2, 1, 8, 4>), dim3(unsigned(g.N + 15) / 16), dim3(512), 0, s, g,
-                         Int8RowsArgs{});
-    } else {  // 24 rows by 6144 x 4096 10.8 us, 13.4 with 16 columns
-      hipLaunchKernelGGL((int8_gemm_few_kernel<-1, 2, 2, 8, 4>), dim3(unsigned(g.N + 31) / 32), dim3(512), 0, s, g,
-                         Int8RowsArgs{});
-    }
+    if (g.any) launch_few_rows<true>(g, s);
+    else launch_few_rows<false>(g, s);
     return true;
   }
   const Int8Tile& t = kInt8Tile[plan.tile];
@@ -106,6 +127,11 @@ bool launch_int8_gemm(const Int8GemmPlan& plan, const Int8GemmArgs& g, hipStream
     hipLaunchKernelGGL(int8_gemm_join_kernel, dim3(unsigned((units + 255) / 256)), dim3(256), 0, s, g, plan.splits);
   }
   return true;
+}
+
+void launch_int8_align(const Int8AlignArgs& a, hipStream_t s) {
+  const long long units = (long long)(a.rows[0] + (long long)(a.rows[1])) * (a.width / 16);
+  hipLaunchKernelGGL(int8_align_kernel, dim3(unsigned(std::min((units + 255) / 256, 16384LL))), dim3(256), 0, s, a);
 }
 
 }  // namespace fx

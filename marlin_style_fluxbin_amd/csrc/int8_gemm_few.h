@@ -8,17 +8,32 @@ namespace fx {
 
 constexpr int kFewCodes = 16384;  // bytes of codes that a workgroup quantizes for itself
 
+// 16 bytes at any address, and n <= 16 of them (the others 0).
+__device__ __forceinline__ u32x4_t any_b128(const int8_t* p) {
+  u32x4_t v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+__device__ __forceinline__ u32x4_t part_b128(const int8_t* p, int n) {
+  if (n >= 16) return any_b128(p);
+  u32x4_t v = {0u, 0u, 0u, 0u};
+  for (int e = 0; e < n; ++e) v[e >> 2] |= unsigned(uint8_t(p[e])) << (8 * (e & 3));
+  return v;
+}
+
 // RT x 16 rows of the weight by MT x 16 of the activations a workgroup, its W waves dealing the
 // columns in pieces of 128: a wave's sums are over its own columns and are added through LDS, so that
 // one launch has a burst of the whole weight in flight.  Bound by the weight's bytes (24576 x 4096 at
 // one row 19.7 us, 5.1 TB/s; 4096 x 4096 5.1 us, of which a launch is 4): every wave issues UN pieces'
 // loads in front of its first product (left to the compiler's order, 20.4).
 //
-// XDT kBF16 or kF16: the rows come unquantized, and every workgroup quantizes them for itself while
+// ANY: rows of any length at any address (elsewhere they begin at 16-byte boundaries and are whole 16
+// bytes long).  XDT kBF16 or kF16: the rows come unquantized, and every workgroup quantizes them for itself while
 // its part of the weight is on the way: a launch less than codes that another kernel leaves.
-template <int XDT, int MT, int RT, int W, int UN>
+template <int XDT, bool ANY, int MT, int RT, int W, int UN>
 __global__ __launch_bounds__(W * 64) void int8_gemm_few_kernel(const Int8GemmArgs g, const Int8RowsArgs rows) {
   constexpr bool kQuantize = XDT >= 0;
+  static_assert(!(kQuantize && ANY), "the rows that are quantized here are whole 16 bytes");
   constexpr int kTiles = MT * RT;
   static_assert(!kQuantize || MT == 1, "sixteen rows of codes at most in LDS");
   __shared__ i32x4_t sums[W][kTiles][64];
@@ -44,14 +59,30 @@ __global__ __launch_bounds__(W * 64) void int8_gemm_few_kernel(const Int8GemmArg
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) acc[i / MT][i % MT] = i32x4_t{0, 0, 0, 0};
   u32x4_t w[UN][2][RT], a[UN][2][MT];
+  // ANY: rows past the last are the last again, not stored
+  const int8_t *w_row[RT], *a_row[MT];
+  if constexpr (ANY) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) w_row[t] = g.w + min(n0 + 16 * t + r, g.N - 1) * g.w_stride + k16;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) a_row[t] = g.a + min(16 * t + r, g.M - 1) * g.a_stride + k16;
+  }
   // (an offset with kOutOfRange's bit is past every range)
   auto past = [&](int k) __attribute__((always_inline)) { return k + k16 < g.K ? 0 : kOutOfRange; };
-  auto load_w = [&](int k0) __attribute__((always_inline)) {
+  auto load = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < UN; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int k = k0 + u * W * 128 + h * 64;
+        if constexpr (ANY) {
+          const bool whole = k + 64 <= g.K;
+#pragma unroll
+          for (int t = 0; t < RT; ++t) w[u][h][t] = whole ? any_b128(w_row[t] + k) : part_b128(w_row[t] + k, g.K - k - k16);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) a[u][h][t] = whole ? any_b128(a_row[t] + k) : part_b128(a_row[t] + k, g.K - k - k16);
+          continue;
+        }
 #pragma unroll
         for (int t = 0; t < RT; ++t) w[u][h][t] = load_b128_stream(rw, (w_at[t] + k) | past(k), 0);
         if constexpr (!kQuantize) {
@@ -62,7 +93,7 @@ __global__ __launch_bounds__(W * 64) void int8_gemm_few_kernel(const Int8GemmArg
     __builtin_amdgcn_sched_barrier(0);
   };
   int k0 = wave * 128;
-  load_w(k0);
+  load(k0);
   if constexpr (kQuantize) {
     RowPointers p{};
     for (int m = 0; m < g.M; ++m) {
@@ -92,7 +123,7 @@ __global__ __launch_bounds__(W * 64) void int8_gemm_few_kernel(const Int8GemmArg
           for (int j = 0; j < MT; ++j) acc[i][j] = mfma_i8_16(w[u][h][i], a[u][h][j], acc[i][j]);
     k0 += W * 128 * UN;
     if (k0 >= g.K) break;
-    load_w(k0);
+    load(k0);
   }
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) sums[wave][i][lane] = acc[i / MT][i % MT];

@@ -26,6 +26,5 @@ constexpr Int8Tile kInt8Tile[] = {
     {256, 256, 1, 1.2f, 1.6f, 8.f, launch_int8_tile_256},
 };
 constexpr int kInt8Tiles = sizeof(kInt8Tile) / sizeof(kInt8Tile[0]);
-constexpr int kInt8Few = -1;  // int8_gemm_few.h
 
 }  // namespace fx

@@ -43,6 +43,7 @@ struct Int8GemmArgs {
   int M, N, K;
   int dt;            // of out and bias
   int k_per_split;   // a multiple of the kernel's K step
+  int any;           // few rows: a's and w's at any address, K any; else whole 16 bytes at 16-byte boundaries
 };
 constexpr long long kInt8RowLimit = 1LL << 22;  // bytes between rows: 256 rows stay within 31 bits
 constexpr int kInt8MaxK = 131071;               // 2^14 * 131071 < 2^31: the sums are exact
@@ -52,7 +53,19 @@ struct Int8GemmPlan {
   int splits;  // workgroups along K
   int k_per_split;
 };
-Int8GemmPlan plan_int8_gemm(int M, int N, int K);
+// any: rows that do not lie at 16-byte boundaries or are not whole 16 bytes.  Few of them are read in
+// place, more are copied first (launch_int8_align) and K is then whole 16.
+constexpr int kInt8Few = -1;  // int8_gemm_few.h
+Int8GemmPlan plan_int8_gemm(int M, int N, int K, bool any);
+
+struct Int8AlignArgs {
+  const int8_t* from[2];  // the activations, the weight
+  int8_t* to[2];          // rows of `width` bytes
+  long long stride[2];
+  int rows[2];            // 0: none
+  int columns, width;
+};
+void launch_int8_align(const Int8AlignArgs& a, hipStream_t s);
 // Whether a Linear's rows are quantized in the product's own launch, and that launch.
 bool int8_linear_fuses(const Int8GemmPlan& plan, int M, int K);
 void launch_int8_linear_few(int x_dt, const Int8RowsArgs& rows, const Int8GemmArgs& g, hipStream_t s);

@@ -27,8 +27,8 @@ from .packed_linear import PACKED_M1, PACKED_SMALL_M, DENSE_FALLBACK, PackedLine
 _HALF = (torch.float16, torch.bfloat16)
 _OUT = (torch.float16, torch.bfloat16, torch.float32)
 MAX_IN_FEATURES = 131056  # sums of so many products of codes stay within 32 bits
-_STEP = 16                # columns of the products' rows come in whole 16 bytes
-_ROW_LIMIT = 1 << 22      # bytes between two rows of codes that the products take
+_STEP = 16                # the module's rows are whole 16 bytes
+_ROW_LIMIT = 1 << 22      # bytes between two rows that every product reads in place
 _WHAT = "an 8-bit operator"
 
 _BF16, _FP16, _INT8, _FP32 = torch.bfloat16, torch.float16, torch.int8, torch.float32
@@ -36,8 +36,8 @@ _CODES = {dtype: _lib.dtype_code(dtype) for dtype in _OUT}
 
 
 @lru_cache(maxsize=4096)
-def _workspace_bytes(m: int, n: int, k: int) -> int:
-    return _lib.library().fx_int8_gemm_workspace_bytes(m, n, k)
+def _workspace_bytes(m: int, n: int, k: int, loose: int) -> int:
+    return _lib.library().fx_int8_gemm_workspace_bytes(m, n, k, loose)
 
 
 @lru_cache(maxsize=4096)
@@ -225,20 +225,16 @@ def _check_codes(codes: torch.Tensor, scales: torch.Tensor, name: str, scales_na
         raise ValueError(f"{scales_name} must be fp32, one for each row of {name}, on its device")
 
 
-def _code_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
-    """Rows as the products read them (whole 16 bytes at 16-byte boundaries): ``t`` or a padded
-    copy of it, rows, row stride and columns."""
-    columns = t.shape[-1]
-    if columns % _STEP == 0:
+def _code_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int, bool]:
+    """``t`` (or a copy whose rows lie evenly), its rows and row stride, and whether the products
+    read its rows in place however many they are (whole 16 bytes at 16-byte boundaries)."""
+    found = _rows_of(t)
+    if found is None or (found[0] > 1 and 0 != found[1] < t.shape[-1]):
+        t = t.contiguous()
         found = _rows_of(t)
-        if found is not None:
-            rows, stride = found
-            if not t.data_ptr() % 16 and (rows == 1 or (not stride % 16 and (stride >= columns or stride == 0)
-                                                        and stride <= _ROW_LIMIT)):
-                return t, rows, stride if rows > 1 else columns, columns
-    width = -(-columns // _STEP) * _STEP
-    t = F.pad(t, (0, width - columns)) if width != columns else t.clone(memory_format=torch.contiguous_format)
-    return t, t.numel() // width, width, width
+    rows, stride = found
+    loose = (t.shape[-1] | t.data_ptr()) & 15 or (rows > 1 and (stride & 15 or stride > _ROW_LIMIT))
+    return t, rows, stride, bool(loose)
 
 
 def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, *,
@@ -248,8 +244,8 @@ def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, w
 
     ``a [..., K]`` and ``weight [N, K]`` int8, their scales fp32 (one per row), ``bias [N]`` and the
     result of ``dtype`` (fp16, bf16 or fp32).  The sum is exact (K up to 131056); scales and bias are
-    applied in fp32, rounded once.  Rows are read in place where they are 16-byte aligned and K is a
-    multiple of 16; others are copied first."""
+    applied in fp32, rounded once.  Rows that lie at 16-byte boundaries are read in place where K is a
+    multiple of 16, and any where ``a`` has at most 32; others are copied first."""
     shape, wide, index = a.shape, weight.shape, a.get_device()
     if not (a.dtype is _INT8 and weight.dtype is _INT8 and a_scales.dtype is _FP32 and weight_scales.dtype is _FP32
             and index >= 0 and a_scales.get_device() == index and weight.get_device() == index
@@ -282,18 +278,19 @@ def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, w
             raise ValueError("out must have contiguous rows, each its own memory")
         out_stride = found[1]
     a_ptr, w_ptr = a.data_ptr(), weight.data_ptr()
+    loose = 0
     if a.is_contiguous() and weight.is_contiguous() and not (k | a_ptr | w_ptr) & 15:
-        rows, a_stride, w_stride, width = a.numel() // k, k, k, k
+        rows, a_stride, w_stride = a.numel() // k, k, k
     else:
-        a, rows, a_stride, width = _code_rows(a)
-        weight, _, w_stride, _ = _code_rows(weight)
-        a_ptr, w_ptr = a.data_ptr(), weight.data_ptr()
+        a, rows, a_stride, a_loose = _code_rows(a)
+        weight, _, w_stride, w_loose = _code_rows(weight)
+        a_ptr, w_ptr, loose = a.data_ptr(), weight.data_ptr(), a_loose + 2 * w_loose
     a_scales, weight_scales = a_scales.contiguous(), weight_scales.contiguous()
-    nbytes = _workspace_bytes(rows, n, width)
+    nbytes = _workspace_bytes(rows, n, k, loose)
     workspace = _new((nbytes,), torch.uint8, device) if nbytes else None
     _launch("fx_int8_gemm", device, a_ptr, a_stride, a_scales.data_ptr(), w_ptr, w_stride,
             weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), out_stride,
-            None if workspace is None else workspace.data_ptr(), nbytes, rows, n, width, code)
+            None if workspace is None else workspace.data_ptr(), nbytes, rows, n, k, code)
     return out
 
 
@@ -340,9 +337,11 @@ class PackedInt8Linear(PackedLinearBase):
         # rows of whole 16 bytes, the columns behind K zero, as the kernels read them
         self._width = -(-self.in_features // _STEP) * _STEP
         codes = codes.detach()
-        self.register_buffer("codes", F.pad(codes, (0, self._width - self.in_features)).contiguous()
-                             if self._width != self.in_features else codes.clone(memory_format=torch.contiguous_format))
-        self.register_buffer("scales", scales.detach().clone())
+        if self._width != self.in_features:
+            codes = F.pad(codes, (0, self._width - self.in_features))
+        codes = codes.contiguous()
+        self.register_buffer("codes", codes.clone() if codes.data_ptr() % 16 else codes)
+        self.register_buffer("scales", scales.detach().contiguous())
 
     @classmethod
     def from_linear(cls, linear: nn.Linear, *, fallback: str = "error") -> "PackedInt8Linear":

@@ -35,7 +35,7 @@ DEFAULTS = {
     "fx_int8_silu_mul": dict(ROWS, gate=D, gate_stride=200, up=D, up_stride=200),
     "fx_int8_restore": dict(codes=D, code_stride=112, scales=D, out=D, out_stride=100, rows=3, columns=100, dtype=2,
                             stream=None),
-    "fx_int8_gemm_workspace_bytes": dict(M=1, N=1, K=16),
+    "fx_int8_gemm_workspace_bytes": dict(M=1, N=1, K=16, loose=0),
     "fx_int8_linear_workspace_bytes": dict(M=1, N=1, K=16),
     "fx_int8_linear": dict(x=D, x_stride=60, x_dtype=2, w=D, w_stride=64, w_scales=D, bias=D, out=D, out_stride=8,
                            workspace=D, workspace_bytes=1 << 20, M=3, N=8, K=60, out_dtype=2, stream=None),
@@ -64,7 +64,7 @@ def test_header_compiles_alone_as_c_and_cxx(tmp_path):
         if shutil.which(compiler) is None:
             pytest.skip(f"no {compiler}")
         src = tmp_path / f"probe.{suffix}"
-        src.write_text('#include "fluxbin_int8.h"\nint main(void) { return (int)fx_int8_gemm_workspace_bytes(1, 1, 16); }\n')
+        src.write_text('#include "fluxbin_int8.h"\nint main(void) { return (int)fx_int8_gemm_workspace_bytes(1, 1, 16, 0); }\n')
         subprocess.run([compiler, *flags, "-Wall", "-Wextra", "-Werror", "-I", str(ROOT / "include"), "-c", str(src),
                         "-o", str(tmp_path / "probe.o")], check=True)
 
@@ -97,11 +97,13 @@ CASES += [("fx_int8_restore", *c) for c in [
     (dict(code_stride=-1), "do not fit rows"), (dict(out_stride=99), "do not fit rows")]]
 CASES += [("fx_int8_gemm", *c) for c in [
     (dict(M=-1), "M must be in"), (dict(M=(1 << 21) + 1), "M must be in"), (dict(N=0), "N must be in"),
-    (dict(N=(1 << 20) + 1), "N must be in"), (dict(K=0), "K must be"), (dict(K=72), "K must be"),
-    (dict(K=131072, a_stride=131072, w_stride=131072), "up to 131056"), (dict(dtype=3), "dtype must be fp32"),
+    (dict(N=(1 << 20) + 1), "N must be in"), (dict(K=0), "K must be"), (dict(K=-16), "K must be"),
+    (dict(K=131072, a_stride=131072, w_stride=131072), "K must be in [1, 131056]"), (dict(dtype=3), "dtype must be fp32"),
     (dict(a=None), "a must be non-null"), (dict(w=None), "w must be non-null"),
-    (dict(a=D + 8), "a must have 16-byte aligned rows"), (dict(w_stride=72), "w must have 16-byte aligned rows"),
-    (dict(a_stride=48), "a stride must be"), (dict(w_stride=(1 << 22) + 16), "w stride must be"),
+    (dict(a_stride=48), "a stride must be"), (dict(w_stride=63), "w stride must be"),
+    (dict(a=D + 8, M=100), "workspace needs"), (dict(w_stride=72, M=100), "workspace needs"),
+    (dict(K=60, M=100, workspace=D, workspace_bytes=64 * 108 - 1), "workspace needs"),
+    (dict(w_stride=(1 << 22) + 16, M=100), "workspace needs"),
     (dict(a_stride=-64), "a stride must be"), (dict(a_scales=None), "scales and out must be non-null"),
     (dict(out=None), "scales and out must be non-null"), (dict(w_scales=D + 2), "aligned to their elements"),
     (dict(bias=D + 2, dtype=0), "aligned to their elements"), (dict(out=D + 1), "aligned to their elements"),
@@ -112,7 +114,7 @@ CASES += [("fx_int8_linear", *c) for c in [
     (dict(workspace=None), "workspace needs"), (dict(workspace_bytes=511), "workspace needs"),
     (dict(workspace=D + 8), "workspace must be 16-byte aligned"), (dict(x=None), "x must be non-null"),
     (dict(x_stride=-2), "x stride"), (dict(w=None), "w must be non-null"), (dict(w_stride=48), "w stride"),
-    (dict(w=D + 8), "w must have 16-byte aligned rows"), (dict(w_scales=None), "scales and out must be non-null"),
+    (dict(w=D + 8), "w must have rows of whole 16 bytes"), (dict(w_scales=None), "scales and out must be non-null"),
     (dict(bias=D + 1), "aligned to their elements"), (dict(out_stride=7), "out stride")]]
 
 
@@ -132,20 +134,25 @@ def test_no_rows_do_nothing(name):
 
 def test_workspace_query_refuses_bad_sizes():
     size = _lib.library().fx_int8_gemm_workspace_bytes
-    assert size(-1, 8, 64) == size(1, 0, 64) == size(1, 8, 65) == size(0, 8, 64) == 0
+    assert size(-1, 8, 64, 0) == size(1, 0, 64, 0) == size(1, 8, 0, 0) == size(0, 8, 64, 3) == 0
+    # up to 32 rows are read wherever they lie; copies of more are whole 16 bytes wide
+    assert size(32, 8, 65, 3) == size(32, 8, 64, 0) == 0
+    one = size(100, 8, 64, 0)
+    assert size(100, 8, 64, 1) == one + 100 * 64 and size(100, 8, 64, 2) == one + 8 * 64
+    assert size(100, 8, 60, 0) == size(100, 8, 60, 3) == one + 108 * 64
     whole = _lib.library().fx_int8_linear_workspace_bytes
     assert whole(-1, 8, 64) == whole(1, 0, 64) == whole(1, 8, 0) == whole(0, 8, 64) == whole(1, 8, 131057) == 0
     # codes padded to whole 16 columns, a scale for each row, the product's own
-    assert whole(3, 8, 60) == 256 + 256 + size(3, 8, 64)
+    assert whole(3, 8, 60) == 256 + 256 + size(3, 8, 64, 0)
 
 
 def test_a_split_products_workspace_is_checked():
     size = _lib.library().fx_int8_gemm_workspace_bytes
-    split = [s for s in ((64, 256, 65536), (128, 1024, 12288), (200, 64, 131056)) if size(*s)]
+    split = [s for s in ((64, 256, 65536), (128, 1024, 12288), (200, 64, 131056)) if size(*s, 0)]
     for m, n, k in split:
         sizes = dict(M=m, N=n, K=k, a_stride=k, w_stride=k, out_stride=n)
         assert "workspace needs" in call("fx_int8_gemm", **sizes)[1]
-        assert "workspace needs" in call("fx_int8_gemm", **sizes, workspace=D, workspace_bytes=size(m, n, k) - 1)[1]
+        assert "workspace needs" in call("fx_int8_gemm", **sizes, workspace=D, workspace_bytes=size(m, n, k, 0) - 1)[1]
         assert "16-byte aligned" in call("fx_int8_gemm", **sizes, workspace=D + 4, workspace_bytes=1 << 40)[1]
 
 

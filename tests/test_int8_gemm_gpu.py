@@ -84,15 +84,42 @@ def test_columns_behind_k_and_rows_behind_m_are_not_read_into_the_sum(gpu, m):
             assert bool((out == 5).all())
 
 
-@pytest.mark.parametrize("k", [1, 15, 17, 100, 2077])
-def test_odd_columns_and_addresses_are_copied(gpu, k):
-    store = codes(40, k + 21, gpu, 5)
-    w = codes(50, k, gpu, 6)
-    sa, sw = scales(40, gpu, 7), scales(50, gpu, 8)
-    for a in (store[:, 3:3 + k], store[:, 16:16 + k].contiguous(), store[:, :k].t().contiguous().t()):
+@pytest.mark.parametrize("m", [1, 3, 16, 17, 32, 33, 130, 300])
+@pytest.mark.parametrize("k", [1, 15, 17, 64, 100, 2077, 8200])
+def test_rows_at_any_address_and_of_any_length(gpu, m, k):
+    """Odd K, odd strides and addresses, rows in reverse memory order, broadcast rows; large values around
+    every row; an output at an odd address."""
+    store = torch.full((m + 2, k + 21), 127, dtype=torch.int8, device=gpu)
+    wide = torch.full((72, k + 7), 127, dtype=torch.int8, device=gpu)
+    sa, sw = scales(m, gpu, 7), scales(70, gpu, 8)
+    bias = torch.randn(70, generator=torch.Generator(device=gpu).manual_seed(9), device=gpu).half()
+    for left, off in ((3, 1), (16, 2), (0, 0)):
+        a, w = store[1:1 + m, left:left + k], wide[1:71, off:off + k]
+        a.copy_(codes(m, k, gpu, left))
+        w.copy_(codes(70, k, gpu, off + 50))
+        out = torch.full((m, 73), 3.0, dtype=torch.float16, device=gpu)
+        int8_matmul(a, sa, w, sw, bias=bias, dtype=torch.float16, out=out[:, 1:71])
+        assert_product(out[:, 1:71], a, sa, w, sw, bias, context=(m, k, left))
+        assert bool((out[:, 0] == 3).all()) and bool((out[:, 71:] == 3).all())
+        aligned = torch.empty(70, -(-k // 16) * 16 + 16, dtype=torch.int8, device=gpu)[:, :k]
+        aligned.copy_(w)
+        assert torch.equal(int8_matmul(a, sa, aligned, sw), int8_matmul(a.contiguous(), sa, w.contiguous(), sw))
+    a = codes(k, m, gpu, 5).t()  # columns far apart: copied by torch
+    assert_product(int8_matmul(a, sa, w, sw), a, sa, w, sw)
+    flat = codes(1, k, gpu, 6)
+    assert torch.equal(int8_matmul(flat.expand(m, k), sa, w, sw), int8_matmul(flat.repeat(m, 1), sa, w, sw))
+
+
+def test_rows_far_apart(gpu):
+    """Strides beyond 2^22 bytes, read in place by few rows and copied for many; a weight of one row."""
+    store = torch.zeros(70, (1 << 22) + 32, dtype=torch.int8, device=gpu)
+    w = store[:, 16:16 + 256]
+    w.copy_(codes(70, 256, gpu, 1))
+    sw = scales(70, gpu, 2)
+    for m in (3, 20, 100):
+        a, sa = codes(m, 256, gpu, 3), scales(m, gpu, 4)
         assert_product(int8_matmul(a, sa, w, sw), a, sa, w, sw)
-    a = store[:, 1:17]
-    assert_product(int8_matmul(a, sa, w[:, :1].expand(50, 16), sw), a, sa, w[:, :1].expand(50, 16), sw)
+        assert_product(int8_matmul(a, sa, w[:1], sw[:1]), a, sa, w[:1], sw[:1])
 
 
 def test_leading_axes_and_no_rows(gpu):
