@@ -21,7 +21,7 @@ from torch import nn
 from torch.nn import functional as F
 
 from . import _lib
-from .cached_attention import _launch, _refuse_records
+from .cached_attention import _current_device, _refuse_records
 from .packed_linear import PACKED_M1, PACKED_SMALL_M, DENSE_FALLBACK, PackedLinearBase, replace_linears_atomically
 
 _HALF = (torch.float16, torch.bfloat16)
@@ -52,6 +52,21 @@ def _new(shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     if len(shape) == 1:
         return torch.empty_strided(shape, (1,), dtype=dtype, device=device)
     return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _launch(name: str, index: int, *args) -> None:
+    """The library call on GPU ``index`` and its current stream."""
+    call = getattr(_lib.library(), name)
+    if _current_device() == index:
+        rc = call(*args, _stream_of(index))
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args, _stream_of(index))
+    if rc:
+        _lib.check(rc, name)
+
+
+_stream_of = _lib._raw_stream or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _refuse(*tensors: torch.Tensor | None) -> None:
@@ -130,7 +145,7 @@ def quantize_int8(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | N
     shape, device = x.shape, x.device
     codes, scales, code_stride = _code_outputs(shape, device, out)
     columns = shape[-1]
-    _launch("fx_int8_quantize", device, x.data_ptr(), stride, codes.data_ptr(), code_stride, scales.data_ptr(), rows,
+    _launch("fx_int8_quantize", device.index, x.data_ptr(), stride, codes.data_ptr(), code_stride, scales.data_ptr(), rows,
             columns, columns, _CODES[x.dtype])
     return codes, scales
 
@@ -151,7 +166,7 @@ def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, *, dtype: torch.d
     scales = scales.contiguous()
     out = _new(codes.shape, dtype, codes.device)
     columns = codes.shape[-1]
-    _launch("fx_int8_restore", codes.device, codes.data_ptr(), found[1], scales.data_ptr(), out.data_ptr(), columns,
+    _launch("fx_int8_restore", codes.get_device(), codes.data_ptr(), found[1], scales.data_ptr(), out.data_ptr(), columns,
             found[0], columns, _lib.dtype_code(dtype))
     return out
 
@@ -180,7 +195,7 @@ def _norm(x, residual, weight, eps, residual_out, out):
             s_stride = found[1]
         r_ptr, s_ptr = residual.data_ptr(), residual_out.data_ptr()
     codes, scales, code_stride = _code_outputs(shape, device, out)
-    _launch("fx_int8_rmsnorm", device, x.data_ptr(), stride, r_ptr, r_stride, s_ptr, s_stride, weight.data_ptr(),
+    _launch("fx_int8_rmsnorm", device.index, x.data_ptr(), stride, r_ptr, r_stride, s_ptr, s_stride, weight.data_ptr(),
             codes.data_ptr(), code_stride, scales.data_ptr(), rows, columns, columns, eps, _CODES[dtype])
     return codes, scales, residual_out
 
@@ -212,7 +227,7 @@ def silu_mul_int8(gate: torch.Tensor, up: torch.Tensor, *, out: tuple[torch.Tens
     shape, device = gate.shape, gate.device
     codes, scales, code_stride = _code_outputs(shape, device, out)
     columns = shape[-1]
-    _launch("fx_int8_silu_mul", device, gate.data_ptr(), stride, up.data_ptr(), up_stride, codes.data_ptr(), code_stride,
+    _launch("fx_int8_silu_mul", device.index, gate.data_ptr(), stride, up.data_ptr(), up_stride, codes.data_ptr(), code_stride,
             scales.data_ptr(), rows, columns, columns, _CODES[gate.dtype])
     return codes, scales
 
@@ -288,7 +303,7 @@ def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, w
     a_scales, weight_scales = a_scales.contiguous(), weight_scales.contiguous()
     nbytes = _workspace_bytes(rows, n, k, loose)
     workspace = _new((nbytes,), torch.uint8, device) if nbytes else None
-    _launch("fx_int8_gemm", device, a_ptr, a_stride, a_scales.data_ptr(), w_ptr, w_stride,
+    _launch("fx_int8_gemm", index, a_ptr, a_stride, a_scales.data_ptr(), w_ptr, w_stride,
             weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), out_stride,
             None if workspace is None else workspace.data_ptr(), nbytes, rows, n, k, code)
     return out
@@ -372,11 +387,12 @@ class PackedInt8Linear(PackedLinearBase):
         width, k, o = self._width, self.in_features, self.out_features
         nbytes = _linear_workspace_bytes(rows, o, k)
         workspace = _new((nbytes,), torch.uint8, device)
+        index = device.index
 
         def run(x2: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
             code = _CODES[x2.dtype]
             added = bias if bias is None or bias.dtype == out.dtype else bias.to(out.dtype)
-            _launch("fx_int8_linear", device, x2.data_ptr(), x2.stride(0), code, codes.data_ptr(), width,
+            _launch("fx_int8_linear", index, x2.data_ptr(), x2.stride(0), code, codes.data_ptr(), width,
                     scales.data_ptr(), None if added is None else added.data_ptr(), out.data_ptr(), o,
                     workspace.data_ptr(), nbytes, rows, o, k, _CODES[out.dtype])
             return out
