@@ -43,7 +43,7 @@ __global__ __launch_bounds__(W * 64) void int8_gemm_few_kernel(const Int8GemmArg
   const int lane = threadIdx.x & 63, wave = wave_index();
   const int r = lane & 15, k16 = (lane >> 4) * 16;
   const int n0 = xcd_local_index8(blockIdx.x, gridDim.x) * (16 * RT);
-  const int w_stride = int(g.w_stride), a_stride = int(g.a_stride);
+  const int w_stride = ANY ? 0 : int(g.w_stride), a_stride = ANY ? 0 : int(g.a_stride);
   // rows past the last: no access, zeros
   const auto rw = buffer_resource_2g(g.w + n0 * g.w_stride, unsigned(min(16 * RT, g.N - n0) - 1) * w_stride + g.K);
   const auto ra = buffer_resource_2g(g.a, kQuantize ? 0u : unsigned(g.M - 1) * a_stride + g.K);

@@ -212,6 +212,25 @@ __device__ __forceinline__ void quantize_row(const Int8RowsArgs& a, const RowPoi
       plain = plain && squares < INFINITY && squares >= kSmall;
       inverse = rsqrtf(squares / float(a.columns) + a.eps);
     }
+    // Zeros (a padded batch's rows), and infinities and NaN where no product can overflow, need no second look.
+    constexpr bool kBounded = MODE == kRowsPlain || (MODE == kRowsNorm && DT == kF16);
+    if (top_bits == 0u || (kBounded && top_bits >= 0x7f800000u)) {
+      unsigned any = 0u;
+      if (top_bits == 0u) {
+        const uint16_t* from = MODE == kRowsNorm && p.second ? p.sum : p.x;
+        for (int c = tl; 8 * c < a.columns; c += TPR) {
+          const u32x4_t x = load8(from + 8 * c, a.columns - 8 * c);
+          any |= (x[0] | x[1] | x[2] | x[3]) & 0x7fff7fffu;
+        }
+        any = row_reduce<TPR>(any, [](unsigned u, unsigned w) { return u | w; }, reinterpret_cast<unsigned*>(red));
+      }
+      if (any == 0u) {
+        if (tl == 0) *scale_out = top_bits == 0u ? 0.f : __uint_as_float(0x7fc00000u);
+        const unsigned none[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+        for (int c = tl; 8 * c < a.code_columns; c += TPR) store_codes(p.codes + 8 * c, none, a.code_columns - 8 * c);
+        return;
+      }
+    }
     const float scale = top * inverse / 127.f;
     if (!plain || !(scale < INFINITY)) {
       row_in_64_bits<DT, MODE, TPR>(a, p, scale_out, tl, true, red);

@@ -156,7 +156,7 @@ def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, *, dtype: torch.d
     _check_codes(codes, scales, "codes", "scales")
     if dtype not in _OUT:
         raise ValueError("dtype must be fp16, bf16 or fp32")
-    _refuse_records(codes, scales, what=_WHAT)
+    _refuse(codes, scales)
     if codes.shape[-1] < 1:
         raise ValueError("codes must have shape [..., columns] with columns to hold")
     found = _rows_of(codes)
@@ -196,7 +196,7 @@ def _norm(x, residual, weight, eps, residual_out, out):
         r_ptr, s_ptr = residual.data_ptr(), residual_out.data_ptr()
     codes, scales, code_stride = _code_outputs(shape, device, out)
     _launch("fx_int8_rmsnorm", device.index, x.data_ptr(), stride, r_ptr, r_stride, s_ptr, s_stride, weight.data_ptr(),
-            codes.data_ptr(), code_stride, scales.data_ptr(), rows, columns, columns, eps, _CODES[dtype])
+            codes.data_ptr(), code_stride, scales.data_ptr(), rows, columns, columns, float(eps), _CODES[dtype])
     return codes, scales, residual_out
 
 
