@@ -2270,7 +2270,7 @@ int fx_int8_linear(const void* x, long long x_stride, int x_dtype, const int8_t*
   if (loose_rows(w, w_stride, N, p.width)) return fail(FX_EINVAL, "w must have rows of whole 16 bytes at 16-byte boundaries");
   if (plan.splits > 1) g.partial = reinterpret_cast<int*>(base + p.partial);
   g.k_per_split = plan.k_per_split;
-  if (fx::int8_linear_fuses(plan, M, p.width)) {
+  if (fx::int8_linear_fuses(M, N, p.width)) {
     fx::Int8RowsArgs rows{};
     rows.x = static_cast<const uint16_t*>(x);
     rows.x_stride = x_stride;

@@ -50,17 +50,30 @@ __global__ __launch_bounds__(256) void int8_align_kernel(const Int8AlignArgs a) 
 constexpr int kFewRows = 32;
 constexpr int kMaxSplits = 16;
 
+// Columns of a workgroup of the few-rows kernel.  From 17 rows on 32 of them share what is read of the
+// activations, where one workgroup a compute unit would not do (24 rows by 6144 x 4096 10.8 us, with 16
+// columns 13.4; 32 rows by 4096 x 4096 8.9 with 16 columns, with 32 11.1).
+int few_columns(int M, int N) { return M > 16 && N > 4096 ? 32 : 16; }
+
 }  // namespace
 
-// Which kernel, and how many workgroups along K, by an estimate of the time (us): rounds of
-// workgroups, each its stages of 128 columns at what a stage takes, and the operands' bytes, of which
-// the shorter hides but in part; for splits the join's launch and the partial sums written and read.
+// Which kernel, and how many workgroups along K, by an estimate of the time (us).  Few rows: rounds of
+// workgroups on a compute unit, each its rows of the weight (and some of the activations' from L2) at
+// 25.5 bytes a ns, whether the other units are at work or not.  Tiles: rounds of workgroups, each its
+// stages of 128 columns at what a stage takes, and the operands' bytes, of which the shorter hides but
+// in part; for splits the join's launch and the partial sums written and read.  Fitted to 408 sizes (1
+// to 4096 rows, 24 shapes of weights) timed with every tile and 1 to 16 splits: within 5% of the best
+// measured choice at 402 of them (fitted to half of the weights, at 195 of the other 204).
 Int8GemmPlan plan_int8_gemm(int M, int N, int K, bool any) {
   if (any && M <= kFewRows) return {kInt8Few, 1, K};
   const int stages = (K + 127) / 128;
-  const float bytes = (float(M) + N) * K / 4.8e6f;
+  const float bytes = (float(M) + N) * K / 6.3e6f;
   Int8GemmPlan best{kInt8Few, 1, K};
-  float least = M <= kFewRows ? 3.f + float(N) * K / 4.9e6f * (M <= 16 ? 1.f + 0.016f * M : 1.45f) : 1e30f;
+  float least = 1e30f;
+  if (M <= kFewRows) {
+    const int columns = few_columns(M, N), rounds = N / (columns * 256) + (N % (columns * 256) != 0);
+    least = 3.1f + rounds * (0.5f + K * (columns + 0.62f * M) / 25500.f);
+  }
   // (32 rows fill half of the smallest tile; the plan itself is then 0.2 us of a call, and 0.7 of a search)
   for (int tile = 0; tile < (M <= kFewRows ? 1 : kInt8Tiles); ++tile) {
     const Int8Tile& t = kInt8Tile[tile];
@@ -70,11 +83,13 @@ Int8GemmPlan plan_int8_gemm(int M, int N, int K, bool any) {
       const int per = (stages + splits - 1) / splits;
       if ((stages + per - 1) / per != splits) continue;  // a last split would be empty
       const long groups = tiles * splits, rounds = (groups + slots - 1) / slots;
-      const float filled = std::max(2.f * float(groups - (rounds - 1) * slots) / float(slots) - 1.f, 0.f);
+      const float last = float(groups - (rounds - 1) * slots) / float(slots);
+      // (a second workgroup on some compute unit already costs most of what one on each does)
+      const float filled = last <= 0.5f ? 0.f : t.places > 1 ? 0.4f + 0.6f * last : 2.f * last - 1.f;
       const float stage = (rounds - 1) * t.full + t.half + (t.full - t.half) * filled;
       const float work = per * stage + rounds * t.ends;
-      float time = 3.f + std::max(work, bytes) + 0.3f * std::min(work, bytes);
-      if (splits > 1) time += 3.5f + 2.f * splits * float(M) * N * 4.f / 5e6f;
+      float time = 1.6f + std::max(work, bytes) + 0.36f * std::min(work, bytes);
+      if (splits > 1) time += 2.8f + 0.2f * splits + 2.f * splits * float(M) * N * 4.f / 8.3e6f;
       if (time < least) least = time, best = {tile, splits, splits == 1 ? K : per * 128};
     }
   }
@@ -91,20 +106,19 @@ void launch_few(const Int8GemmArgs& g, const Int8RowsArgs& rows, hipStream_t s) 
 
 template <bool ANY>
 void launch_few_rows(const Int8GemmArgs& g, hipStream_t s) {
-  if (g.M <= 16) {
-    launch_few<-1, ANY>(g, {}, s);
-  } else if (g.N <= 4096) {  // one workgroup a compute unit at most: 32 rows by 4096 x 4096 8.9 us, 11.1 with 32 columns
-    hipLaunchKernelGGL((int8_gemm_few_kernel<-1, ANY, 2, 1, 8, 4>), dim3(unsigned(g.N + 15) / 16), dim3(512), 0, s, g,
-                       Int8RowsArgs{});
-  } else {  // 24 rows by 6144 x 4096 10.8 us, 13.4 with 16 columns
-    hipLaunchKernelGGL((int8_gemm_few_kernel<-1, ANY, 2, 2, 8, 4>), dim3(unsigned(g.N + 31) / 32), dim3(512), 0, s, g,
-                       Int8RowsArgs{});
-  }
+  const int columns = few_columns(g.M, g.N);
+  const dim3 grid(unsigned(g.N + columns - 1) / columns);
+  if (g.M <= 16) launch_few<-1, ANY>(g, {}, s);
+  else if (columns == 16) hipLaunchKernelGGL((int8_gemm_few_kernel<-1, ANY, 2, 1, 8, 4>), grid, dim3(512), 0, s, g, Int8RowsArgs{});
+  else hipLaunchKernelGGL((int8_gemm_few_kernel<-1, ANY, 2, 2, 8, 4>), grid, dim3(512), 0, s, g, Int8RowsArgs{});
 }
 
-// Rows that every workgroup of the few-rows kernel had better quantize for itself.
-bool int8_linear_fuses(const Int8GemmPlan& plan, int M, int K) {
-  return plan.tile == kInt8Few && M <= 16 && long(M) * K <= kFewCodes;
+// Every workgroup quantizes the rows again, 1.5 us for each and each round of workgroups, where codes
+// from a launch of their own cost 2 to 3 us (one row by 4096 x 4096 7.1 us for 8.3, by 12288 x 1536 10.6
+// for 10.7, by 24576 x 4096 24.3 for 22.8; two rows by 1024 x 2000 6.7 for 7.0, by 4096 x 4096 8.9 for
+// 8.6 and a launch less for the host, by 9728 x 896 11.4 for 9.8; four by 1024 x 2000 9.8 for 7.2).
+bool int8_linear_fuses(int M, int N, int K) {
+  return M <= 2 && long(M) * N <= 12288 && long(M) * K <= kFewCodes;
 }
 
 void launch_int8_linear_few(int x_dt, const Int8RowsArgs& rows, const Int8GemmArgs& g, hipStream_t s) {

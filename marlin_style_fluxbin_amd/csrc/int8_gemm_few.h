@@ -35,7 +35,7 @@ __global__ __launch_bounds__(W * 64) void int8_gemm_few_kernel(const Int8GemmArg
   constexpr bool kQuantize = XDT >= 0;
   static_assert(!(kQuantize && ANY), "the rows that are quantized here are whole 16 bytes");
   constexpr int kTiles = MT * RT;
-  static_assert(!kQuantize || MT == 1, "sixteen rows of codes at most in LDS");
+  static_assert(!kQuantize || MT == 1, "at most sixteen rows are quantized here");
   __shared__ i32x4_t sums[W][kTiles][64];
   __shared__ __attribute__((aligned(16))) int8_t codes[kQuantize ? kFewCodes : 16];
   __shared__ double red[W];

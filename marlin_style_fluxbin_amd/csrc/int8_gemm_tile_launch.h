@@ -20,10 +20,10 @@ struct Int8Tile {
 // (of 2048 x 4096 x 4096 the four take 63, 43.7, 37.6 and 45.5 us; of 1024 x 4096 x 4096 34, 22.6, 32 and 44;
 // 128 x 128 tiles with two stages, two workgroups a compute unit: 39.4 and 25.7)
 constexpr Int8Tile kInt8Tile[] = {
-    {64, 64, 2, 0.28f, 0.43f, 1.5f, launch_int8_tile_64},
-    {128, 128, 1, 0.48f, 0.58f, 3.f, launch_int8_tile_128},
-    {128, 256, 1, 0.8f, 1.f, 5.f, launch_int8_tile_128x256},
-    {256, 256, 1, 1.2f, 1.6f, 8.f, launch_int8_tile_256},
+    {64, 64, 2, 0.24f, 0.475f, 1.45f, launch_int8_tile_64},
+    {128, 128, 1, 0.44f, 0.58f, 3.f, launch_int8_tile_128},
+    {128, 256, 1, 0.755f, 0.9f, 3.95f, launch_int8_tile_128x256},
+    {256, 256, 1, 1.335f, 1.57f, 5.3f, launch_int8_tile_256},
 };
 constexpr int kInt8Tiles = sizeof(kInt8Tile) / sizeof(kInt8Tile[0]);
 

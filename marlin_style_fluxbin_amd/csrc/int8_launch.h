@@ -67,7 +67,7 @@ struct Int8AlignArgs {
 };
 void launch_int8_align(const Int8AlignArgs& a, hipStream_t s);
 // Whether a Linear's rows are quantized in the product's own launch, and that launch.
-bool int8_linear_fuses(const Int8GemmPlan& plan, int M, int K);
+bool int8_linear_fuses(int M, int N, int K);
 void launch_int8_linear_few(int x_dt, const Int8RowsArgs& rows, const Int8GemmArgs& g, hipStream_t s);
 bool launch_int8_gemm(const Int8GemmPlan& plan, const Int8GemmArgs& a, hipStream_t s);
 
