@@ -93,7 +93,7 @@ __device__ __forceinline__ void tile_store_as(const Int8GemmArgs& g, const i32x1
       const u32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(lds + row * kRow + col * kSize);
       char* to = out + ((m + row) * stride + n0 + col) * kSize;
       if (left >= kEach) {
-        // at whatever address the row begins (301 x 1001 x 2000 8.2 us, element by element 10.6); a result is
+        // at whatever address the row begins (301 x 1001 x 2000 8.8 us, element by element 10.6); a result is
         // not read again here (8192 x 12288 x 4096 356 us, with plain stores 371)
         if constexpr (OUT < 0) __builtin_memcpy(to, &v, 16);
         else __builtin_nontemporal_store(v, reinterpret_cast<any16_t*>(to));

@@ -260,7 +260,8 @@ def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, w
     ``a [..., K]`` and ``weight [N, K]`` int8, their scales fp32 (one per row), ``bias [N]`` and the
     result of ``dtype`` (fp16, bf16 or fp32).  The sum is exact (K up to 131056); scales and bias are
     applied in fp32, rounded once.  Rows that lie at 16-byte boundaries are read in place where K is a
-    multiple of 16, and any where ``a`` has at most 32; others are copied first."""
+    multiple of 16, and any where ``a`` has at most 32; others are copied first.  ``out`` shares no memory
+    with the inputs."""
     shape, wide, index = a.shape, weight.shape, a.get_device()
     if not (a.dtype is _INT8 and weight.dtype is _INT8 and a_scales.dtype is _FP32 and weight_scales.dtype is _FP32
             and index >= 0 and a_scales.get_device() == index and weight.get_device() == index
@@ -316,7 +317,10 @@ def quantize_weight_int8(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tens
         raise ValueError("weight must have shape [O, K]")
     weight = weight.detach()
     if weight.is_cuda and weight.dtype in _HALF:
-        return quantize_int8(weight)
+        codes, scales = quantize_int8(weight)
+        if not bool(torch.isfinite(scales).all()):
+            raise ValueError("weight must be finite")
+        return codes, scales
     wide = weight.double()
     top = wide.abs().amax(1, keepdim=True)
     if not bool(torch.isfinite(top).all()):
@@ -329,7 +333,8 @@ class PackedInt8Linear(PackedLinearBase):
     """Linear with 8-bit weights (a scale per output channel) and activations (a scale per row,
     formed in the call).
 
-    ``codes [O, K]`` int8 and ``scales [O]`` fp32 stand for the weight ``codes * scales[:, None]``.
+    ``codes [O, K]`` int8 and ``scales [O]`` fp32 stand for the weight ``codes * scales[:, None]``; the
+    module keeps the tensors it is given where they lie as the kernels read them.
     Any number of fp16 or bf16 rows on the GPU take the kernels; other inputs are refused unless
     ``fallback='dense'`` (``F.linear`` with the weight that the codes stand for).  Routes, counters
     and the bound one-row decode call are those of ``packed_linear.PackedLinearBase``."""

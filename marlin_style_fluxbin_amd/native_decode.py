@@ -21,8 +21,10 @@ same with the hybrid GEMV's normalising prologue and residual epilogue
 (``fx_hybrid_gemv_segments_rmsnormed``, ``fx_hybrid_gemv_residual``), the
 SwiGLU formed in the down GEMV's prologue (6 per layer).  Other Linears (dense bf16, the bf16
 arm, ``torch.matmul``) run between add+RMSNorm kernels and the same attention
-launches; with 8-bit Linears (``PackedInt8Linear``) the norms and the SwiGLU write codes.  The arithmetic and rounding points are the stock HF Qwen3 modules'
-(RMSNorm, RoPE, SDPA with fp32 softmax, SwiGLU).
+launches; with 8-bit Linears (``PackedInt8Linear``) the norms and the SwiGLU
+write codes.  The arithmetic and rounding points are the stock HF Qwen3 modules'
+(RMSNorm, RoPE, SDPA with fp32 softmax, SwiGLU), except that the codes are
+rounded from fp32 values, without the rounding to 16 bits between.
 """
 from __future__ import annotations
 
@@ -62,7 +64,7 @@ class _Linear:
     module's own table route (``groups_per_split > 1``: ``fx_w3_m1_out`` with its
     row tile and split, as ``PackedW3Linear.forward`` runs it), the hybrid two-base
     GEMV (``fx_hybrid_gemv`` through the module's own packed kernel and
-    workspace), or a dense matmul."""
+    workspace), the 8-bit product (``fx_int8_linear``, the same way), or a dense matmul."""
 
     def __init__(self, module):
         self.gemv = None
@@ -93,7 +95,7 @@ class _FusedLinear:
     concatenated rows (q|k|v, gate|up): one launch instead of several.  W3 payloads
     concatenate along O when K, arithmetic, scale dtype, zero-point presence and
     the column permutation agree; hybrid two-base payloads run as one
-    ``fx_hybrid_gemv_segments`` launch; dense weights concatenate along O.  Each output
+    ``fx_hybrid_gemv_segments`` launch; 8-bit codes and dense weights concatenate along O.  Each output
     row is computed exactly as it would be alone, so the outputs are bit-identical
     to separate calls.  ``None`` from :meth:`build` when the modules do not fuse."""
 

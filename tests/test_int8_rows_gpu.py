@@ -11,15 +11,16 @@ leave 2^-21 of a value, a and the quotient's own rounding as much again: a code 
 import pytest
 import torch
 
-from marlin_style_fluxbin_amd import (add_rms_norm_int8, dequantize_int8, quantize_int8, rms_norm_int8, silu_mul_int8)
+from marlin_style_fluxbin_amd import (add_rms_norm_int8, dequantize_int8, quantize_int8, quantize_weight_int8,
+                                      rms_norm_int8, silu_mul_int8)
 from tests.int8_reference import HALVES, held, norm_rows, swiglu_rows
 
 pytestmark = pytest.mark.gpu
 
 EPS = 1e-6
-# around every kernel's width: 512, 1024, 2048, 4096, 8192, 16384, and beyond
+# around every kernel's width: 512, 1024, 2048, 4096, 8192, 12288, 16384, and beyond
 SHAPES = [(1, 1), (3, 7), (5, 8), (2, 63), (9, 512), (4, 513), (7, 1000), (5, 1024), (3, 1032), (2, 2047), (3, 2049),
-          (4, 4096), (2, 4104), (3, 8192), (2, 8200), (2, 16384), (2, 16392), (1, 40000)]
+          (4, 4096), (2, 4104), (3, 8192), (2, 8200), (300, 4090), (2, 12288), (2, 12296), (2, 16384), (2, 16392), (1, 40000)]
 
 
 def states(rows, columns, dtype, gpu, seed=0):
@@ -271,3 +272,14 @@ def test_streams_and_graphs(gpu):
         torch.cuda.synchronize()
         assert torch.equal(codes, eager[0]) and torch.equal(scales, eager[1]) and torch.equal(total, eager[2])
         assert torch.equal(act[0], act_eager[0]) and torch.equal(act[1], act_eager[1])
+
+
+def test_a_weight_that_is_not_finite_is_refused(gpu):
+    """As on the CPU: no channel becomes NaN without a word."""
+    weight = torch.randn(5, 48, device=gpu, dtype=torch.bfloat16)
+    weight[3, 7] = float("nan")
+    with pytest.raises(ValueError, match="finite"):
+        quantize_weight_int8(weight)
+    weight[3, 7] = 0
+    codes, scales = quantize_weight_int8(weight)
+    assert torch.equal(codes, quantize_int8(weight)[0]) and torch.equal(scales, quantize_int8(weight)[1])
