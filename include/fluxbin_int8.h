@@ -25,8 +25,7 @@ extern "C" {
 /*
  * Rows x [rows, columns] to codes [rows, code_columns] and scales [rows].  code_columns >=
  * columns: the codes behind a row's last column become 0 (rows padded to what fx_int8_gemm
- * takes).  Tensors at 16-byte boundaries with strides of whole 8 elements are read 16 bytes at
- * a time, others element by element.  Codes of inputs as they are (quantize, rmsnorm) are the
+ * takes).  Rows begin at any element.  Codes of inputs as they are (quantize, rmsnorm) are the
  * exact quotient's.
  */
 int fx_int8_quantize(const void *x, long long x_stride, int8_t *codes, long long code_stride, float *scales, int rows,
