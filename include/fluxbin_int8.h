@@ -9,8 +9,8 @@
  *
  * Codes are int8 rows of contiguous columns; strides count elements between rows, all
  * non-negative.  dtype: FX_F16 or FX_BF16 for the rows' inputs, also FX_F32 for the outputs of
- * fx_int8_restore and fx_int8_gemm.  rows up to 2^21 (0 launches
- * nothing), columns up to 2^20.
+ * fx_int8_restore and fx_int8_gemm.  rows up to 2^21 (0 launches nothing), columns up to 2^20.
+ * Outputs overlap no input but where it says so.
  */
 #ifndef FLUXBIN_INT8_H
 #define FLUXBIN_INT8_H

@@ -125,10 +125,11 @@ def _code_outputs(shape: torch.Size, device: torch.device, out) -> tuple[torch.T
     if out is None:
         return _new(shape, _INT8, device), _new(shape[:-1], _FP32, device), shape[-1]
     codes, scales = out
+    _refuse(scales)
     if codes.shape != shape or codes.dtype is not _INT8 or codes.device != device:
         raise ValueError("out's codes must be int8 of the input's shape on its device")
     if (scales.shape != shape[:-1] or scales.dtype is not _FP32 or scales.device != device
-            or not scales.is_contiguous()):
+            or not scales.is_contiguous() or scales.is_neg()):
         raise ValueError("out's scales must be contiguous fp32 of the input's leading shape on its device")
     found = _rows_of(codes)
     if found is None or (found[0] > 1 and found[1] < shape[-1]):
@@ -139,7 +140,8 @@ def _code_outputs(shape: torch.Size, device: torch.device, out) -> tuple[torch.T
 def quantize_int8(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | None = None):
     """Each row of ``x [..., columns]`` (fp16 or bf16) as ``codes`` (int8, x's shape) and ``scales``
     (fp32, x's leading shape): with a the row's largest magnitude, code = round(127 x / a), ties to
-    even, scale = a / 127.  A row with an infinity or NaN stands for NaN (its scale is NaN)."""
+    even, scale = a / 127.  A row with an infinity or NaN stands for NaN (its scale is NaN).  ``out``
+    gives both their memory, none of it an input's."""
     _refuse(x)
     x, rows, stride = _half_input(x, "x")
     shape, device = x.shape, x.device
@@ -163,7 +165,7 @@ def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, *, dtype: torch.d
     if found is None:
         codes = codes.contiguous()
         found = _rows_of(codes)
-    scales = scales.contiguous()
+    scales = scales.resolve_neg().contiguous()
     out = _new(codes.shape, dtype, codes.device)
     columns = codes.shape[-1]
     _launch("fx_int8_restore", codes.get_device(), codes.data_ptr(), found[1], scales.data_ptr(), out.data_ptr(), columns,
@@ -301,7 +303,10 @@ def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, w
         a, rows, a_stride, a_loose = _code_rows(a)
         weight, _, w_stride, w_loose = _code_rows(weight)
         a_ptr, w_ptr, loose = a.data_ptr(), weight.data_ptr(), a_loose + 2 * w_loose
-    a_scales, weight_scales = a_scales.contiguous(), weight_scales.contiguous()
+    if not a_scales.is_contiguous() or a_scales.is_neg():
+        a_scales = a_scales.resolve_neg().contiguous()
+    if not weight_scales.is_contiguous() or weight_scales.is_neg():
+        weight_scales = weight_scales.resolve_neg().contiguous()
     nbytes = _workspace_bytes(rows, n, k, loose)
     workspace = _new((nbytes,), torch.uint8, device) if nbytes else None
     _launch("fx_int8_gemm", index, a_ptr, a_stride, a_scales.data_ptr(), w_ptr, w_stride,

@@ -48,6 +48,18 @@ def test_larger_products(gpu, m, n, k):
     assert_product(int8_matmul(*args, bias=b), *args, b, context=(m, n, k))
 
 
+# every kernel, whole and in K splits (few rows: 16 and 32 rows by 16 and 32 columns, eight and sixteen
+# waves; tiles of 64, 128, 128 x 256 and 256), its last stage not whole
+@pytest.mark.parametrize("m,n,k", [(16, 1000, 528), (9, 1000, 8208), (17, 17, 528), (17, 4097, 1040), (31, 8200, 1040),
+                                   (200, 100, 48), (16, 6001, 4112), (90, 17, 12304), (200, 8200, 48), (1300, 1000, 8208),
+                                   (90, 4097, 8208), (2050, 2049, 48), (260, 8200, 12304), (130, 6001, 8208),
+                                   (1300, 6001, 48), (130, 8200, 16400)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_every_kernel_and_split(gpu, m, n, k, dtype):
+    args, b = case(m, n, k, gpu, dtype, True, seed=11)
+    assert_product(int8_matmul(*args, bias=b, dtype=dtype), *args, b, context=(m, n, k))
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_sums_are_exact_at_their_largest(gpu, m):
     """Every product 2^14 or -127 * 128, as many of them as K may be; scales 1 and fp32 results."""
@@ -172,6 +184,7 @@ def test_refusals(gpu):
         (lambda: int8_matmul(a, sa, w, sw, out=torch.empty(1, 32, dtype=torch.bfloat16, device=gpu).expand(4, 32)), "out must"),
         (lambda: int8_matmul(a, sa, w, sw, out=torch.empty(32, 4, dtype=torch.bfloat16, device=gpu).t()), "out must"),
         (lambda: int8_matmul(a, sa.clone().requires_grad_(), w, sw), "no backward"),
+        (lambda: quantize_int8(b[None], out=(w.view(-1)[:32].view(1, 32), sw[:1].clone().requires_grad_())), "no backward"),
     ]
     for call, message in bad:
         with pytest.raises(ValueError, match=message):
