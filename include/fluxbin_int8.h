@@ -66,8 +66,9 @@ int fx_int8_gemm(const int8_t *a, long long a_stride, const float *a_scales, con
 /*
  * A Linear in one call: rows x [M, K] of x_dtype (fp16 or bf16) quantized (fx_int8_quantize) and
  * multiplied (fx_int8_gemm) with w [N, K padded to whole 16, zeros behind K] to out of out_dtype.
- * `workspace`: fx_int8_linear_workspace_bytes bytes, 16-byte aligned, no initial contents; it
- * holds the codes, their scales and the product's partial sums.
+ * `workspace`: fx_int8_linear_workspace_bytes bytes (NULL when 0: few rows that the product's launch
+ * quantizes), 16-byte aligned, no initial contents; it holds the codes, their scales and the
+ * product's partial sums; calls that share one must be ordered on one stream.
  */
 size_t fx_int8_linear_workspace_bytes(int M, int N, int K);
 int fx_int8_linear(const void *x, long long x_stride, int x_dtype, const int8_t *w, long long w_stride,

@@ -2229,21 +2229,19 @@ int fx_int8_gemm(const int8_t* a, long long a_stride, const float* a_scales, con
 namespace {
 // The parts of a Linear's workspace: codes, scales, partial sums.
 struct Int8LinearParts {
-  int width;  // of a row of codes
   size_t scales, partial, bytes;
 };
 Int8LinearParts int8_linear_parts(const fx::Int8GemmPlan& plan, int M, int N, int K) {
   Int8LinearParts p;
-  p.width = whole16(K);
-  p.scales = align_up(size_t(M) * p.width, 256);
+  p.scales = align_up(size_t(M) * whole16(K), 256);
   p.partial = align_up(p.scales + size_t(M) * sizeof(float), 256);
-  p.bytes = p.partial + int8_gemm_parts(plan, M, N, p.width, 0).bytes;
+  p.bytes = p.partial + int8_gemm_parts(plan, M, N, whole16(K), 0).bytes;
   return p;
 }
 }  // namespace
 
 size_t fx_int8_linear_workspace_bytes(int M, int N, int K) {
-  if (validate_int8_gemm_sizes(M, N, K) || M == 0) return 0;
+  if (validate_int8_gemm_sizes(M, N, K) || M == 0 || fx::int8_linear_fuses(M, N, whole16(K))) return 0;
   return int8_linear_parts(fx::plan_int8_gemm(M, N, whole16(K), false), M, N, K).bytes;
 }
 
@@ -2254,7 +2252,25 @@ int fx_int8_linear(const void* x, long long x_stride, int x_dtype, const int8_t*
   if (!is_half_dtype(x_dtype)) return fail(FX_EINVAL, "x dtype must be fp16 or bf16");
   if (!is_half_dtype(out_dtype) && out_dtype != FX_F32) return fail(FX_EINVAL, "out dtype must be fp32, fp16 or bf16");
   if (M == 0) return FX_OK;
-  const fx::Int8GemmPlan plan = fx::plan_int8_gemm(M, N, whole16(K), false);
+  if (int rc = validate_half_rows("x", x, x_stride)) return rc;
+  const int width = whole16(K);
+  fx::Int8GemmArgs g{};
+  if (fx::int8_linear_fuses(M, N, width)) {
+    // (no codes in memory: the launch reads neither of the two)
+    if (int rc = prepare_int8_gemm(static_cast<const int8_t*>(x), width, w_scales, w, w_stride, w_scales, bias, out,
+                                   out_stride, M, N, width, out_dtype, &g))
+      return rc;
+    if (loose_rows(w, w_stride, N, width)) return fail(FX_EINVAL, "w must have rows of whole 16 bytes at 16-byte boundaries");
+    fx::Int8RowsArgs rows{};
+    rows.x = static_cast<const uint16_t*>(x);
+    rows.x_stride = x_stride;
+    rows.rows = M;
+    rows.columns = K;
+    rows.code_columns = width;
+    fx::launch_int8_linear_few(x_dtype, rows, g, static_cast<hipStream_t>(stream));
+    return check_launch("fx_int8_linear");
+  }
+  const fx::Int8GemmPlan plan = fx::plan_int8_gemm(M, N, width, false);
   const Int8LinearParts p = int8_linear_parts(plan, M, N, K);
   if (!workspace || workspace_bytes < p.bytes)
     return fail(FX_EINVAL, "linear workspace needs %zu bytes, got %zu", p.bytes, workspace_bytes);
@@ -2262,25 +2278,13 @@ int fx_int8_linear(const void* x, long long x_stride, int x_dtype, const int8_t*
   char* base = static_cast<char*>(workspace);
   int8_t* codes = reinterpret_cast<int8_t*>(base);
   float* scales = reinterpret_cast<float*>(base + p.scales);
-  if (int rc = validate_half_rows("x", x, x_stride)) return rc;
-  fx::Int8GemmArgs g{};
-  if (int rc = prepare_int8_gemm(codes, p.width, scales, w, w_stride, w_scales, bias, out, out_stride, M, N, p.width,
+  if (int rc = prepare_int8_gemm(codes, width, scales, w, w_stride, w_scales, bias, out, out_stride, M, N, width,
                                  out_dtype, &g))
     return rc;
-  if (loose_rows(w, w_stride, N, p.width)) return fail(FX_EINVAL, "w must have rows of whole 16 bytes at 16-byte boundaries");
+  if (loose_rows(w, w_stride, N, width)) return fail(FX_EINVAL, "w must have rows of whole 16 bytes at 16-byte boundaries");
   if (plan.splits > 1) g.partial = reinterpret_cast<int*>(base + p.partial);
   g.k_per_split = plan.k_per_split;
-  if (fx::int8_linear_fuses(M, N, p.width)) {
-    fx::Int8RowsArgs rows{};
-    rows.x = static_cast<const uint16_t*>(x);
-    rows.x_stride = x_stride;
-    rows.rows = M;
-    rows.columns = K;
-    rows.code_columns = p.width;
-    fx::launch_int8_linear_few(x_dtype, rows, g, static_cast<hipStream_t>(stream));
-    return check_launch("fx_int8_linear");
-  }
-  if (int rc = fx_int8_quantize(x, x_stride, codes, p.width, scales, M, K, p.width, x_dtype, stream)) return rc;
+  if (int rc = fx_int8_quantize(x, x_stride, codes, width, scales, M, K, width, x_dtype, stream)) return rc;
   return run_int8_gemm(g, plan, stream);
 }
 

@@ -396,7 +396,7 @@ class PackedInt8Linear(PackedLinearBase):
         codes, scales, bias = self._tensor("codes"), self._tensor("scales"), self._tensor("bias")
         width, k, o = self._width, self.in_features, self.out_features
         nbytes = _linear_workspace_bytes(rows, o, k)
-        workspace = _new((nbytes,), torch.uint8, device)
+        workspace = _new((nbytes,), torch.uint8, device) if nbytes else None
         index = device.index
 
         def run(x2: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
@@ -404,7 +404,7 @@ class PackedInt8Linear(PackedLinearBase):
             added = bias if bias is None or bias.dtype == out.dtype else bias.to(out.dtype)
             _launch("fx_int8_linear", index, x2.data_ptr(), x2.stride(0), code, codes.data_ptr(), width,
                     scales.data_ptr(), None if added is None else added.data_ptr(), out.data_ptr(), o,
-                    workspace.data_ptr(), nbytes, rows, o, k, _CODES[out.dtype])
+                    workspace if workspace is None else workspace.data_ptr(), nbytes, rows, o, k, _CODES[out.dtype])
             return out
         return run
 
