@@ -21,27 +21,31 @@ __device__ __forceinline__ float load_value(const void* p, long long i) {
 
 typedef float f32x4v_t __attribute__((ext_vector_type(4)));
 
-// The scales of columns n .. n + 3 (0 past the last).
-__device__ __forceinline__ f32x4v_t column_scales(const Int8GemmArgs& g, int n) {
-  return __builtin_bit_cast(f32x4v_t, load_b128(buffer_resource(g.w_scales, size_t(g.N) * 4), n * 4, 0));
+// What the results of columns n .. n + 3 take besides their sums (scales 0 past the last).
+struct Columns4 {
+  f32x4v_t scales, bias;
+};
+__device__ __forceinline__ float bias_value(const Int8GemmArgs& g, int n) {
+  if (g.dt == kF32) return load_value<kF32>(g.bias, n);
+  return g.dt == kBF16 ? load_value<kBF16>(g.bias, n) : load_value<kF16>(g.bias, n);
 }
-template <int DT>
-__device__ __forceinline__ f32x4v_t column_bias(const Int8GemmArgs& g, int n) {
-  f32x4v_t b = {0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ Columns4 load_columns(const Int8GemmArgs& g, int n) {
+  Columns4 c{__builtin_bit_cast(f32x4v_t, load_b128(buffer_resource(g.w_scales, size_t(g.N) * 4), n * 4, 0)),
+             {0.f, 0.f, 0.f, 0.f}};
   if (g.bias)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) b[r] = load_value<DT>(g.bias, min(n + r, g.N - 1));
-  return b;
+    for (int r = 0; r < 4; ++r) c.bias[r] = bias_value(g, min(n + r, g.N - 1));
+  return c;
 }
 
 // Columns n .. n + 3 (those below N) of row m: one rounding of (acc a_scale) w_scale + bias in fp32.
 // (sa: the row's scale.)  acc's own float is rounded once beyond 2^24 (2^-24 of it).
 template <int DT>
-__device__ __forceinline__ void store4_as(const Int8GemmArgs& g, int m, int n, const i32x4_t& acc, float sa) {
-  const f32x4v_t ws = column_scales(g, n), bias = column_bias<DT>(g, n);
+__device__ __forceinline__ void store4_as(const Int8GemmArgs& g, int m, int n, const i32x4_t& acc, float sa,
+                                          const Columns4& c) {
   float y[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) y[r] = fmaf(float(acc[r]) * sa, ws[r], bias[r]);
+  for (int r = 0; r < 4; ++r) y[r] = fmaf(float(acc[r]) * sa, c.scales[r], c.bias[r]);
   const long long at = m * g.out_stride + n;
   if constexpr (DT == kF32) {
     float* out = static_cast<float*>(g.out) + at;
@@ -62,10 +66,11 @@ __device__ __forceinline__ void store4_as(const Int8GemmArgs& g, int m, int n, c
     }
   }
 }
-__device__ __forceinline__ void store4(const Int8GemmArgs& g, int m, int n, const i32x4_t& acc, float sa) {
-  if (g.dt == kBF16) store4_as<kBF16>(g, m, n, acc, sa);
-  else if (g.dt == kF16) store4_as<kF16>(g, m, n, acc, sa);
-  else store4_as<kF32>(g, m, n, acc, sa);
+__device__ __forceinline__ void store4(const Int8GemmArgs& g, int m, int n, const i32x4_t& acc, float sa,
+                                       const Columns4& c) {
+  if (g.dt == kBF16) store4_as<kBF16>(g, m, n, acc, sa, c);
+  else if (g.dt == kF16) store4_as<kF16>(g, m, n, acc, sa, c);
+  else store4_as<kF32>(g, m, n, acc, sa, c);
 }
 
 }  // namespace fx

@@ -15,6 +15,8 @@ __global__ __launch_bounds__(256) void int8_gemm_join_kernel(const Int8GemmArgs 
   const unsigned unit = blockIdx.x * 256u + threadIdx.x;
   const int m = int(unit / quads), n = int(unit - unsigned(m) * quads) * 4;
   if (m >= g.M) return;
+  const Columns4 columns = load_columns(g, n);
+  const float sa = g.a_scales[m];
   const size_t plane = size_t(g.M) * g.N;
   const int* p = g.partial + size_t(m) * g.N + n;
   i32x4_t total = {0, 0, 0, 0};
@@ -30,7 +32,7 @@ __global__ __launch_bounds__(256) void int8_gemm_join_kernel(const Int8GemmArgs 
       for (int r = 0; r < 4; ++r)
         if (n + r < g.N) total[r] += p[s * plane + r];
   }
-  store4(g, m, n, total, g.a_scales[m]);
+  store4(g, m, n, total, sa, columns);
 }
 
 // Rows at whatever address copied to whole 16 bytes at 16-byte boundaries, zeros behind them: those of

@@ -133,7 +133,8 @@ __global__ __launch_bounds__(W * 64) void int8_gemm_few_kernel(const Int8GemmArg
 #pragma unroll
     for (int v = 1; v < W; ++v) total += sums[v][tile][lane];
     const int m = (tile % MT) * 16 + r, n = n0 + (tile / MT) * 16 + (lane >> 4) * 4;
-    if (m < g.M && n < g.N) store4(g, m, n, total, kQuantize ? row_scales[m & 15] : g.a_scales[m]);
+    // (their scales loaded in front of the products: 4096 x 12288 12.3 us for 11.9)
+    if (m < g.M && n < g.N) store4(g, m, n, total, kQuantize ? row_scales[m & 15] : g.a_scales[m], load_columns(g, n));
   }
 }
 

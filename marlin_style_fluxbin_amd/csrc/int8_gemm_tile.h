@@ -16,13 +16,13 @@ __device__ __forceinline__ i32x16_t mfma_i8_32(const u32x4_t& a, const u32x4_t& 
   return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
 }
 
-// 16 bytes per lane from `resource` at the lane's offset to lds + 16 * lane, asynchronously
-// (vmcnt).  The instruction has no result register; written as the builtin, every later LDS
-// read of the kernel waits for it, whichever buffer it fills.
-__device__ __forceinline__ void fill_lds(const u32x4_t& resource, int offset, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset),
-               "s"(resource)
-               : "memory", "m0");
+// 16 bytes per lane from `resource` at the lane's offset and `column` to lds + at + 16 * lane,
+// asynchronously (vmcnt).  The instruction has no result register; written as the builtin, every later
+// LDS read of the kernel waits for it, whichever buffer it fills.
+__device__ __forceinline__ void fill_lds(const u32x4_t& resource, int offset, int column, unsigned lds, int at) {
+  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds" ::"s"(lds), "i"(at),
+               "v"(offset), "s"(resource), "s"(column)
+               : "memory", "m0", "scc");
 }
 
 template <int N>
@@ -43,9 +43,14 @@ __device__ __forceinline__ void tile_barrier() {
 // and more write a row's neighbours: written from the registers (8 bytes a lane and 32 rows at a time)
 // the results of a 256 x 256 tile took 20 us.
 // OUT: kBF16, kF16, kF32, or -1 for the sums of a K split.
+// (w_scales, bias, a_scales: those of this wave's columns and rows, in LDS)
+typedef const __attribute__((address_space(3))) float lds_float_t;
+struct TileScales {
+  lds_float_t *w_scales, *bias, *a_scales;
+};
 template <int OUT, int NT, int MT>
 __device__ __forceinline__ void tile_store_as(const Int8GemmArgs& g, const i32x16_t (&acc)[NT][MT], int m0, int n0,
-                                              int split, lds8_t* lds, int lane) {
+                                              int split, lds8_t* lds, int lane, const TileScales& scales) {
   constexpr int kSize = OUT == kBF16 || OUT == kF16 ? 2 : 4, kRow = NT * 32 * kSize + 16;
   constexpr int kLanes = NT * 32 * kSize / 16, kPass = 64 / kLanes;  // lanes of a row, rows of a wave store
   const int half = lane >> 5, low = lane & 31;
@@ -55,15 +60,15 @@ __device__ __forceinline__ void tile_store_as(const Int8GemmArgs& g, const i32x1
   if constexpr (OUT >= 0) {
 #pragma unroll
     for (int q = 0; q < NT * 4; ++q) {
-      const int n = n0 + q * 8 + half * 4;
-      ws[q] = column_scales(g, n);
-      bias[q] = column_bias<OUT>(g, n);
+      typedef const __attribute__((address_space(3))) f32x4v_t* lds128_t;
+      ws[q] = *reinterpret_cast<lds128_t>(scales.w_scales + q * 8 + half * 4);
+      bias[q] = *reinterpret_cast<lds128_t>(scales.bias + q * 8 + half * 4);
     }
   }
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
     const int m = m0 + j * 32;
-    const float sa = OUT < 0 ? 0.f : g.a_scales[min(m + low, g.M - 1)];
+    const float sa = OUT < 0 ? 0.f : scales.a_scales[j * 32 + low];
     wave_lds_order();
 #pragma unroll
     for (int q = 0; q < NT * 4; ++q) {
@@ -110,11 +115,11 @@ __device__ __forceinline__ void tile_store_as(const Int8GemmArgs& g, const i32x1
 }
 template <int NT, int MT>
 __device__ __forceinline__ void tile_store(const Int8GemmArgs& g, const i32x16_t (&acc)[NT][MT], int m0, int n0,
-                                           int split, lds8_t* lds, int lane) {
-  if (g.partial) tile_store_as<-1>(g, acc, m0, n0, split, lds, lane);
-  else if (g.dt == kBF16) tile_store_as<kBF16>(g, acc, m0, n0, split, lds, lane);
-  else if (g.dt == kF16) tile_store_as<kF16>(g, acc, m0, n0, split, lds, lane);
-  else tile_store_as<kF32>(g, acc, m0, n0, split, lds, lane);
+                                           int split, lds8_t* lds, int lane, const TileScales& scales) {
+  if (g.partial) tile_store_as<-1>(g, acc, m0, n0, split, lds, lane, scales);
+  else if (g.dt == kBF16) tile_store_as<kBF16>(g, acc, m0, n0, split, lds, lane, scales);
+  else if (g.dt == kF16) tile_store_as<kF16>(g, acc, m0, n0, split, lds, lane, scales);
+  else tile_store_as<kF32>(g, acc, m0, n0, split, lds, lane, scales);
 }
 constexpr int tile_store_bytes(int NT) { return 32 * (NT * 32 * 4 + 16); }  // of LDS, a wave
 
@@ -139,6 +144,7 @@ __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8G
   static_assert(BN % (2 * kRows * kWaves) == 0 && BM % (2 * kRows * kWaves) == 0 && S >= 2, "waves share a stage's loads evenly");
   constexpr int kResults = kWaves * tile_store_bytes(NT);
   __shared__ __attribute__((aligned(1024))) char ring[S * kStage > kResults ? S * kStage : kResults];
+  __shared__ __attribute__((aligned(16))) float side[2 * BN + BM];  // scales of the columns, their bias, scales of the rows
   const int lane = threadIdx.x & 63, wave = wave_index();
   const unsigned lds0 = unsigned(size_t((lds8_t*)ring));
 
@@ -154,6 +160,16 @@ __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8G
   const int k_begin = split * g.k_per_split, k_end = min(g.K, k_begin + g.k_per_split);
   const int stages = (k_end - k_begin + kTileK - 1) / kTileK;
 
+  // Scales and bias, on the way during the products (loaded behind them 0.3 us more a workgroup).
+  static_assert(WM * WN * 64 >= BN && WM * WN * 64 >= BM, "a thread has one of each");
+  const int thread = threadIdx.x;
+  float w_scale = 0.f, bias = 0.f, a_scale = 0.f;
+  if (!g.partial) {
+    w_scale = thread < BN ? g.w_scales[min(n0 + thread, g.N - 1)] : 0.f;
+    a_scale = thread < BM ? g.a_scales[min(m0 + thread, g.M - 1)] : 0.f;
+    if (g.bias && thread < BN) bias = bias_value(g, min(n0 + thread, g.N - 1));
+  }
+
   // This wave's loads: kRows rows of kTileK bytes each, lane l bytes 16 c .. of row l / kPlaces, where it
   // fills place l % kPlaces: c is that place with swizzle(row) applied, so that 16 lanes that read one c
   // of 16 rows in a row meet 16 places of 16 bytes within 256 bytes (64 banks).
@@ -168,42 +184,34 @@ __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8G
   for (int i = 0; i < PA; ++i) a_off[i] = (i * kRows + lane / kPlaces) * a_stride + chunk[i & 1];
   const int w_row = n0 + wave * (PW * kRows), a_row = m0 + wave * (PA * kRows);
   const int w_left = min(PW * kRows, g.N - w_row), a_left = min(PA * kRows, g.M - a_row);
-  const size_t w_base = reinterpret_cast<size_t>(g.w) + w_row * g.w_stride + k_begin;
-  const size_t a_base = reinterpret_cast<size_t>(g.a) + a_row * g.a_stride + k_begin;
   const int columns = k_end - k_begin;
-  const int w_bytes = w_left > 0 ? (w_left - 1) * w_stride + columns : 0;
-  const int a_bytes = a_left > 0 ? (a_left - 1) * a_stride + columns : 0;
+  // (rows past the last lie past these ranges: no access, zeros)
+  const auto range = [&](const int8_t* p, long long stride, int row, int rows) {
+    const size_t at = reinterpret_cast<size_t>(p) + row * stride + k_begin;
+    return u32x4_t{unsigned(at), unsigned(at >> 32) & 0xffffu, rows > 0 ? unsigned((rows - 1) * int(stride) + columns) : 0u,
+                   0x00020000u};
+  };
+  const u32x4_t rw = range(g.w, g.w_stride, w_row, w_left), ra = range(g.a, g.a_stride, a_row, a_left);
+  const unsigned w_dst = lds0 + wave * (PW * 1024), a_dst = lds0 + BN * kTileK + wave * (PA * 1024);
   // The XCDs begin at different columns: they read the same rows at different times, and rows of a
   // power of two apart meet more of the memory's channels at any one (5% of the time in tiles of 256,
   // 11 to 17% in the others at 12288 columns and at 48 rows).
-  int issued = 0, next = int(blockIdx.x % kXcdCount) * stages / kXcdCount, slot = 0;  // stages
-  auto issue = [&]() __attribute__((always_inline)) {
-    const int k = next * kTileK, left = issued < stages ? columns - k : 0;
-    const unsigned w_dst = lds0 + unsigned(slot) * kStage + wave * (PW * 1024);
-    const unsigned a_dst = lds0 + unsigned(slot) * kStage + BN * kTileK + wave * (PA * 1024);
-    const size_t wp = w_base + k, ap = a_base + k;
-    // (past the last stage, and for rows past the last: no access, zeros)
-    const u32x4_t rw = {unsigned(wp), unsigned(wp >> 32) & 0xffffu, left > 0 ? unsigned(max(w_bytes - k, 0)) : 0u, 0x00020000u};
-    const u32x4_t ra = {unsigned(ap), unsigned(ap >> 32) & 0xffffu, left > 0 ? unsigned(max(a_bytes - k, 0)) : 0u, 0x00020000u};
-    if (left >= kTileK || left <= 0) {
+  int unissued = stages, column = int(blockIdx.x % kXcdCount) * stages / kXcdCount * kTileK;
+  auto issue = [&](int slot) __attribute__((always_inline)) {
+    // (the columns behind the last, and past the last stage: no access, zeros)
+    const int left = columns - column, there = unissued > 0 ? left : 0;
 #pragma unroll
-      for (int i = 0; i < PW; ++i) fill_lds(rw, w_off[i], w_dst + i * 1024);
+    for (int i = 0; i < PW; ++i)
+      fill_lds(rw, chunk[i & 1] < there ? w_off[i] : kOutOfRange, column, w_dst, slot * kStage + i * 1024);
 #pragma unroll
-      for (int i = 0; i < PA; ++i) fill_lds(ra, a_off[i], a_dst + i * 1024);
-    } else {  // the last columns, not a whole stage of them
-#pragma unroll
-      for (int i = 0; i < PW; ++i) fill_lds(rw, chunk[i & 1] < left ? w_off[i] : kOutOfRange, w_dst + i * 1024);
-#pragma unroll
-      for (int i = 0; i < PA; ++i) fill_lds(ra, chunk[i & 1] < left ? a_off[i] : kOutOfRange, a_dst + i * 1024);
-    }
-    ++issued;
-    next = next + 1 == stages ? 0 : next + 1;
-    slot = slot + 1 == S ? 0 : slot + 1;
+    for (int i = 0; i < PA; ++i)
+      fill_lds(ra, chunk[i & 1] < there ? a_off[i] : kOutOfRange, column, a_dst, slot * kStage + i * 1024);
+    --unissued;
+    column = left <= kTileK ? 0 : column + kTileK;
   };
 
   const int wm = wave / WN, wn = wave % WN;
-  const char* w_at = ring + (wn * TN + (lane & 31)) * kTileK;
-  const char* a_at = ring + (BN + wm * TM + (lane & 31)) * kTileK;
+  const int w_at = int(lds0) + (wn * TN + (lane & 31)) * kTileK, a_at = int(lds0) + (BN + wm * TM + (lane & 31)) * kTileK;
   const int place = ((lane >> 5) ^ swizzle(lane & 31)) * 16;
 
   i32x16_t acc[NT][MT];
@@ -214,12 +222,13 @@ __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8G
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
   u32x4_t w[2][NT], a[2][MT];
-  auto read = [&](int h, int step, int stage) __attribute__((always_inline)) {
-    const int at = stage * kStage + (place ^ (step * 32));
+  auto read = [&](int h, int step, int slot) __attribute__((always_inline)) {
+    typedef const __attribute__((address_space(3))) u32x4_t* lds128_t;
+    const int at = place ^ (step * 32), stage = slot * kStage;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) w[h][i] = *reinterpret_cast<const u32x4_t*>(w_at + at + i * 32 * kTileK);
+    for (int i = 0; i < NT; ++i) w[h][i] = *reinterpret_cast<lds128_t>(w_at + at + (stage + i * 32 * kTileK));
 #pragma unroll
-    for (int j = 0; j < MT; ++j) a[h][j] = *reinterpret_cast<const u32x4_t*>(a_at + at + j * 32 * kTileK);
+    for (int j = 0; j < MT; ++j) a[h][j] = *reinterpret_cast<lds128_t>(a_at + at + (stage + j * 32 * kTileK));
     // (the compiler otherwise reads a step's operands just in front of its products)
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -232,31 +241,39 @@ __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8G
   };
 
 #pragma unroll
-  for (int s = 0; s < S; ++s) issue();
+  for (int s = 0; s < S; ++s) issue(s);
   tile_wait<(S - 1) * P>();
   tile_barrier();
   read(0, 0, 0);
-  int here = 0;
-  for (int s = 0; s < stages; ++s) {
+  for (int s = 0; s < stages;) {
 #pragma unroll
-    for (int t = 0; t < kSteps; ++t) {
-      if (t < kSteps - 1) {
-        read((t + 1) & 1, t + 1, here);
-      } else {
-        // stage s is in every wave's registers, and stage s + 1 is there
-        tile_wait<(S - 2) * P>();
-        tile_barrier();
-        issue();
-        here = here + 1 == S ? 0 : here + 1;
-        read(0, 0, here);
+    for (int slot = 0; slot < S; ++slot) {
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) {
+        if (t < kSteps - 1) {
+          read((t + 1) & 1, t + 1, slot);
+        } else {
+          // this stage is in every wave's registers, and the next one is there
+          tile_wait<(S - 2) * P>();
+          tile_barrier();
+          read(0, 0, (slot + 1) % S);
+        }
+        multiply(t & 1);
       }
-      multiply(t & 1);
+      issue(slot);
+      if (++s == stages) break;
     }
   }
+  if (thread < BN) {
+    side[thread] = w_scale;
+    side[BN + thread] = bias;
+  }
+  if (thread < BM) side[2 * BN + thread] = a_scale;
   tile_wait<0>();  // nothing fills this workgroup's LDS after its last wave has left
-
   tile_barrier();  // nor does a wave read it any more
-  tile_store(g, acc, m0 + wm * TM, n0 + wn * TN, split, (lds8_t*)ring + wave * tile_store_bytes(NT), lane);
+  lds_float_t* at = (lds_float_t*)side;
+  tile_store(g, acc, m0 + wm * TM, n0 + wn * TN, split, (lds8_t*)ring + wave * tile_store_bytes(NT), lane,
+             TileScales{at + wn * TN, at + BN + wn * TN, at + 2 * BN + wm * TM});
 }
 
 }  // namespace fx
