@@ -61,23 +61,23 @@ int few_columns(int M, int N) { return M > 16 && N > 4096 ? 32 : 16; }
 
 // Which kernel, and how many workgroups along K, by an estimate of the time (us).  Few rows: rounds of
 // workgroups on a compute unit, each its rows of the weight (and some of the activations' from L2) at
-// 25.5 bytes a ns, whether the other units are at work or not.  Tiles: rounds of workgroups, each its
+// 25.4 bytes a ns, whether the other units are at work or not.  Tiles: rounds of workgroups, each its
 // stages of 128 columns at what a stage takes, and the operands' bytes, of which the shorter hides but
 // in part; for splits the join's launch and the partial sums written and read.  Fitted to 408 sizes (1
 // to 4096 rows, 24 shapes of weights) timed with every tile and 1 to 16 splits: within 5% of the best
-// measured choice at 402 of them (fitted to half of the weights, at 195 of the other 204).
+// measured choice at 386 of them (fitted to half of the weights, at 188 of the other 204).
 Int8GemmPlan plan_int8_gemm(int M, int N, int K, bool any) {
   if (any && M <= kFewRows) return {kInt8Few, 1, K};
   const int stages = (K + 127) / 128;
-  const float bytes = (float(M) + N) * K / 6.3e6f;
+  const float bytes = (float(M) + N) * K / 6.9e6f;
   Int8GemmPlan best{kInt8Few, 1, K};
   float least = 1e30f;
   if (M <= kFewRows) {
     const int columns = few_columns(M, N), rounds = N / (columns * 256) + (N % (columns * 256) != 0);
-    least = 3.1f + rounds * (0.5f + K * (columns + 0.62f * M) / 25500.f);
+    least = 2.54f + rounds * (0.71f + K * (columns + 0.64f * M) / 25400.f);
   }
-  // (32 rows fill half of the smallest tile; the plan itself is then 0.2 us of a call, and 0.7 of a search)
-  for (int tile = 0; tile < (M <= kFewRows ? 1 : kInt8Tiles); ++tile) {
+  // (32 rows fill half of the smallest tiles; the plan itself is then 0.2 us of a call, and 0.7 of a search)
+  for (int tile = 0; tile < (M <= kFewRows ? 2 : kInt8Tiles); ++tile) {
     const Int8Tile& t = kInt8Tile[tile];
     const long tiles = long((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn), slots = 256 * t.places;
     for (int splits = 1; splits <= std::min(stages, kMaxSplits); ++splits) {
@@ -86,12 +86,12 @@ Int8GemmPlan plan_int8_gemm(int M, int N, int K, bool any) {
       if ((stages + per - 1) / per != splits) continue;  // a last split would be empty
       const long groups = tiles * splits, rounds = (groups + slots - 1) / slots;
       const float last = float(groups - (rounds - 1) * slots) / float(slots);
-      // (a second workgroup on some compute unit already costs most of what one on each does)
-      const float filled = last <= 0.5f ? 0.f : t.places > 1 ? 0.4f + 0.6f * last : 2.f * last - 1.f;
+      // (a second workgroup on some compute unit already costs what one on each does)
+      const float filled = last <= 0.5f ? 0.f : t.places > 1 ? 1.f : 2.f * last - 1.f;
       const float stage = (rounds - 1) * t.full + t.half + (t.full - t.half) * filled;
       const float work = per * stage + rounds * t.ends;
-      float time = 1.6f + std::max(work, bytes) + 0.36f * std::min(work, bytes);
-      if (splits > 1) time += 2.8f + 0.2f * splits + 2.f * splits * float(M) * N * 4.f / 8.3e6f;
+      float time = 1.5f + std::max(work, bytes) + 0.56f * std::min(work, bytes);
+      if (splits > 1) time += 1.83f + 0.27f * splits + 2.f * splits * float(M) * N * 4.f / 6.5e6f;
       if (time < least) least = time, best = {tile, splits, splits == 1 ? K : per * 128};
     }
   }

@@ -5,6 +5,7 @@
 namespace fx {
 
 void launch_int8_tile_64(const Int8GemmArgs& g, unsigned groups, hipStream_t s);
+void launch_int8_tile_64x128(const Int8GemmArgs& g, unsigned groups, hipStream_t s);
 void launch_int8_tile_128(const Int8GemmArgs& g, unsigned groups, hipStream_t s);
 void launch_int8_tile_128x256(const Int8GemmArgs& g, unsigned groups, hipStream_t s);
 void launch_int8_tile_256(const Int8GemmArgs& g, unsigned groups, hipStream_t s);
@@ -17,13 +18,15 @@ struct Int8Tile {
   float half, full, ends;
   void (*launch)(const Int8GemmArgs& g, unsigned groups, hipStream_t s);
 };
-// (of 2048 x 4096 x 4096 the four take 63, 43.7, 37.6 and 45.5 us; of 1024 x 4096 x 4096 34, 22.6, 32 and 44;
-// 128 x 128 tiles with two stages, two workgroups a compute unit: 39.4 and 25.7)
+// (of 300 x 4096 x 4096 the five take 13.9, 12.7, 15.0, 23.5 and 40.8 us, of 1024 x 4096 x 4096 28.8, 23.6, 21.4,
+// 25.5 and 42.1, of 2048 x 4096 x 4096 54.8, 44.8, 42.2, 35.6 and 42.4; 128 x 128 with two stages, two
+// workgroups a compute unit, 22.3, 24.3 and 36.7)
 constexpr Int8Tile kInt8Tile[] = {
-    {64, 64, 2, 0.24f, 0.475f, 1.45f, launch_int8_tile_64},
-    {128, 128, 1, 0.44f, 0.58f, 3.f, launch_int8_tile_128},
-    {128, 256, 1, 0.755f, 0.9f, 3.95f, launch_int8_tile_128x256},
-    {256, 256, 1, 1.335f, 1.57f, 5.3f, launch_int8_tile_256},
+    {64, 64, 2, 0.198f, 0.407f, 1.58f, launch_int8_tile_64},
+    {64, 128, 2, 0.325f, 0.657f, 2.01f, launch_int8_tile_64x128},
+    {128, 128, 1, 0.397f, 0.44f, 2.81f, launch_int8_tile_128},
+    {128, 256, 1, 0.697f, 0.697f, 3.42f, launch_int8_tile_128x256},
+    {256, 256, 1, 1.32f, 1.42f, 3.82f, launch_int8_tile_256},
 };
 constexpr int kInt8Tiles = sizeof(kInt8Tile) / sizeof(kInt8Tile[0]);
 
