@@ -182,16 +182,18 @@ __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8G
   for (int i = 0; i < PW; ++i) w_off[i] = (i * kRows + lane / kPlaces) * w_stride + chunk[i & 1];
 #pragma unroll
   for (int i = 0; i < PA; ++i) a_off[i] = (i * kRows + lane / kPlaces) * a_stride + chunk[i & 1];
-  const int w_row = n0 + wave * (PW * kRows), a_row = m0 + wave * (PA * kRows);
-  const int w_left = min(PW * kRows, g.N - w_row), a_left = min(PA * kRows, g.M - a_row);
   const int columns = k_end - k_begin;
-  // (rows past the last lie past these ranges: no access, zeros)
-  const auto range = [&](const int8_t* p, long long stride, int row, int rows) {
+  // A wave's range ends with the last of its rows that there are: no access behind it, zeros.  A wave
+  // without any has the matrix's last row, so that every range holds more bytes than `column` below: a
+  // lane within `chunk < there` is in bounds, and one behind the rows is not, whether the range check
+  // counts `column` or not.
+  const auto range = [&](const int8_t* p, long long stride, int first, int rows, int all) {
+    const int row = min(first, all - 1), there = min(rows, all - row);
     const size_t at = reinterpret_cast<size_t>(p) + row * stride + k_begin;
-    return u32x4_t{unsigned(at), unsigned(at >> 32) & 0xffffu, rows > 0 ? unsigned((rows - 1) * int(stride) + columns) : 0u,
-                   0x00020000u};
+    return u32x4_t{unsigned(at), unsigned(at >> 32) & 0xffffu, unsigned((there - 1) * int(stride) + columns), 0x00020000u};
   };
-  const u32x4_t rw = range(g.w, g.w_stride, w_row, w_left), ra = range(g.a, g.a_stride, a_row, a_left);
+  const u32x4_t rw = range(g.w, g.w_stride, n0 + wave * (PW * kRows), PW * kRows, g.N);
+  const u32x4_t ra = range(g.a, g.a_stride, m0 + wave * (PA * kRows), PA * kRows, g.M);
   const unsigned w_dst = lds0 + wave * (PW * 1024), a_dst = lds0 + BN * kTileK + wave * (PA * 1024);
   // The XCDs begin at different columns: they read the same rows at different times, and rows of a
   // power of two apart meet more of the memory's channels at any one (5% of the time in tiles of 256,
