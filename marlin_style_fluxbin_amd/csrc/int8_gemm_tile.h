@@ -98,8 +98,8 @@ __device__ __forceinline__ void tile_store_as(const Int8GemmArgs& g, const i32x1
       const u32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(lds + row * kRow + col * kSize);
       char* to = out + ((m + row) * stride + n0 + col) * kSize;
       if (left >= kEach) {
-        // at whatever address the row begins (301 x 1001 x 2000 8.8 us, element by element 10.6); a result is
-        // not read again here (8192 x 12288 x 4096 356 us, with plain stores 371)
+        // at whatever address the row begins (301 x 1001 x 2000: element by element 1.8 us more); a result is
+        // not read again here (8192 x 12288 x 4096 4% faster than with plain stores)
         if constexpr (OUT < 0) __builtin_memcpy(to, &v, 16);
         else __builtin_nontemporal_store(v, reinterpret_cast<any16_t*>(to));
       } else {
@@ -131,11 +131,14 @@ constexpr int kTileK = 128;
 // products of the step before, one barrier a stage: behind it the stage that every wave has read makes
 // room for the load of the one S ahead.
 //
-// What bounds it: of 8192 x 12288 x 4096 (256 x 256, 356 us, 2.3e15 operations a second; the library's
+// What bounds it: of 8192 x 12288 x 4096 (256 x 256, 336 us, 2.4e15 operations a second; the library's
 // int8 product takes 385) the matrix cores are busy 60% of the clocks, at 1.9 GHz, where the chip's
 // power holds it (2.5 GHz with operands of zeros).  Without its loads 74%; with a third place in the
 // ring for one operand 1% faster; with the next tile's first stages under a tile's results slower
-// (registers).  Reads of LDS: 24% of the clocks, no bank conflicts.
+// (registers).  Reads of LDS: 26% of the clocks, conflicts 5% of these.  With one wave a SIMD (64 x 64)
+// a stage's time is its instructions, 4 clocks each: places in the ring are constants, and a scalar
+// offset is all that a load adds up (64 x 4096 x 4096 8.7 us, with descriptors and places formed in
+// every stage 10.8).
 template <int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(WM* WN * 64) void int8_gemm_tile_kernel(const Int8GemmArgs g) {
   constexpr int kWaves = WM * WN, TM = BM / WM, TN = BN / WN, MT = TM / 32, NT = TN / 32;

@@ -49,11 +49,12 @@ def test_larger_products(gpu, m, n, k):
 
 
 # every kernel, whole and in K splits (few rows: 16 and 32 rows by 16 and 32 columns, eight and sixteen
-# waves; tiles of 64, 128, 128 x 256 and 256), its last stage not whole
+# waves; tiles of 64, 64 x 128, 128, 128 x 256 and 256), its last stage not whole
 @pytest.mark.parametrize("m,n,k", [(16, 1000, 528), (9, 1000, 8208), (17, 17, 528), (17, 4097, 1040), (31, 8200, 1040),
                                    (200, 100, 48), (16, 6001, 4112), (90, 17, 12304), (200, 8200, 48), (1300, 1000, 8208),
                                    (90, 4097, 8208), (2050, 2049, 48), (260, 8200, 12304), (130, 6001, 8208),
-                                   (1300, 6001, 48), (130, 8200, 16400)])
+                                   (1300, 6001, 48), (130, 8200, 16400), (9, 3001, 8208), (200, 8200, 528),
+                                   (260, 4097, 8208), (390, 8200, 12304)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_every_kernel_and_split(gpu, m, n, k, dtype):
     args, b = case(m, n, k, gpu, dtype, True, seed=11)
