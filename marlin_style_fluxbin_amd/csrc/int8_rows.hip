@@ -36,7 +36,8 @@ void launch_rows(const Int8RowsArgs& a, hipStream_t s) {
   // The fewest threads whose registers hold the row, eight columns a thread and chunk; wider ones have up
   // to four chunks rather than more threads, whose reductions cost more (norm of 8192 rows: 1024 columns
   // 14.2 us, with 256 threads 18.8; 8192 columns 85, with 1024 threads 91; 12288 columns 127 and 175,
-  // 16384 columns 168 and 206; one row of 12288 5.1 and 5.8).
+  // 16384 columns 168 and 206; one row of 12288 5.1 and 5.8; SwiGLU of 8192 x 6144 38 us, with 512
+  // threads 46).
   if (width <= 512) go(int8_rows_kernel<DT, MODE, 64, 1>, 256, 4);
   else if (width <= 1024) go(int8_rows_kernel<DT, MODE, 64, 2>, 256, 4);
   else if (width <= 2048) go(int8_rows_kernel<DT, MODE, 256, 1>, 256, 1);
@@ -45,6 +46,7 @@ void launch_rows(const Int8RowsArgs& a, hipStream_t s) {
     if (a.rows <= 256) go(int8_rows_kernel<DT, MODE, 512, 1>, 512, 1);
     else go(int8_rows_kernel<DT, MODE, 256, 2>, 256, 1);
   }
+  else if (width <= 6144) go(int8_rows_kernel<DT, MODE, 256, 3>, 256, 1);
   else if (width <= 8192) go(int8_rows_kernel<DT, MODE, 512, 2>, 512, 1);
   else if (width <= 12288) go(int8_rows_kernel<DT, MODE, 512, 3>, 512, 1);
   else if (width <= 16384) go(int8_rows_kernel<DT, MODE, 512, 4>, 512, 1);

@@ -18,9 +18,10 @@ from tests.int8_reference import HALVES, held, norm_rows, swiglu_rows
 pytestmark = pytest.mark.gpu
 
 EPS = 1e-6
-# around every kernel's width: 512, 1024, 2048, 4096, 8192, 12288, 16384, and beyond
+# around every kernel's width: 512, 1024, 2048, 4096, 6144, 8192, 12288, 16384, and beyond
 SHAPES = [(1, 1), (3, 7), (5, 8), (2, 63), (9, 512), (4, 513), (7, 1000), (5, 1024), (3, 1032), (2, 2047), (3, 2049),
-          (4, 4096), (2, 4104), (3, 8192), (2, 8200), (300, 4090), (2, 12288), (2, 12296), (2, 16384), (2, 16392), (1, 40000)]
+          (4, 4096), (2, 4104), (2, 6144), (3, 6152), (3, 8192), (2, 8200), (300, 4090), (2, 12288), (2, 12296), (2, 16384),
+          (2, 16392), (1, 40000)]
 
 
 def states(rows, columns, dtype, gpu, seed=0):
