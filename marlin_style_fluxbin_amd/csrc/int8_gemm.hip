@@ -61,20 +61,20 @@ int few_columns(int M, int N) { return M > 16 && N > 4096 ? 32 : 16; }
 
 // Which kernel, and how many workgroups along K, by an estimate of the time (us).  Few rows: rounds of
 // workgroups on a compute unit, each its rows of the weight (and some of the activations' from L2) at
-// 25.4 bytes a ns, whether the other units are at work or not.  Tiles: rounds of workgroups, each its
+// 26 bytes a ns, whether the other units are at work or not.  Tiles: rounds of workgroups, each its
 // stages of 128 columns at what a stage takes, and the operands' bytes, of which the shorter hides but
 // in part; for splits the join's launch and the partial sums written and read.  Fitted to 408 sizes (1
 // to 4096 rows, 24 shapes of weights) timed with every tile and 1 to 16 splits: within 5% of the best
-// measured choice at 386 of them (fitted to half of the weights, at 188 of the other 204).
+// measured choice at 386 of them (fitted to half of the weights, at 195 of the other 204).
 Int8GemmPlan plan_int8_gemm(int M, int N, int K, bool any) {
   if (any && M <= kFewRows) return {kInt8Few, 1, K};
   const int stages = (K + 127) / 128;
-  const float bytes = (float(M) + N) * K / 6.9e6f;
+  const float bytes = (float(M) + N) * K / 7.4e6f;
   Int8GemmPlan best{kInt8Few, 1, K};
   float least = 1e30f;
   if (M <= kFewRows) {
     const int columns = few_columns(M, N), rounds = N / (columns * 256) + (N % (columns * 256) != 0);
-    least = 2.54f + rounds * (0.71f + K * (columns + 0.64f * M) / 25400.f);
+    least = 2.08f + rounds * (0.345f + K * (columns + 0.78f * M) / 26100.f);
   }
   // (32 rows fill half of the smallest tiles; the plan itself is then 0.2 us of a call, and 0.7 of a search)
   for (int tile = 0; tile < (M <= kFewRows ? 2 : kInt8Tiles); ++tile) {
@@ -90,42 +90,51 @@ Int8GemmPlan plan_int8_gemm(int M, int N, int K, bool any) {
       const float filled = last <= 0.5f ? 0.f : t.places > 1 ? 1.f : 2.f * last - 1.f;
       const float stage = (rounds - 1) * t.full + t.half + (t.full - t.half) * filled;
       const float work = per * stage + rounds * t.ends;
-      float time = 1.5f + std::max(work, bytes) + 0.56f * std::min(work, bytes);
-      if (splits > 1) time += 1.83f + 0.27f * splits + 2.f * splits * float(M) * N * 4.f / 6.5e6f;
+      float time = 1.25f + std::max(work, bytes) + 0.695f * std::min(work, bytes);
+      if (splits > 1) time += 1.73f + 0.3f * splits + 2.f * splits * float(M) * N * 4.f / 7.6e6f;
       if (time < least) least = time, best = {tile, splits, splits == 1 ? K : per * 128};
     }
   }
   return best;
 }
 
-template <int XDT, bool ANY>
+// A wave's pieces of 128 columns in flight: two, eight waves of them (2048 columns), so that few loads run
+// past the last column; four where one pass of them is all (one row by 24576 x 4096 19.7 us, with two 20.1;
+// by 5120 x 5120 12.2 and 10.9).  Sixteen waves where passes of 4096 columns come out even (one row by
+// 4096 x 12288 11.9 us, with eight 12.4; by 4096 x 14336 13.7 and 13.1).
+template <int XDT, bool ANY, int MT, int RT>
 void launch_few(const Int8GemmArgs& g, const Int8RowsArgs& rows, hipStream_t s) {
-  const dim3 grid(unsigned(g.N + 15) / 16);
-  // long rows: more of them in flight (4096 x 12288 11.8 us, with eight waves 12.5; 24576 x 4096 20.4 and 19.7)
-  if (g.K > 8192) hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, ANY, 1, 1, 16, 2>), grid, dim3(1024), 0, s, g, rows);
-  else hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, ANY, 1, 1, 8, 4>), grid, dim3(512), 0, s, g, rows);
+  const dim3 grid(unsigned(g.N + 16 * RT - 1) / (16 * RT));
+  if constexpr (MT == 1) {
+    const int past = -g.K & 4095;
+    if (g.K > 8192 && (XDT >= 0 || past <= g.K / 16)) {  // (rows quantized here: at most 16 columns a thread)
+      hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, ANY, 1, 1, 16, 2>), grid, dim3(1024), 0, s, g, rows);
+      return;
+    }
+  }
+  if (g.K > 3584 && g.K <= 4096) hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, ANY, MT, RT, 8, 4>), grid, dim3(512), 0, s, g, rows);
+  else hipLaunchKernelGGL((int8_gemm_few_kernel<XDT, ANY, MT, RT, 8, 2>), grid, dim3(512), 0, s, g, rows);
 }
 
 template <bool ANY>
 void launch_few_rows(const Int8GemmArgs& g, hipStream_t s) {
-  const int columns = few_columns(g.M, g.N);
-  const dim3 grid(unsigned(g.N + columns - 1) / columns);
-  if (g.M <= 16) launch_few<-1, ANY>(g, {}, s);
-  else if (columns == 16) hipLaunchKernelGGL((int8_gemm_few_kernel<-1, ANY, 2, 1, 8, 4>), grid, dim3(512), 0, s, g, Int8RowsArgs{});
-  else hipLaunchKernelGGL((int8_gemm_few_kernel<-1, ANY, 2, 2, 8, 4>), grid, dim3(512), 0, s, g, Int8RowsArgs{});
+  if (g.M <= 16) launch_few<-1, ANY, 1, 1>(g, {}, s);
+  else if (few_columns(g.M, g.N) == 16) launch_few<-1, ANY, 2, 1>(g, {}, s);
+  else launch_few<-1, ANY, 2, 2>(g, {}, s);
 }
 
 // Every workgroup quantizes the rows again, 1.5 us for each and each round of workgroups, where codes
-// from a launch of their own cost 2 to 3 us (one row by 4096 x 4096 7.1 us for 8.3, by 12288 x 1536 10.6
-// for 10.7, by 24576 x 4096 24.3 for 22.8; two rows by 1024 x 2000 6.7 for 7.0, by 4096 x 4096 8.9 for
-// 8.6 and a launch less for the host, by 9728 x 896 11.4 for 9.8; four by 1024 x 2000 9.8 for 7.2).
+// from a launch of their own cost 2 to 3 us (one row by 4096 x 4096 7.5 us for 8.5, by 1024 x 2000 5.2
+// for 6.4, by 12288 x 1536 9.7 for 9.9, by 24576 x 4096 24.3 for 22.8; two rows by 1024 x 2000 6.7 for
+// 6.7 and by 4096 x 4096 8.7 for 8.4, and a launch less for the host, by 9728 x 896 11.4 for 9.8; four by
+// 1024 x 2000 9.8 for 7.2).
 bool int8_linear_fuses(int M, int N, int K) {
   return M <= 2 && long(M) * N <= 12288 && long(M) * K <= kFewCodes;
 }
 
 void launch_int8_linear_few(int x_dt, const Int8RowsArgs& rows, const Int8GemmArgs& g, hipStream_t s) {
-  if (x_dt == kBF16) launch_few<kBF16, false>(g, rows, s);
-  else launch_few<kF16, false>(g, rows, s);
+  if (x_dt == kBF16) launch_few<kBF16, false, 1, 1>(g, rows, s);
+  else launch_few<kF16, false, 1, 1>(g, rows, s);
 }
 
 bool launch_int8_gemm(const Int8GemmPlan& plan, const Int8GemmArgs& g, hipStream_t s) {

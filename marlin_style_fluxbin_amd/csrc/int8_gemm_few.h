@@ -24,7 +24,7 @@ __device__ __forceinline__ u32x4_t part_b128(const int8_t* p, int n) {
 // RT x 16 rows of the weight by MT x 16 of the activations a workgroup, its W waves dealing the
 // columns in pieces of 128: a wave's sums are over its own columns and are added through LDS, so that
 // one launch has a burst of the whole weight in flight.  Bound by the weight's bytes (24576 x 4096 at
-// one row 19.7 us, 5.1 TB/s; 4096 x 4096 5.1 us, of which a launch is 4): every wave issues UN pieces'
+// one row 19.7 us, 5.1 TB/s; 4096 x 4096 5.4 us, of which a launch is 2): every wave issues UN pieces'
 // loads in front of its first product (left to the compiler's order, 20.4).
 //
 // ANY: rows of any length at any address (elsewhere they begin at 16-byte boundaries and are whole 16

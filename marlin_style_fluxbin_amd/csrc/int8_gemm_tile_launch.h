@@ -22,11 +22,11 @@ struct Int8Tile {
 // 25.5 and 42.1, of 2048 x 4096 x 4096 54.8, 44.8, 42.2, 35.6 and 42.4; 128 x 128 with two stages, two
 // workgroups a compute unit, 22.3, 24.3 and 36.7)
 constexpr Int8Tile kInt8Tile[] = {
-    {64, 64, 2, 0.198f, 0.407f, 1.58f, launch_int8_tile_64},
-    {64, 128, 2, 0.325f, 0.657f, 2.01f, launch_int8_tile_64x128},
-    {128, 128, 1, 0.397f, 0.44f, 2.81f, launch_int8_tile_128},
-    {128, 256, 1, 0.697f, 0.697f, 3.42f, launch_int8_tile_128x256},
-    {256, 256, 1, 1.32f, 1.42f, 3.82f, launch_int8_tile_256},
+    {64, 64, 2, 0.19f, 0.389f, 1.91f, launch_int8_tile_64},
+    {64, 128, 2, 0.33f, 0.645f, 2.31f, launch_int8_tile_64x128},
+    {128, 128, 1, 0.39f, 0.409f, 2.97f, launch_int8_tile_128},
+    {128, 256, 1, 0.68f, 0.775f, 3.76f, launch_int8_tile_128x256},
+    {256, 256, 1, 1.21f, 1.5f, 4.68f, launch_int8_tile_256},
 };
 constexpr int kInt8Tiles = sizeof(kInt8Tile) / sizeof(kInt8Tile[0]);
 
