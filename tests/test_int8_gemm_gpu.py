@@ -49,12 +49,14 @@ def test_larger_products(gpu, m, n, k):
 
 
 # every kernel, whole and in K splits (few rows: 16 and 32 rows by 16 and 32 columns, eight and sixteen
-# waves; tiles of 64, 64 x 128, 128, 128 x 256 and 256), its last stage not whole
+# waves, two and four pieces in flight; tiles of 64, 64 x 128, 128, 128 x 256 and 256), its last stage not whole
 @pytest.mark.parametrize("m,n,k", [(16, 1000, 528), (9, 1000, 8208), (17, 17, 528), (17, 4097, 1040), (31, 8200, 1040),
                                    (200, 100, 48), (16, 6001, 4112), (90, 17, 12304), (200, 8200, 48), (1300, 1000, 8208),
                                    (90, 4097, 8208), (2050, 2049, 48), (260, 8200, 12304), (130, 6001, 8208),
                                    (1300, 6001, 48), (130, 8200, 16400), (9, 3001, 8208), (200, 8200, 528),
-                                   (260, 4097, 8208), (390, 8200, 12304)])
+                                   (260, 4097, 8208), (390, 8200, 12304), (3, 300, 3712), (20, 100, 3712),
+                                   (20, 5001, 3712), (7, 4000, 12288), (1, 4097, 12304), (40, 4097, 12304),
+                                   (130, 6001, 12304), (2050, 4097, 48)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_every_kernel_and_split(gpu, m, n, k, dtype):
     args, b = case(m, n, k, gpu, dtype, True, seed=11)
@@ -98,7 +100,7 @@ def test_columns_behind_k_and_rows_behind_m_are_not_read_into_the_sum(gpu, m):
 
 
 @pytest.mark.parametrize("m", [1, 3, 16, 17, 32, 33, 130, 300])
-@pytest.mark.parametrize("k", [1, 15, 17, 64, 100, 2077, 8200])
+@pytest.mark.parametrize("k", [1, 15, 17, 64, 100, 2077, 4090, 8200, 12275])
 def test_rows_at_any_address_and_of_any_length(gpu, m, k):
     """Odd K, odd strides and addresses, rows in reverse memory order, broadcast rows; large values around
     every row; an output at an odd address."""
