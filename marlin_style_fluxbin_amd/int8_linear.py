@@ -27,6 +27,10 @@ from .packed_linear import PACKED_M1, PACKED_SMALL_M, DENSE_FALLBACK, PackedLine
 _HALF = (torch.float16, torch.bfloat16)
 _OUT = (torch.float16, torch.bfloat16, torch.float32)
 MAX_IN_FEATURES = 131056  # sums of so many products of codes stay within 32 bits
+# The library's limits, checked here on the whole number: its size arguments are 32 bits wide, and
+# the binding would drop the bits above them without a word.
+MAX_ROWS, MAX_COLUMNS = 1 << 21, 1 << 20
+MAX_OUT_FEATURES = 1 << 20
 _STEP = 16                # the module's rows are whole 16 bytes
 _ROW_LIMIT = 1 << 22      # bytes between two rows that every product reads in place
 _WHAT = "an 8-bit operator"
@@ -101,6 +105,14 @@ def _rows_of(t: torch.Tensor) -> tuple[int, int] | None:
     return rows, step
 
 
+def _check_sizes(t: torch.Tensor, name: str) -> None:
+    """``t [..., columns]``, columns not 0, is within what one call takes."""
+    columns = t.shape[-1]
+    if columns > MAX_COLUMNS or t.numel() > MAX_ROWS * columns:
+        raise ValueError(f"{name} must have at most {MAX_ROWS} rows of at most {MAX_COLUMNS} columns, "
+                         f"got {t.numel() // columns} of {columns}")
+
+
 def _half_input(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> tuple[torch.Tensor, int, int]:
     """``t`` or a copy of it as the kernels read it, its row count and row stride."""
     dtype, shape = t.dtype, t.shape
@@ -111,6 +123,7 @@ def _half_input(t: torch.Tensor, name: str, like: torch.Tensor | None = None) ->
         raise ValueError(f"{name} must have shape [..., columns] with columns to hold")
     if like is not None and (shape != like.shape or dtype is not like.dtype or t.get_device() != like.get_device()):
         raise ValueError(f"{name} must have the input's shape, dtype and device")
+    _check_sizes(t, name)
     if t.is_neg():
         t = t.resolve_neg()
     found = _rows_of(t)
@@ -140,8 +153,9 @@ def _code_outputs(shape: torch.Size, device: torch.device, out) -> tuple[torch.T
 def quantize_int8(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | None = None):
     """Each row of ``x [..., columns]`` (fp16 or bf16) as ``codes`` (int8, x's shape) and ``scales``
     (fp32, x's leading shape): with a the row's largest magnitude, code = round(127 x / a), ties to
-    even, scale = a / 127.  A row with an infinity or NaN stands for NaN (its scale is NaN).  ``out``
-    gives both their memory, none of it an input's."""
+    even, scale = a / 127.  A row with an infinity or NaN stands for NaN (its scale is NaN).  At most
+    2^21 rows of 2^20 columns, here and in the calls below.  ``out`` gives both their memory, none of
+    it an input's."""
     _refuse(x)
     x, rows, stride = _half_input(x, "x")
     shape, device = x.shape, x.device
@@ -161,6 +175,7 @@ def dequantize_int8(codes: torch.Tensor, scales: torch.Tensor, *, dtype: torch.d
     _refuse(codes, scales)
     if codes.shape[-1] < 1:
         raise ValueError("codes must have shape [..., columns] with columns to hold")
+    _check_sizes(codes, "codes")
     found = _rows_of(codes)
     if found is None:
         codes = codes.contiguous()
@@ -261,7 +276,7 @@ def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, w
 
     ``a [..., K]`` and ``weight [N, K]`` int8, their scales fp32 (one per row), ``bias [N]`` and the
     result of ``dtype`` (fp16, bf16 or fp32).  The sum is exact (K up to 131056); scales and bias are
-    applied in fp32, rounded once.  Rows that lie at 16-byte boundaries are read in place where K is a
+    applied in fp32, rounded once.  At most 2^21 rows and N up to 2^20.  Rows that lie at 16-byte boundaries are read in place where K is a
     multiple of 16, and any where ``a`` has at most 32; others are copied first.  ``out`` shares no memory
     with the inputs."""
     shape, wide, index = a.shape, weight.shape, a.get_device()
@@ -274,8 +289,9 @@ def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, w
         raise ValueError("weight must be [N, K] with a's K, on a's device")
     n, k = wide
     device = a.device
-    if not 1 <= k <= MAX_IN_FEATURES or n < 1:
-        raise ValueError(f"K must be in [1, {MAX_IN_FEATURES}] and N positive, got {k} and {n}")
+    if not 1 <= k <= MAX_IN_FEATURES or not 1 <= n <= MAX_OUT_FEATURES or a.numel() > MAX_ROWS * k:
+        raise ValueError(f"K must be in [1, {MAX_IN_FEATURES}], N positive and at most {MAX_OUT_FEATURES} and a of at "
+                         f"most {MAX_ROWS} rows, got K {k}, N {n} and {a.numel() // max(k, 1)} rows")
     code = _CODES.get(dtype)
     if code is None:
         raise ValueError("dtype must be fp16, bf16 or fp32")
@@ -340,11 +356,11 @@ class PackedInt8Linear(PackedLinearBase):
 
     ``codes [O, K]`` int8 and ``scales [O]`` fp32 stand for the weight ``codes * scales[:, None]``; the
     module keeps the tensors it is given where they lie as the kernels read them.
-    Any number of fp16 or bf16 rows on the GPU take the kernels; other inputs are refused unless
-    ``fallback='dense'`` (``F.linear`` with the weight that the codes stand for).  Routes, counters
+    fp16 or bf16 rows on the GPU, up to 2^21 of them, take the kernels, by up to 2^20 outputs; the rest
+    is refused unless ``fallback='dense'`` (``F.linear`` with the weight that the codes stand for).  Routes, counters
     and the bound one-row decode call are those of ``packed_linear.PackedLinearBase``."""
 
-    max_packed_rows = 1 << 21
+    max_packed_rows = MAX_ROWS
     bias_in_kernel = True
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, *, bias: torch.Tensor | None = None,
@@ -395,6 +411,8 @@ class PackedInt8Linear(PackedLinearBase):
         """The rows quantized and multiplied, through a workspace of this callable's own."""
         codes, scales, bias = self._tensor("codes"), self._tensor("scales"), self._tensor("bias")
         width, k, o = self._width, self.in_features, self.out_features
+        if rows > MAX_ROWS or o > MAX_OUT_FEATURES:
+            raise ValueError(f"at most {MAX_ROWS} rows by {MAX_OUT_FEATURES} outputs take the kernels, got {rows} by {o}")
         nbytes = _linear_workspace_bytes(rows, o, k)
         workspace = _new((nbytes,), torch.uint8, device) if nbytes else None
         index = device.index
@@ -420,7 +438,7 @@ class PackedInt8Linear(PackedLinearBase):
         device = self._tensor("codes").device
         rows = x.numel() // k
         if (not x.is_cuda or (dtype is not _BF16 and dtype is not _FP16) or x.get_device() != device.index
-                or rows > self.max_packed_rows):
+                or rows > self.max_packed_rows or self.out_features > MAX_OUT_FEATURES):
             if self.fallback != "dense":
                 raise ValueError("unsupported input; enable explicit dense fallback if needed")
             self._count(DENSE_FALLBACK)
