@@ -355,7 +355,7 @@ class PackedInt8Linear(PackedLinearBase):
     formed in the call).
 
     ``codes [O, K]`` int8 and ``scales [O]`` fp32 stand for the weight ``codes * scales[:, None]``; the
-    module keeps the tensors it is given where they lie as the kernels read them.
+    module holds copies of them.
     fp16 or bf16 rows on the GPU, up to 2^21 of them, take the kernels, by up to 2^20 outputs; the rest
     is refused unless ``fallback='dense'`` (``F.linear`` with the weight that the codes stand for).  Routes, counters
     and the bound one-row decode call are those of ``packed_linear.PackedLinearBase``."""
@@ -377,12 +377,10 @@ class PackedInt8Linear(PackedLinearBase):
         self._init_protocol(fallback=fallback, bias=bias)
         # rows of whole 16 bytes, the columns behind K zero, as the kernels read them
         self._width = -(-self.in_features // _STEP) * _STEP
-        codes = codes.detach()
-        if self._width != self.in_features:
-            codes = F.pad(codes, (0, self._width - self.in_features))
-        codes = codes.contiguous()
-        self.register_buffer("codes", codes.clone() if codes.data_ptr() % 16 else codes)
-        self.register_buffer("scales", scales.detach().contiguous())
+        padded = self._width != self.in_features
+        codes = F.pad(codes.detach(), (0, self._width - self.in_features)) if padded else codes.detach()
+        self.register_buffer("codes", codes.contiguous() if padded else codes.clone(memory_format=torch.contiguous_format))
+        self.register_buffer("scales", scales.detach().clone(memory_format=torch.contiguous_format))
 
     @classmethod
     def from_linear(cls, linear: nn.Linear, *, fallback: str = "error") -> "PackedInt8Linear":
