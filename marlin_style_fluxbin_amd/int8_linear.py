@@ -18,6 +18,7 @@ from functools import lru_cache
 
 import torch
 from torch import nn
+from torch.autograd.graph import increment_version
 from torch.nn import functional as F
 
 from . import _lib
@@ -163,6 +164,8 @@ def quantize_int8(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | N
     columns = shape[-1]
     _launch("fx_int8_quantize", device.index, x.data_ptr(), stride, codes.data_ptr(), code_stride, scales.data_ptr(), rows,
             columns, columns, _CODES[x.dtype])
+    if out is not None:
+        increment_version(out)  # a graph that saved the memory before refuses its backward, as for torch's own out=
     return codes, scales
 
 
@@ -199,6 +202,7 @@ def _norm(x, residual, weight, eps, residual_out, out):
         weight = weight.resolve_neg().contiguous()
     r_ptr = s_ptr = None
     r_stride = s_stride = 0
+    written = () if out is None else tuple(out)
     if residual is not None:
         residual, _, r_stride = _half_input(residual, "residual", x)
         if residual_out is None:
@@ -210,10 +214,13 @@ def _norm(x, residual, weight, eps, residual_out, out):
             if found is None or (found[0] > 1 and found[1] < columns):
                 raise ValueError("residual_out must have contiguous rows, each its own memory")
             s_stride = found[1]
+            written += (residual_out,)
         r_ptr, s_ptr = residual.data_ptr(), residual_out.data_ptr()
     codes, scales, code_stride = _code_outputs(shape, device, out)
     _launch("fx_int8_rmsnorm", device.index, x.data_ptr(), stride, r_ptr, r_stride, s_ptr, s_stride, weight.data_ptr(),
             codes.data_ptr(), code_stride, scales.data_ptr(), rows, columns, columns, float(eps), _CODES[dtype])
+    if written:
+        increment_version(written)
     return codes, scales, residual_out
 
 
@@ -246,6 +253,8 @@ def silu_mul_int8(gate: torch.Tensor, up: torch.Tensor, *, out: tuple[torch.Tens
     columns = shape[-1]
     _launch("fx_int8_silu_mul", device.index, gate.data_ptr(), stride, up.data_ptr(), up_stride, codes.data_ptr(), code_stride,
             scales.data_ptr(), rows, columns, columns, _CODES[gate.dtype])
+    if out is not None:
+        increment_version(out)
     return codes, scales
 
 
@@ -301,7 +310,8 @@ def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, w
         bias = bias.resolve_neg().contiguous()
     _refuse(a_scales, weight_scales, bias, out)
     shape = (*shape[:-1], n)
-    if out is None:
+    given = out is not None
+    if not given:
         out = _new(shape, dtype, device)
         out_stride = n
     else:
@@ -328,6 +338,8 @@ def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, w
     _launch("fx_int8_gemm", index, a_ptr, a_stride, a_scales.data_ptr(), w_ptr, w_stride,
             weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), out_stride,
             None if workspace is None else workspace.data_ptr(), nbytes, rows, n, k, code)
+    if given:
+        increment_version(out)
     return out
 
 
