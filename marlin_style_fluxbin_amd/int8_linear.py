@@ -408,9 +408,25 @@ class PackedInt8Linear(PackedLinearBase):
     def _dense_weight(self, dtype: torch.dtype) -> torch.Tensor:
         return (self.codes[:, :self.in_features].float() * self.scales[:, None]).to(dtype)
 
+    def _load_from_state_dict(self, *args, **kwargs):
+        """Tensors that ``assign=True`` puts in place of the buffers are held as the kernels read them, and
+        a decode binding of the old ones ends."""
+        before = [id(t) for t in self._buffers.values()]
+        super()._load_from_state_dict(*args, **kwargs)
+        for name in ("codes", "scales", "bias"):
+            t = self._buffers[name]
+            if t is not None and (not t.is_contiguous() or t.is_neg() or t.data_ptr() % 16):
+                self._buffers[name] = t.detach().clone(memory_format=torch.contiguous_format)
+        if before != [id(t) for t in self._buffers.values()]:
+            self.clear_prepared_decode()
+
     def _check_before_call(self) -> None:
-        if self._tensor("scales").dtype is not torch.float32 or self._tensor("codes").dtype is not torch.int8:
+        codes, scales, bias = self._tensor("codes"), self._tensor("scales"), self._tensor("bias")
+        if scales.dtype is not torch.float32 or codes.dtype is not torch.int8:
             raise ValueError("codes or scales were cast; move devices without dtype conversion")
+        index = codes.get_device()
+        if scales.get_device() != index or (bias is not None and bias.get_device() != index):
+            raise ValueError("codes, scales and bias must be on one device")
 
     def _check_before_bind(self, device: torch.device) -> None:
         if self.scales.device != device or not self.codes.is_contiguous():

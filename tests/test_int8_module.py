@@ -1,8 +1,10 @@
-"""PackedInt8Linear's payload: memory of its own.  CPU-only."""
+"""PackedInt8Linear's payload: memory of its own, laid out as the kernels read it whatever brings it.
+CPU-only."""
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
-from marlin_style_fluxbin_amd import PackedInt8Linear
+from marlin_style_fluxbin_amd import PackedInt8Linear, int8_linear
 
 
 def payload(columns, seed=0):
@@ -45,3 +47,64 @@ def test_any_layout_becomes_whole_rows():
         assert torch.equal(module.codes, given) and torch.equal(module.scales, scales)
     one = PackedInt8Linear(codes[:1].expand(7, 48), scales[:1].expand(7))
     assert torch.equal(one.codes, codes[:1].repeat(7, 1)) and one.codes.is_contiguous() and one.scales.is_contiguous()
+
+
+# ------------------------------------------------------------------ tensors that a state dict assigns
+class Launched(Exception):
+    pass
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    """Fake tensors of a GPU device; a call that would reach the library ends."""
+    def launch(name, index, *args):
+        raise Launched(name)
+
+    monkeypatch.setattr(int8_linear, "_launch", launch)
+    with FakeTensorMode(), torch.no_grad():
+        yield lambda *shape, dtype=torch.bfloat16, device="cuda:0": torch.empty(*shape, dtype=dtype, device=device)
+
+
+def fake_module(fake, bias=True):
+    return PackedInt8Linear(fake(8, 32, dtype=torch.int8), fake(8, dtype=torch.float32), bias=fake(8) if bias else None)
+
+
+@torch.no_grad()
+def test_assigned_tensors_are_held_as_the_kernels_read_them():
+    """Strided, lazily negated and unaligned ones as copies, others as they are."""
+    codes, scales = payload(48)
+    bias = torch.rand(7)
+    module = PackedInt8Linear(codes, scales, bias=bias)
+    odd = torch.empty(7 * 48 + 3, dtype=torch.int8)[3:].view(7, 48).copy_(codes)
+    for given in (dict(codes=codes.t().contiguous().t(), scales=scales.repeat_interleave(2)[::2],
+                       bias=bias.repeat_interleave(2)[::2]),
+                  dict(codes=odd, scales=torch._neg_view(-scales), bias=torch._neg_view(-bias))):
+        module.load_state_dict(given, assign=True)
+        for name, want in (("codes", codes), ("scales", scales), ("bias", bias)):
+            held = getattr(module, name)
+            assert held.is_contiguous() and not held.is_neg() and held.data_ptr() % 16 == 0 and torch.equal(held, want)
+    module.load_state_dict(dict(codes=codes, scales=scales, bias=bias), assign=True)
+    assert module.codes.data_ptr() == codes.data_ptr()
+
+
+@pytest.mark.parametrize("which", ["codes", "scales", "bias"])
+def test_tensors_of_two_devices_are_refused(fake, which):
+    module = fake_module(fake)
+    with pytest.raises(Launched):
+        module(fake(3, 32))
+    shape, dtype = dict(codes=((8, 32), torch.int8), scales=((8,), torch.float32), bias=((8,), torch.bfloat16))[which]
+    module.load_state_dict({which: fake(*shape, dtype=dtype, device="cpu")}, assign=True, strict=False)
+    for x in (fake(3, 32), fake(1, 1, 32)):
+        with pytest.raises(ValueError, match="device|fallback"):
+            module(x)
+    with pytest.raises(ValueError, match="device|CUDA"):
+        module.bind_prepared_decode(torch.bfloat16)
+
+
+def test_an_assigned_payload_ends_a_binding_of_the_old_one(fake):
+    module = fake_module(fake)
+    module.bind_prepared_decode(torch.bfloat16)
+    module.load_state_dict(fake_module(fake).state_dict())  # written into the buffers that are bound
+    assert module._decode_binding is not None
+    module.load_state_dict(fake_module(fake).state_dict(), assign=True)
+    assert module._decode_binding is None and module._decode_output is None
