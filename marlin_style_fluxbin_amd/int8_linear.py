@@ -454,7 +454,8 @@ class PackedInt8Linear(PackedLinearBase):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if self._decode_binding is not None:
-            return self._decode_binding(x)
+            _refuse_records(x, what=_WHAT)
+            return self._decode_binding(x.resolve_neg() if x.is_neg() else x)
         if torch.is_grad_enabled():
             raise RuntimeError("packed inference requires no_grad/inference_mode")
         shape, k, dtype = x.shape, self.in_features, x.dtype

@@ -1,5 +1,5 @@
 """PackedInt8Linear's payload: memory of its own, laid out as the kernels read it whatever brings it.
-CPU-only."""
+CPU-only but for the last test."""
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -108,3 +108,41 @@ def test_an_assigned_payload_ends_a_binding_of_the_old_one(fake):
     assert module._decode_binding is not None
     module.load_state_dict(fake_module(fake).state_dict(), assign=True)
     assert module._decode_binding is None and module._decode_output is None
+
+
+# ------------------------------------------------------------------ bound calls
+def test_a_bound_call_reads_values_and_refuses_records(fake, monkeypatch):
+    from torch.autograd import forward_ad
+
+    module = fake_module(fake)
+    module.bind_prepared_decode(torch.bfloat16)
+    x = fake(1, 1, 32)
+    addresses = []
+    monkeypatch.setattr(module, "_decode_binding", lambda t: addresses.append(t.is_neg()))
+    module(x)
+    module(torch._neg_view(x))
+    assert addresses == [False, False]
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="tangent"):
+            module(forward_ad.make_dual(x, torch.ones_like(x)))
+        module(x)
+    assert len(addresses) == 3
+
+
+@pytest.mark.gpu
+def test_bound_calls_on_the_gpu(gpu):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    codes, scales = payload(48)
+    module = PackedInt8Linear(codes.to(gpu), scales.to(gpu))
+    x = torch.randn(1, 1, 48, generator=torch.Generator().manual_seed(2)).bfloat16().to(gpu)
+    with torch.no_grad():
+        want, minus = module(x), module(-x)
+        module.bind_prepared_decode(torch.bfloat16)
+        assert torch.equal(module(x), want) and torch.equal(module(torch._neg_view(x)), minus)
+        for record in (lambda: torch.jit.trace(module, (x,), check_trace=False), lambda: make_fx(module)(x)):
+            with pytest.raises(ValueError, match="traced"):
+                record()
+        module.load_state_dict({name: t.clone() for name, t in PackedInt8Linear(codes.to(gpu), 2 * scales.to(gpu))
+                                .state_dict().items()}, assign=True)
+        assert torch.equal(module(x), 2 * want)  # a power of two: exact
