@@ -9,7 +9,8 @@
  *
  * Codes are int8 rows of contiguous columns; strides count elements between rows, all
  * non-negative.  dtype: FX_F16 or FX_BF16 for the rows' inputs, also FX_F32 for the outputs of
- * fx_int8_restore and fx_int8_gemm.  rows up to 2^21 (0 launches nothing), columns up to 2^20.
+ * fx_int8_restore and fx_int8_gemm.  rows up to 2^21 (0 launches nothing), columns up to 2^20 (codes of
+ * more than 16384 columns are formed in 64 bits, at two to six times the time per value).
  * Outputs overlap no input but where it says so.
  */
 #ifndef FLUXBIN_INT8_H
@@ -52,8 +53,8 @@ int fx_int8_restore(const int8_t *codes, long long code_stride, const float *sca
  * fp32, rounded once to dtype (out's and bias's; bias may be NULL).  a [M, K], w [N, K] and
  * out [M, N]; K up to 131056, M up to 2^21, N up to 2^20; strides of a and w 0 or at least K.  out
  * overlaps no input.  Rows of whole 16 bytes (K a multiple of 16) at 16-byte boundaries, at most
- * 2^22 bytes apart, are read where they are, and so are those of a product of up to 32 rows; others
- * are copied into the workspace first.
+ * 2^22 bytes apart, are read where they are, and so are those of a product of up to 32 rows (without
+ * K splits, so slower where K is long and N short); others are copied into the workspace in every call.
  * `workspace` (16-byte aligned, no initial contents, NULL when 0 bytes) also holds the partial sums
  * of a product that is split along K; calls that share one must be ordered on one stream.  `loose`: 1
  * when a's rows do not lie so, plus 2 when w's do not (3 by itself where K is no multiple of 16).

@@ -53,8 +53,8 @@ constexpr int kFewRows = 32;
 constexpr int kMaxSplits = 16;
 
 // Columns of a workgroup of the few-rows kernel.  From 17 rows on 32 of them share what is read of the
-// activations, where one workgroup a compute unit would not do (24 rows by 6144 x 4096 10.8 us, with 16
-// columns 13.4; 32 rows by 4096 x 4096 8.9 with 16 columns, with 32 11.1).
+// activations, where one workgroup a compute unit would not do (24 rows by 6144 x 4096 10.9 us, with 16
+// columns 13.6; 32 rows by 4096 x 4096 9.2 with 16 columns, with 32 11.3).
 int few_columns(int M, int N) { return M > 16 && N > 4096 ? 32 : 16; }
 
 }  // namespace
@@ -66,6 +66,9 @@ int few_columns(int M, int N) { return M > 16 && N > 4096 ? 32 : 16; }
 // in part; for splits the join's launch and the partial sums written and read.  Fitted to 408 sizes (1
 // to 4096 rows, 24 shapes of weights) timed with every tile and 1 to 16 splits: within 5% of the best
 // measured choice at 386 of them (fitted to half of the weights, at 195 of the other 204).
+//
+// Rows at any address (`any`) skip the estimate where they are few: read in place, without K splits, 16
+// bytes at a time (32 x 300 x 15999 87 us, where 16000 columns in K splits take 10).
 Int8GemmPlan plan_int8_gemm(int M, int N, int K, bool any) {
   if (any && M <= kFewRows) return {kInt8Few, 1, K};
   const int stages = (K + 127) / 128;
@@ -99,9 +102,11 @@ Int8GemmPlan plan_int8_gemm(int M, int N, int K, bool any) {
 }
 
 // A wave's pieces of 128 columns in flight: two, eight waves of them (2048 columns), so that few loads run
-// past the last column; four where one pass of them is all (one row by 24576 x 4096 19.7 us, with two 20.1;
-// by 5120 x 5120 12.2 and 10.9).  Sixteen waves where passes of 4096 columns come out even (one row by
-// 4096 x 12288 11.9 us, with eight 12.4; by 4096 x 14336 13.7 and 13.1).
+// past the last column; four where one pass of them is all and an eighth of it at most runs past.  One row
+// by 24576 x K, with two and with four: K 2560 15.5 and 16.4 us, 3328 18.2 and 18.0, 3584 19.0 and 18.8, 4096
+// 20.2 and 19.6, 5120 29.8 and 32.9, 6144 31.2 and 33.9, 8192 37.5 and 37.3 (two there: 4096 x 8192 8.3 and
+// 8.7).  Sixteen waves where passes of 4096 columns come out even (one row by 4096 x 12288 11.9 us, with
+// eight 12.5; by 4096 x 14336 13.7 and 13.1).
 template <int XDT, bool ANY, int MT, int RT>
 void launch_few(const Int8GemmArgs& g, const Int8RowsArgs& rows, hipStream_t s) {
   const dim3 grid(unsigned(g.N + 16 * RT - 1) / (16 * RT));
@@ -124,10 +129,12 @@ void launch_few_rows(const Int8GemmArgs& g, hipStream_t s) {
 }
 
 // Every workgroup quantizes the rows again, 1.5 us for each and each round of workgroups, where codes
-// from a launch of their own cost 2 to 3 us (one row by 4096 x 4096 7.5 us for 8.5, by 1024 x 2000 5.2
-// for 6.4, by 12288 x 1536 9.7 for 9.9, by 24576 x 4096 24.3 for 22.8; two rows by 1024 x 2000 6.7 for
-// 6.7 and by 4096 x 4096 8.7 for 8.4, and a launch less for the host, by 9728 x 896 11.4 for 9.8; four by
-// 1024 x 2000 9.8 for 7.2).
+// from a launch of their own cost 2 to 3 us (one row by 4096 x 4096 7.1 us for 8.2, by 1024 x 2000 5.4
+// for 6.6, by 12288 x 1536 9.2 for 9.1, by 24576 x 4096 24.3 for 22.8; two rows by 1024 x 2000 6.6 for
+// 6.7 and by 4096 x 4096 9.1 for 8.7, by 9728 x 896 11.4 for 9.8; four by 1024 x 2000 9.8 for 7.2).  Where
+// the two are near, the rule takes the launch less: the host's part of it, 3 us, bounds such a call.  It
+// costs the GPU most where several rounds of workgroups have few columns each (one row by 9728 x 896 8.6
+// for 7.8).
 bool int8_linear_fuses(int M, int N, int K) {
   return M <= 2 && long(M) * N <= 12288 && long(M) * K <= kFewCodes;
 }

@@ -2,10 +2,14 @@
 // even, and scale = a / 127, a = max|p|.  p is a row as it is, its RMSNorm (after the residual's
 // addition) or SiLU(gate) * up, so that no 16-bit copy of it is written and read again.
 //
-// One pass: a row's values stay in registers between its maximum and its codes.  Bound by the bytes of
-// the rows: the norm of 8192 rows of 4096 with the residual 44 us, 5.3 TB/s where a large copy reaches
-// 4.7 (results stay in the memory-side cache), the SwiGLU of 4096 rows of 12288 50 us; one row 3 us, of
-// which the launch is 2.
+// Up to 16384 columns one pass: a row's values stay in registers between its maximum and its codes.  Bound
+// by the bytes of the rows: the norm of 8192 rows of 4096 with the residual 44 us, 5.3 TB/s where a large
+// copy reaches 4.7 (results stay in the memory-side cache), the SwiGLU of 4096 rows of 12288 50 us; one row
+// 3 us, of which the launch is 2.
+//
+// Wider rows are formed in 64 bits and read twice (with a residual its sum too), bound by that arithmetic:
+// 4096 rows of 18944 columns as they are 111 us, normalised with the residual 164, SwiGLU 328, where their
+// bytes take 50, 117 and 83 at a copy's rate; one row 11, 14 and 24 us.
 #include "int8_row.h"
 
 namespace fx {
@@ -50,7 +54,7 @@ void launch_rows(const Int8RowsArgs& a, hipStream_t s) {
   else if (width <= 8192) go(int8_rows_kernel<DT, MODE, 512, 2>, 512, 1);
   else if (width <= 12288) go(int8_rows_kernel<DT, MODE, 512, 3>, 512, 1);
   else if (width <= 16384) go(int8_rows_kernel<DT, MODE, 512, 4>, 512, 1);
-  else go(int8_rows_kernel<DT, MODE, 1024, 0>, 1024, 1);
+  else go(int8_rows_kernel<DT, MODE, 1024, 0>, 1024, 1);  // no registers: 4096 rows of 16384 SwiGLU 64 us, of 18944 328
 }
 
 // 16 codes a thread, at whatever address (int8_row.h).

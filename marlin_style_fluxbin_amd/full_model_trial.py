@@ -28,7 +28,7 @@ PACKED_TYPES = (PackedHybridLinear, PackedW3Linear, PackedInt8Linear)
 
 
 def packed_modules(model) -> dict:
-    """Every packed Linear of ``model`` (W3 and hybrid two-base), by module name."""
+    """Every packed Linear of ``model`` (W3, hybrid two-base and 8-bit), by module name."""
     return {name: module for name, module in model.named_modules() if isinstance(module, PACKED_TYPES)}
 
 
@@ -169,7 +169,8 @@ def compare_trace(candidate: dict, reference: dict, *, logprob_tolerance: float)
 def validate_routes(trace: dict, *, expected_linears: int, steps: int) -> bool:
     """Every packed Linear served the prompt once -- densely, or on the small-M
     packed route when the module opts into 2..8-row inputs and the prompt is that
-    short -- and each decode step packed.  Counters at zero are ignored."""
+    short (an 8-bit Linear takes it for every prompt) -- and each decode step packed.
+    Counters at zero are ignored."""
     wanted = ({"dense_fallback": 1, "packed_m1": steps}, {"packed_small_m": 1, "packed_m1": steps})
     routes = trace["routes"]
 

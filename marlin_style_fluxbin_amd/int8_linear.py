@@ -3,10 +3,12 @@
 No reference counterpart: the reference's Linears keep 16-bit activations
 (``w3_lut_deployment.py:190-359``, ``deployment.py:182-297``).  Here a row of activations (a
 token) and a row of the weight (an output channel) are 8-bit codes with an fp32 scale each, the
-products run on the int8 matrix cores with exact sums, and what produces a Linear's input
-writes it as codes at once: :func:`add_rms_norm_int8` in front of q|k|v and gate|up,
+products run on the int8 matrix cores with exact sums, and what produces a Linear's input can
+write it as codes at once: :func:`add_rms_norm_int8` in front of q|k|v and gate|up,
 :func:`silu_mul_int8` in front of down, :func:`quantize_int8` elsewhere.
-:class:`PackedInt8Linear` is the module; ``include/fluxbin_int8.h`` has the format.
+:class:`PackedInt8Linear` is the module, which quantizes its own 16-bit input: a model of them
+does so in every Linear, ``NativeDecodeSession``'s steps take the operators instead.
+``include/fluxbin_int8.h`` has the format.
 
 Every call goes to the HIP kernels on the current stream of the tensors' device; there is no
 CPU substitute, no backward pass and no forward-mode derivative, and calls are not traced.
@@ -285,9 +287,10 @@ def int8_matmul(a: torch.Tensor, a_scales: torch.Tensor, weight: torch.Tensor, w
 
     ``a [..., K]`` and ``weight [N, K]`` int8, their scales fp32 (one per row), ``bias [N]`` and the
     result of ``dtype`` (fp16, bf16 or fp32).  The sum is exact (K up to 131056); scales and bias are
-    applied in fp32, rounded once.  At most 2^21 rows and N up to 2^20.  Rows that lie at 16-byte boundaries are read in place where K is a
-    multiple of 16, and any where ``a`` has at most 32; others are copied first.  ``out`` shares no memory
-    with the inputs."""
+    applied in fp32, rounded once.  At most 2^21 rows and N up to 2^20.  Rows that lie at 16-byte
+    boundaries are read in place where K is a multiple of 16, and any where ``a`` has at most 32; others
+    are copied in every call (512 x 4096 x 4090 31 us, 4096 columns 18).  ``out`` shares no memory with
+    the inputs."""
     shape, wide, index = a.shape, weight.shape, a.get_device()
     if not (a.dtype is _INT8 and weight.dtype is _INT8 and a_scales.dtype is _FP32 and weight_scales.dtype is _FP32
             and index >= 0 and a_scales.get_device() == index and weight.get_device() == index
@@ -367,7 +370,8 @@ class PackedInt8Linear(PackedLinearBase):
     formed in the call).
 
     ``codes [O, K]`` int8 and ``scales [O]`` fp32 stand for the weight ``codes * scales[:, None]``; the
-    module holds copies of them.
+    module holds copies of them (and of a bias, which is rounded to the result's type where its own is
+    another).
     fp16 or bf16 rows on the GPU, up to 2^21 of them, take the kernels, by up to 2^20 outputs; the rest
     is refused unless ``fallback='dense'`` (``F.linear`` with the weight that the codes stand for).  Routes, counters
     and the bound one-row decode call are those of ``packed_linear.PackedLinearBase``."""
