@@ -167,7 +167,7 @@ def quantize_int8(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | N
     _launch("fx_int8_quantize", device.index, x.data_ptr(), stride, codes.data_ptr(), code_stride, scales.data_ptr(), rows,
             columns, columns, _CODES[x.dtype])
     if out is not None:
-        increment_version(out)  # a graph that saved the memory before refuses its backward, as for torch's own out=
+        increment_version((codes, scales))  # a graph that saved the memory before refuses its backward, as for torch's own out=
     return codes, scales
 
 
@@ -204,7 +204,7 @@ def _norm(x, residual, weight, eps, residual_out, out):
         weight = weight.resolve_neg().contiguous()
     r_ptr = s_ptr = None
     r_stride = s_stride = 0
-    written = () if out is None else tuple(out)
+    written = ()
     if residual is not None:
         residual, _, r_stride = _half_input(residual, "residual", x)
         if residual_out is None:
@@ -219,6 +219,8 @@ def _norm(x, residual, weight, eps, residual_out, out):
             written += (residual_out,)
         r_ptr, s_ptr = residual.data_ptr(), residual_out.data_ptr()
     codes, scales, code_stride = _code_outputs(shape, device, out)
+    if out is not None:
+        written += (codes, scales)
     _launch("fx_int8_rmsnorm", device.index, x.data_ptr(), stride, r_ptr, r_stride, s_ptr, s_stride, weight.data_ptr(),
             codes.data_ptr(), code_stride, scales.data_ptr(), rows, columns, columns, float(eps), _CODES[dtype])
     if written:
@@ -256,7 +258,7 @@ def silu_mul_int8(gate: torch.Tensor, up: torch.Tensor, *, out: tuple[torch.Tens
     _launch("fx_int8_silu_mul", device.index, gate.data_ptr(), stride, up.data_ptr(), up_stride, codes.data_ptr(), code_stride,
             scales.data_ptr(), rows, columns, columns, _CODES[gate.dtype])
     if out is not None:
-        increment_version(out)
+        increment_version((codes, scales))
     return codes, scales
 
 

@@ -36,6 +36,19 @@ def test_outputs_given_count_a_change(monkeypatch, which):
     assert all(n >= 1 for n in change[:len(written)]) and not any(change[len(written):]), change
 
 
+@pytest.mark.parametrize("kind", [tuple, list, iter])
+def test_outputs_given_by_any_pair_count_a_change(monkeypatch, kind):
+    monkeypatch.setattr(int8_linear, "_launch", lambda *args: None)
+    with FakeTensorMode(), torch.no_grad():
+        make = lambda *a: torch.empty(*a[:-1], dtype=a[-1], device="cuda:0")
+        x, w, pair = make(4, 64, BF), make(64, BF), (make(4, 64, I8), make(4, F32))
+        for call in (lambda: quantize_int8(x, out=kind(pair)), lambda: rms_norm_int8(x, w, 1e-6, out=kind(pair)),
+                     lambda: silu_mul_int8(x, x, out=kind(pair))):
+            before = [t._version for t in pair]
+            call()
+            assert all(t._version > v for t, v in zip(pair, before))
+
+
 @pytest.mark.gpu
 def test_a_graph_does_not_read_what_a_call_overwrote(gpu):
     x, w = torch.randn(4, 64, device=gpu).to(BF), torch.ones(64, dtype=BF, device=gpu)
