@@ -417,13 +417,13 @@ class PackedInt8Linear(PackedLinearBase):
     def _load_from_state_dict(self, *args, **kwargs):
         """Tensors that ``assign=True`` puts in place of the buffers are held as the kernels read them, and
         a decode binding of the old ones ends."""
-        before = [id(t) for t in self._buffers.values()]
+        before = list(self._buffers.values())  # (held, so that no new tensor is taken for a freed one)
         super()._load_from_state_dict(*args, **kwargs)
         for name in ("codes", "scales", "bias"):
             t = self._buffers[name]
             if t is not None and (not t.is_contiguous() or t.is_neg() or t.data_ptr() % 16):
                 self._buffers[name] = t.detach().clone(memory_format=torch.contiguous_format)
-        if before != [id(t) for t in self._buffers.values()]:
+        if any(t is not b for t, b in zip(self._buffers.values(), before)):
             self.clear_prepared_decode()
 
     def _check_before_call(self) -> None:

@@ -108,6 +108,11 @@ def test_an_assigned_payload_ends_a_binding_of_the_old_one(fake):
     assert module._decode_binding is not None
     module.load_state_dict(fake_module(fake).state_dict(), assign=True)
     assert module._decode_binding is None and module._decode_output is None
+    for given in (dict(codes=fake(32, 8, dtype=torch.int8).t()), dict(scales=fake(16, dtype=torch.float32)[::2]),
+                  dict(bias=fake(16)[::2])):  # each held as a copy
+        module.bind_prepared_decode(torch.bfloat16)
+        module.load_state_dict(given, assign=True, strict=False)
+        assert module._decode_binding is None
 
 
 # ------------------------------------------------------------------ bound calls
